@@ -27,6 +27,8 @@ _MODULES = (
     "components.dist_configs",
     "components.ops",
     "components.layers",
+    "components.attention",
+    "components.dropout",
     "components.sparse_utils",
 )
 

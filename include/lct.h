@@ -804,6 +804,114 @@ int32_t lct_skinny_linear(const void *a, const void *w, void *out, int32_t token
 int32_t lct_bandwidth_probe(int32_t kind, const void *src, int64_t src_bytes, void *dst,
                             int64_t dst_bytes, int32_t workgroups, hipStream_t stream);
 
+/* ---- attention with a sliding window and sinks (scores, softmax and products
+ * of LCT/components/layers.py:232-305's causal attention, whose every query sees
+ * all keys up to its own).
+ *
+ * BF16 or FP16 (fp16 != 0) tensors [batch, head, token, channel] by strides in
+ * elements (batch, head, token; channels adjacent), multiples of 8, the token's
+ * below 2^24; pointers 16-byte aligned.  head_dim: a multiple of 8 up to 128.
+ * heads: a multiple of kv_heads; query head h reads key head
+ * h / (heads / kv_heads).  Query i stands at position i + keys - queries.  It
+ * sees key j where j <= its position, both lie below lengths[b] (NULL: keys),
+ * and window == 0 or its position - j < window or j < sinks.  A query that sees
+ * no key has output zero and no gradient.  scale: positive.
+ *
+ * out = softmax(scale q k^T) v.  lse[batch][heads][queries rounded up to 128]:
+ * log2 of the sum of the scores' exponentials, +infinity where a query sees no
+ * key; NULL: not written (lct_attention_forward only).  Scores, sums and products are FP32; the
+ * weights are rounded to the tensors' type for the product with v. */
+#define LCT_MAX_HEAD_DIM 128
+#define LCT_MAX_ATTENTION_SPLITS 64
+typedef struct {
+    const void *q, *k, *v;
+    void *out;
+    float *lse;
+    const int32_t *lengths;      /* int32[batch] or NULL */
+    int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];
+    int32_t batch, heads, kv_heads, queries, keys, head_dim, window, sinks, fp16;
+    float scale;
+} lct_attention;
+
+/* splits > 1: each query's keys are shared among that many workgroups, whose
+ * parts meet in `workspace` (8-byte aligned), splits * batch * heads * queries *
+ * (head_dim + 2) floats, and are joined by a second launch.  splits == 1:
+ * workspace may be NULL. */
+int32_t lct_attention_forward(const lct_attention *a, int32_t splits, float *workspace,
+                              int64_t workspace_floats, hipStream_t stream);
+
+/* The gradients of q, k and v from that of out, a->out and a->lse as the forward
+ * call wrote them; those of a key head that several query heads share are
+ * their sum.  delta: working array of lse's size.  The queries that see a block
+ * of 128 keys are shared among `splits` workgroups, among `sink_splits` where
+ * the block holds sinks (and window > 0); with either above 1, `workspace`
+ * holds batch * kv_heads * (sink blocks * sink_splits + other blocks * splits) *
+ * 256 * head_dim floats, added by a further launch in their order. */
+typedef struct {
+    const void *grad;
+    void *dq, *dk, *dv;
+    float *delta;
+    int64_t grad_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
+} lct_attention_gradients;
+
+int32_t lct_attention_backward(const lct_attention *a, const lct_attention_gradients *d,
+                               int32_t splits, int32_t sink_splits, float *workspace,
+                               int64_t workspace_floats, hipStream_t stream);
+
+/* One query per sequence against its cache: a->queries == 1, a->keys the caches'
+ * capacity, a->lengths the sequences' lengths with the query's own token (0:
+ * output zero; NULL: the capacity), the query at position length - 1; else as
+ * lct_attention_forward, with a->lse NULL.  splits > 1: workspace of splits *
+ * batch * heads * (head_dim + 2) floats, 8-byte aligned. */
+int32_t lct_attention_decode(const lct_attention *a, int32_t splits, float *workspace,
+                             int64_t workspace_floats, hipStream_t stream);
+
+/* Value types of lct_rotate and lct_dropout. */
+#define LCT_BF16 0
+#define LCT_FP16 1
+#define LCT_FP32 2
+
+/* ---- rotary positions (examples/nanogpt/train_gpt_lct.py:150-165): the first
+ * rotary_dim (even) of head_dim <= LCT_MAX_ROTARY_DIM channels of q and, unless
+ * k_in is NULL, k, [batch, token, head, channel] by strides in elements (batch,
+ * token, head; channels adjacent), turn in pairs (i, i + rotary_dim / 2) or, if
+ * interleaved, (2 i, 2 i + 1):
+ *     (x, y) -> magnitude (x cos - y sin, y cos + x sin),
+ * the angle being the position times turns[i] / 2^64 of a turn; `inverse` turns
+ * the other way (the gradient).  The other channels are copied.  Token t of
+ * sequence b is at start + t + positions[b * position_stride[0]] where
+ * position_stride[1] is 0, else at start + positions[b * position_stride[0] + t *
+ * position_stride[1]]; positions NULL: at start + t.
+ * capacity > 0: k_out (and v_out, v_in copied) are caches of that many tokens,
+ * written at the token's position; positions outside are not written.  Without
+ * a capacity, out may be in, with the same strides. */
+#define LCT_MAX_ROTARY_DIM 256
+typedef struct {
+    const void *q_in, *k_in, *v_in;
+    void *q_out, *k_out, *v_out;
+    const int64_t *turns;        /* int64[rotary_dim / 2], fixed point modulo one turn */
+    const int32_t *positions;
+    int64_t q_in_stride[3], k_in_stride[3], v_in_stride[3];
+    int64_t q_out_stride[3], k_out_stride[3], v_out_stride[3];
+    int64_t position_stride[2];
+    int64_t start;
+    int32_t batch, tokens, heads, kv_heads, head_dim, rotary_dim, interleaved, inverse, type,
+        capacity;
+    float magnitude;
+} lct_rotary;
+
+int32_t lct_rotate(const lct_rotary *r, hipStream_t stream);
+
+/* ---- out = residual + dropout(x) (residual NULL: dropout(x)), n contiguous
+ * values, pointers 16-byte aligned, n up to 2^35 - 2048.  Value i is kept, and
+ * multiplied by 65536 / (65536 - below), where the 16-bit half i % 8 (the low
+ * half of a word first) of Philox-4x32-10's four words at counter (i / 8,
+ * offset + *offset_more) under the key `seed` is at least `below` (0..65536).
+ * offset_more: NULL, or a device value that is read when the launch runs. */
+int32_t lct_dropout(const void *x, const void *residual, void *out, int64_t n, int32_t type,
+                    int32_t below, uint64_t seed, uint64_t offset, const int64_t *offset_more,
+                    hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -30,6 +30,10 @@ SOURCES = [
     "noalloc.hip",
     "layers.hip",
     "linear.hip",
+    "attention.hip",
+    "attention_decode.hip",
+    "rotary.hip",
+    "dropout.hip",
     "bandwidth.hip",
 ]
 

@@ -1,0 +1,792 @@
+// Attention with a sliding window and sinks, forward.
+#include <algorithm>
+#include <type_traits>
+
+#include "attention_core.h"
+
+namespace lct {
+namespace {
+
+constexpr int kQueryTile = 128;      // queries of a workgroup, 32 per wave
+constexpr int kKeyTile = 64;         // keys per step
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRescale = 8.0f;     // how far (log2) a running maximum may lag
+constexpr float kHalfWeights = 256.0f;
+
+// lse's and delta's values per head: whole query tiles, the last one's extra
+// rows among them.
+__host__ __device__ __forceinline__ int64_t lse_pitch(int32_t queries) {
+    return (int64_t{queries} + kQueryTile - 1) / kQueryTile * kQueryTile;
+}
+
+// A lane's share of one row (4 of each 8 channels), times `factor`.
+template <bool kHalf, int kColumns>
+__device__ __forceinline__ void store_row(uint16_t *dst, const f32x16 (&x)[kColumns], float factor,
+                                          int32_t dim) {
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int32_t channel = 32 * c + 8 * g + 4 * (wave_lane() >> 5);
+            if (channel >= dim) continue;
+            u32x2 pairs;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                pairs[i] = Element<kHalf>::round_pair(x[c][4 * g + 2 * i] * factor,
+                                                      x[c][4 * g + 2 * i + 1] * factor);
+            *reinterpret_cast<u32x2 *>(dst + channel) = pairs;
+        }
+}
+
+template <bool kHalf, int kDim, bool kSplit>
+__global__ __launch_bounds__(kAttentionThreads, 2) void attention_forward_kernel(
+    lct_attention a, int32_t tiles, int32_t splits, float *__restrict__ parts) {
+    constexpr int kPitch = kPitchOf<kDim>;
+    constexpr int kSteps = kDim / 16, kColumns = kDim / 32;
+    __shared__ __attribute__((aligned(1024))) uint16_t k_even[kKeyTile * kPitch];
+    __shared__ __attribute__((aligned(1024))) uint16_t v_even[kKeyTile * kPitch];
+    __shared__ __attribute__((aligned(1024))) uint16_t k_odd[kKeyTile * kPitch];
+    __shared__ __attribute__((aligned(1024))) uint16_t v_odd[kKeyTile * kPitch];
+
+    const int64_t per_head = int64_t{tiles} * splits;
+    const int64_t item = xcd_item(per_head * a.batch * a.heads);
+    if (item >= per_head * a.batch * a.heads) return;
+    const int32_t bh = static_cast<int32_t>(item / per_head);
+    const int32_t part = static_cast<int32_t>(item % per_head);
+    const int32_t b = bh / a.heads, h = bh % a.heads, kv = h / (a.heads / a.kv_heads);
+    // The last queries see the most keys: they go first.
+    const int32_t tile = tiles - 1 - part / splits, split = part % splits;
+
+    const int lane = wave_lane(), half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int32_t shift = a.keys - a.queries;
+    const int32_t length = sequence_length(a, b);
+    const int32_t first = tile * kQueryTile;
+    const int32_t last = min(first + kQueryTile, a.queries) - 1;
+    const KeyTiles all(a, first + shift, last + shift, length, kKeyTile);
+    const int32_t per_split = (all.count + splits - 1) / splits;
+    const int32_t begin = split * per_split, end = min(all.count, begin + per_split);
+
+    // This wave's queries, one per lane (twice): q, and what each sees.
+    const int32_t wave_first = first + 32 * wave;
+    const int32_t row = wave_first + (lane & 31);
+    const uint16_t *q = static_cast<const uint16_t *>(a.q) + b * a.q_stride[0] + h * a.q_stride[1];
+    u32x4 q_operand[kSteps];
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s)
+        q_operand[s] = load_operand(q, a.q_stride[2], row, a.queries, a.head_dim, s);
+    const Sight sight = sight_of(a, row < a.queries ? row + shift : -1, length);
+    const int32_t low_position = wave_first + shift;
+    const int32_t high_position = min(wave_first + 31, a.queries - 1) + shift;
+
+    const uint16_t *k = static_cast<const uint16_t *>(a.k) + b * a.k_stride[0] + kv * a.k_stride[1];
+    const uint16_t *v = static_cast<const uint16_t *>(a.v) + b * a.v_stride[0] + kv * a.v_stride[1];
+    TileLoads<kKeyTile, kPitch> k_loads, v_loads;
+    k_loads.prepare(a.k_stride[2], a.head_dim);
+    v_loads.prepare(a.v_stride[2], a.head_dim);
+    const auto load = [&](int32_t t, uint16_t *keys, uint16_t *values) __attribute__((always_inline)) {
+        const int32_t key = all.first_key(t, kKeyTile);
+        k_loads.issue(k + key * a.k_stride[2], length - key, a.k_stride[2], a.head_dim,
+                      keys);
+        v_loads.issue(v + key * a.v_stride[2], length - key, a.v_stride[2], a.head_dim,
+                      values);
+    };
+
+    const float factor = a.scale * kLog2e;
+    f32x16 out[kColumns];
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c) out[c] = f32x16{};
+    float most = -INFINITY;     // the scores' running maximum, or up to kRescale below
+    float shifted = 0.0f;       // its product with factor, 0 while no key was seen
+    float total = 0.0f;         // this lane's keys' weights
+
+    const auto step = [&](int32_t t, const uint16_t *keys, const uint16_t *values) __attribute__((always_inline)) {
+        const int32_t key = all.first_key(t, kKeyTile);
+        const bool seen_by_some =
+            key <= high_position
+            && (a.window == 0 || key + kKeyTile > low_position - a.window + 1 || key < a.sinks);
+        if (!seen_by_some) return;
+        const bool seen_by_all =
+            key + kKeyTile - 1 <= low_position && high_position < length
+            && (a.window == 0 || high_position - key < a.window || key + kKeyTile <= a.sinks);
+        f32x16 s[2];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            s[n] = f32x16{};
+#pragma unroll
+            for (int d = 0; d < kSteps; ++d)
+                s[n] = Element<kHalf>::multiply(read_rows<kPitch>(keys, n, d), q_operand[d], s[n]);
+        }
+        if (!seen_by_all) {
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int32_t at = key + 32 * n + 8 * (r / 4) + 4 * half + r % 4;
+                    s[n][r] = sight(at) ? s[n][r] : -INFINITY;
+                }
+        }
+        float top = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+        for (int r = 1; r < 16; ++r) top = fmaxf(fmaxf(top, s[0][r]), s[1][r]);
+        top = across_max(top);
+        if (__any(top * factor > most * factor + kRescale)) {
+            const float next = fmaxf(most, top);
+            const float scaled = next == -INFINITY ? 0.0f : next * factor;
+            const float change = exp2_fast(most * factor - scaled);
+            most = next;
+            shifted = scaled;
+            total *= change;
+#pragma unroll
+            for (int c = 0; c < kColumns; ++c)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) out[c][r] *= change;
+        }
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[n][r] = exp2_fast(__builtin_fmaf(s[n][r], factor, -shifted));
+                total += s[n][r];
+            }
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                const u32x4 weights = as_operand<kHalf>(s[n], p);
+#pragma unroll
+                for (int c = 0; c < kColumns; ++c)
+                    out[c] = Element<kHalf>::multiply(
+                        read_columns<kPitch>(values, 32 * n + 16 * p, c), weights, out[c]);
+            }
+    };
+
+    if (begin < end) load(begin, k_even, v_even);
+    for (int32_t t = begin; t < end; t += 2) {
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        if (t + 1 < end) load(t + 1, k_odd, v_odd);
+        step(t, k_even, v_even);
+        if (t + 1 >= end) break;
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        if (t + 2 < end) load(t + 2, k_even, v_even);
+        step(t + 1, k_odd, v_odd);
+    }
+
+    total = across_sum(total);
+    if constexpr (kSplit) {
+        if (row >= a.queries) return;
+        float *part_out = parts + ((int64_t{bh} * splits + split) * a.queries + row) * (a.head_dim + 2);
+#pragma unroll
+        for (int c = 0; c < kColumns; ++c)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int32_t channel = 32 * c + 8 * g + 4 * half;
+                if (channel >= a.head_dim) continue;
+#pragma unroll
+                for (int i = 0; i < 4; i += 2)
+                    *reinterpret_cast<f32x2 *>(part_out + channel + i) =
+                        f32x2{out[c][4 * g + i], out[c][4 * g + i + 1]};
+            }
+        if (half == 0)
+            *reinterpret_cast<f32x2 *>(part_out + a.head_dim) = f32x2{shifted, total};
+        return;
+    }
+    // Rows past the last query have no output but a place in lse.
+    if (a.lse != nullptr && half == 0)
+        a.lse[int64_t{bh} * lse_pitch(a.queries) + row] =
+            total == 0.0f || row >= a.queries ? INFINITY : shifted + __log2f(total);
+    if (row >= a.queries) return;
+    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+    uint16_t *dst = static_cast<uint16_t *>(a.out) + b * a.out_stride[0] + h * a.out_stride[1]
+                    + row * a.out_stride[2];
+    store_row<kHalf, kColumns>(dst, out, inverse, a.head_dim);
+}
+
+// Joins the parts of a query's keys: sum of 2^(shift - largest) out, over the
+// same sum of the weights.  A wave per query, two channels per lane.
+template <bool kHalf>
+__global__ __launch_bounds__(kAttentionThreads) void attention_join_kernel(
+    lct_attention a, int64_t pitch, int32_t splits, const float *__restrict__ parts) {
+    const int64_t item = int64_t{blockIdx.x} * kAttentionWaves + threadIdx.x / kWave;
+    if (item >= int64_t{a.batch} * a.heads * pitch) return;
+    const int32_t bh = static_cast<int32_t>(item / pitch), row = static_cast<int32_t>(item % pitch);
+    if (row >= a.queries) {
+        if (a.lse != nullptr && wave_lane() == 0) a.lse[item] = INFINITY;
+        return;
+    }
+    const int32_t width = a.head_dim + 2, channel = 2 * wave_lane();
+    const float *part = parts + (int64_t{bh} * splits * a.queries + row) * width;
+    const int64_t step = int64_t{a.queries} * width;
+    float largest = -INFINITY;
+    for (int32_t s = 0; s < splits; ++s) {
+        const f32x2 stats = *reinterpret_cast<const f32x2 *>(part + s * step + a.head_dim);
+        if (stats[1] != 0.0f) largest = fmaxf(largest, stats[0]);
+    }
+    float total = 0.0f, x = 0.0f, y = 0.0f;
+    for (int32_t s = 0; s < splits; ++s) {
+        const f32x2 stats = *reinterpret_cast<const f32x2 *>(part + s * step + a.head_dim);
+        if (stats[1] == 0.0f) continue;
+        const float weight = exp2_fast(stats[0] - largest);
+        total += weight * stats[1];
+        if (channel < a.head_dim) {
+            const f32x2 o = *reinterpret_cast<const f32x2 *>(part + s * step + channel);
+            x += weight * o[0];
+            y += weight * o[1];
+        }
+    }
+    if (a.lse != nullptr && wave_lane() == 0)
+        a.lse[item] = total == 0.0f ? INFINITY : largest + __log2f(total);
+    if (channel >= a.head_dim) return;
+    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+    uint16_t *dst = static_cast<uint16_t *>(a.out) + (bh / a.heads) * a.out_stride[0]
+                    + (bh % a.heads) * a.out_stride[1] + row * a.out_stride[2];
+    *reinterpret_cast<uint32_t *>(dst + channel) =
+        Element<kHalf>::round_pair(x * inverse, y * inverse);
+}
+
+// ---- backward
+//
+// With P = 2^(factor s - lse), dP = dO v^T and delta = sum(dO out):
+// dS = P (dP - delta), dq = scale dS k, dk = scale dS^T q, dv = P^T dO.  Two
+// kernels, one per side that is summed over, each of which computes the scores
+// again: seven products in place of five, but no sum is shared between
+// workgroups, so results do not depend on timing.
+
+// A wave's 32 queries, the keys in tiles.  delta is stored for the other kernel.
+template <bool kHalf, int kDim>
+__global__ __launch_bounds__(kAttentionThreads, 2) void attention_dq_kernel(
+    lct_attention a, lct_attention_gradients d, int32_t tiles) {
+    constexpr int kPitch = kPitchOf<kDim>;
+    constexpr int kSteps = kDim / 16, kColumns = kDim / 32;
+    __shared__ __attribute__((aligned(1024))) uint16_t k_even[kKeyTile * kPitch];
+    __shared__ __attribute__((aligned(1024))) uint16_t v_even[kKeyTile * kPitch];
+    __shared__ __attribute__((aligned(1024))) uint16_t k_odd[kKeyTile * kPitch];
+    __shared__ __attribute__((aligned(1024))) uint16_t v_odd[kKeyTile * kPitch];
+
+    const int64_t items = int64_t{tiles} * a.batch * a.heads;
+    const int64_t item = xcd_item(items);
+    if (item >= items) return;
+    const int32_t bh = static_cast<int32_t>(item / tiles);
+    const int32_t b = bh / a.heads, h = bh % a.heads, kv = h / (a.heads / a.kv_heads);
+    const int32_t tile = tiles - 1 - static_cast<int32_t>(item % tiles);
+
+    const int lane = wave_lane(), half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int32_t shift = a.keys - a.queries;
+    const int32_t length = sequence_length(a, b);
+    const int32_t first = tile * kQueryTile;
+    const int32_t last = min(first + kQueryTile, a.queries) - 1;
+    const KeyTiles all(a, first + shift, last + shift, length, kKeyTile);
+
+    const int32_t wave_first = first + 32 * wave;
+    const int32_t row = wave_first + (lane & 31);
+    const Sight sight = sight_of(a, row < a.queries ? row + shift : -1, length);
+    const int32_t low_position = wave_first + shift;
+    const int32_t high_position = min(wave_first + 31, a.queries - 1) + shift;
+    // Queries that see nothing take part as zeros.
+    const int32_t rows = sight.limit > 0 ? a.queries : 0;
+
+    u32x4 q_operand[kSteps], g_operand[kSteps];
+    float delta = 0.0f;
+    {
+        const uint16_t *q =
+            static_cast<const uint16_t *>(a.q) + b * a.q_stride[0] + h * a.q_stride[1];
+        const uint16_t *g = static_cast<const uint16_t *>(d.grad) + b * d.grad_stride[0]
+                            + h * d.grad_stride[1];
+        const uint16_t *o =
+            static_cast<const uint16_t *>(a.out) + b * a.out_stride[0] + h * a.out_stride[1];
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            q_operand[s] = load_operand(q, a.q_stride[2], row, rows, a.head_dim, s);
+            g_operand[s] = load_operand(g, d.grad_stride[2], row, rows, a.head_dim, s);
+            const u32x4 out = load_operand(o, a.out_stride[2], row, rows, a.head_dim, s);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                delta += Element<kHalf>::low(g_operand[s][i]) * Element<kHalf>::low(out[i]);
+                delta += Element<kHalf>::high(g_operand[s][i]) * Element<kHalf>::high(out[i]);
+            }
+        }
+    }
+    delta = across_sum(delta);
+    const int64_t at = int64_t{bh} * lse_pitch(a.queries) + row;
+    if (half == 0) d.delta[at] = delta;
+    const float lse = a.lse[at];
+
+    const uint16_t *k = static_cast<const uint16_t *>(a.k) + b * a.k_stride[0] + kv * a.k_stride[1];
+    const uint16_t *v = static_cast<const uint16_t *>(a.v) + b * a.v_stride[0] + kv * a.v_stride[1];
+    TileLoads<kKeyTile, kPitch> k_loads, v_loads;
+    k_loads.prepare(a.k_stride[2], a.head_dim);
+    v_loads.prepare(a.v_stride[2], a.head_dim);
+    const auto load = [&](int32_t t, uint16_t *keys, uint16_t *values)
+                          __attribute__((always_inline)) {
+        const int32_t key = all.first_key(t, kKeyTile);
+        k_loads.issue(k + key * a.k_stride[2], length - key, a.k_stride[2], a.head_dim, keys);
+        v_loads.issue(v + key * a.v_stride[2], length - key, a.v_stride[2], a.head_dim, values);
+    };
+
+    const float factor = a.scale * kLog2e;
+    f32x16 dq[kColumns];
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c) dq[c] = f32x16{};
+
+    const auto step = [&](int32_t t, const uint16_t *keys, const uint16_t *values)
+                          __attribute__((always_inline)) {
+        const int32_t key = all.first_key(t, kKeyTile);
+        const bool seen_by_some =
+            key <= high_position
+            && (a.window == 0 || key + kKeyTile > low_position - a.window + 1 || key < a.sinks);
+        if (!seen_by_some) return;
+        const bool seen_by_all =
+            key + kKeyTile - 1 <= low_position && high_position < length
+            && (a.window == 0 || high_position - key < a.window || key + kKeyTile <= a.sinks);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            f32x16 s{}, e;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) e[r] = -delta;
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                s = Element<kHalf>::multiply(read_rows<kPitch>(keys, n, i), q_operand[i], s);
+                e = Element<kHalf>::multiply(read_rows<kPitch>(values, n, i), g_operand[i], e);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = exp2_fast(__builtin_fmaf(s[r], factor, -lse)) * e[r];
+            if (!seen_by_all) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int32_t column = key + 32 * n + 8 * (r / 4) + 4 * half + r % 4;
+                    s[r] = sight(column) ? s[r] : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                const u32x4 ds = as_operand<kHalf>(s, p);
+#pragma unroll
+                for (int c = 0; c < kColumns; ++c)
+                    dq[c] = Element<kHalf>::multiply(
+                        read_columns<kPitch>(keys, 32 * n + 16 * p, c), ds, dq[c]);
+            }
+        }
+    };
+
+    if (all.count > 0) load(0, k_even, v_even);
+    for (int32_t t = 0; t < all.count; t += 2) {
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        if (t + 1 < all.count) load(t + 1, k_odd, v_odd);
+        step(t, k_even, v_even);
+        if (t + 1 >= all.count) break;
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        if (t + 2 < all.count) load(t + 2, k_even, v_even);
+        step(t + 1, k_odd, v_odd);
+    }
+    if (row >= a.queries) return;
+    uint16_t *dst = static_cast<uint16_t *>(d.dq) + b * d.dq_stride[0] + h * d.dq_stride[1]
+                    + row * d.dq_stride[2];
+    store_row<kHalf, kColumns>(dst, dq, a.scale, a.head_dim);
+}
+
+// How a key block's queries are shared: blocks that hold sinks are seen by all
+// later queries and have parts of their own number.
+struct KeyBlocks {
+    int32_t blocks, sink_blocks, splits, sink_splits;
+    __host__ __device__ __forceinline__ int64_t parts() const {
+        return int64_t{sink_blocks} * sink_splits + int64_t{blocks - sink_blocks} * splits;
+    }
+    __host__ __device__ __forceinline__ int64_t first_part(int32_t block) const {
+        return block < sink_blocks
+                   ? int64_t{block} * sink_splits
+                   : int64_t{sink_blocks} * sink_splits + int64_t{block - sink_blocks} * splits;
+    }
+    __host__ __device__ __forceinline__ int32_t parts_of(int32_t block) const {
+        return block < sink_blocks ? sink_splits : splits;
+    }
+};
+
+constexpr int kKeyBlock = 128;       // keys of a workgroup, 32 per wave
+constexpr int kQueryStep = 64;       // queries per step
+
+// A wave's 32 keys, the queries (of all heads that share them) in tiles.
+template <bool kHalf, int kDim>
+__global__ __launch_bounds__(kAttentionThreads, kDim > 64 ? 1 : 2) void attention_dkdv_kernel(
+    lct_attention a, lct_attention_gradients d, KeyBlocks blocks, float *__restrict__ parts) {
+    constexpr int kPitch = kPitchOf<kDim>;
+    constexpr int kSteps = kDim / 16, kColumns = kDim / 32;
+    __shared__ __attribute__((aligned(1024))) uint16_t q_even[kQueryStep * kPitch];
+    __shared__ __attribute__((aligned(1024))) uint16_t g_even[kQueryStep * kPitch];
+    __shared__ __attribute__((aligned(1024))) uint16_t q_odd[kQueryStep * kPitch];
+    __shared__ __attribute__((aligned(1024))) uint16_t g_odd[kQueryStep * kPitch];
+    __shared__ __attribute__((aligned(1024))) float stats_even[2 * kQueryStep];
+    __shared__ __attribute__((aligned(1024))) float stats_odd[2 * kQueryStep];
+
+    const int64_t per_head = blocks.parts();
+    const int64_t items = per_head * a.batch * a.kv_heads;
+    const int64_t item = xcd_item(items);
+    if (item >= items) return;
+    const int32_t bkv = static_cast<int32_t>(item / per_head);
+    const int32_t b = bkv / a.kv_heads, kv = bkv % a.kv_heads, group = a.heads / a.kv_heads;
+    const int64_t part = item % per_head;
+    const int64_t sink_parts = int64_t{blocks.sink_blocks} * blocks.sink_splits;
+    int32_t block, split;
+    if (part < sink_parts) {
+        block = static_cast<int32_t>(part / blocks.sink_splits);
+        split = static_cast<int32_t>(part % blocks.sink_splits);
+    } else {
+        block = blocks.sink_blocks + static_cast<int32_t>((part - sink_parts) / blocks.splits);
+        split = static_cast<int32_t>((part - sink_parts) % blocks.splits);
+    }
+
+    const int lane = wave_lane(), half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int32_t shift = a.keys - a.queries;
+    const int32_t length = sequence_length(a, b);
+    const int32_t first = block * kKeyBlock;
+    // Positions that see some of the block's keys, and their queries' tiles.
+    const int32_t last_key = min(first + kKeyBlock, length) - 1;
+    const int32_t last_position =
+        last_key < first                            ? -1
+        : a.window == 0 || first < a.sinks          ? length - 1
+        : last_key > length - a.window              ? length - 1
+                                                    : last_key + a.window - 1;
+    const int32_t live = min(a.queries, length - shift);     // queries below the length
+    const int32_t low = max(0, first - shift), high = min(live, last_position + 1 - shift);
+    const int32_t low_tile = low / kQueryStep;
+    const int32_t per_query_head =
+        high > low ? (high + kQueryStep - 1) / kQueryStep - low_tile : 0;
+    const int32_t steps = per_query_head * group;
+    const int32_t per_split = (steps + blocks.parts_of(block) - 1) / blocks.parts_of(block);
+    const int32_t begin = split * per_split, end = min(steps, begin + per_split);
+
+    const int32_t wave_first = first + 32 * wave;
+    const int32_t key = wave_first + (lane & 31);
+    const uint16_t *k = static_cast<const uint16_t *>(a.k) + b * a.k_stride[0] + kv * a.k_stride[1];
+    const uint16_t *v = static_cast<const uint16_t *>(a.v) + b * a.v_stride[0] + kv * a.v_stride[1];
+    u32x4 k_operand[kSteps], v_operand[kSteps];
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+        k_operand[s] = load_operand(k, a.k_stride[2], key, length, a.head_dim, s);
+        v_operand[s] = load_operand(v, a.v_stride[2], key, length, a.head_dim, s);
+    }
+
+    TileLoads<kQueryStep, kPitch> q_loads, g_loads;
+    q_loads.prepare(a.q_stride[2], a.head_dim);
+    g_loads.prepare(d.grad_stride[2], a.head_dim);
+    const auto load = [&](int32_t t, uint16_t *q_tile, uint16_t *g_tile, float *stats)
+                          __attribute__((always_inline)) {
+        const int32_t h = kv * group + t / per_query_head;
+        const int32_t query = (low_tile + t % per_query_head) * kQueryStep;
+        q_loads.issue(static_cast<const uint16_t *>(a.q) + b * a.q_stride[0] + h * a.q_stride[1]
+                          + query * a.q_stride[2],
+                      live - query, a.q_stride[2], a.head_dim, q_tile);
+        g_loads.issue(static_cast<const uint16_t *>(d.grad) + b * d.grad_stride[0]
+                          + h * d.grad_stride[1] + query * d.grad_stride[2],
+                      live - query, d.grad_stride[2], a.head_dim, g_tile);
+        if (wave < 2) {
+            const float *from = (wave == 0 ? a.lse : d.delta)
+                                + (int64_t{b} * a.heads + h) * lse_pitch(a.queries) + query;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                make_rsrc(from, kQueryStep * 4),
+                (__attribute__((address_space(3))) void *)(stats + wave * kQueryStep), 4, lane * 4,
+                0, 0, 0);
+        }
+    };
+
+    const float factor = a.scale * kLog2e;
+    f32x16 dk[kColumns], dv[kColumns];
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c) dk[c] = dv[c] = f32x16{};
+
+    const auto step = [&](int32_t t, const uint16_t *q_tile, const uint16_t *g_tile,
+                          const float *stats) __attribute__((always_inline)) {
+        const int32_t tile_position = (low_tile + t % per_query_head) * kQueryStep + shift;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const int32_t position = tile_position + 32 * n, last_here = position + 31;
+            const bool seen_by_some =
+                last_here >= wave_first
+                && (a.window == 0 || position - (wave_first + 31) < a.window
+                    || wave_first < a.sinks);
+            if (!seen_by_some) continue;
+            const bool seen_by_all =
+                wave_first + 31 <= position && last_here < length
+                && (a.window == 0 || last_here - wave_first < a.window
+                    || wave_first + 32 <= a.sinks);
+            f32x16 s{}, e;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 delta = *reinterpret_cast<const f32x4 *>(
+                    stats + kQueryStep + 32 * n + 8 * g + 4 * half);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) e[4 * g + i] = -delta[i];
+            }
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                s = Element<kHalf>::multiply(read_rows<kPitch>(q_tile, n, i), k_operand[i], s);
+                e = Element<kHalf>::multiply(read_rows<kPitch>(g_tile, n, i), v_operand[i], e);
+            }
+            // In FP16 the weights of long rows lie below the normal numbers:
+            // they are held 2^8 larger until the sums of dv are stored.
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 lse =
+                    *reinterpret_cast<const f32x4 *>(stats + 32 * n + 8 * g + 4 * half);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = 4 * g + i;
+                    s[r] = exp2_fast(__builtin_fmaf(s[r], factor, -lse[i]));
+                    e[r] *= s[r];
+                    if (kHalf) s[r] *= kHalfWeights;
+                }
+            }
+            if (!seen_by_all) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int32_t at = position + 8 * (r / 4) + 4 * half + r % 4;
+                    const bool seen = sight_of(a, at, length)(key);
+                    s[r] = seen ? s[r] : 0.0f;
+                    e[r] = seen ? e[r] : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                const u32x4 weights = as_operand<kHalf>(s, p), ds = as_operand<kHalf>(e, p);
+#pragma unroll
+                for (int c = 0; c < kColumns; ++c) {
+                    dv[c] = Element<kHalf>::multiply(
+                        read_columns<kPitch>(g_tile, 32 * n + 16 * p, c), weights, dv[c]);
+                    dk[c] = Element<kHalf>::multiply(
+                        read_columns<kPitch>(q_tile, 32 * n + 16 * p, c), ds, dk[c]);
+                }
+            }
+        }
+    };
+
+    if (begin < end) load(begin, q_even, g_even, stats_even);
+    for (int32_t t = begin; t < end; t += 2) {
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        if (t + 1 < end) load(t + 1, q_odd, g_odd, stats_odd);
+        step(t, q_even, g_even, stats_even);
+        if (t + 1 >= end) break;
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        if (t + 2 < end) load(t + 2, q_even, g_even, stats_even);
+        step(t + 1, q_odd, g_odd, stats_odd);
+    }
+
+    if (key >= a.keys) return;
+    const float dv_scale = kHalf ? 1.0f / kHalfWeights : 1.0f;
+    if (blocks.parts_of(block) > 1) {
+        float *dst = parts
+                     + (int64_t{bkv} * per_head + blocks.first_part(block) + split) * 2 * kKeyBlock
+                           * a.head_dim
+                     + int64_t{key - first} * a.head_dim;
+#pragma unroll
+        for (int c = 0; c < kColumns; ++c)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int32_t channel = 32 * c + 8 * g + 4 * half;
+                if (channel >= a.head_dim) continue;
+                f32x4 x, y;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[i] = dk[c][4 * g + i] * a.scale;
+                    y[i] = dv[c][4 * g + i] * dv_scale;
+                }
+                *reinterpret_cast<f32x4 *>(dst + channel) = x;
+                *reinterpret_cast<f32x4 *>(dst + kKeyBlock * a.head_dim + channel) = y;
+            }
+        return;
+    }
+    store_row<kHalf, kColumns>(static_cast<uint16_t *>(d.dk) + b * d.dk_stride[0]
+                                   + kv * d.dk_stride[1] + key * d.dk_stride[2],
+                               dk, a.scale, a.head_dim);
+    store_row<kHalf, kColumns>(static_cast<uint16_t *>(d.dv) + b * d.dv_stride[0]
+                                   + kv * d.dv_stride[1] + key * d.dv_stride[2],
+                               dv, dv_scale, a.head_dim);
+}
+
+// Adds the parts of the blocks from `first_block` on that have several, in
+// their order.  Four channels of one key per thread.
+template <bool kHalf>
+__global__ __launch_bounds__(kAttentionThreads) void attention_sum_parts_kernel(
+    lct_attention a, lct_attention_gradients d, KeyBlocks blocks, const float *__restrict__ parts,
+    int32_t end_block) {
+    const int32_t quads = a.head_dim / 4;
+    const int64_t item = int64_t{blockIdx.x} * kAttentionThreads + threadIdx.x;
+    const int32_t channel = 4 * static_cast<int32_t>(item % quads);
+    const int64_t keys = min(a.keys, end_block * kKeyBlock);
+    const int32_t key = static_cast<int32_t>(item / quads % keys);
+    const int64_t bkv = item / quads / keys;
+    if (bkv >= int64_t{a.batch} * a.kv_heads) return;
+    const int32_t block = key / kKeyBlock;
+    const int32_t count = blocks.parts_of(block);
+    if (count == 1) return;
+    const int64_t step = int64_t{2} * kKeyBlock * a.head_dim;
+    const float *src = parts + (bkv * blocks.parts() + blocks.first_part(block)) * step
+                       + int64_t{key % kKeyBlock} * a.head_dim + channel;
+    f32x4 x{}, y{};
+    for (int32_t s = 0; s < count; ++s) {
+        x += *reinterpret_cast<const f32x4 *>(src + s * step);
+        y += *reinterpret_cast<const f32x4 *>(src + s * step + kKeyBlock * a.head_dim);
+    }
+    const int64_t b = bkv / a.kv_heads, kv = bkv % a.kv_heads;
+    u32x2 dk, dv;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        dk[i] = Element<kHalf>::round_pair(x[2 * i], x[2 * i + 1]);
+        dv[i] = Element<kHalf>::round_pair(y[2 * i], y[2 * i + 1]);
+    }
+    *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(d.dk) + b * d.dk_stride[0]
+                               + kv * d.dk_stride[1] + key * d.dk_stride[2] + channel) = dk;
+    *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(d.dv) + b * d.dv_stride[0]
+                               + kv * d.dv_stride[1] + key * d.dv_stride[2] + channel) = dv;
+}
+
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+bool strides_ok(const int64_t (&stride)[3]) {
+    for (const int64_t s : stride)
+        if (s < 0 || (s & 7) != 0) return false;
+    return stride[2] < (int64_t{1} << 24);
+}
+
+constexpr int32_t kMaxTokens = 1 << 30;
+
+}  // namespace
+
+int32_t check_attention(const lct_attention *a) {
+    if (!a || !a->q || !a->k || !a->v || !a->out) return LCT_E_NULL;
+    if (a->batch <= 0 || a->heads <= 0 || a->kv_heads <= 0 || a->heads % a->kv_heads != 0
+        || a->queries <= 0 || a->keys <= 0 || a->queries > kMaxTokens || a->keys > kMaxTokens
+        || a->head_dim <= 0 || a->head_dim > LCT_MAX_HEAD_DIM || (a->head_dim & 7) != 0
+        || int64_t{a->batch} * a->heads > kMaxAttentionItems)
+        return LCT_E_SIZE;
+    if (a->window < 0 || a->window > kMaxTokens || a->sinks < 0 || a->sinks > kMaxTokens
+        || !(a->scale > 0.0f) || !(a->scale < INFINITY) || !strides_ok(a->q_stride)
+        || !strides_ok(a->k_stride) || !strides_ok(a->v_stride) || !strides_ok(a->out_stride)
+        || !aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->out)
+        || !aligned16(a->lse))
+        return LCT_E_ARG;
+    return LCT_OK;
+}
+
+int32_t join_parts(const lct_attention &a, int32_t splits, const float *parts,
+                   hipStream_t stream) {
+    const int64_t pitch = a.lse != nullptr ? lse_pitch(a.queries) : a.queries;
+    const int64_t rows = int64_t{a.batch} * a.heads * pitch;
+    const uint32_t grid = static_cast<uint32_t>((rows + kAttentionWaves - 1) / kAttentionWaves);
+    if (a.fp16)
+        attention_join_kernel<true>
+            <<<grid, kAttentionThreads, 0, stream>>>(a, pitch, splits, parts);
+    else
+        attention_join_kernel<false>
+            <<<grid, kAttentionThreads, 0, stream>>>(a, pitch, splits, parts);
+    return static_cast<int32_t>(hipGetLastError());
+}
+
+namespace {
+
+template <bool kHalf>
+int32_t forward(const lct_attention &a, int32_t splits, float *workspace, hipStream_t stream) {
+    const int32_t tiles = (a.queries + kQueryTile - 1) / kQueryTile;
+    const int64_t items = int64_t{tiles} * splits * a.batch * a.heads;
+    if (items > kMaxAttentionItems) return LCT_E_SIZE;
+    const uint32_t grid = static_cast<uint32_t>(xcd_grid(items));
+    by_width(a.head_dim, [&](auto width) {
+        constexpr int kDim = decltype(width)::value;
+        if (splits > 1)
+            attention_forward_kernel<kHalf, kDim, true>
+                <<<grid, kAttentionThreads, 0, stream>>>(a, tiles, splits, workspace);
+        else
+            attention_forward_kernel<kHalf, kDim, false>
+                <<<grid, kAttentionThreads, 0, stream>>>(a, tiles, splits, workspace);
+    });
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess || splits == 1) return static_cast<int32_t>(err);
+    return join_parts(a, splits, workspace, stream);
+}
+
+template <bool kHalf>
+int32_t backward(const lct_attention &a, const lct_attention_gradients &d, const KeyBlocks &blocks,
+                 float *workspace, hipStream_t stream) {
+    const int32_t tiles = (a.queries + kQueryTile - 1) / kQueryTile;
+    const int64_t items = int64_t{tiles} * a.batch * a.heads;
+    const int64_t parts = blocks.parts() * a.batch * a.kv_heads;
+    by_width(a.head_dim, [&](auto width) {
+        constexpr int kDim = decltype(width)::value;
+        attention_dq_kernel<kHalf, kDim>
+            <<<static_cast<uint32_t>(xcd_grid(items)), kAttentionThreads, 0, stream>>>(a, d, tiles);
+        attention_dkdv_kernel<kHalf, kDim>
+            <<<static_cast<uint32_t>(xcd_grid(parts)), kAttentionThreads, 0, stream>>>(
+                a, d, blocks, workspace);
+    });
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess) return static_cast<int32_t>(err);
+    const int32_t end_block = blocks.splits > 1        ? blocks.blocks
+                              : blocks.sink_splits > 1 ? blocks.sink_blocks
+                                                       : 0;
+    if (end_block == 0) return LCT_OK;
+    const int64_t keys = std::min<int64_t>(a.keys, int64_t{end_block} * kKeyBlock);
+    const int64_t threads = keys * (a.head_dim / 4) * a.batch * a.kv_heads;
+    attention_sum_parts_kernel<kHalf>
+        <<<static_cast<uint32_t>((threads + kAttentionThreads - 1) / kAttentionThreads),
+           kAttentionThreads, 0, stream>>>(a, d, blocks, workspace, end_block);
+    return static_cast<int32_t>(hipGetLastError());
+}
+
+}  // namespace
+}  // namespace lct
+
+using namespace lct;
+
+extern "C" int32_t lct_attention_forward(const lct_attention *a, int32_t splits, float *workspace,
+                                         int64_t workspace_floats, hipStream_t stream) {
+    if (const int32_t code = check_attention(a); code != LCT_OK) return code;
+    if (splits <= 0 || splits > LCT_MAX_ATTENTION_SPLITS) return LCT_E_ARG;
+    if (splits > 1) {
+        if (!workspace) return LCT_E_NULL;
+        if (workspace_floats / (a->head_dim + 2) / splits / a->queries
+            < int64_t{a->batch} * a->heads)
+            return LCT_E_SIZE;
+        if ((reinterpret_cast<uintptr_t>(workspace) & 7) != 0) return LCT_E_ARG;
+        if (int64_t{a->batch} * a->heads * lse_pitch(a->queries) > kMaxAttentionItems * kAttentionWaves)
+            return LCT_E_SIZE;
+    }
+    return a->fp16 ? forward<true>(*a, splits, workspace, stream)
+                   : forward<false>(*a, splits, workspace, stream);
+}
+
+extern "C" int32_t lct_attention_backward(const lct_attention *a, const lct_attention_gradients *d,
+                                          int32_t splits, int32_t sink_splits, float *workspace,
+                                          int64_t workspace_floats, hipStream_t stream) {
+    if (const int32_t code = check_attention(a); code != LCT_OK) return code;
+    if (!d || !a->lse || !d->grad || !d->dq || !d->dk || !d->dv || !d->delta) return LCT_E_NULL;
+    if (splits <= 0 || splits > LCT_MAX_ATTENTION_SPLITS || sink_splits <= 0
+        || sink_splits > LCT_MAX_ATTENTION_SPLITS || !strides_ok(d->grad_stride)
+        || !strides_ok(d->dq_stride) || !strides_ok(d->dk_stride) || !strides_ok(d->dv_stride)
+        || !aligned16(d->grad) || !aligned16(d->dq) || !aligned16(d->dk) || !aligned16(d->dv)
+        || !aligned16(d->delta) || !aligned16(workspace))
+        return LCT_E_ARG;
+    KeyBlocks blocks;
+    blocks.blocks = (a->keys + kKeyBlock - 1) / kKeyBlock;
+    blocks.sink_blocks =
+        a->window > 0 ? (std::min(a->sinks, a->keys) + kKeyBlock - 1) / kKeyBlock : 0;
+    blocks.splits = splits;
+    blocks.sink_splits = sink_splits;
+    const int64_t parts = blocks.parts() * a->batch * a->kv_heads;
+    if (parts > kMaxAttentionItems
+        || int64_t{(a->queries + kQueryTile - 1) / kQueryTile} * a->batch * a->heads > kMaxAttentionItems
+        || int64_t{a->keys} * (a->head_dim / 4) * a->batch * a->kv_heads
+               > kMaxAttentionItems * kAttentionThreads)
+        return LCT_E_SIZE;
+    if (splits > 1 || (sink_splits > 1 && blocks.sink_blocks > 0)) {
+        if (!workspace) return LCT_E_NULL;
+        if (workspace_floats < parts * 2 * kKeyBlock * a->head_dim) return LCT_E_SIZE;
+    }
+    return a->fp16 ? backward<true>(*a, *d, blocks, workspace, stream)
+                   : backward<false>(*a, *d, blocks, workspace, stream);
+}

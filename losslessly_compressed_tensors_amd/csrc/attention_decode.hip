@@ -1,0 +1,278 @@
+// One query per sequence against its cache of keys and values, with a sliding
+// window and sinks.
+//
+// A workgroup takes a key head (16 of its query heads at most, the columns of
+// 16x16x32 matrix instructions) and a share of the visible keys; its 4 waves
+// take tiles of 32 keys in turn, each by itself, with the next tile's loads in
+// registers.  Keys go from memory straight into operands; values pass through
+// the wave's own LDS rows for the transposed read.  As in attention_core.h a
+// lane's scores are the next product's operand: lane l holds keys 4 (l >> 4) + i
+// and 16 more of query l & 15, and the values are read in that order.
+#include "attention_core.h"
+
+namespace lct {
+namespace {
+
+constexpr int kDecodeKeys = 32;      // keys per tile
+constexpr int kQueries = 16;         // query heads per workgroup
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRescale = 8.0f;
+
+template <bool kHalf>
+__device__ __forceinline__ f32x4 multiply16(u32x4 a, u32x4 b, f32x4 c) {
+    if constexpr (kHalf)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                      __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                       __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// Over the four lanes l & 15 + 16 i.
+__device__ __forceinline__ float quarters_max(float v) {
+    const uint32_t u = __float_as_uint(v);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    return across_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float quarters_sum(float v) {
+    const uint32_t u = __float_as_uint(v);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    return across_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+template <bool kHalf, int kDim, bool kSplit>
+__global__ __launch_bounds__(kAttentionThreads, 2) void attention_decode_kernel(
+    lct_attention a, int32_t splits, float *__restrict__ parts) {
+    constexpr int kPitch = kPitchOf<kDim>;
+    constexpr int kSteps = kDim / 32, kColumns = kDim / 16;
+    constexpr int kChunks = kPitch / 8;                        // 16-byte chunks of an LDS row
+    constexpr int kValueLoads = kDecodeKeys * kChunks / kWave;
+    constexpr int kMergePitch = kDim + 4;
+    constexpr int kValueBytes = kAttentionWaves * kDecodeKeys * kPitch * 2;
+    constexpr int kMergeBytes = kAttentionWaves * kQueries * kMergePitch * 4;
+    __shared__ __attribute__((aligned(1024))) char
+        shared[kValueBytes > kMergeBytes ? kValueBytes : kMergeBytes];
+
+    const int lane = wave_lane(), column = lane & 15, quarter = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int32_t group = a.heads / a.kv_heads;
+    const int32_t chunks = (group + kQueries - 1) / kQueries;
+    const int64_t item = blockIdx.x;
+    const int32_t split = static_cast<int32_t>(item % splits);
+    const int64_t rest = item / splits;
+    const int32_t chunk = static_cast<int32_t>(rest % chunks);
+    const int32_t kv = static_cast<int32_t>(rest / chunks % a.kv_heads);
+    const int32_t b = static_cast<int32_t>(rest / chunks / a.kv_heads);
+
+    const int32_t length = sequence_length(a, b);
+    const KeyTiles all(a, length - 1, length - 1, length, kDecodeKeys);
+    const Sight sight = sight_of(a, length - 1, length);
+    const int32_t per_split = (all.count + splits - 1) / splits;
+    const int32_t begin = split * per_split, end = min(all.count, begin + per_split);
+
+    const int32_t in_group = chunk * kQueries + column;
+    const int32_t h = kv * group + in_group;
+    const uint16_t *q = static_cast<const uint16_t *>(a.q) + b * a.q_stride[0] + h * a.q_stride[1];
+    const uint16_t *k = static_cast<const uint16_t *>(a.k) + b * a.k_stride[0] + kv * a.k_stride[1];
+    const uint16_t *v = static_cast<const uint16_t *>(a.v) + b * a.v_stride[0] + kv * a.v_stride[1];
+    u32x4 q_operand[kSteps];
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+        const int32_t channel = 32 * s + 8 * quarter;
+        q_operand[s] = u32x4{0u, 0u, 0u, 0u};
+        if (in_group < group && channel < a.head_dim)
+            q_operand[s] = *reinterpret_cast<const u32x4 *>(q + channel);
+    }
+
+    struct Tile {
+        u32x4 k[2][kSteps], v[kValueLoads];
+    };
+    // Keys and values that the query does not see are zeros.
+    const auto load = [&](int32_t t, Tile &tile) __attribute__((always_inline)) {
+        const int32_t first = all.first_key(t, kDecodeKeys);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const int32_t key = first + 16 * n + column;
+            const bool seen = sight(key);
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                const int32_t channel = 32 * s + 8 * quarter;
+                tile.k[n][s] = u32x4{0u, 0u, 0u, 0u};
+                if (seen && channel < a.head_dim)
+                    tile.k[n][s] =
+                        *reinterpret_cast<const u32x4 *>(k + key * a.k_stride[2] + channel);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kValueLoads; ++i) {
+            const int slot = i * kWave + lane;
+            const int32_t key = first + slot / kChunks, channel = slot % kChunks * 8;
+            tile.v[i] = u32x4{0u, 0u, 0u, 0u};
+            if (channel < a.head_dim && sight(key))
+                tile.v[i] = *reinterpret_cast<const u32x4 *>(v + key * a.v_stride[2] + channel);
+        }
+    };
+
+    const float factor = a.scale * kLog2e;
+    uint16_t *values = reinterpret_cast<uint16_t *>(shared) + wave * kDecodeKeys * kPitch;
+    f32x4 out[kColumns];
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c) out[c] = f32x4{};
+    float most = -INFINITY, shifted = 0.0f, total = 0.0f;
+
+    const auto step = [&](int32_t t, const Tile &tile) __attribute__((always_inline)) {
+        const int32_t first = all.first_key(t, kDecodeKeys);
+#pragma unroll
+        for (int i = 0; i < kValueLoads; ++i) {
+            const int slot = i * kWave + lane;
+            const int row = slot / kChunks, at = (slot % kChunks) ^ swizzle(row);
+            *reinterpret_cast<u32x4 *>(values + row * kPitch + at * 8) = tile.v[i];
+        }
+        f32x4 s[2];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            s[n] = f32x4{};
+#pragma unroll
+            for (int d = 0; d < kSteps; ++d)
+                s[n] = multiply16<kHalf>(tile.k[n][d], q_operand[d], s[n]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                s[n][i] = sight(first + 16 * n + 4 * quarter + i) ? s[n][i] : -INFINITY;
+        }
+        float top = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+        for (int i = 1; i < 4; ++i) top = fmaxf(fmaxf(top, s[0][i]), s[1][i]);
+        top = quarters_max(top);
+        if (__any(top * factor > most * factor + kRescale)) {
+            const float next = fmaxf(most, top);
+            const float scaled = next == -INFINITY ? 0.0f : next * factor;
+            const float change = exp2_fast(most * factor - scaled);
+            most = next;
+            shifted = scaled;
+            total *= change;
+#pragma unroll
+            for (int c = 0; c < kColumns; ++c) out[c] *= change;
+        }
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s[n][i] = exp2_fast(__builtin_fmaf(s[n][i], factor, -shifted));
+                total += s[n][i];
+            }
+        u32x4 weights;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                weights[2 * n + i] = Element<kHalf>::round_pair(s[n][2 * i], s[n][2 * i + 1]);
+#pragma unroll
+        for (int c = 0; c < kColumns; ++c) {
+            const int row = 4 * quarter + ((lane & 15) >> 2);
+            const int at = (2 * c + ((lane >> 1) & 1)) ^ swizzle(row);
+            const uint16_t *from = values + row * kPitch + at * 8 + (lane & 1) * 4;
+            const u32x2 low = __builtin_bit_cast(
+                u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                           (__attribute__((address_space(3))) i16x4 *)(from)));
+            const u32x2 high = __builtin_bit_cast(
+                u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                           (__attribute__((address_space(3))) i16x4 *)(from + 16 * kPitch)));
+            out[c] = multiply16<kHalf>(u32x4{low[0], low[1], high[0], high[1]}, weights, out[c]);
+        }
+    };
+
+    int32_t t = begin + wave;
+    Tile next;
+    if (t < end) load(t, next);
+    for (; t < end; t += kAttentionWaves) {
+        const Tile tile = next;
+        if (t + kAttentionWaves < end) load(t + kAttentionWaves, next);
+        step(t, tile);
+        // The wave's own rows: its LDS operations run in order.
+        __builtin_amdgcn_wave_barrier();
+    }
+    total = quarters_sum(total);
+
+    // The waves' parts meet in LDS, in wave order.
+    __syncthreads();
+    float *merge = reinterpret_cast<float *>(shared);
+    float *mine = merge + (wave * kQueries + column) * kMergePitch;
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c)
+        *reinterpret_cast<f32x4 *>(mine + 16 * c + 4 * quarter) = out[c];
+    if (quarter == 0) *reinterpret_cast<f32x2 *>(mine + kDim) = f32x2{shifted, total};
+    __syncthreads();
+    const int32_t pairs = a.head_dim / 2;
+    const int32_t rows = min(kQueries, group - chunk * kQueries);
+    for (int32_t i = threadIdx.x; i < rows * pairs; i += kAttentionThreads) {
+        const int32_t row = i / pairs, channel = 2 * (i % pairs);
+        float largest = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kAttentionWaves; ++w) {
+            const float *from = merge + (w * kQueries + row) * kMergePitch + kDim;
+            if (from[1] != 0.0f) largest = fmaxf(largest, from[0]);
+        }
+        float sum = 0.0f, x = 0.0f, y = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kAttentionWaves; ++w) {
+            const float *from = merge + (w * kQueries + row) * kMergePitch;
+            if (from[kDim + 1] == 0.0f) continue;
+            const float weight = exp2_fast(from[kDim] - largest);
+            sum += weight * from[kDim + 1];
+            x += weight * from[channel];
+            y += weight * from[channel + 1];
+        }
+        const int32_t head = kv * group + chunk * kQueries + row;
+        if constexpr (kSplit) {
+            float *part = parts
+                          + ((int64_t{b} * a.heads + head) * splits + split) * (a.head_dim + 2);
+            *reinterpret_cast<f32x2 *>(part + channel) = f32x2{x, y};
+            if (channel == 0) *reinterpret_cast<f32x2 *>(part + a.head_dim) = f32x2{largest, sum};
+        } else {
+            const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+            uint16_t *dst = static_cast<uint16_t *>(a.out) + b * a.out_stride[0]
+                            + head * a.out_stride[1];
+            *reinterpret_cast<uint32_t *>(dst + channel) =
+                Element<kHalf>::round_pair(x * inverse, y * inverse);
+        }
+    }
+}
+
+template <bool kHalf>
+int32_t decode(const lct_attention &a, int32_t splits, float *workspace, hipStream_t stream) {
+    const int64_t chunks = (a.heads / a.kv_heads + kQueries - 1) / kQueries;
+    const uint32_t grid = static_cast<uint32_t>(chunks * a.kv_heads * a.batch * splits);
+    by_width(a.head_dim, [&](auto width) {
+        constexpr int kDim = decltype(width)::value;
+        if (splits > 1)
+            attention_decode_kernel<kHalf, kDim, true>
+                <<<grid, kAttentionThreads, 0, stream>>>(a, splits, workspace);
+        else
+            attention_decode_kernel<kHalf, kDim, false>
+                <<<grid, kAttentionThreads, 0, stream>>>(a, splits, workspace);
+    });
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess || splits == 1) return static_cast<int32_t>(err);
+    return join_parts(a, splits, workspace, stream);
+}
+
+}  // namespace
+}  // namespace lct
+
+using namespace lct;
+
+extern "C" int32_t lct_attention_decode(const lct_attention *a, int32_t splits, float *workspace,
+                                        int64_t workspace_floats, hipStream_t stream) {
+    if (const int32_t code = check_attention(a); code != LCT_OK) return code;
+    if (a->queries != 1 || a->lse != nullptr || splits <= 0 || splits > LCT_MAX_ATTENTION_SPLITS)
+        return LCT_E_ARG;
+    if (int64_t{a->batch} * a->heads * splits > kMaxAttentionItems) return LCT_E_SIZE;
+    if (splits > 1) {
+        if (!workspace) return LCT_E_NULL;
+        if (workspace_floats / (a->head_dim + 2) / splits < int64_t{a->batch} * a->heads)
+            return LCT_E_SIZE;
+        if ((reinterpret_cast<uintptr_t>(workspace) & 7) != 0) return LCT_E_ARG;
+    }
+    return a->fp16 ? decode<true>(*a, splits, workspace, stream)
+                   : decode<false>(*a, splits, workspace, stream);
+}

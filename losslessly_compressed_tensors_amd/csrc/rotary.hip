@@ -1,0 +1,242 @@
+// Rotary positions of queries and keys, and a new token's way into the caches.
+//
+// A pair (x, y) of channels at position p turns by the angle p f of its
+// frequency: (x cos - y sin, y cos + x sin), times a magnitude.  Frequencies are
+// fractions of a turn per position in 64-bit fixed point, so the product with
+// the position wraps modulo one turn exactly, whatever the position: no table
+// bounds the context, and the angle's only rounding is to FP32 in [-1/2, 1/2].
+//
+// Follows examples/nanogpt/train_gpt_lct.py:150-165 (whose rotation has the
+// other sense: negative frequencies).
+#include <algorithm>
+
+#include "attention_core.h"
+
+namespace lct {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxPairs = LCT_MAX_ROTARY_DIM / 2;
+constexpr int kMaxTokens = 16;       // tokens of a workgroup
+
+template <int kType>
+struct Value;
+template <>
+struct Value<LCT_BF16> {
+    using Bits = uint16_t;
+    static __device__ __forceinline__ float load(Bits b) { return bf16_to_float(b); }
+    static __device__ __forceinline__ Bits store(float x) {
+        return __builtin_bit_cast(Bits, static_cast<__bf16>(x));
+    }
+};
+template <>
+struct Value<LCT_FP16> {
+    using Bits = uint16_t;
+    static __device__ __forceinline__ float load(Bits b) {
+        return static_cast<float>(__builtin_bit_cast(_Float16, b));
+    }
+    static __device__ __forceinline__ Bits store(float x) {
+        return __builtin_bit_cast(Bits, static_cast<_Float16>(x));
+    }
+};
+template <>
+struct Value<LCT_FP32> {
+    using Bits = uint32_t;
+    static __device__ __forceinline__ float load(Bits b) { return __uint_as_float(b); }
+    static __device__ __forceinline__ Bits store(float x) { return __float_as_uint(x); }
+};
+
+// How the (token, head, unit) items of a workgroup's tokens are counted: units
+// of kVector adjacent channels (with those half the rotated part further on in
+// the half layout), pairs first, then the channels that are only copied.
+struct Counts {
+    int32_t per_group;      // tokens of a workgroup
+    int32_t pair_units, units, per_token;
+    uint32_t units_inverse, per_token_inverse;   // ceil(2^32 / .), 0 for 1
+};
+
+__device__ __forceinline__ int32_t divide(int32_t x, uint32_t inverse) {
+    return inverse == 0u ? x : static_cast<int32_t>(__umulhi(static_cast<uint32_t>(x), inverse));
+}
+
+__device__ __forceinline__ int64_t position_of(const lct_rotary &r, int64_t b, int64_t t) {
+    int64_t p = r.start + (r.positions == nullptr || r.position_stride[1] == 0 ? t : 0);
+    if (r.positions != nullptr)
+        p += r.positions[b * r.position_stride[0] + t * r.position_stride[1]];
+    return p;
+}
+
+template <int kType, int kVector>
+__global__ __launch_bounds__(kThreads) void rotary_kernel(lct_rotary r, Counts n) {
+    using V = Value<kType>;
+    using Bits = typename V::Bits;
+    struct alignas(sizeof(Bits) * kVector) Pack {
+        Bits v[kVector];
+    };
+    __shared__ f32x2 turn[kMaxTokens * kMaxPairs];
+    __shared__ int64_t place[kMaxTokens];
+    const int64_t tokens = int64_t{r.batch} * r.tokens;
+    const int64_t first = int64_t{blockIdx.x} * n.per_group;
+    const int32_t here = static_cast<int32_t>(min(int64_t{n.per_group}, tokens - first));
+    const int32_t pairs = r.rotary_dim / 2;
+    for (int32_t i = threadIdx.x; i < here * pairs; i += kThreads) {
+        const int32_t token = i / pairs, pair = i % pairs;
+        const int64_t b = (first + token) / r.tokens, t = (first + token) % r.tokens;
+        const int64_t p = position_of(r, b, t);
+        const int64_t angle = static_cast<int64_t>(static_cast<uint64_t>(p)
+                                                   * static_cast<uint64_t>(r.turns[pair]));
+        float sine, cosine;
+        sincospif(static_cast<float>(angle) * 0x1p-63f, &sine, &cosine);
+        turn[i] = f32x2{cosine * r.magnitude, (r.inverse ? -sine : sine) * r.magnitude};
+        if (pair == 0) place[token] = p;
+    }
+    __syncthreads();
+
+    for (int32_t i = threadIdx.x; i < here * n.per_token; i += kThreads) {
+        const int32_t token = divide(i, n.per_token_inverse);
+        const int32_t in_token = i - token * n.per_token;
+        int32_t head = divide(in_token, n.units_inverse);
+        const int32_t unit = in_token - head * n.units;
+        const int64_t b = (first + token) / r.tokens, t = (first + token) % r.tokens;
+        // q's heads, then k's, then v's.
+        const bool is_q = head < r.heads;
+        if (!is_q) head -= r.heads;
+        const bool is_k = !is_q && head < r.kv_heads;
+        if (!is_q && !is_k) head -= r.kv_heads;
+        const bool rotate = is_q || is_k;
+        int64_t out_token = t;
+        if (!is_q && r.capacity > 0) {
+            out_token = place[token];
+            if (out_token < 0 || out_token >= r.capacity) continue;
+        }
+        const auto pick = [&](auto q, auto k, auto v) { return is_q ? q : is_k ? k : v; };
+        const Bits *src = static_cast<const Bits *>(pick(r.q_in, r.k_in, r.v_in))
+                          + b * pick(r.q_in_stride[0], r.k_in_stride[0], r.v_in_stride[0])
+                          + t * pick(r.q_in_stride[1], r.k_in_stride[1], r.v_in_stride[1])
+                          + head * pick(r.q_in_stride[2], r.k_in_stride[2], r.v_in_stride[2]);
+        Bits *dst = static_cast<Bits *>(pick(r.q_out, r.k_out, r.v_out))
+                    + b * pick(r.q_out_stride[0], r.k_out_stride[0], r.v_out_stride[0])
+                    + out_token * pick(r.q_out_stride[1], r.k_out_stride[1], r.v_out_stride[1])
+                    + head * pick(r.q_out_stride[2], r.k_out_stride[2], r.v_out_stride[2]);
+        const f32x2 *angles = turn + token * pairs;
+        if (unit >= n.pair_units) {          // channels past the rotated part
+            const int32_t c = r.rotary_dim + (unit - n.pair_units) * kVector;
+            *reinterpret_cast<Pack *>(dst + c) = *reinterpret_cast<const Pack *>(src + c);
+        } else if (!r.interleaved) {
+            const int32_t c = unit * kVector;
+            Pack x = *reinterpret_cast<const Pack *>(src + c);
+            Pack y = *reinterpret_cast<const Pack *>(src + c + pairs);
+#pragma unroll
+            for (int j = 0; j < kVector; ++j) {
+                if (!rotate) continue;
+                const f32x2 a = angles[c + j];
+                const float u = V::load(x.v[j]), w = V::load(y.v[j]);
+                x.v[j] = V::store(u * a[0] - w * a[1]);
+                y.v[j] = V::store(w * a[0] + u * a[1]);
+            }
+            *reinterpret_cast<Pack *>(dst + c) = x;
+            *reinterpret_cast<Pack *>(dst + c + pairs) = y;
+        } else if constexpr (kVector > 1) {
+            const int32_t c = unit * kVector;
+            Pack x = *reinterpret_cast<const Pack *>(src + c);
+#pragma unroll
+            for (int j = 0; j < kVector; j += 2) {
+                if (!rotate) continue;
+                const f32x2 a = angles[(c + j) / 2];
+                const float u = V::load(x.v[j]), w = V::load(x.v[j + 1]);
+                x.v[j] = V::store(u * a[0] - w * a[1]);
+                x.v[j + 1] = V::store(w * a[0] + u * a[1]);
+            }
+            *reinterpret_cast<Pack *>(dst + c) = x;
+        } else {
+            const int32_t c = 2 * unit;
+            const Bits u = src[c], w = src[c + 1];
+            const f32x2 a = angles[unit];
+            dst[c] = rotate ? V::store(V::load(u) * a[0] - V::load(w) * a[1]) : u;
+            dst[c + 1] = rotate ? V::store(V::load(w) * a[0] + V::load(u) * a[1]) : w;
+        }
+    }
+}
+
+// x / d is the high half of x ceil(2^32 / d) for x and d up to 2^16.
+constexpr int32_t kMaxItems = 1 << 16;
+
+uint32_t inverse_of(int32_t x) {
+    return static_cast<uint32_t>(((uint64_t{1} << 32) + x - 1) / x);
+}
+
+bool multiples(const int64_t (&stride)[3], int32_t of) {
+    return stride[0] % of == 0 && stride[1] % of == 0 && stride[2] % of == 0;
+}
+
+bool aligned_to(const void *p, uintptr_t bytes) {
+    return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0;
+}
+
+template <int kType, int kVector>
+int32_t launch(const lct_rotary &r, hipStream_t stream) {
+    const int32_t pairs = r.rotary_dim / 2;
+    Counts n;
+    n.pair_units = r.interleaved && kVector > 1 ? r.rotary_dim / kVector : pairs / kVector;
+    n.units = n.pair_units + (r.head_dim - r.rotary_dim) / kVector;
+    n.per_token = (r.heads + (r.k_in ? r.kv_heads : 0) + (r.v_in ? r.kv_heads : 0)) * n.units;
+    if (n.per_token >= kMaxItems) return LCT_E_SIZE;
+    const int64_t tokens = int64_t{r.batch} * r.tokens;
+    // Enough tokens that a workgroup's threads take a few units each and share
+    // the angles, while there are workgroups for every compute unit.
+    int64_t per = std::min<int64_t>(kMaxTokens, std::max(1, 4 * kThreads / n.per_token));
+    per = std::min(per, std::max<int64_t>(1, tokens / 1024));
+    n.per_group = static_cast<int32_t>(std::min<int64_t>(per, kMaxItems / n.per_token));
+    n.units_inverse = inverse_of(n.units);
+    n.per_token_inverse = inverse_of(n.per_token);
+    const int64_t grid = (tokens + n.per_group - 1) / n.per_group;
+    if (grid >= int64_t{1} << 24) return LCT_E_SIZE;
+    rotary_kernel<kType, kVector>
+        <<<static_cast<uint32_t>(grid), kThreads, 0, stream>>>(r, n);
+    return static_cast<int32_t>(hipGetLastError());
+}
+
+template <int kType>
+int32_t by_vector(const lct_rotary &r, hipStream_t stream) {
+    constexpr int kVector = 16 / sizeof(typename Value<kType>::Bits);
+    const int32_t pairs = r.rotary_dim / 2;
+    bool wide = (r.interleaved ? r.rotary_dim : pairs) % kVector == 0 && r.head_dim % kVector == 0
+                && r.rotary_dim % kVector == 0;
+    const auto fits = [&](const void *in, void *out, const int64_t (&is)[3],
+                          const int64_t (&os)[3]) {
+        return in == nullptr
+               || (aligned_to(in, 16) && aligned_to(out, 16) && multiples(is, kVector)
+                   && multiples(os, kVector));
+    };
+    wide = wide && fits(r.q_in, r.q_out, r.q_in_stride, r.q_out_stride)
+           && fits(r.k_in, r.k_out, r.k_in_stride, r.k_out_stride)
+           && fits(r.v_in, r.v_out, r.v_in_stride, r.v_out_stride);
+    return wide ? launch<kType, kVector>(r, stream) : launch<kType, 1>(r, stream);
+}
+
+}  // namespace
+}  // namespace lct
+
+using namespace lct;
+
+extern "C" int32_t lct_rotate(const lct_rotary *r, hipStream_t stream) {
+    if (!r || !r->q_in || !r->q_out || !r->turns || (r->k_in && !r->k_out)
+        || (r->v_in && (!r->v_out || !r->k_in)))
+        return LCT_E_NULL;
+    if (r->batch <= 0 || r->tokens <= 0 || r->heads <= 0 || (r->k_in && r->kv_heads <= 0)
+        || r->head_dim <= 0 || r->head_dim > LCT_MAX_ROTARY_DIM || r->rotary_dim <= 0
+        || r->rotary_dim > r->head_dim || (r->rotary_dim & 1) != 0 || r->capacity < 0
+        || r->heads > 4096 || r->kv_heads > 4096)
+        return LCT_E_SIZE;
+    const uintptr_t size = r->type == LCT_FP32 ? 4 : 2;
+    if (!aligned_to(r->q_in, size) || !aligned_to(r->q_out, size) || !aligned_to(r->k_in, size)
+        || !aligned_to(r->k_out, size) || !aligned_to(r->v_in, size) || !aligned_to(r->v_out, size)
+        || (r->v_in && r->capacity <= 0))
+        return LCT_E_ARG;
+    switch (r->type) {
+    case LCT_BF16: return by_vector<LCT_BF16>(*r, stream);
+    case LCT_FP16: return by_vector<LCT_FP16>(*r, stream);
+    case LCT_FP32: return by_vector<LCT_FP32>(*r, stream);
+    default: return LCT_E_ARG;
+    }
+}

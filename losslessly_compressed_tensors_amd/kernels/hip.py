@@ -7,6 +7,7 @@ and the current torch stream as the ``hipStream_t`` argument.
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from pathlib import Path
 
@@ -163,6 +164,17 @@ class UpdateJob(ctypes.Structure):
     ]
 
 
+# lct_attention, lct_attention_gradients and lct_rotary, packed in one step (a
+# ctypes.Structure's field writes took 12 us of a 20 us call); entry points take
+# the bytes.  Fields as include/lct.h declares them.
+ATTENTION = struct.Struct("@6P12q9if")
+ATTENTION_GRADIENTS = struct.Struct("@5P12q")
+ROTARY = struct.Struct("@8P21q10if4x")
+
+# Value types (LCT_BF16, LCT_FP16, LCT_FP32).
+BF16, FP16, FP32 = 0, 1, 2
+
+
 # name -> argument types (all entry points return int32).
 _SIGNATURES = {
     "lct_estimate_and_shift_tables": [_ptr, _c_int32, _c_int64, _c_int64, _ptr, _ptr, _ptr, _ptr,
@@ -250,6 +262,12 @@ _SIGNATURES = {
     "lct_rms_norm_backward": [_ptr, _ptr, _ptr, _ptr, _c_int32, _ptr, _ptr, _ptr, _c_int64, _ptr,
                               _c_int32, _c_int64, _c_int32, _ptr],
     "lct_skinny_linear": [_ptr, _ptr, _ptr, _c_int32, _c_int32, _c_int32, _ptr],
+    "lct_attention_forward": [_ptr, _c_int32, _ptr, _c_int64, _ptr],
+    "lct_attention_backward": [_ptr, _ptr, _c_int32, _c_int32, _ptr, _c_int64, _ptr],
+    "lct_attention_decode": [_ptr, _c_int32, _ptr, _c_int64, _ptr],
+    "lct_rotate": [_ptr, _ptr],
+    "lct_dropout": [_ptr, _ptr, _ptr, _c_int64, _c_int32, _c_int32, ctypes.c_uint64,
+                    ctypes.c_uint64, _ptr, _ptr],
     "lct_bandwidth_probe": [_c_int32, _ptr, _c_int64, _ptr, _c_int64, _c_int32, _ptr],
     "lct_compress_buffered_noalloc": [_ptr, _c_int64, _c_int64, Geometry, _ptr, _ptr, _ptr, _ptr,
                                       _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int32, _ptr,
