@@ -843,10 +843,11 @@ int32_t lct_attention_forward(const lct_attention *a, int32_t splits, float *wor
 /* The gradients of q, k and v from that of out, a->out and a->lse as the forward
  * call wrote them; those of a key head that several query heads share are
  * their sum.  delta: working array of lse's size.  The queries that see a block
- * of 128 keys are shared among `splits` workgroups, among `sink_splits` where
- * the block holds sinks (and window > 0); with either above 1, `workspace`
- * holds batch * kv_heads * (sink blocks * sink_splits + other blocks * splits) *
- * 256 * head_dim floats, added by a further launch in their order. */
+ * of n keys (128, 256 where head_dim > 64) are shared among `splits` workgroups,
+ * among `sink_splits` where the block holds sinks (and window > 0); with either
+ * above 1, `workspace` holds batch * kv_heads * (sink blocks * sink_splits + other
+ * blocks * splits) * 2 n * head_dim floats, added by a further launch in their
+ * order. */
 typedef struct {
     const void *grad;
     void *dq, *dk, *dv;

@@ -12,6 +12,7 @@ constexpr int kKeyTile = 64;         // keys per step
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescale = 8.0f;     // how far (log2) a running maximum may lag
 constexpr float kHalfWeights = 256.0f;
+constexpr int32_t kMaxTokens = 1 << 30;
 
 // lse's and delta's values per head: whole query tiles, the last one's extra
 // rows among them.
@@ -49,7 +50,7 @@ __global__ __launch_bounds__(kAttentionThreads, 2) void attention_forward_kernel
     __shared__ __attribute__((aligned(1024))) uint16_t v_odd[kKeyTile * kPitch];
 
     const int64_t per_head = int64_t{tiles} * splits;
-    const int64_t item = xcd_item(per_head * a.batch * a.heads);
+    const int64_t item = xcd_item(per_head * a.batch * a.heads, blockIdx.x);
     if (item >= per_head * a.batch * a.heads) return;
     const int32_t bh = static_cast<int32_t>(item / per_head);
     const int32_t part = static_cast<int32_t>(item % per_head);
@@ -266,7 +267,7 @@ __global__ __launch_bounds__(kAttentionThreads, 2) void attention_dq_kernel(
     __shared__ __attribute__((aligned(1024))) uint16_t v_odd[kKeyTile * kPitch];
 
     const int64_t items = int64_t{tiles} * a.batch * a.heads;
-    const int64_t item = xcd_item(items);
+    const int64_t item = xcd_item(items, blockIdx.x);
     if (item >= items) return;
     const int32_t bh = static_cast<int32_t>(item / tiles);
     const int32_t b = bh / a.heads, h = bh % a.heads, kv = h / (a.heads / a.kv_heads);
@@ -393,51 +394,62 @@ __global__ __launch_bounds__(kAttentionThreads, 2) void attention_dq_kernel(
 // later queries and have parts of their own number.
 struct KeyBlocks {
     int32_t blocks, sink_blocks, splits, sink_splits;
+    __host__ __device__ __forceinline__ int64_t sink_parts() const {
+        return int64_t{sink_blocks} * sink_splits;
+    }
+    __host__ __device__ __forceinline__ int64_t other_parts() const {
+        return int64_t{blocks - sink_blocks} * splits;
+    }
     __host__ __device__ __forceinline__ int64_t parts() const {
-        return int64_t{sink_blocks} * sink_splits + int64_t{blocks - sink_blocks} * splits;
+        return sink_parts() + other_parts();
     }
     __host__ __device__ __forceinline__ int64_t first_part(int32_t block) const {
-        return block < sink_blocks
-                   ? int64_t{block} * sink_splits
-                   : int64_t{sink_blocks} * sink_splits + int64_t{block - sink_blocks} * splits;
+        return block < sink_blocks ? int64_t{block} * sink_splits
+                                   : sink_parts() + int64_t{block - sink_blocks} * splits;
     }
     __host__ __device__ __forceinline__ int32_t parts_of(int32_t block) const {
         return block < sink_blocks ? sink_splits : splits;
     }
 };
 
-constexpr int kKeyBlock = 128;       // keys of a workgroup, 32 per wave
 constexpr int kQueryStep = 64;       // queries per step
 
-// A wave's 32 keys, the queries (of all heads that share them) in tiles.
+// Keys of a workgroup of the kernel below.
+__host__ __device__ constexpr int key_block(int dim) { return dim > 64 ? 256 : 128; }
+
+// A wave's 32 or 64 keys, the queries (of all heads that share them) in tiles.
 template <bool kHalf, int kDim>
-__global__ __launch_bounds__(kAttentionThreads, kDim > 64 ? 1 : 2) void attention_dkdv_kernel(
+__global__ __launch_bounds__(key_block(kDim) * 2, 2) void attention_dkdv_kernel(
     lct_attention a, lct_attention_gradients d, KeyBlocks blocks, float *__restrict__ parts) {
     constexpr int kPitch = kPitchOf<kDim>;
     constexpr int kSteps = kDim / 16, kColumns = kDim / 32;
+    constexpr int kKeyBlock = key_block(kDim), kWaveKeys = 32, kThreads = kKeyBlock * 2;
+    constexpr int kGroups = kWaveKeys / 32;
     __shared__ __attribute__((aligned(1024))) uint16_t q_even[kQueryStep * kPitch];
     __shared__ __attribute__((aligned(1024))) uint16_t g_even[kQueryStep * kPitch];
     __shared__ __attribute__((aligned(1024))) uint16_t q_odd[kQueryStep * kPitch];
     __shared__ __attribute__((aligned(1024))) uint16_t g_odd[kQueryStep * kPitch];
     __shared__ __attribute__((aligned(1024))) float stats_even[2 * kQueryStep];
     __shared__ __attribute__((aligned(1024))) float stats_odd[2 * kQueryStep];
+    // Wide heads leave no registers for the values' operands beside the sums.
+    constexpr bool kStaged = kDim > 64;
+    __shared__ __attribute__((aligned(1024))) uint16_t v_block[kStaged ? kKeyBlock * kPitch : 512];
 
-    const int64_t per_head = blocks.parts();
-    const int64_t items = per_head * a.batch * a.kv_heads;
-    const int64_t item = xcd_item(items);
+    // The blocks without sinks, then those with: each kind dealt out over the
+    // XCDs by itself, since their parts are of unequal length.
+    const int64_t heads = int64_t{a.batch} * a.kv_heads;
+    const int64_t other_items = blocks.other_parts() * heads, sink_items = blocks.sink_parts() * heads;
+    const bool sinks = blockIdx.x >= xcd_grid(other_items);
+    const int64_t items = sinks ? sink_items : other_items;
+    const int64_t item =
+        xcd_item(items, sinks ? blockIdx.x - static_cast<uint32_t>(xcd_grid(other_items)) : blockIdx.x);
     if (item >= items) return;
+    const int64_t per_head = sinks ? blocks.sink_parts() : blocks.other_parts();
     const int32_t bkv = static_cast<int32_t>(item / per_head);
     const int32_t b = bkv / a.kv_heads, kv = bkv % a.kv_heads, group = a.heads / a.kv_heads;
-    const int64_t part = item % per_head;
-    const int64_t sink_parts = int64_t{blocks.sink_blocks} * blocks.sink_splits;
-    int32_t block, split;
-    if (part < sink_parts) {
-        block = static_cast<int32_t>(part / blocks.sink_splits);
-        split = static_cast<int32_t>(part % blocks.sink_splits);
-    } else {
-        block = blocks.sink_blocks + static_cast<int32_t>((part - sink_parts) / blocks.splits);
-        split = static_cast<int32_t>((part - sink_parts) % blocks.splits);
-    }
+    const int32_t part = static_cast<int32_t>(item % per_head);
+    const int32_t splits = sinks ? blocks.sink_splits : blocks.splits;
+    const int32_t block = (sinks ? 0 : blocks.sink_blocks) + part / splits, split = part % splits;
 
     const int lane = wave_lane(), half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -457,21 +469,32 @@ __global__ __launch_bounds__(kAttentionThreads, kDim > 64 ? 1 : 2) void attentio
     const int32_t per_query_head =
         high > low ? (high + kQueryStep - 1) / kQueryStep - low_tile : 0;
     const int32_t steps = per_query_head * group;
-    const int32_t per_split = (steps + blocks.parts_of(block) - 1) / blocks.parts_of(block);
+    const int32_t per_split = (steps + splits - 1) / splits;
     const int32_t begin = split * per_split, end = min(steps, begin + per_split);
 
-    const int32_t wave_first = first + 32 * wave;
-    const int32_t key = wave_first + (lane & 31);
+    const int32_t wave_first = first + kWaveKeys * wave;
     const uint16_t *k = static_cast<const uint16_t *>(a.k) + b * a.k_stride[0] + kv * a.k_stride[1];
     const uint16_t *v = static_cast<const uint16_t *>(a.v) + b * a.v_stride[0] + kv * a.v_stride[1];
-    u32x4 k_operand[kSteps], v_operand[kSteps];
+    u32x4 k_operand[kGroups][kSteps], v_operand[kStaged ? 1 : kGroups][kStaged ? 1 : kSteps];
+    if constexpr (kStaged) {
+        TileLoads<kQueryStep, kPitch, kThreads> v_loads;
+        v_loads.prepare(a.v_stride[2], a.head_dim);
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-        k_operand[s] = load_operand(k, a.k_stride[2], key, length, a.head_dim, s);
-        v_operand[s] = load_operand(v, a.v_stride[2], key, length, a.head_dim, s);
+        for (int i = 0; i < kKeyBlock; i += kQueryStep)
+            v_loads.issue(v + (first + i) * a.v_stride[2], length - first - i, a.v_stride[2],
+                          a.head_dim, v_block + i * kPitch);
     }
+#pragma unroll
+    for (int m = 0; m < kGroups; ++m)
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const int32_t key = wave_first + 32 * m + (lane & 31);
+            k_operand[m][s] = load_operand(k, a.k_stride[2], key, length, a.head_dim, s);
+            if constexpr (!kStaged)
+                v_operand[m][s] = load_operand(v, a.v_stride[2], key, length, a.head_dim, s);
+        }
 
-    TileLoads<kQueryStep, kPitch> q_loads, g_loads;
+    TileLoads<kQueryStep, kPitch, kThreads> q_loads, g_loads;
     q_loads.prepare(a.q_stride[2], a.head_dim);
     g_loads.prepare(d.grad_stride[2], a.head_dim);
     const auto load = [&](int32_t t, uint16_t *q_tile, uint16_t *g_tile, float *stats)
@@ -495,72 +518,110 @@ __global__ __launch_bounds__(kAttentionThreads, kDim > 64 ? 1 : 2) void attentio
     };
 
     const float factor = a.scale * kLog2e;
-    f32x16 dk[kColumns], dv[kColumns];
+    f32x16 dk[kGroups][kColumns], dv[kGroups][kColumns];
 #pragma unroll
-    for (int c = 0; c < kColumns; ++c) dk[c] = dv[c] = f32x16{};
+    for (int m = 0; m < kGroups; ++m)
+#pragma unroll
+        for (int c = 0; c < kColumns; ++c) dk[m][c] = dv[m][c] = f32x16{};
 
-    const auto step = [&](int32_t t, const uint16_t *q_tile, const uint16_t *g_tile,
-                          const float *stats) __attribute__((always_inline)) {
-        const int32_t tile_position = (low_tile + t % per_query_head) * kQueryStep + shift;
+    // 32 of the step's queries, at `position`; `all`: each sees all the wave's keys.
+    const auto rows = [&](int n, bool all, int32_t position, const uint16_t *q_tile,
+                          const uint16_t *g_tile, const float *stats)
+                          __attribute__((always_inline)) {
+        f32x16 s[kGroups], e[kGroups];
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            const int32_t position = tile_position + 32 * n, last_here = position + 31;
-            const bool seen_by_some =
-                last_here >= wave_first
-                && (a.window == 0 || position - (wave_first + 31) < a.window
-                    || wave_first < a.sinks);
-            if (!seen_by_some) continue;
-            const bool seen_by_all =
-                wave_first + 31 <= position && last_here < length
-                && (a.window == 0 || last_here - wave_first < a.window
-                    || wave_first + 32 <= a.sinks);
-            f32x16 s{}, e;
+        for (int g = 0; g < 4; ++g) {
+            const f32x4 delta = *reinterpret_cast<const f32x4 *>(stats + kQueryStep + 32 * n + 8 * g
+                                                                 + 4 * half);
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const f32x4 delta = *reinterpret_cast<const f32x4 *>(
-                    stats + kQueryStep + 32 * n + 8 * g + 4 * half);
+            for (int m = 0; m < kGroups; ++m)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) e[4 * g + i] = -delta[i];
+                for (int i = 0; i < 4; ++i) {
+                    s[m][4 * g + i] = 0.0f;
+                    e[m][4 * g + i] = -delta[i];
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            const u32x4 q_rows = read_rows<kPitch>(q_tile, n, i);
+            const u32x4 g_rows = read_rows<kPitch>(g_tile, n, i);
+#pragma unroll
+            for (int m = 0; m < kGroups; ++m) {
+                s[m] = Element<kHalf>::multiply(q_rows, k_operand[m][i], s[m]);
+                if constexpr (kStaged)
+                    e[m] = Element<kHalf>::multiply(
+                        g_rows, read_rows<kPitch>(v_block, kGroups * wave + m, i), e[m]);
+                else
+                    e[m] = Element<kHalf>::multiply(g_rows, v_operand[m][i], e[m]);
             }
+        }
+        // In FP16 the weights of long rows lie below the normal numbers: they are
+        // held 2^8 larger until the sums of dv are stored.
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-                s = Element<kHalf>::multiply(read_rows<kPitch>(q_tile, n, i), k_operand[i], s);
-                e = Element<kHalf>::multiply(read_rows<kPitch>(g_tile, n, i), v_operand[i], e);
-            }
-            // In FP16 the weights of long rows lie below the normal numbers:
-            // they are held 2^8 larger until the sums of dv are stored.
+        for (int g = 0; g < 4; ++g) {
+            const f32x4 lse = *reinterpret_cast<const f32x4 *>(stats + 32 * n + 8 * g + 4 * half);
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const f32x4 lse =
-                    *reinterpret_cast<const f32x4 *>(stats + 32 * n + 8 * g + 4 * half);
+            for (int m = 0; m < kGroups; ++m)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int r = 4 * g + i;
-                    s[r] = exp2_fast(__builtin_fmaf(s[r], factor, -lse[i]));
-                    e[r] *= s[r];
-                    if (kHalf) s[r] *= kHalfWeights;
+                    s[m][r] = exp2_fast(__builtin_fmaf(s[m][r], factor, -lse[i]));
+                    e[m][r] *= s[m][r];
+                    if (kHalf) s[m][r] *= kHalfWeights;
                 }
-            }
-            if (!seen_by_all) {
+        }
+        if (!all) {
+            // Query at - key: from 0 to below what the key's place allows.
+            const int32_t at = position + 4 * half;
+#pragma unroll
+            for (int m = 0; m < kGroups; ++m) {
+                const int32_t key = wave_first + 32 * m + (lane & 31);
+                const uint32_t reach =
+                    a.window == 0 || key < a.sinks ? kMaxTokens : static_cast<uint32_t>(a.window);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const int32_t at = position + 8 * (r / 4) + 4 * half + r % 4;
-                    const bool seen = sight_of(a, at, length)(key);
-                    s[r] = seen ? s[r] : 0.0f;
-                    e[r] = seen ? e[r] : 0.0f;
+                    const int32_t c = 8 * (r / 4) + r % 4;
+                    const bool seen =
+                        static_cast<uint32_t>(at - key + c) < reach && at < length - c;
+                    s[m][r] = seen ? s[m][r] : 0.0f;
+                    e[m][r] = seen ? e[m][r] : 0.0f;
                 }
             }
+        }
 #pragma unroll
-            for (int p = 0; p < 2; ++p) {
-                const u32x4 weights = as_operand<kHalf>(s, p), ds = as_operand<kHalf>(e, p);
+        for (int p = 0; p < 2; ++p) {
+            u32x4 weights[kGroups], ds[kGroups];
 #pragma unroll
-                for (int c = 0; c < kColumns; ++c) {
-                    dv[c] = Element<kHalf>::multiply(
-                        read_columns<kPitch>(g_tile, 32 * n + 16 * p, c), weights, dv[c]);
-                    dk[c] = Element<kHalf>::multiply(
-                        read_columns<kPitch>(q_tile, 32 * n + 16 * p, c), ds, dk[c]);
+            for (int m = 0; m < kGroups; ++m) {
+                weights[m] = as_operand<kHalf>(s[m], p);
+                ds[m] = as_operand<kHalf>(e[m], p);
+            }
+#pragma unroll
+            for (int c = 0; c < kColumns; ++c) {
+                const u32x4 g_columns = read_columns<kPitch>(g_tile, 32 * n + 16 * p, c);
+                const u32x4 q_columns = read_columns<kPitch>(q_tile, 32 * n + 16 * p, c);
+#pragma unroll
+                for (int m = 0; m < kGroups; ++m) {
+                    dv[m][c] = Element<kHalf>::multiply(g_columns, weights[m], dv[m][c]);
+                    dk[m][c] = Element<kHalf>::multiply(q_columns, ds[m], dk[m][c]);
                 }
             }
+        }
+    };
+    const auto step = [&](int32_t t, const uint16_t *q_tile, const uint16_t *g_tile,
+                          const float *stats) __attribute__((always_inline)) {
+        const int32_t position = (low_tile + t % per_query_head) * kQueryStep + shift;
+        const int32_t last_here = position + kQueryStep - 1, wave_last = wave_first + kWaveKeys - 1;
+        const bool all =
+            wave_last <= position && last_here < length
+            && (a.window == 0 || last_here - wave_first < a.window || wave_last < a.sinks);
+#pragma unroll 1
+        for (int n = 0; n < 2; ++n) {
+            const int32_t here = position + 32 * n;
+            if (all
+                || (here + 31 >= wave_first
+                    && (a.window == 0 || here - wave_last < a.window || wave_first < a.sinks)))
+                rows(n, all, here, q_tile, g_tile, stats);
         }
     };
 
@@ -577,11 +638,22 @@ __global__ __launch_bounds__(kAttentionThreads, kDim > 64 ? 1 : 2) void attentio
         step(t + 1, q_odd, g_odd, stats_odd);
     }
 
-    if (key >= a.keys) return;
     const float dv_scale = kHalf ? 1.0f / kHalfWeights : 1.0f;
-    if (blocks.parts_of(block) > 1) {
+#pragma unroll
+    for (int m = 0; m < kGroups; ++m) {
+        const int32_t key = wave_first + 32 * m + (lane & 31);
+        if (key >= a.keys) continue;
+        if (splits == 1) {
+            store_row<kHalf, kColumns>(static_cast<uint16_t *>(d.dk) + b * d.dk_stride[0]
+                                           + kv * d.dk_stride[1] + key * d.dk_stride[2],
+                                       dk[m], a.scale, a.head_dim);
+            store_row<kHalf, kColumns>(static_cast<uint16_t *>(d.dv) + b * d.dv_stride[0]
+                                           + kv * d.dv_stride[1] + key * d.dv_stride[2],
+                                       dv[m], dv_scale, a.head_dim);
+            continue;
+        }
         float *dst = parts
-                     + (int64_t{bkv} * per_head + blocks.first_part(block) + split) * 2 * kKeyBlock
+                     + (bkv * blocks.parts() + blocks.first_part(block) + split) * 2 * kKeyBlock
                            * a.head_dim
                      + int64_t{key - first} * a.head_dim;
 #pragma unroll
@@ -593,20 +665,13 @@ __global__ __launch_bounds__(kAttentionThreads, kDim > 64 ? 1 : 2) void attentio
                 f32x4 x, y;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    x[i] = dk[c][4 * g + i] * a.scale;
-                    y[i] = dv[c][4 * g + i] * dv_scale;
+                    x[i] = dk[m][c][4 * g + i] * a.scale;
+                    y[i] = dv[m][c][4 * g + i] * dv_scale;
                 }
                 *reinterpret_cast<f32x4 *>(dst + channel) = x;
                 *reinterpret_cast<f32x4 *>(dst + kKeyBlock * a.head_dim + channel) = y;
             }
-        return;
     }
-    store_row<kHalf, kColumns>(static_cast<uint16_t *>(d.dk) + b * d.dk_stride[0]
-                                   + kv * d.dk_stride[1] + key * d.dk_stride[2],
-                               dk, a.scale, a.head_dim);
-    store_row<kHalf, kColumns>(static_cast<uint16_t *>(d.dv) + b * d.dv_stride[0]
-                                   + kv * d.dv_stride[1] + key * d.dv_stride[2],
-                               dv, dv_scale, a.head_dim);
 }
 
 // Adds the parts of the blocks from `first_block` on that have several, in
@@ -615,23 +680,23 @@ template <bool kHalf>
 __global__ __launch_bounds__(kAttentionThreads) void attention_sum_parts_kernel(
     lct_attention a, lct_attention_gradients d, KeyBlocks blocks, const float *__restrict__ parts,
     int32_t end_block) {
-    const int32_t quads = a.head_dim / 4;
+    const int32_t quads = a.head_dim / 4, per_block = key_block(a.head_dim);
     const int64_t item = int64_t{blockIdx.x} * kAttentionThreads + threadIdx.x;
     const int32_t channel = 4 * static_cast<int32_t>(item % quads);
-    const int64_t keys = min(a.keys, end_block * kKeyBlock);
+    const int64_t keys = min(int64_t{a.keys}, int64_t{end_block} * per_block);
     const int32_t key = static_cast<int32_t>(item / quads % keys);
     const int64_t bkv = item / quads / keys;
     if (bkv >= int64_t{a.batch} * a.kv_heads) return;
-    const int32_t block = key / kKeyBlock;
+    const int32_t block = key / per_block;
     const int32_t count = blocks.parts_of(block);
     if (count == 1) return;
-    const int64_t step = int64_t{2} * kKeyBlock * a.head_dim;
+    const int64_t step = int64_t{2} * per_block * a.head_dim;
     const float *src = parts + (bkv * blocks.parts() + blocks.first_part(block)) * step
-                       + int64_t{key % kKeyBlock} * a.head_dim + channel;
+                       + int64_t{key % per_block} * a.head_dim + channel;
     f32x4 x{}, y{};
     for (int32_t s = 0; s < count; ++s) {
         x += *reinterpret_cast<const f32x4 *>(src + s * step);
-        y += *reinterpret_cast<const f32x4 *>(src + s * step + kKeyBlock * a.head_dim);
+        y += *reinterpret_cast<const f32x4 *>(src + s * step + per_block * a.head_dim);
     }
     const int64_t b = bkv / a.kv_heads, kv = bkv % a.kv_heads;
     u32x2 dk, dv;
@@ -654,7 +719,6 @@ bool strides_ok(const int64_t (&stride)[3]) {
     return stride[2] < (int64_t{1} << 24);
 }
 
-constexpr int32_t kMaxTokens = 1 << 30;
 
 }  // namespace
 
@@ -715,14 +779,15 @@ int32_t backward(const lct_attention &a, const lct_attention_gradients &d, const
                  float *workspace, hipStream_t stream) {
     const int32_t tiles = (a.queries + kQueryTile - 1) / kQueryTile;
     const int64_t items = int64_t{tiles} * a.batch * a.heads;
-    const int64_t parts = blocks.parts() * a.batch * a.kv_heads;
+    const int64_t heads = int64_t{a.batch} * a.kv_heads;
+    const uint32_t parts = static_cast<uint32_t>(xcd_grid(blocks.other_parts() * heads)
+                                                 + xcd_grid(blocks.sink_parts() * heads));
     by_width(a.head_dim, [&](auto width) {
         constexpr int kDim = decltype(width)::value;
         attention_dq_kernel<kHalf, kDim>
             <<<static_cast<uint32_t>(xcd_grid(items)), kAttentionThreads, 0, stream>>>(a, d, tiles);
         attention_dkdv_kernel<kHalf, kDim>
-            <<<static_cast<uint32_t>(xcd_grid(parts)), kAttentionThreads, 0, stream>>>(
-                a, d, blocks, workspace);
+            <<<parts, 2 * key_block(kDim), 0, stream>>>(a, d, blocks, workspace);
     });
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return static_cast<int32_t>(err);
@@ -730,7 +795,7 @@ int32_t backward(const lct_attention &a, const lct_attention_gradients &d, const
                               : blocks.sink_splits > 1 ? blocks.sink_blocks
                                                        : 0;
     if (end_block == 0) return LCT_OK;
-    const int64_t keys = std::min<int64_t>(a.keys, int64_t{end_block} * kKeyBlock);
+    const int64_t keys = std::min<int64_t>(a.keys, int64_t{end_block} * key_block(a.head_dim));
     const int64_t threads = keys * (a.head_dim / 4) * a.batch * a.kv_heads;
     attention_sum_parts_kernel<kHalf>
         <<<static_cast<uint32_t>((threads + kAttentionThreads - 1) / kAttentionThreads),
@@ -772,9 +837,10 @@ extern "C" int32_t lct_attention_backward(const lct_attention *a, const lct_atte
         || !aligned16(d->delta) || !aligned16(workspace))
         return LCT_E_ARG;
     KeyBlocks blocks;
-    blocks.blocks = (a->keys + kKeyBlock - 1) / kKeyBlock;
+    const int32_t per_block = key_block(a->head_dim);
+    blocks.blocks = (a->keys + per_block - 1) / per_block;
     blocks.sink_blocks =
-        a->window > 0 ? (std::min(a->sinks, a->keys) + kKeyBlock - 1) / kKeyBlock : 0;
+        a->window > 0 ? (std::min(a->sinks, a->keys) + per_block - 1) / per_block : 0;
     blocks.splits = splits;
     blocks.sink_splits = sink_splits;
     const int64_t parts = blocks.parts() * a->batch * a->kv_heads;
@@ -785,7 +851,7 @@ extern "C" int32_t lct_attention_backward(const lct_attention *a, const lct_atte
         return LCT_E_SIZE;
     if (splits > 1 || (sink_splits > 1 && blocks.sink_blocks > 0)) {
         if (!workspace) return LCT_E_NULL;
-        if (workspace_floats < parts * 2 * kKeyBlock * a->head_dim) return LCT_E_SIZE;
+        if (workspace_floats < parts * 2 * per_block * a->head_dim) return LCT_E_SIZE;
     }
     return a->fp16 ? backward<true>(*a, *d, blocks, workspace, stream)
                    : backward<false>(*a, *d, blocks, workspace, stream);

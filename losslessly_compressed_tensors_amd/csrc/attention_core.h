@@ -13,8 +13,9 @@
 // LDS tiles hold rows of 64 or 128 values (kPitch; narrower heads padded with
 // zeros by the loads' range check).  Each row's 16-byte chunks are permuted by
 // an exclusive or with swizzle(row), a permutation of 0..7 over 8 rows that
-// also keeps 4 rows' chunk pairs apart: rows read by 32 lanes at one chunk, and
-// transposed reads of 4 rows by 16 columns, both touch every bank once.
+// also keeps 4 rows' chunk pairs apart: rows read by 8 lanes at one chunk, and
+// transposed reads of 4 rows by 32 bytes, lie in different 16-byte columns of
+// the 128 bytes that LDS returns in a clock.
 #pragma once
 
 #include <type_traits>
@@ -103,16 +104,16 @@ __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t rsrc, uint16_
 // wave w's load i fills the 1024 bytes at (i * waves + w) * 1024, and lane l's
 // 16 bytes of them hold the chunk that belongs there.  Chunks past the head's
 // width get an offset that the range check rejects (LDS receives zeros).
-template <int kRows, int kPitch>
+template <int kRows, int kPitch, int kThreads = kAttentionThreads>
 struct TileLoads {
-    static constexpr int kCount = kRows * kPitch * 2 / (kAttentionThreads * 16);
+    static constexpr int kCount = kRows * kPitch * 2 / (kThreads * 16);
     uint32_t offset[kCount];
 
     __device__ __forceinline__ void prepare(int64_t row_stride, int32_t dim) {
         constexpr int kChunks = kPitch / 8;
 #pragma unroll
         for (int i = 0; i < kCount; ++i) {
-            const int slot = (i * kAttentionThreads + threadIdx.x);
+            const int slot = i * kThreads + threadIdx.x;
             const int row = slot / kChunks;
             const int chunk = (slot % kChunks) ^ swizzle(row);
             offset[i] = chunk * 8 < dim
@@ -130,7 +131,7 @@ struct TileLoads {
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
 #pragma unroll
         for (int i = 0; i < kCount; ++i)
-            load_to_lds(rsrc, tile + (i * kAttentionWaves + wave) * 512, offset[i]);
+            load_to_lds(rsrc, tile + (i * (kThreads / kWave) + wave) * 512, offset[i]);
     }
 };
 
@@ -226,12 +227,11 @@ struct KeyTiles {
 // Workgroups are handed to the 8 XCDs in turn, each with an L2 of its own: the
 // items (all of a head next to each other) are dealt out in 8 runs, so that a
 // head's workgroups share one L2.  Returns items or more past the last one.
-__device__ __forceinline__ int64_t xcd_item(int64_t items) {
+__device__ __forceinline__ int64_t xcd_item(int64_t items, uint32_t place) {
     const int64_t per = (items + 7) / 8;
-    const int64_t run = blockIdx.x & 7, at = blockIdx.x >> 3;
-    return run * per + at;
+    return (place & 7) * per + (place >> 3);
 }
-inline int64_t xcd_grid(int64_t items) { return (items + 7) / 8 * 8; }
+__host__ __device__ inline int64_t xcd_grid(int64_t items) { return (items + 7) / 8 * 8; }
 
 constexpr int64_t kMaxAttentionItems = int64_t{1} << 23;   // 256 threads each: below 2^32
 

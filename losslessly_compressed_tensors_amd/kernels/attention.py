@@ -21,7 +21,7 @@ MAX_HEAD_DIM = 128       # LCT_MAX_HEAD_DIM
 MAX_ROTARY_DIM = 256     # LCT_MAX_ROTARY_DIM
 MAX_TOKENS = 1 << 30
 
-_QUERY_TILE, _KEY_TILE, _KEY_BLOCK = 128, 64, 128
+_QUERY_TILE, _KEY_TILE = 128, 64
 _DECODE_TILE = 4 * 32    # keys that a workgroup's waves take at a time
 _MAX_SPLITS = 64
 _CUS = 256
@@ -110,21 +110,41 @@ def attention_forward(q: Tensor, k: Tensor, v: Tensor, window: int, sinks: int, 
     return out, lse
 
 
-def backward_splits(batch: int, heads: int, kv_heads: int, queries: int, keys: int, window: int,
-                    sinks: int) -> tuple:
+def key_block(dim: int) -> int:
+    """Keys of a workgroup of the kernel of dk and dv."""
+    return 256 if dim > 64 else 128
+
+
+def backward_splits(batch: int, heads: int, kv_heads: int, queries: int, keys: int, dim: int,
+                    window: int, sinks: int) -> tuple:
     """Workgroups that share the queries of a key block without and with sinks.
-    Blocks are shared until there are two workgroups per compute unit, with 4
-    query tiles each at least; a block with sinks, which all later queries see,
-    then gets parts as long as the others'."""
-    blocks = -(-keys // _KEY_BLOCK)
-    group = heads // kv_heads
-    tiles = -(-min(queries, keys if window == 0 else window + _KEY_BLOCK) // 64) * group
+
+    Without: what ends first by the steps (of 64 queries) that the busiest compute
+    unit takes, and what the parts' sums cost (the traffic of a part's FP32 sums
+    is 0.04 steps of one compute unit, over all of them).  With a window all
+    blocks see about as many queries, without one the first sees all and the last
+    few.  A block with sinks, which all later queries see, gets parts of an
+    eighth of the others' length, which fill what the others leave."""
+    per_block = key_block(dim)
+    blocks, group = -(-keys // per_block), heads // kv_heads
+    slots = _CUS if dim > 64 else 2 * _CUS
+    steps = -(-min(queries, keys if window == 0 else window + per_block) // 64) * group
     items = batch * kv_heads * blocks
-    splits = max(1, min(_MAX_SPLITS, -(-2 * _CUS // items), tiles // 4))
+    best = None
+    for splits in range(1, min(_MAX_SPLITS, max(1, steps // 4)) + 1):
+        part = -(-steps // splits)
+        if window == 0:
+            time = items * steps / 2 / slots + part
+        else:
+            time = -(-items * splits // slots) * part
+        time += 0.04 * items * splits / slots * (splits > 1) * _CUS
+        if best is None or time < best[0]:
+            best = time, splits
+    splits = best[1]
     if window == 0 or sinks == 0:
         return splits, 1
-    per_part = -(-tiles // splits)
-    return splits, max(1, min(_MAX_SPLITS, -(-(-(-queries // 64) * group) // per_part)))
+    part = max(4, -(-steps // splits) // 8)
+    return splits, max(1, min(_MAX_SPLITS, -(-(-(-queries // 64) * group) // part)))
 
 
 def attention_backward(grad: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor,
@@ -136,11 +156,13 @@ def attention_backward(grad: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tenso
     with on_device(q):
         dq, dk, dv = _btHD(q), _btHD(k), _btHD(v)
         delta = _lse(q)
-        splits, sink_splits = backward_splits(batch, heads, kv_heads, queries, keys, window, sinks)
-        blocks = -(-keys // _KEY_BLOCK)
-        sink_blocks = -(-min(sinks, keys) // _KEY_BLOCK) if window else 0
+        splits, sink_splits = backward_splits(batch, heads, kv_heads, queries, keys, dim, window,
+                                              sinks)
+        per_block = key_block(dim)
+        blocks = -(-keys // per_block)
+        sink_blocks = -(-min(sinks, keys) // per_block) if window else 0
         parts = sink_blocks * sink_splits + (blocks - sink_blocks) * splits
-        floats = (batch * kv_heads * parts * 2 * _KEY_BLOCK * dim
+        floats = (batch * kv_heads * parts * 2 * per_block * dim
                   if splits > 1 or (sink_splits > 1 and sink_blocks) else 0)
         workspace = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
         hip.call("lct_attention_backward",
