@@ -40,27 +40,41 @@ def _whole(value, name: str, least: int, most: int) -> int:
     return int(value)
 
 
+_PLAIN = (Tensor, torch.nn.Parameter)
+_wrapped = torch._C._functorch.is_functorch_wrapped_tensor
+
+
 def _check_tensor(t, name: str, ndim: int, dtypes) -> None:
-    if not isinstance(t, Tensor):
-        raise TypeError(f"{name} must be a torch.Tensor")
-    if (type(t) not in (Tensor, torch.nn.Parameter)
-            or torch._C._functorch.is_functorch_wrapped_tensor(t)):
-        raise TypeError(f"{name} must be a plain tensor, got {type(t).__name__}")
+    if type(t) not in _PLAIN or _wrapped(t) or t.is_neg():
+        raise TypeError(f"{name} must be a plain torch.Tensor, got {type(t).__name__}")
     if not t.is_cuda:
         raise ValueError(f"{name} must be a GPU tensor")
     if t.dtype not in dtypes:
         raise TypeError(f"{name} must be one of {', '.join(map(str, dtypes))}, got {t.dtype}")
     if t.ndim != ndim:
         raise ValueError(f"{name} must have {ndim} dimensions, got {t.ndim}")
-    if t.is_neg():
-        raise TypeError(f"{name} must not be a negated view")
 
 
-def _check_like(t, name: str, other: Tensor, other_name: str) -> None:
-    if t.dtype != other.dtype:
-        raise TypeError(f"{name} and {other_name} must have one type")
+def _check_like(t, name: str, other: Tensor, ndim: int) -> None:
+    """``t`` against ``other``, q or x, which has been checked."""
+    if type(t) not in _PLAIN or _wrapped(t) or t.is_neg():
+        raise TypeError(f"{name} must be a plain torch.Tensor, got {type(t).__name__}")
     if t.device != other.device:
-        raise ValueError(f"{name} and {other_name} must be on one device")
+        raise ValueError(f"all tensors must be on {other.device}, {name} is on {t.device}")
+    if t.dtype != other.dtype:
+        raise TypeError(f"all tensors must have one type, {other.dtype}: {name} has {t.dtype}")
+    if t.ndim != ndim:
+        raise ValueError(f"{name} must have {ndim} dimensions, got {t.ndim}")
+
+
+def _recorded(*tensors) -> bool:
+    """Whether autograd has to see the call."""
+    if not torch.is_grad_enabled():
+        return False
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return True
+    return False
 
 
 def _indices(t, name: str, shapes, device) -> Tensor:
@@ -74,7 +88,7 @@ def _indices(t, name: str, shapes, device) -> Tensor:
                          f"got {tuple(t.shape)}")
     if t.device != device:
         raise ValueError(f"{name} must be on {device}")
-    return t.to(torch.int32)
+    return t if t.dtype == torch.int32 else t.to(torch.int32)
 
 
 # ---- rotary positions
@@ -154,20 +168,19 @@ class Rotary:
 
 
 _ROTARY_TYPES = tuple(kernels.TYPES)
+_MAX_HEADS = 4096
 
 
-def _check_rotary(plan, q, others) -> None:
-    if not isinstance(plan, Rotary):
+def _check_rotary(plan, q) -> None:
+    if type(plan) is not Rotary:
         raise TypeError("plan must be a Rotary")
     if plan.turns.device != q.device:
         raise ValueError("plan and q must be on one device")
-    if q.shape[-1] < plan.dim or q.shape[-1] > kernels.MAX_ROTARY_DIM:
+    if not plan.dim <= q.shape[-1] <= kernels.MAX_ROTARY_DIM:
         raise ValueError(f"heads must have {plan.dim} to {kernels.MAX_ROTARY_DIM} channels, "
                          f"got {q.shape[-1]}")
-    if q.shape[-2] > 4096:
-        raise ValueError("at most 4096 heads")
-    for name, t in others:
-        _check_like(t, name, q, "q")
+    if q.shape[-2] > _MAX_HEADS:
+        raise ValueError(f"at most {_MAX_HEADS} heads")
 
 
 class _ApplyRotary(torch.autograd.Function):
@@ -180,16 +193,23 @@ class _ApplyRotary(torch.autograd.Function):
         return q_out if k is None else (q_out, k_out)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_q, grad_k=None):
-        positions, = ctx.saved_tensors
-        if grad_q is None and grad_k is None:
-            return None, None, None, None, None
-        if grad_q is None:
-            grad_k, _ = kernels.rotate(ctx.plan, grad_k, None, positions, ctx.start, True)
-        else:
-            grad_q, grad_k = kernels.rotate(ctx.plan, grad_q, grad_k, positions, ctx.start, True)
-        return grad_q, grad_k, None, None, None
+        # With a graph of the backward pass asked for, a second one is an error.
+        if torch.is_grad_enabled():
+            return _rotary_backward_once(ctx, grad_q, grad_k)
+        return _rotary_backward(ctx, grad_q, grad_k)
+
+
+def _rotary_backward(ctx, grad_q, grad_k):
+    positions, = ctx.saved_tensors
+    if grad_q is None and grad_k is not None:
+        grad_k, _ = kernels.rotate(ctx.plan, grad_k, None, positions, ctx.start, True)
+    elif grad_q is not None:
+        grad_q, grad_k = kernels.rotate(ctx.plan, grad_q, grad_k, positions, ctx.start, True)
+    return grad_q, grad_k, None, None, None
+
+
+_rotary_backward_once = once_differentiable(_rotary_backward)
 
 
 @torch.compiler.disable
@@ -200,30 +220,29 @@ def apply_rotary(plan: Rotary, q: Tensor, k: Tensor | None = None, positions=Non
     as [batch, token] (INT32; INT64 is converted).  Angles and products are FP32,
     rounded once.  Differentiable in ``q`` and ``k``."""
     _check_tensor(q, "q", 4, _ROTARY_TYPES)
-    others = []
+    _check_rotary(plan, q)
     if k is not None:
-        _check_tensor(k, "k", 4, _ROTARY_TYPES)
-        others.append(("k", k))
+        _check_like(k, "k", q, 4)
         if k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3]:
             raise ValueError("q and k must agree in batch, tokens and channels")
-        if k.shape[2] > 4096:
-            raise ValueError("at most 4096 heads")
-    _check_rotary(plan, q, others)
+        if k.shape[2] > _MAX_HEADS:
+            raise ValueError(f"at most {_MAX_HEADS} heads")
     start = 0
-    if positions is None:
-        pass
-    elif isinstance(positions, numbers.Integral):
-        start, positions = _whole(positions, "positions", -2 ** 62, 2 ** 62), None
-    else:
+    if isinstance(positions, Tensor):
         positions = _indices(positions, "positions", ((q.shape[0],), tuple(q.shape[:2])), q.device)
+    elif positions is not None:
+        start, positions = _whole(positions, "positions", -2 ** 62, 2 ** 62), None
     if q.numel() == 0 or (k is not None and k.numel() == 0):
-        if q.numel() == 0 and (k is None or k.numel() == 0):
-            return q.clone() if k is None else (q.clone(), k.clone())
-        return ((q.clone(), apply_rotary(plan, k, None, positions if positions is not None
-                                         else start)) if q.numel() == 0 else
-                (apply_rotary(plan, q, None, positions if positions is not None else start),
-                 k.clone()))
-    return _ApplyRotary.apply(q, k, plan, positions, start)
+        if k is None:
+            return q.clone()
+        # Of the two, one may have heads.
+        return tuple(t.clone() if t.numel() == 0 else
+                     apply_rotary(plan, t, positions=start if positions is None else positions)
+                     for t in (q, k))
+    if _recorded(q, k):
+        return _ApplyRotary.apply(q, k, plan, positions, start)
+    out = kernels.rotate(plan, q, k, positions, start, False)
+    return out[0] if k is None else out
 
 
 @torch.compiler.disable
@@ -234,28 +253,27 @@ def rotary_append(plan: Rotary, q: Tensor, k: Tensor, v: Tensor, k_cache: Tensor
     to the caches [batch, capacity, head, channel] there.  A position outside the
     cache is not written.  Not differentiable."""
     _check_tensor(q, "q", 3, _ROTARY_TYPES)
-    for name, t in (("k", k), ("v", v)):
-        _check_tensor(t, name, 3, _ROTARY_TYPES)
-        if t.shape != k.shape or t.shape[0] != q.shape[0] or t.shape[2] != q.shape[2]:
-            raise ValueError("q, k and v must agree in batch and channels, k and v in heads")
-    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
-        _check_tensor(t, name, 4, _ROTARY_TYPES)
-        if (t.shape[0], t.shape[2], t.shape[3]) != tuple(k.shape) or t.shape != k_cache.shape:
-            raise ValueError("the caches must be [batch, capacity, head, channel] of k's heads")
-        if t.stride(3) != 1 and t.shape[3] != 1:
-            raise ValueError(f"{name}'s channels must be adjacent")
-        _no_gradient(t, name)
-    _check_rotary(plan, q, (("k", k), ("v", v), ("k_cache", k_cache), ("v_cache", v_cache)))
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        _no_gradient(t, name)
-    if k.shape[1] > 4096 or k_cache.shape[1] > kernels.MAX_TOKENS:
-        raise ValueError(f"at most 4096 heads and {kernels.MAX_TOKENS} tokens")
-    positions = _indices(positions, "positions", ((q.shape[0],),), q.device)
+    _check_rotary(plan, q)
+    _check_like(k, "k", q, 3)
+    _check_like(v, "v", q, 3)
+    _check_like(k_cache, "k_cache", q, 4)
+    _check_like(v_cache, "v_cache", q, 4)
+    batch, kv_heads, dim = k.shape
+    if v.shape != k.shape or q.shape[0] != batch or q.shape[2] != dim:
+        raise ValueError("q, k and v must agree in batch and channels, k and v in heads")
+    if (k_cache.shape != v_cache.shape or k_cache.shape[0] != batch
+            or k_cache.shape[2] != kv_heads or k_cache.shape[3] != dim):
+        raise ValueError("the caches must be [batch, capacity, head, channel] of k's heads")
+    if k_cache.stride(3) != 1 or v_cache.stride(3) != 1:
+        raise ValueError("the caches' channels must be adjacent")
+    if _recorded(q, k, v, k_cache, v_cache):
+        raise ValueError(_NO_GRADIENT)
+    if kv_heads > _MAX_HEADS or k_cache.shape[1] > kernels.MAX_TOKENS:
+        raise ValueError(f"at most {_MAX_HEADS} heads and {kernels.MAX_TOKENS} tokens")
+    positions = _indices(positions, "positions", ((batch,),), q.device)
     if q.numel() == 0 or k_cache.numel() == 0:
         raise ValueError("rotary_append needs a token and a cache")
-    out, _ = kernels.rotate(plan, q.unsqueeze(1), k.unsqueeze(1), positions, 0, False,
-                            (v.unsqueeze(1), k_cache, v_cache))
-    return out.squeeze(1)
+    return kernels.rotate_into(plan, q, k, v, k_cache, v_cache, positions)
 
 
 # ---- attention
@@ -263,10 +281,8 @@ def rotary_append(plan: Rotary, q: Tensor, k: Tensor, v: Tensor, k_cache: Tensor
 _ATTENTION_TYPES = (torch.bfloat16, torch.float16)
 
 
-def _no_gradient(t: Tensor, name: str) -> None:
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{name} requires a gradient, which this operator does not have; "
-                         "call it under torch.no_grad()")
+_NO_GRADIENT = ("an input requires a gradient, which this operator does not have: "
+                "call it under torch.no_grad()")
 
 
 def _sight(window, sinks, scale, dim: int) -> tuple:
@@ -290,28 +306,33 @@ def _check_heads(heads: int, kv_heads: int, dim: int) -> None:
 class _WindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lengths, window, sinks, scale):
-        needed = any(ctx.needs_input_grad[:3])
-        out, lse = kernels.attention_forward(q, k, v, window, sinks, scale, lengths, needed)
-        if needed:
-            ctx.save_for_backward(q, k, v, out, lse, lengths)
-            ctx.sight = window, sinks, scale
+        out, lse = kernels.attention_forward(q, k, v, window, sinks, scale, lengths, True)
+        ctx.save_for_backward(q, k, v, out, lse, lengths)
+        ctx.sight = window, sinks, scale
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad):
-        q, k, v, out, lse, lengths = ctx.saved_tensors
-        window, sinks, scale = ctx.sight
-        return (*kernels.attention_backward(grad, q, k, v, out, lse, window, sinks, scale,
-                                            lengths), None, None, None, None)
+        if torch.is_grad_enabled():
+            return _attention_backward_once(ctx, grad)
+        return _attention_backward(ctx, grad)
+
+
+def _attention_backward(ctx, grad):
+    q, k, v, out, lse, lengths = ctx.saved_tensors
+    return (*kernels.attention_backward(grad, q, k, v, out, lse, *ctx.sight, lengths), None, None,
+            None, None)
+
+
+_attention_backward_once = once_differentiable(_attention_backward)
 
 
 def check_attention(q, k, v, window, sinks, scale, lengths) -> tuple:
     """:func:`window_attention`'s checks; its ``(window, sinks, scale, lengths)``
     as the kernels take them."""
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        _check_tensor(t, name, 4, _ATTENTION_TYPES)
-        _check_like(t, name, q, "q")
+    _check_tensor(q, "q", 4, _ATTENTION_TYPES)
+    _check_like(k, "k", q, 4)
+    _check_like(v, "v", q, 4)
     batch, heads, queries, dim = q.shape
     if k.shape != v.shape or k.shape[0] != batch or k.shape[3] != dim:
         raise ValueError("q, k and v must agree in batch and channels, k and v in shape")
@@ -346,7 +367,9 @@ def window_attention(q: Tensor, k: Tensor, v: Tensor, *, window: int | None = No
     if q.numel() == 0 or k.shape[2] == 0:
         # Nothing to compute, or nothing to see: zero, with zero gradients.
         return q * 0 + (k.sum() + v.sum()) * 0
-    return _WindowAttention.apply(q, k, v, lengths, window, sinks, scale)
+    if _recorded(q, k, v):
+        return _WindowAttention.apply(q, k, v, lengths, window, sinks, scale)
+    return kernels.attention_forward(q, k, v, window, sinks, scale, lengths, False)[0]
 
 
 @torch.compiler.disable
@@ -359,11 +382,10 @@ def decode_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, lengths: Tenso
     gives zeros; lengths above the capacity count as the capacity.  Only keys
     that are seen are read.  Not differentiable."""
     _check_tensor(q, "q", 3, _ATTENTION_TYPES)
-    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
-        _check_tensor(t, name, 4, _ATTENTION_TYPES)
-        _check_like(t, name, q, "q")
-        _no_gradient(t, name)
-    _no_gradient(q, "q")
+    _check_like(k_cache, "k_cache", q, 4)
+    _check_like(v_cache, "v_cache", q, 4)
+    if _recorded(q, k_cache, v_cache):
+        raise ValueError(_NO_GRADIENT)
     batch, heads, dim = q.shape
     if (k_cache.shape != v_cache.shape or k_cache.shape[0] != batch or k_cache.shape[3] != dim):
         raise ValueError("q and the caches must agree in batch and channels, the caches in shape")
@@ -376,8 +398,7 @@ def decode_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, lengths: Tenso
     window, sinks, scale = _sight(window, sinks, scale, dim)
     if q.numel() == 0 or k_cache.shape[1] == 0:
         return torch.zeros_like(q)
-    return kernels.attention_decode(q, k_cache.transpose(1, 2), v_cache.transpose(1, 2), window,
-                                    sinks, scale, lengths)
+    return kernels.attention_decode(q, k_cache, v_cache, window, sinks, scale, lengths)
 
 
 class KVCache:

@@ -12,7 +12,7 @@ from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from ..kernels import attention as kernels
-from .attention import _check_like, _check_tensor, _whole
+from .attention import _check_like, _check_tensor, _recorded, _whole
 
 __all__ = ["dropout_add"]
 
@@ -34,14 +34,23 @@ class _DropoutAdd(torch.autograd.Function):
                                below, seed, offset, more)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad):
-        below, seed, offset = ctx.draw
-        more, = ctx.saved_tensors
-        grad_x = None
-        if ctx.needs_input_grad[0]:
-            grad_x = kernels.dropout(_whole_rows(grad), None, below, seed, offset, more)
-        return grad_x, grad if ctx.needs_input_grad[1] else None, None, None, None, None
+        # With a graph of the backward pass asked for, a second one is an error.
+        if torch.is_grad_enabled():
+            return _backward_once(ctx, grad)
+        return _backward(ctx, grad)
+
+
+def _backward(ctx, grad):
+    below, seed, offset = ctx.draw
+    more, = ctx.saved_tensors
+    grad_x = None
+    if ctx.needs_input_grad[0]:
+        grad_x = kernels.dropout(_whole_rows(grad), None, below, seed, offset, more)
+    return grad_x, grad if ctx.needs_input_grad[1] else None, None, None, None, None
+
+
+_backward_once = once_differentiable(_backward)
 
 
 @torch.compiler.disable
@@ -56,14 +65,9 @@ def dropout_add(x: Tensor, residual: Tensor | None, p: float, seed: int, offset=
     layer and step.  ``seed`` and ``offset``: integers modulo 2^64; ``offset`` may be
     a one-element INT64 tensor on the device, which a captured step can advance.
     Differentiable in both; the mask is drawn again in backward."""
-    if not isinstance(x, Tensor):
-        raise TypeError("x must be a torch.Tensor")
-    _check_tensor(x, "x", x.ndim, _TYPES)
+    _check_tensor(x, "x", x.ndim if isinstance(x, Tensor) else 0, _TYPES)
     if residual is not None:
-        if not isinstance(residual, Tensor):
-            raise TypeError("residual must be a torch.Tensor")
-        _check_tensor(residual, "residual", residual.ndim, _TYPES)
-        _check_like(residual, "residual", x, "x")
+        _check_like(residual, "residual", x, x.ndim)
         if residual.shape != x.shape:
             raise ValueError(f"x has shape {tuple(x.shape)}, residual {tuple(residual.shape)}")
     if not (math.isfinite(p) and 0 <= p <= 1):
@@ -80,4 +84,8 @@ def dropout_add(x: Tensor, residual: Tensor | None, p: float, seed: int, offset=
         raise ValueError("at most 2^35 - 2048 values")
     if x.numel() == 0:
         return x.clone() if residual is None else x + residual
-    return _DropoutAdd.apply(x, residual, round(p * 65536), seed, offset, more)
+    below = round(p * 65536)
+    if _recorded(x, residual):
+        return _DropoutAdd.apply(x, residual, below, seed, offset, more)
+    return kernels.dropout(_whole_rows(x), None if residual is None else _whole_rows(residual),
+                           below, seed, offset, more)

@@ -10,7 +10,7 @@ allocated on the current stream, and the work is shared out.
 """
 from __future__ import annotations
 
-import contextlib
+from functools import lru_cache
 
 import torch
 from torch import Tensor
@@ -23,58 +23,64 @@ MAX_TOKENS = 1 << 30
 
 _QUERY_TILE, _KEY_TILE = 128, 64
 _DECODE_TILE = 4 * 32    # keys that a workgroup's waves take at a time
-_MAX_SPLITS = 64
+_MAX_SPLITS = 64        # LCT_MAX_ATTENTION_SPLITS
+_MAX_PARTS = 8          # of dk and dv: FP32 copies of both in the workspace
 _CUS = 256
 
 TYPES = {torch.bfloat16: hip.BF16, torch.float16: hip.FP16, torch.float32: hip.FP32}
 
 
-def on_device(tensor: Tensor):
-    """The tensor's device as the current one, for the launch."""
-    if tensor.get_device() == torch._C._cuda_getDevice():
-        return contextlib.nullcontext()
-    return torch.cuda.device(tensor.device)
-
-
-def _stream(tensor: Tensor) -> int:
-    return torch._C._cuda_getCurrentRawStream(tensor.get_device())
-
-
-def _strides(t: Tensor) -> tuple:
-    """Strides of all dimensions but the last; 0 where there is one element."""
-    return tuple([0 if n == 1 else s for n, s in zip(t.shape[:-1], t.stride())])
+def _launch(name: str, device: int, *args) -> None:
+    """An entry point on ``device``'s current stream."""
+    if device == torch._C._cuda_getDevice():
+        hip.call(name, *args, torch._C._cuda_getCurrentRawStream(device))
+    else:
+        with torch.cuda.device(device):
+            hip.call(name, *args, torch._C._cuda_getCurrentRawStream(device))
 
 
 def _readable(t: Tensor) -> Tensor:
-    """``t``, or a copy with strides and alignment that the attention kernels
-    read: [batch, head, token, channel], 16-byte rows."""
-    b, h, n = _strides(t)
-    if (t.stride(3) != 1 and t.shape[3] != 1 or t.data_ptr() & 15 or (b | h | n) & 7
-            or n >= 1 << 24):
-        return t.clone(memory_format=torch.contiguous_format)
-    return t
+    """``t``, or a copy, of four dimensions with strides and alignment that the
+    attention kernels read: rows of 16-byte pieces, tokens in dimension 2."""
+    b, h, n, c = t.stride()
+    if c == 1 and not (b | h | n) & 7 and n < 1 << 24 and not t.data_ptr() & 15:
+        return t
+    # Dimensions of one element have any stride: only 0 is sure to be in range.
+    size = t.shape
+    b, h, n = b * (size[0] > 1), h * (size[1] > 1), n * (size[2] > 1)
+    if (c == 1 or size[3] == 1) and not (b | h | n) & 7 and n < 1 << 24 and not t.data_ptr() & 15:
+        return t.as_strided(size, (b, h, n, 1))
+    return t.clone(memory_format=torch.contiguous_format)
 
 
-def _btHD(like: Tensor) -> Tensor:
+def _token_major(like: Tensor) -> Tensor:
     """A new [batch, head, token, channel] tensor in token-major storage."""
     b, h, t, d = like.shape
-    return torch.empty((b, t, h, d), dtype=like.dtype, device=like.device).transpose(1, 2)
+    return like.new_empty_strided((b, h, t, d), (t * h * d, d, h * d, 1))
 
 
 def _record(q, k, v, out, lse, lengths, window, sinks, scale) -> bytes:
     batch, heads, queries, dim = q.shape
+    _, kv_heads, keys, _ = k.shape
     return hip.ATTENTION.pack(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
         0 if lse is None else lse.data_ptr(), 0 if lengths is None else lengths.data_ptr(),
-        *_strides(q), *_strides(k), *_strides(v), *_strides(out), batch, heads, k.shape[1],
-        queries, k.shape[2], dim, window, sinks, q.dtype == torch.float16, scale)
+        *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], batch, heads,
+        kv_heads, queries, keys, dim, window, sinks, q.dtype == torch.float16, scale)
 
 
 def _lse(q: Tensor) -> Tensor:
     """A value per query and head, in whole query tiles."""
     tiles = -(-q.shape[2] // _QUERY_TILE)
-    return torch.empty(q.shape[0] * q.shape[1] * tiles * _QUERY_TILE, dtype=torch.float32,
-                       device=q.device)
+    return q.new_empty(q.shape[0] * q.shape[1] * tiles * _QUERY_TILE, dtype=torch.float32)
+
+
+def _workspace(q: Tensor, floats: int):
+    """FP32 working memory and its address, None for none."""
+    if not floats:
+        return None, None
+    workspace = q.new_empty(floats, dtype=torch.float32)
+    return workspace, workspace.data_ptr()
 
 
 def _seen(keys: int, window: int, sinks: int, rows: int) -> int:
@@ -82,6 +88,7 @@ def _seen(keys: int, window: int, sinks: int, rows: int) -> int:
     return keys if window == 0 else min(keys, window + rows - 1 + sinks)
 
 
+@lru_cache(maxsize=1024)
 def forward_splits(batch: int, heads: int, queries: int, keys: int, window: int,
                    sinks: int) -> int:
     """Workgroups that share a query tile's keys: as many as fill the compute
@@ -98,15 +105,13 @@ def attention_forward(q: Tensor, k: Tensor, v: Tensor, window: int, sinks: int, 
     """``(out, lse)``; ``lse`` is what :func:`attention_backward` needs, or None."""
     q, k, v = _readable(q), _readable(k), _readable(v)
     batch, heads, queries, dim = q.shape
-    with on_device(q):
-        out = _btHD(q)
-        lse = _lse(q) if need_lse else None
-        splits = forward_splits(batch, heads, queries, k.shape[2], window, sinks)
-        floats = batch * heads * queries * splits * (dim + 2) if splits > 1 else 0
-        workspace = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
-        hip.call("lct_attention_forward",
-                 _record(q, k, v, out, lse, lengths, window, sinks, scale), splits,
-                 workspace.data_ptr() if floats else None, floats, _stream(q))
+    out = _token_major(q)
+    lse = _lse(q) if need_lse else None
+    splits = forward_splits(batch, heads, queries, k.shape[2], window, sinks)
+    floats = batch * heads * queries * splits * (dim + 2) if splits > 1 else 0
+    workspace, address = _workspace(q, floats)
+    _launch("lct_attention_forward", q.get_device(),
+            _record(q, k, v, out, lse, lengths, window, sinks, scale), splits, address, floats)
     return out, lse
 
 
@@ -115,6 +120,7 @@ def key_block(dim: int) -> int:
     return 256 if dim > 64 else 128
 
 
+@lru_cache(maxsize=1024)
 def backward_splits(batch: int, heads: int, kv_heads: int, queries: int, keys: int, dim: int,
                     window: int, sinks: int) -> tuple:
     """Workgroups that share the queries of a key block without and with sinks.
@@ -131,7 +137,7 @@ def backward_splits(batch: int, heads: int, kv_heads: int, queries: int, keys: i
     steps = -(-min(queries, keys if window == 0 else window + per_block) // 64) * group
     items = batch * kv_heads * blocks
     best = None
-    for splits in range(1, min(_MAX_SPLITS, max(1, steps // 4)) + 1):
+    for splits in range(1, min(_MAX_PARTS, max(1, steps // 4)) + 1):
         part = -(-steps // splits)
         if window == 0:
             time = items * steps / 2 / slots + part
@@ -153,29 +159,27 @@ def attention_backward(grad: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tenso
     q, k, v, out, grad = (_readable(t) for t in (q, k, v, out, grad))
     batch, heads, queries, dim = q.shape
     kv_heads, keys = k.shape[1], k.shape[2]
-    with on_device(q):
-        dq, dk, dv = _btHD(q), _btHD(k), _btHD(v)
-        delta = _lse(q)
-        splits, sink_splits = backward_splits(batch, heads, kv_heads, queries, keys, dim, window,
-                                              sinks)
-        per_block = key_block(dim)
-        blocks = -(-keys // per_block)
-        sink_blocks = -(-min(sinks, keys) // per_block) if window else 0
-        parts = sink_blocks * sink_splits + (blocks - sink_blocks) * splits
-        floats = (batch * kv_heads * parts * 2 * per_block * dim
-                  if splits > 1 or (sink_splits > 1 and sink_blocks) else 0)
-        workspace = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
-        hip.call("lct_attention_backward",
-                 _record(q, k, v, out, lse, lengths, window, sinks, scale),
-                 hip.ATTENTION_GRADIENTS.pack(
-                     grad.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                     delta.data_ptr(), *_strides(grad), *_strides(dq), *_strides(dk),
-                     *_strides(dv)),
-                 splits, sink_splits, workspace.data_ptr() if floats else None, floats,
-                 _stream(q))
+    dq, dk, dv = _token_major(q), _token_major(k), _token_major(v)
+    delta = _lse(q)
+    splits, sink_splits = backward_splits(batch, heads, kv_heads, queries, keys, dim, window,
+                                          sinks)
+    per_block = key_block(dim)
+    blocks = -(-keys // per_block)
+    sink_blocks = -(-min(sinks, keys) // per_block) if window else 0
+    parts = sink_blocks * sink_splits + (blocks - sink_blocks) * splits
+    floats = (batch * kv_heads * parts * 2 * per_block * dim
+              if splits > 1 or (sink_splits > 1 and sink_blocks) else 0)
+    workspace, address = _workspace(q, floats)
+    _launch("lct_attention_backward", q.get_device(),
+            _record(q, k, v, out, lse, lengths, window, sinks, scale),
+            hip.ATTENTION_GRADIENTS.pack(
+                grad.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr(),
+                *grad.stride()[:3], *dq.stride()[:3], *dk.stride()[:3], *dv.stride()[:3]),
+            splits, sink_splits, address, floats)
     return dq, dk, dv
 
 
+@lru_cache(maxsize=1024)
 def decode_splits(batch: int, heads: int, kv_heads: int, capacity: int, window: int,
                   sinks: int) -> int:
     """Workgroups that share a sequence's keys: as many as fill the compute units
@@ -185,60 +189,79 @@ def decode_splits(batch: int, heads: int, kv_heads: int, capacity: int, window: 
     return max(1, min(_MAX_SPLITS, -(-2 * _CUS // items), tiles))
 
 
-def attention_decode(q: Tensor, k: Tensor, v: Tensor, window: int, sinks: int, scale: float,
-                     lengths) -> Tensor:
-    """[batch, heads, channel] of queries of that shape over
-    [batch, head, token, channel] caches."""
-    q, k, v = _readable(q.unsqueeze(2)), _readable(k), _readable(v)
-    batch, heads, _, dim = q.shape
-    with on_device(q):
-        out = torch.empty((batch, heads, 1, dim), dtype=q.dtype, device=q.device)
-        splits = decode_splits(batch, heads, k.shape[1], k.shape[2], window, sinks)
-        floats = batch * heads * splits * (dim + 2) if splits > 1 else 0
-        workspace = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
-        hip.call("lct_attention_decode",
-                 _record(q, k, v, out, None, lengths, window, sinks, scale), splits,
-                 workspace.data_ptr() if floats else None, floats, _stream(q))
-    return out.squeeze(2)
+def attention_decode(q: Tensor, k_cache: Tensor, v_cache: Tensor, window: int, sinks: int,
+                     scale: float, lengths) -> Tensor:
+    """[batch, head, channel] of queries of that shape over [batch, token, head,
+    channel] caches."""
+    if (q.stride(2) != 1 or (q.stride(0) | q.stride(1)) & 7 or q.data_ptr() & 15):
+        q = q.clone(memory_format=torch.contiguous_format)
+    k, v = (_readable(t.transpose(1, 2)) for t in (k_cache, v_cache))
+    batch, heads, dim = q.shape
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    _, kv_heads, capacity, _ = k.shape
+    splits = decode_splits(batch, heads, kv_heads, capacity, window, sinks)
+    floats = batch * heads * splits * (dim + 2) if splits > 1 else 0
+    workspace, address = _workspace(q, floats)
+    _launch("lct_attention_decode", q.get_device(), hip.ATTENTION.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0,
+        0 if lengths is None else lengths.data_ptr(), *q.stride()[:2], 0, *k.stride()[:3],
+        *v.stride()[:3], heads * dim, dim, 0, batch, heads, kv_heads, 1, capacity, dim, window,
+        sinks, q.dtype == torch.float16, scale), splits, address, floats)
+    return out
 
 
-def rotate(plan, q: Tensor, k, positions, start: int, inverse: bool, cache=None):
-    """The rotated ``(q, k)`` of [batch, token, head, channel] tensors (``k`` may
-    be None); with ``cache`` = (v, k_cache, v_cache) ``k`` and ``v`` go there."""
-    if q.stride(3) != 1 and q.shape[3] != 1:
+_NO_STRIDES = (0, 0, 0)
+
+
+def rotate(plan, q: Tensor, k, positions, start: int, inverse: bool):
+    """The rotated ``(q, k)`` of [batch, token, head, channel] tensors; ``k`` may be
+    None."""
+    if q.stride(3) != 1:
         q = q.contiguous()
-    if k is not None and k.stride(3) != 1 and k.shape[3] != 1:
-        k = k.contiguous()
     batch, tokens, heads, dim = q.shape
-    zeros = (0, 0, 0)
-    with on_device(q):
-        q_out = torch.empty((batch, tokens, heads, dim), dtype=q.dtype, device=q.device)
-        v = v_out = k_out = None
-        if cache is not None:
-            v, k_out, v_out = cache
-            if v.stride(3) != 1 and v.shape[3] != 1:
-                v = v.contiguous()
-        elif k is not None:
-            k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        given = [0 if t is None else t.data_ptr() for t in (q, k, v, q_out, k_out, v_out)]
-        strides = [s for t in (q, k, v, q_out, k_out, v_out)
-                   for s in (zeros if t is None else _strides(t))]
-        by_token = positions is not None and positions.ndim == 2
-        hip.call("lct_rotate", hip.ROTARY.pack(
-            *given, plan.turns.data_ptr(), 0 if positions is None else positions.data_ptr(),
-            *strides, 0 if positions is None else positions.stride(0),
-            positions.stride(1) if by_token else 0, start, batch, tokens, heads,
-            0 if k is None else k.shape[2], dim, plan.dim, plan.interleaved, inverse,
-            TYPES[q.dtype], k_out.shape[1] if cache is not None else 0, plan.magnitude),
-            _stream(q))
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if k is None:
+        k_out, k_in_at, k_out_at, kv_heads = None, 0, 0, 0
+        k_in_stride = k_out_stride = _NO_STRIDES
+    else:
+        if k.stride(3) != 1:
+            k = k.contiguous()
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+        k_in_at, k_out_at, kv_heads = k.data_ptr(), k_out.data_ptr(), k.shape[2]
+        k_in_stride, k_out_stride = k.stride()[:3], k_out.stride()[:3]
+    at = b = t = 0
+    if positions is not None:
+        at, b = positions.data_ptr(), positions.stride(0)
+        t = positions.stride(1) if positions.ndim == 2 else 0
+    _launch("lct_rotate", q.get_device(), hip.ROTARY.pack(
+        q.data_ptr(), k_in_at, 0, q_out.data_ptr(), k_out_at, 0, plan.turns.data_ptr(), at,
+        *q.stride()[:3], *k_in_stride, 0, 0, 0, *q_out.stride()[:3], *k_out_stride, 0, 0, 0, b, t,
+        start, batch, tokens, heads, kv_heads, dim, plan.dim, plan.interleaved, inverse,
+        TYPES[q.dtype], 0, plan.magnitude))
     return q_out, k_out
+
+
+def rotate_into(plan, q: Tensor, k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor,
+                positions: Tensor) -> Tensor:
+    """The rotated ``q`` [batch, head, channel]; ``k``, rotated, and ``v`` go to the
+    [batch, token, head, channel] caches at ``positions``."""
+    q, k, v = (t if t.stride(2) == 1 else t.contiguous() for t in (q, k, v))
+    batch, heads, dim = q.shape
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    (qb, qh, _), (kb, kh, _), (vb, vh, _) = q.stride(), k.stride(), v.stride()
+    _launch("lct_rotate", q.get_device(), hip.ROTARY.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), k_cache.data_ptr(),
+        v_cache.data_ptr(), plan.turns.data_ptr(), positions.data_ptr(), qb, 0, qh, kb, 0, kh, vb,
+        0, vh, heads * dim, 0, dim, *k_cache.stride()[:3], *v_cache.stride()[:3],
+        positions.stride(0), 0, 0, batch, 1, heads, k.shape[1], dim, plan.dim, plan.interleaved,
+        False, TYPES[q.dtype], k_cache.shape[1], plan.magnitude))
+    return out
 
 
 def dropout(x: Tensor, residual, below: int, seed: int, offset: int, more) -> Tensor:
     """``residual + dropout(x)`` of contiguous, 16-byte aligned tensors."""
-    with on_device(x):
-        out = torch.empty_like(x)
-        hip.call("lct_dropout", x.data_ptr(), None if residual is None else residual.data_ptr(),
-                 out.data_ptr(), x.numel(), TYPES[x.dtype], below, seed, offset,
-                 None if more is None else more.data_ptr(), _stream(x))
+    out = torch.empty_like(x)
+    _launch("lct_dropout", x.get_device(), x.data_ptr(),
+            None if residual is None else residual.data_ptr(), out.data_ptr(), x.numel(),
+            TYPES[x.dtype], below, seed, offset, None if more is None else more.data_ptr())
     return out
