@@ -875,8 +875,8 @@ int32_t lct_attention_decode(const lct_attention *a, int32_t splits, float *work
 /* ---- rotary positions (examples/nanogpt/train_gpt_lct.py:150-165): the first
  * rotary_dim (even) of head_dim <= LCT_MAX_ROTARY_DIM channels of q and, unless
  * k_in is NULL, k, [batch, token, head, channel] by strides in elements (batch,
- * token, head; channels adjacent), turn in pairs (i, i + rotary_dim / 2) or, if
- * interleaved, (2 i, 2 i + 1):
+ * token, head, the head's below 2^31; channels adjacent), turn in pairs (i, i +
+ * rotary_dim / 2) or, if interleaved, (2 i, 2 i + 1):
  *     (x, y) -> magnitude (x cos - y sin, y cos + x sin),
  * the angle being the position times turns[i] / 2^64 of a turn; `inverse` turns
  * the other way (the gradient).  The other channels are copied.  Token t of

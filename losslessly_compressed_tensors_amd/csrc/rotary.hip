@@ -66,15 +66,24 @@ __device__ __forceinline__ int64_t position_of(const lct_rotary &r, int64_t b, i
     return p;
 }
 
-template <int kType, int kVector>
+// Where a token's q, k and v are and go (elements; k's and v's place -1: nowhere).
+struct Places {
+    int64_t in[3], out[3];
+};
+
+// A workgroup takes a few tokens: it computes their angles' sines and cosines
+// once, into LDS, for all of their heads, then moves its units, kAhead of a
+// thread's in flight.
+template <int kType, int kVector, bool kInterleaved>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(lct_rotary r, Counts n) {
     using V = Value<kType>;
     using Bits = typename V::Bits;
     struct alignas(sizeof(Bits) * kVector) Pack {
         Bits v[kVector];
     };
+    constexpr int kAhead = 4;
     __shared__ f32x2 turn[kMaxTokens * kMaxPairs];
-    __shared__ int64_t place[kMaxTokens];
+    __shared__ Places places[kMaxTokens];
     const int64_t tokens = int64_t{r.batch} * r.tokens;
     const int64_t first = int64_t{blockIdx.x} * n.per_group;
     const int32_t here = static_cast<int32_t>(min(int64_t{n.per_group}, tokens - first));
@@ -88,72 +97,97 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(lct_rotary r, Counts n
         float sine, cosine;
         sincospif(static_cast<float>(angle) * 0x1p-63f, &sine, &cosine);
         turn[i] = f32x2{cosine * r.magnitude, (r.inverse ? -sine : sine) * r.magnitude};
-        if (pair == 0) place[token] = p;
+        if (pair != 0) continue;
+        Places &at = places[token];
+        at.in[0] = b * r.q_in_stride[0] + t * r.q_in_stride[1];
+        at.in[1] = b * r.k_in_stride[0] + t * r.k_in_stride[1];
+        at.in[2] = b * r.v_in_stride[0] + t * r.v_in_stride[1];
+        at.out[0] = b * r.q_out_stride[0] + t * r.q_out_stride[1];
+        const int64_t to = r.capacity > 0 ? p : t;
+        const bool kept = r.capacity == 0 || (p >= 0 && p < r.capacity);
+        at.out[1] = kept ? b * r.k_out_stride[0] + to * r.k_out_stride[1] : -1;
+        at.out[2] = kept ? b * r.v_out_stride[0] + to * r.v_out_stride[1] : -1;
     }
     __syncthreads();
 
-    for (int32_t i = threadIdx.x; i < here * n.per_token; i += kThreads) {
-        const int32_t token = divide(i, n.per_token_inverse);
-        const int32_t in_token = i - token * n.per_token;
-        int32_t head = divide(in_token, n.units_inverse);
-        const int32_t unit = in_token - head * n.units;
-        const int64_t b = (first + token) / r.tokens, t = (first + token) % r.tokens;
-        // q's heads, then k's, then v's.
-        const bool is_q = head < r.heads;
-        if (!is_q) head -= r.heads;
-        const bool is_k = !is_q && head < r.kv_heads;
-        if (!is_q && !is_k) head -= r.kv_heads;
-        const bool rotate = is_q || is_k;
-        int64_t out_token = t;
-        if (!is_q && r.capacity > 0) {
-            out_token = place[token];
-            if (out_token < 0 || out_token >= r.capacity) continue;
+    const int32_t items = here * n.per_token;
+    for (int32_t base = threadIdx.x; base < items; base += kAhead * kThreads) {
+        Pack x[kAhead], y[kAhead];
+        Bits *dst[kAhead];           // null: nothing to store
+        int32_t angles[kAhead];      // first of the unit's in `turn`, or -1: a copy
+        int32_t gap[kAhead];         // from x's channels to y's, or 0: no y
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            dst[u] = nullptr;
+            angles[u] = -1;
+            const int32_t i = base + u * kThreads;
+            if (i >= items) continue;
+            const int32_t token = divide(i, n.per_token_inverse);
+            const int32_t in_token = i - token * n.per_token;
+            int32_t head = divide(in_token, n.units_inverse);
+            const int32_t unit = in_token - head * n.units;
+            // q's heads, then k's, then v's.
+            const bool is_q = head < r.heads;
+            if (!is_q) head -= r.heads;
+            const bool is_k = !is_q && head < r.kv_heads;
+            if (!is_q && !is_k) head -= r.kv_heads;
+            const auto pick = [&](auto q, auto k, auto v) { return is_q ? q : is_k ? k : v; };
+            const int which = pick(0, 1, 2);
+            const int64_t to = places[token].out[which];
+            if (to < 0) continue;
+            const int32_t in_head = static_cast<int32_t>(
+                pick(r.q_in_stride[2], r.k_in_stride[2], r.v_in_stride[2]));
+            const int32_t out_head = static_cast<int32_t>(
+                pick(r.q_out_stride[2], r.k_out_stride[2], r.v_out_stride[2]));
+            int32_t c = unit * kVector;
+            gap[u] = 0;
+            if (unit >= n.pair_units) {              // channels past the rotated part
+                c = r.rotary_dim + (unit - n.pair_units) * kVector;
+            } else if (!kInterleaved) {
+                angles[u] = token * pairs + c;
+                gap[u] = pairs;
+            } else if (kVector > 1) {
+                angles[u] = token * pairs + c / 2;
+            } else {
+                c = 2 * unit;
+                angles[u] = token * pairs + unit;
+                gap[u] = 1;
+            }
+            if (which == 2) angles[u] = -1;
+            const Bits *src = static_cast<const Bits *>(pick(r.q_in, r.k_in, r.v_in))
+                              + places[token].in[which] + int64_t{head} * in_head + c;
+            dst[u] = static_cast<Bits *>(pick(r.q_out, r.k_out, r.v_out)) + to
+                     + int64_t{head} * out_head + c;
+            x[u] = *reinterpret_cast<const Pack *>(src);
+            if (gap[u] != 0) y[u] = *reinterpret_cast<const Pack *>(src + gap[u]);
         }
-        const auto pick = [&](auto q, auto k, auto v) { return is_q ? q : is_k ? k : v; };
-        const Bits *src = static_cast<const Bits *>(pick(r.q_in, r.k_in, r.v_in))
-                          + b * pick(r.q_in_stride[0], r.k_in_stride[0], r.v_in_stride[0])
-                          + t * pick(r.q_in_stride[1], r.k_in_stride[1], r.v_in_stride[1])
-                          + head * pick(r.q_in_stride[2], r.k_in_stride[2], r.v_in_stride[2]);
-        Bits *dst = static_cast<Bits *>(pick(r.q_out, r.k_out, r.v_out))
-                    + b * pick(r.q_out_stride[0], r.k_out_stride[0], r.v_out_stride[0])
-                    + out_token * pick(r.q_out_stride[1], r.k_out_stride[1], r.v_out_stride[1])
-                    + head * pick(r.q_out_stride[2], r.k_out_stride[2], r.v_out_stride[2]);
-        const f32x2 *angles = turn + token * pairs;
-        if (unit >= n.pair_units) {          // channels past the rotated part
-            const int32_t c = r.rotary_dim + (unit - n.pair_units) * kVector;
-            *reinterpret_cast<Pack *>(dst + c) = *reinterpret_cast<const Pack *>(src + c);
-        } else if (!r.interleaved) {
-            const int32_t c = unit * kVector;
-            Pack x = *reinterpret_cast<const Pack *>(src + c);
-            Pack y = *reinterpret_cast<const Pack *>(src + c + pairs);
 #pragma unroll
-            for (int j = 0; j < kVector; ++j) {
-                if (!rotate) continue;
-                const f32x2 a = angles[c + j];
-                const float u = V::load(x.v[j]), w = V::load(y.v[j]);
-                x.v[j] = V::store(u * a[0] - w * a[1]);
-                y.v[j] = V::store(w * a[0] + u * a[1]);
-            }
-            *reinterpret_cast<Pack *>(dst + c) = x;
-            *reinterpret_cast<Pack *>(dst + c + pairs) = y;
-        } else if constexpr (kVector > 1) {
-            const int32_t c = unit * kVector;
-            Pack x = *reinterpret_cast<const Pack *>(src + c);
+        for (int u = 0; u < kAhead; ++u) {
+            if (dst[u] == nullptr) continue;
+            if constexpr (kInterleaved && kVector > 1) {
+                if (angles[u] >= 0) {
 #pragma unroll
-            for (int j = 0; j < kVector; j += 2) {
-                if (!rotate) continue;
-                const f32x2 a = angles[(c + j) / 2];
-                const float u = V::load(x.v[j]), w = V::load(x.v[j + 1]);
-                x.v[j] = V::store(u * a[0] - w * a[1]);
-                x.v[j + 1] = V::store(w * a[0] + u * a[1]);
+                    for (int j = 0; j < kVector; j += 2) {
+                        const f32x2 a = turn[angles[u] + j / 2];
+                        const float v = V::load(x[u].v[j]), w = V::load(x[u].v[j + 1]);
+                        x[u].v[j] = V::store(v * a[0] - w * a[1]);
+                        x[u].v[j + 1] = V::store(w * a[0] + v * a[1]);
+                    }
+                }
+                *reinterpret_cast<Pack *>(dst[u]) = x[u];
+                continue;
             }
-            *reinterpret_cast<Pack *>(dst + c) = x;
-        } else {
-            const int32_t c = 2 * unit;
-            const Bits u = src[c], w = src[c + 1];
-            const f32x2 a = angles[unit];
-            dst[c] = rotate ? V::store(V::load(u) * a[0] - V::load(w) * a[1]) : u;
-            dst[c + 1] = rotate ? V::store(V::load(w) * a[0] + V::load(u) * a[1]) : w;
+            if (angles[u] >= 0) {
+#pragma unroll
+                for (int j = 0; j < kVector; ++j) {
+                    const f32x2 a = turn[angles[u] + j];
+                    const float v = V::load(x[u].v[j]), w = V::load(y[u].v[j]);
+                    x[u].v[j] = V::store(v * a[0] - w * a[1]);
+                    y[u].v[j] = V::store(w * a[0] + v * a[1]);
+                }
+            }
+            *reinterpret_cast<Pack *>(dst[u]) = x[u];
+            if (gap[u] != 0) *reinterpret_cast<Pack *>(dst[u] + gap[u]) = y[u];
         }
     }
 }
@@ -169,6 +203,10 @@ bool multiples(const int64_t (&stride)[3], int32_t of) {
     return stride[0] % of == 0 && stride[1] % of == 0 && stride[2] % of == 0;
 }
 
+bool heads_near(const int64_t (&stride)[3]) {
+    return stride[2] >= 0 && stride[2] <= INT32_MAX;
+}
+
 bool aligned_to(const void *p, uintptr_t bytes) {
     return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0;
 }
@@ -180,19 +218,35 @@ int32_t launch(const lct_rotary &r, hipStream_t stream) {
     n.pair_units = r.interleaved && kVector > 1 ? r.rotary_dim / kVector : pairs / kVector;
     n.units = n.pair_units + (r.head_dim - r.rotary_dim) / kVector;
     n.per_token = (r.heads + (r.k_in ? r.kv_heads : 0) + (r.v_in ? r.kv_heads : 0)) * n.units;
-    if (n.per_token >= kMaxItems) return LCT_E_SIZE;
+    if (n.per_token > kMaxItems) return LCT_E_SIZE;
     const int64_t tokens = int64_t{r.batch} * r.tokens;
-    // Enough tokens that a workgroup's threads take a few units each and share
-    // the angles, while there are workgroups for every compute unit.
-    int64_t per = std::min<int64_t>(kMaxTokens, std::max(1, 4 * kThreads / n.per_token));
-    per = std::min(per, std::max<int64_t>(1, tokens / 1024));
-    n.per_group = static_cast<int32_t>(std::min<int64_t>(per, kMaxItems / n.per_token));
+    // Whole rounds of the threads' units (to a tenth), while there are workgroups
+    // for every compute unit.
+    const int64_t most = std::min<int64_t>(
+        {kMaxTokens, kMaxItems / n.per_token, std::max<int64_t>(1, tokens / 1024)});
+    constexpr int64_t kRound = 4 * kThreads;
+    n.per_group = 1;
+    double best = 0.0;
+    for (int64_t per = 1; per <= most; ++per) {
+        const int64_t units = per * n.per_token;
+        const double used =
+            static_cast<double>(units) / static_cast<double>((units + kRound - 1) / kRound * kRound);
+        if (used > best + 1e-9) {
+            best = used;
+            n.per_group = static_cast<int32_t>(per);
+        }
+        if (best >= 0.9) break;
+    }
     n.units_inverse = inverse_of(n.units);
     n.per_token_inverse = inverse_of(n.per_token);
     const int64_t grid = (tokens + n.per_group - 1) / n.per_group;
     if (grid >= int64_t{1} << 24) return LCT_E_SIZE;
-    rotary_kernel<kType, kVector>
-        <<<static_cast<uint32_t>(grid), kThreads, 0, stream>>>(r, n);
+    if (r.interleaved)
+        rotary_kernel<kType, kVector, true>
+            <<<static_cast<uint32_t>(grid), kThreads, 0, stream>>>(r, n);
+    else
+        rotary_kernel<kType, kVector, false>
+            <<<static_cast<uint32_t>(grid), kThreads, 0, stream>>>(r, n);
     return static_cast<int32_t>(hipGetLastError());
 }
 
@@ -231,7 +285,10 @@ extern "C" int32_t lct_rotate(const lct_rotary *r, hipStream_t stream) {
     const uintptr_t size = r->type == LCT_FP32 ? 4 : 2;
     if (!aligned_to(r->q_in, size) || !aligned_to(r->q_out, size) || !aligned_to(r->k_in, size)
         || !aligned_to(r->k_out, size) || !aligned_to(r->v_in, size) || !aligned_to(r->v_out, size)
-        || (r->v_in && r->capacity <= 0))
+        || (r->v_in && r->capacity <= 0) || !heads_near(r->q_in_stride)
+        || !heads_near(r->k_in_stride) || !heads_near(r->v_in_stride)
+        || !heads_near(r->q_out_stride) || !heads_near(r->k_out_stride)
+        || !heads_near(r->v_out_stride))
         return LCT_E_ARG;
     switch (r->type) {
     case LCT_BF16: return by_vector<LCT_BF16>(*r, stream);
