@@ -206,45 +206,55 @@ __global__ __launch_bounds__(kAttentionThreads, 2) void attention_forward_kernel
 }
 
 // Joins the parts of a query's keys: sum of 2^(shift - largest) out, over the
-// same sum of the weights.  A wave per query, two channels per lane.
+// same sum of the weights.  A workgroup per query, two channels per lane, a
+// quarter of the parts per wave; lane s holds part s's shift and weight.
 template <bool kHalf>
 __global__ __launch_bounds__(kAttentionThreads) void attention_join_kernel(
     lct_attention a, int64_t pitch, int32_t splits, const float *__restrict__ parts) {
-    const int64_t item = int64_t{blockIdx.x} * kAttentionWaves + threadIdx.x / kWave;
-    if (item >= int64_t{a.batch} * a.heads * pitch) return;
+    static_assert(LCT_MAX_ATTENTION_SPLITS <= kWave, "a lane per part");
+    __shared__ f32x2 sums[kAttentionWaves][kWave];
+    const int64_t item = blockIdx.x;
     const int32_t bh = static_cast<int32_t>(item / pitch), row = static_cast<int32_t>(item % pitch);
+    const int lane = wave_lane(), wave = threadIdx.x / kWave;
     if (row >= a.queries) {
-        if (a.lse != nullptr && wave_lane() == 0) a.lse[item] = INFINITY;
+        if (threadIdx.x == 0) a.lse[item] = INFINITY;
         return;
     }
-    const int32_t width = a.head_dim + 2, channel = 2 * wave_lane();
+    const int32_t width = a.head_dim + 2, channel = 2 * lane;
     const float *part = parts + (int64_t{bh} * splits * a.queries + row) * width;
     const int64_t step = int64_t{a.queries} * width;
-    float largest = -INFINITY;
-    for (int32_t s = 0; s < splits; ++s) {
-        const f32x2 stats = *reinterpret_cast<const f32x2 *>(part + s * step + a.head_dim);
-        if (stats[1] != 0.0f) largest = fmaxf(largest, stats[0]);
-    }
-    float total = 0.0f, x = 0.0f, y = 0.0f;
-    for (int32_t s = 0; s < splits; ++s) {
-        const f32x2 stats = *reinterpret_cast<const f32x2 *>(part + s * step + a.head_dim);
-        if (stats[1] == 0.0f) continue;
-        const float weight = exp2_fast(stats[0] - largest);
-        total += weight * stats[1];
-        if (channel < a.head_dim) {
+    f32x2 stats = {0.0f, 0.0f};
+    if (lane < splits) stats = *reinterpret_cast<const f32x2 *>(part + lane * step + a.head_dim);
+    float largest = stats[1] != 0.0f ? stats[0] : -INFINITY;
+#pragma unroll
+    for (int d = kWave / 2; d > 0; d >>= 1) largest = fmaxf(largest, __shfl_xor(largest, d, kWave));
+    const float weight = stats[1] != 0.0f ? exp2_fast(stats[0] - largest) : 0.0f;
+    float total = weight * stats[1];
+#pragma unroll
+    for (int d = kWave / 2; d > 0; d >>= 1) total += __shfl_xor(total, d, kWave);
+    f32x2 sum = {0.0f, 0.0f};
+    if (channel < a.head_dim) {
+#pragma unroll 4
+        for (int32_t s = wave; s < splits; s += kAttentionWaves) {
+            const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), s));
             const f32x2 o = *reinterpret_cast<const f32x2 *>(part + s * step + channel);
-            x += weight * o[0];
-            y += weight * o[1];
+            // A part that saw nothing has no sums.
+            if (w != 0.0f) sum += w * o;
         }
     }
-    if (a.lse != nullptr && wave_lane() == 0)
+    sums[wave][lane] = sum;
+    __syncthreads();
+    if (wave != 0) return;
+    if (a.lse != nullptr && lane == 0)
         a.lse[item] = total == 0.0f ? INFINITY : largest + __log2f(total);
     if (channel >= a.head_dim) return;
+#pragma unroll
+    for (int w = 1; w < kAttentionWaves; ++w) sum += sums[w][lane];
     const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
     uint16_t *dst = static_cast<uint16_t *>(a.out) + (bh / a.heads) * a.out_stride[0]
                     + (bh % a.heads) * a.out_stride[1] + row * a.out_stride[2];
     *reinterpret_cast<uint32_t *>(dst + channel) =
-        Element<kHalf>::round_pair(x * inverse, y * inverse);
+        Element<kHalf>::round_pair(sum[0] * inverse, sum[1] * inverse);
 }
 
 // ---- backward
@@ -741,8 +751,7 @@ int32_t check_attention(const lct_attention *a) {
 int32_t join_parts(const lct_attention &a, int32_t splits, const float *parts,
                    hipStream_t stream) {
     const int64_t pitch = a.lse != nullptr ? lse_pitch(a.queries) : a.queries;
-    const int64_t rows = int64_t{a.batch} * a.heads * pitch;
-    const uint32_t grid = static_cast<uint32_t>((rows + kAttentionWaves - 1) / kAttentionWaves);
+    const uint32_t grid = static_cast<uint32_t>(int64_t{a.batch} * a.heads * pitch);
     if (a.fp16)
         attention_join_kernel<true>
             <<<grid, kAttentionThreads, 0, stream>>>(a, pitch, splits, parts);
@@ -818,7 +827,7 @@ extern "C" int32_t lct_attention_forward(const lct_attention *a, int32_t splits,
             < int64_t{a->batch} * a->heads)
             return LCT_E_SIZE;
         if ((reinterpret_cast<uintptr_t>(workspace) & 7) != 0) return LCT_E_ARG;
-        if (int64_t{a->batch} * a->heads * lse_pitch(a->queries) > kMaxAttentionItems * kAttentionWaves)
+        if (int64_t{a->batch} * a->heads * lse_pitch(a->queries) > kMaxAttentionItems)
             return LCT_E_SIZE;
     }
     return a->fp16 ? forward<true>(*a, splits, workspace, stream)

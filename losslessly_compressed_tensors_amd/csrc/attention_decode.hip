@@ -8,6 +8,9 @@
 // the wave's own LDS rows for the transposed read.  As in attention_core.h a
 // lane's scores are the next product's operand: lane l holds keys 4 (l >> 4) + i
 // and 16 more of query l & 15, and the values are read in that order.
+#include <algorithm>
+#include <type_traits>
+
 #include "attention_core.h"
 
 namespace lct {
@@ -17,6 +20,13 @@ constexpr int kDecodeKeys = 32;      // keys per tile
 constexpr int kQueries = 16;         // query heads per workgroup
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescale = 8.0f;
+
+// Keys and values of more bytes than half the memory side's cache (256 MiB) are
+// read past it: 263 us in place of 292 for 4 sequences of up to 131072 keys, 188
+// for 192 at 64 of 4100 (1.7 and 1.1 GB); 6.3 for 6.0 at one of 257, which
+// stays in it.
+constexpr int kStreaming = 2;
+constexpr int64_t kCacheBytes = int64_t{128} << 20;
 
 template <bool kHalf>
 __device__ __forceinline__ f32x4 multiply16(u32x4 a, u32x4 b, f32x4 c) {
@@ -40,7 +50,7 @@ __device__ __forceinline__ float quarters_sum(float v) {
     return across_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
-template <bool kHalf, int kDim, bool kSplit>
+template <bool kHalf, int kDim, bool kSplit, int kCache>
 __global__ __launch_bounds__(kAttentionThreads, 2) void attention_decode_kernel(
     lct_attention a, int32_t splits, float *__restrict__ parts) {
     constexpr int kPitch = kPitchOf<kDim>;
@@ -87,30 +97,48 @@ __global__ __launch_bounds__(kAttentionThreads, 2) void attention_decode_kernel(
     struct Tile {
         u32x4 k[2][kSteps], v[kValueLoads];
     };
-    // Keys and values that the query does not see are zeros.
+    // This lane's places in a tile; past the head's width, one that the range
+    // check rejects.  So are keys past the sequence: both load zeros.
+    uint32_t k_place[2][kSteps], v_place[kValueLoads];
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const int32_t channel = 32 * s + 8 * quarter;
+            k_place[n][s] = channel < a.head_dim ? static_cast<uint32_t>(
+                                (16 * n + column) * a.k_stride[2] + channel) * 2u
+                                                 : kOutOfRange;
+        }
+#pragma unroll
+    for (int i = 0; i < kValueLoads; ++i) {
+        const int slot = i * kWave + lane, channel = slot % kChunks * 8;
+        v_place[i] = channel < a.head_dim ? static_cast<uint32_t>(
+                         slot / kChunks * a.v_stride[2] + channel) * 2u
+                                          : kOutOfRange;
+    }
     const auto load = [&](int32_t t, Tile &tile) __attribute__((always_inline)) {
         const int32_t first = all.first_key(t, kDecodeKeys);
+        const int32_t rows = min(length - first, kDecodeKeys) - 1;
+        // Past the last tile nothing is in range.  The loads are issued all the
+        // same, so that the wait for the tile before leaves them in flight.
+        const auto records = [&](int64_t stride) {
+            return t < end ? static_cast<uint32_t>(rows * stride + a.head_dim) * 2u : 0u;
+        };
+        const __amdgpu_buffer_rsrc_t k_rows =
+            make_rsrc(k + first * a.k_stride[2], records(a.k_stride[2]));
+        const __amdgpu_buffer_rsrc_t v_rows =
+            make_rsrc(v + first * a.v_stride[2], records(a.v_stride[2]));
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            const int32_t key = first + 16 * n + column;
-            const bool seen = sight(key);
+        for (int n = 0; n < 2; ++n)
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
-                const int32_t channel = 32 * s + 8 * quarter;
-                tile.k[n][s] = u32x4{0u, 0u, 0u, 0u};
-                if (seen && channel < a.head_dim)
-                    tile.k[n][s] =
-                        *reinterpret_cast<const u32x4 *>(k + key * a.k_stride[2] + channel);
-            }
-        }
+            for (int s = 0; s < kSteps; ++s)
+                tile.k[n][s] = __builtin_bit_cast(
+                    u32x4, __builtin_amdgcn_raw_buffer_load_b128(k_rows, k_place[n][s], 0,
+                                                                 kCache));
 #pragma unroll
-        for (int i = 0; i < kValueLoads; ++i) {
-            const int slot = i * kWave + lane;
-            const int32_t key = first + slot / kChunks, channel = slot % kChunks * 8;
-            tile.v[i] = u32x4{0u, 0u, 0u, 0u};
-            if (channel < a.head_dim && sight(key))
-                tile.v[i] = *reinterpret_cast<const u32x4 *>(v + key * a.v_stride[2] + channel);
-        }
+        for (int i = 0; i < kValueLoads; ++i)
+            tile.v[i] = __builtin_bit_cast(
+                u32x4, __builtin_amdgcn_raw_buffer_load_b128(v_rows, v_place[i], 0, kCache));
     };
 
     const float factor = a.scale * kLog2e;
@@ -120,8 +148,17 @@ __global__ __launch_bounds__(kAttentionThreads, 2) void attention_decode_kernel(
     for (int c = 0; c < kColumns; ++c) out[c] = f32x4{};
     float most = -INFINITY, shifted = 0.0f, total = 0.0f;
 
-    const auto step = [&](int32_t t, const Tile &tile) __attribute__((always_inline)) {
+    const auto step = [&](int32_t t, Tile &tile) __attribute__((always_inline)) {
         const int32_t first = all.first_key(t, kDecodeKeys);
+        const bool seen_by_all = first + kDecodeKeys <= length
+                                 && (first >= sight.low || first + kDecodeKeys <= sight.sinks);
+        // What the query does not see may be anything: its values become zeros.
+        if (!seen_by_all) {
+#pragma unroll
+            for (int i = 0; i < kValueLoads; ++i)
+                if (!sight(first + (i * kWave + lane) / kChunks))
+                    tile.v[i] = u32x4{0u, 0u, 0u, 0u};
+        }
 #pragma unroll
         for (int i = 0; i < kValueLoads; ++i) {
             const int slot = i * kWave + lane;
@@ -135,9 +172,13 @@ __global__ __launch_bounds__(kAttentionThreads, 2) void attention_decode_kernel(
 #pragma unroll
             for (int d = 0; d < kSteps; ++d)
                 s[n] = multiply16<kHalf>(tile.k[n][d], q_operand[d], s[n]);
+        }
+        if (!seen_by_all) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                s[n][i] = sight(first + 16 * n + 4 * quarter + i) ? s[n][i] : -INFINITY;
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    s[n][i] = sight(first + 16 * n + 4 * quarter + i) ? s[n][i] : -INFINITY;
         }
         float top = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
@@ -181,15 +222,16 @@ __global__ __launch_bounds__(kAttentionThreads, 2) void attention_decode_kernel(
         }
     };
 
+    // The wave's own LDS rows: its operations on them run in order.
+    Tile even, odd;
     int32_t t = begin + wave;
-    Tile next;
-    if (t < end) load(t, next);
-    for (; t < end; t += kAttentionWaves) {
-        const Tile tile = next;
-        if (t + kAttentionWaves < end) load(t + kAttentionWaves, next);
-        step(t, tile);
-        // The wave's own rows: its LDS operations run in order.
-        __builtin_amdgcn_wave_barrier();
+    load(t, even);
+    for (; t < end; t += 2 * kAttentionWaves) {
+        load(t + kAttentionWaves, odd);
+        step(t, even);
+        if (t + kAttentionWaves >= end) break;
+        load(t + 2 * kAttentionWaves, even);
+        step(t + kAttentionWaves, odd);
     }
     total = quarters_sum(total);
 
@@ -242,14 +284,22 @@ template <bool kHalf>
 int32_t decode(const lct_attention &a, int32_t splits, float *workspace, hipStream_t stream) {
     const int64_t chunks = (a.heads / a.kv_heads + kQueries - 1) / kQueries;
     const uint32_t grid = static_cast<uint32_t>(chunks * a.kv_heads * a.batch * splits);
+    const auto launch = [&](auto width, auto split, auto cache) {
+        attention_decode_kernel<kHalf, decltype(width)::value, decltype(split)::value,
+                                decltype(cache)::value>
+            <<<grid, kAttentionThreads, 0, stream>>>(a, splits, workspace);
+    };
+    const int64_t seen = a.window > 0 ? std::min<int64_t>(a.keys, int64_t{a.window} + a.sinks) : a.keys;
+    const bool stream_once = 4 * seen * a.batch * a.kv_heads * a.head_dim > kCacheBytes;
     by_width(a.head_dim, [&](auto width) {
-        constexpr int kDim = decltype(width)::value;
-        if (splits > 1)
-            attention_decode_kernel<kHalf, kDim, true>
-                <<<grid, kAttentionThreads, 0, stream>>>(a, splits, workspace);
+        if (splits > 1 && stream_once)
+            launch(width, std::true_type{}, std::integral_constant<int, kStreaming>{});
+        else if (splits > 1)
+            launch(width, std::true_type{}, std::integral_constant<int, 0>{});
+        else if (stream_once)
+            launch(width, std::false_type{}, std::integral_constant<int, kStreaming>{});
         else
-            attention_decode_kernel<kHalf, kDim, false>
-                <<<grid, kAttentionThreads, 0, stream>>>(a, splits, workspace);
+            launch(width, std::false_type{}, std::integral_constant<int, 0>{});
     });
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess || splits == 1) return static_cast<int32_t>(err);

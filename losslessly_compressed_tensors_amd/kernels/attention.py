@@ -182,11 +182,18 @@ def attention_backward(grad: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tenso
 @lru_cache(maxsize=1024)
 def decode_splits(batch: int, heads: int, kv_heads: int, capacity: int, window: int,
                   sinks: int) -> int:
-    """Workgroups that share a sequence's keys: as many as fill the compute units
-    twice, with one tile per wave each at least."""
+    """Workgroups that share a sequence's keys.  Up to 1024 keys one is as fast as
+    several with the launch that joins their parts (us at 12 heads: 5.1 | 7.1 at
+    257 keys, 7.6 | 7.4 at 1024, two and four parts); above, three workgroups per
+    compute unit (8 heads of 8192 keys: 73 in one part, 20 in 6, 13.4 in 24, 16 in
+    64; 128 of 4096: 75, 40 in 6, 43 in 8, 59 in 32), with 256 keys each at least,
+    and of long caches parts of 3072 keys at most, so that sequences of unequal
+    length even out (32 heads of 131072: 316 in 16 parts, 275 in 64)."""
     items = batch * kv_heads * -(-(heads // kv_heads) // 16)
     tiles = -(-_seen(capacity, window, sinks, 1) // _DECODE_TILE)
-    return max(1, min(_MAX_SPLITS, -(-2 * _CUS // items), tiles))
+    if tiles <= 8:
+        return 1
+    return max(1, min(_MAX_SPLITS, tiles // 2, max(3 * _CUS // items, tiles // 24)))
 
 
 def attention_decode(q: Tensor, k_cache: Tensor, v_cache: Tensor, window: int, sinks: int,
