@@ -14,7 +14,11 @@ FineWeb shards, no network); the dense regions run eagerly, without a
 tracing compiler; one step is one microbatch of ``batch`` sequences.
 
 ``python examples/nanogpt/train_gpt_lct.py --mode both`` prints, per mode,
-tokens per second and peak device memory of the training step.
+tokens per second and peak device memory of the training step.  With ``--window``
+the blocks' rotary embedding and attention are the kernels of
+``components/attention.py`` (a sliding window with ``--sinks`` first tokens that
+stay visible), and with ``--dropout`` each residual addition drops what it adds
+(``components/dropout.py``); the reference has neither.
 """
 from __future__ import annotations
 
@@ -34,8 +38,13 @@ from torch.utils.checkpoint import checkpoint
 
 from losslessly_compressed_tensors_amd.comp_format import Distribution, DistType, NoiseLevel
 from losslessly_compressed_tensors_amd.LCTensor import LCTTensor
+from losslessly_compressed_tensors_amd.components.attention import Rotary as RotaryPlan
+from losslessly_compressed_tensors_amd.components.attention import (
+    apply_rotary, trainer_frequencies,
+)
+from losslessly_compressed_tensors_amd.components.dropout import dropout_add
 from losslessly_compressed_tensors_amd.components.layers import (
-    Embedding, FlashAttention, Linear, RMSLinear, RMSNormFunction, Relu2Linear,
+    Embedding, FlashAttention, Linear, RMSLinear, RMSNormFunction, Relu2Linear, WindowAttention,
     compress_weight, dense_weight, flush_saved, named_trainable_tensors, prefetch_saved,
     prefetch_weights, queued_saved, rms_norm_qkv,
 )
@@ -163,7 +172,7 @@ class Rotary(nn.Module):
 
 class CausalSelfAttention(nn.Module):
     def __init__(self, dim: int, head_dim=HEAD_DIM, compress_activations=False,
-                 min_compress_elements=MIN_COMPRESS_ELEMENTS):
+                 min_compress_elements=MIN_COMPRESS_ELEMENTS, window=None, sinks=0):
         super().__init__()
         if dim % head_dim:
             raise ValueError("model_dim must be divisible by head_dim")
@@ -175,6 +184,13 @@ class CausalSelfAttention(nn.Module):
         self.q, self.k, self.v = Linear(dim, hdim), Linear(dim, hdim), Linear(dim, hdim)
         self.proj = Linear(hdim, dim)
         self.rotary = Rotary(head_dim)
+        self.window, self.sinks = window, sinks
+        self.rotary_plan = None      # made where the first tokens are
+
+    def plan(self, device) -> RotaryPlan:
+        if self.rotary_plan is None or self.rotary_plan.turns.device != device:
+            self.rotary_plan = RotaryPlan(trainer_frequencies(self.head_dim), device=device)
+        return self.rotary_plan
 
     def forward(self, x: Tensor, norm_weight: Tensor):
         B, T = x.size(0), x.size(1)
@@ -185,6 +201,13 @@ class CausalSelfAttention(nn.Module):
         shape = (B, T, self.num_heads, self.head_dim)
         q, k, v = q.view(shape), k.view(shape), v.view(shape)
         norm_args = (None, self.tensor_buffer, compressed, act_dist, self.min_compress_elements)
+        if self.window is not None:
+            q, k = apply_rotary(self.plan(x.device), RMSNormFunction.apply(q, *norm_args),
+                                RMSNormFunction.apply(k, *norm_args))
+            return WindowAttention.apply(
+                q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), self.proj.weight,
+                self.proj.bias, self.tensor_buffer, compressed, act_dist,
+                self.min_compress_elements, self.window, self.sinks)
         q = self.rotary(RMSNormFunction.apply(q, *norm_args))
         k = self.rotary(RMSNormFunction.apply(k, *norm_args))
         return FlashAttention.apply(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2),
@@ -211,9 +234,11 @@ class MLP(nn.Module):
 
 class Block(nn.Module):
     def __init__(self, dim: int, head_dim=HEAD_DIM, compress_activations=False,
-                 min_compress_elements=MIN_COMPRESS_ELEMENTS):
+                 min_compress_elements=MIN_COMPRESS_ELEMENTS, window=None, sinks=0, dropout=0.0):
         super().__init__()
-        self.attn = CausalSelfAttention(dim, head_dim, compress_activations, min_compress_elements)
+        self.attn = CausalSelfAttention(dim, head_dim, compress_activations, min_compress_elements,
+                                        window, sinks)
+        self.dropout = dropout
         self.mlp = MLP(dim, compress_activations, min_compress_elements)
         self.norm1, self.norm2 = RMSNorm(dim), RMSNorm(dim)
 
@@ -222,7 +247,13 @@ class Block(nn.Module):
         return [attn.q.weight, attn.k.weight, attn.v.weight, attn.proj.weight, mlp.fc.weight,
                 mlp.proj.weight]
 
-    def forward(self, x: Tensor):
+    def add(self, x: Tensor, part: Tensor, seed: int, offset: int) -> Tensor:
+        """The residual's addition; dropped values are drawn from (seed, offset)."""
+        if self.dropout and self.training and torch.is_grad_enabled():
+            return dropout_add(part, x, self.dropout, seed, offset)
+        return x + part
+
+    def forward(self, x: Tensor, seed: int = 0, offset: int = 0):
         # The block's compressed weights are decoded together, once before its
         # forward and once when its backward starts (the hook on its output),
         # instead of one decode launch per use.
@@ -234,11 +265,11 @@ class Block(nn.Module):
         prefetch_weights(weights)
         a = self.attn(x, self.norm1.gains)
         saved_attn = queued_saved()
-        x = x + a
+        x = self.add(x, a, seed, offset)
         m = self.mlp(x, self.norm2.gains)
         attn_ids = {id(s) for s in saved_attn}
         saved_mlp = [s for s in flush_saved() if id(s) not in attn_ids]
-        out = x + m
+        out = self.add(x, m, seed, offset + 1)
         if out.requires_grad:
             if any(isinstance(w, LCTTensor) for w in weights):
                 out.register_hook(lambda grad: prefetch_weights(self.weights()))
@@ -252,11 +283,15 @@ class Block(nn.Module):
 class GPT(nn.Module):
     def __init__(self, vocab_size=VOCAB_SIZE, num_layers=NUM_LAYERS, model_dim=MODEL_DIM,
                  head_dim=HEAD_DIM, compress_activations=False,
-                 min_compress_elements=MIN_COMPRESS_ELEMENTS):
+                 min_compress_elements=MIN_COMPRESS_ELEMENTS, window=None, sinks=0, dropout=0.0,
+                 dropout_seed=0):
         super().__init__()
         self.embed = nn.Embedding(vocab_size, model_dim, dtype=torch.bfloat16)
         self.blocks = nn.ModuleList([Block(model_dim, head_dim, compress_activations,
-                                           min_compress_elements) for _ in range(num_layers)])
+                                           min_compress_elements, window, sinks, dropout)
+                                     for _ in range(num_layers)])
+        # Each step and addition draws its own mask: the offset counts them.
+        self.dropout_seed, self.dropout_offset = dropout_seed, 0
         self.compress_activations = compress_activations
         self.min_compress_elements = min_compress_elements
         self.proj = Linear(model_dim, vocab_size)
@@ -286,7 +321,8 @@ class GPT(nn.Module):
                                   self.tensor_buffer, compressed, act_dist,
                                   self.min_compress_elements)
         for block in self.blocks:
-            x = block(x)
+            x = block(x, self.dropout_seed, self.dropout_offset)
+            self.dropout_offset += 2
         return SoftcapCrossEntropy.head_loss(x, targets, self.proj.weight, self.norm2.gains,
                                              self.proj.bias, self.tensor_buffer,
                                              self.compress_activations, self.min_compress_elements)
@@ -333,11 +369,13 @@ def make_optimizers(model, compressed=False):
 
 def build(device, *, compress_weights, compress_activations, compress_optimizer,
           use_buffer=True, vocab_size=VOCAB_SIZE, num_layers=NUM_LAYERS, model_dim=MODEL_DIM,
-          head_dim=HEAD_DIM, buffer_mib=BUFFER_SIZE_MIB, seed=0):
+          head_dim=HEAD_DIM, buffer_mib=BUFFER_SIZE_MIB, seed=0, window=None, sinks=0,
+          dropout=0.0):
     """Model and optimizers for one mode, initialised from ``seed``."""
     torch.manual_seed(seed)
     model = GPT(vocab_size, num_layers, model_dim, head_dim,
-                compress_activations=compress_activations).to(device)
+                compress_activations=compress_activations, window=window, sinks=sinks,
+                dropout=dropout, dropout_seed=seed).to(device)
     initialize_model(model)
     if use_buffer and (compress_weights or compress_activations or compress_optimizer):
         model.set_tensor_buffer(TensorBuffer(buffer_mib * 2 ** 20, device=device))
@@ -421,6 +459,11 @@ def main():
     parser.add_argument("--warmup", type=int, default=3)
     parser.add_argument("--batch", type=int, default=BATCH)
     parser.add_argument("--layers", type=int, default=NUM_LAYERS)
+    parser.add_argument("--window", type=int, default=None,
+                        help="keys that a query sees up to its own (default: all)")
+    parser.add_argument("--sinks", type=int, default=0,
+                        help="first tokens that stay visible under a window")
+    parser.add_argument("--dropout", type=float, default=0.0)
     args = parser.parse_args()
     if not torch.cuda.is_available():
         raise RuntimeError("training needs a GPU")
@@ -429,7 +472,8 @@ def main():
     modes = ("dense", "lct") if args.mode == "both" else (args.mode,)
     for mode in modes:
         result = measure(device, compressed=mode == "lct", steps=args.steps, warmup=args.warmup,
-                         batch=args.batch, num_layers=args.layers)
+                         batch=args.batch, num_layers=args.layers, window=args.window,
+                         sinks=args.sinks, dropout=args.dropout)
         print(json.dumps({"mode": mode, **result}), flush=True)
 
 

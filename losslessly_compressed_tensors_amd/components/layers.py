@@ -23,14 +23,16 @@ from torch import Tensor, nn
 
 from ..LCTensor import LCTTensor
 from ..codec.decode import decode_batch
+from ..kernels import attention as attention_kernels
 from ..kernels import fused
 from ..operations import compress, compress_batch, decompress
+from .attention import check_attention
 from .dist_configs import act_dist, act_relu_dist, weight_dist
 from .ops import rms_norm, rms_norm_backward
 
 __all__ = [
     "dense_weight", "prefetch_weights", "RMSLinear", "rms_norm_qkv", "RMSNormFunction",
-    "Relu2Linear", "FlashAttention", "compress_weight", "Linear", "Embedding",
+    "Relu2Linear", "FlashAttention", "WindowAttention", "compress_weight", "Linear", "Embedding",
     "named_trainable_tensors", "flush_saved", "queued_saved", "prefetch_saved",
     "batch_saved_compression",
 ]
@@ -383,6 +385,42 @@ class FlashAttention(torch.autograd.Function):
             0.0, True, seed, offset, scale=ATTENTION_SCALE)
         ctx.state = ctx.auxiliary = ctx.weight = None
         return dq, dk, dv, grad_weight, grad_bias, None, None, None, None
+
+
+class WindowAttention(torch.autograd.Function):
+    """:class:`FlashAttention` with a sliding window and sinks
+    (``components/attention.py``'s ``window_attention``; the reference has none): query
+    i sees the last ``window`` keys up to its own and the first ``sinks`` keys, and
+    ``k`` and ``v`` may have fewer heads."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, weight, bias, buffer, compressed, distribution, min_elements,
+                window, sinks=0, scale=ATTENTION_SCALE):
+        window, sinks, scale, _ = check_attention(q, k, v, window, sinks, scale, None)
+        out, lse = attention_kernels.attention_forward(q, k, v, window, sinks, scale, None, True)
+        hidden = out.transpose(1, 2).reshape(q.shape[0], q.shape[2], -1)
+        output = F.linear(hidden, dense_weight(weight), bias.to(out.dtype))
+        ctx.sight, ctx.lse = (window, sinks, scale), lse
+        ctx.weight = weight
+        ctx.bias_dtype = bias.dtype
+        ctx.state = _AttentionState((q, k, v, out), compressed and q.numel() >= min_elements,
+                                    buffer, distribution)
+        return output
+
+    @staticmethod
+    def backward(ctx, grad_output):
+        q, k, v, out = ctx.state.unpack()
+        batch, heads, length, head_dim = q.shape
+        g = grad_output.reshape(-1, grad_output.shape[-1])
+        hidden = out.transpose(1, 2).reshape(-1, heads * head_dim)
+        grad_weight = g.T @ hidden
+        grad_bias = _bias_grad(g, ctx.bias_dtype)
+        grad_attention = (g @ dense_weight(ctx.weight)).reshape(
+            batch, length, heads, head_dim).transpose(1, 2)
+        dq, dk, dv = attention_kernels.attention_backward(grad_attention, q, k, v, out, ctx.lse,
+                                                          *ctx.sight, None)
+        ctx.state = ctx.lse = ctx.weight = None
+        return (dq, dk, dv, grad_weight, grad_bias, None, None, None, None, None, None, None)
 
 
 def compress_weight(module, buffer=None, distribution=None):
