@@ -39,6 +39,45 @@ __device__ __forceinline__ void store_row(uint16_t *dst, const f32x16 (&x)[kColu
         }
 }
 
+// ---- infinities and NaN in masked places
+//
+// A masked weight is an exact zero, but the matrix instructions multiply it, and
+// zero times an infinity or a NaN is a NaN: values that a query does not see
+// reach it where they share a tile with some that it does.  Padding is loaded
+// as zeros; for the rest a wave looks at its sums when they are done, and where
+// one is not finite it computes its rows again, key by key, from what they see
+// alone: 100 cycles per pair, and only then.
+
+// Whether a sum of the wave is an infinity or a NaN.
+template <int kCount>
+__device__ __forceinline__ bool not_finite(const f32x16 (&x)[kCount]) {
+    float probe = 0.0f;
+#pragma unroll
+    for (int c = 0; c < kCount; ++c)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) probe = __builtin_fmaf(x[c][r], 0.0f, probe);
+    return __any(!(probe == 0.0f));
+}
+
+// One row's two channels of this lane; zeros past the head's width.
+__device__ __forceinline__ uint32_t lane_pair(const uint16_t *row, int32_t dim) {
+    const int32_t channel = 2 * wave_lane();
+    return channel < dim ? *reinterpret_cast<const uint32_t *>(row + channel) : 0u;
+}
+
+template <bool kHalf>
+__device__ __forceinline__ float row_product(uint32_t a, uint32_t b) {
+    using E = Element<kHalf>;
+    float sum = E::low(a) * E::low(b) + E::high(a) * E::high(b);
+#pragma unroll
+    for (int d = kWave / 2; d > 0; d >>= 1) sum += __shfl_xor(sum, d, kWave);
+    return sum;
+}
+
+__device__ __forceinline__ float of_lane(float v, int lane) {
+    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane));
+}
+
 template <bool kHalf, int kDim, bool kSplit>
 __global__ __launch_bounds__(kAttentionThreads, 2) void attention_forward_kernel(
     lct_attention a, int32_t tiles, int32_t splits, float *__restrict__ parts) {
@@ -176,6 +215,54 @@ __global__ __launch_bounds__(kAttentionThreads, 2) void attention_forward_kernel
     }
 
     total = across_sum(total);
+    if (not_finite(out)) {
+        const int32_t channel = 2 * lane;
+        for (int r = 0; r < 32; ++r) {
+            const int32_t at = wave_first + r;
+            if (at >= a.queries) break;
+            const Sight seen = sight_of(a, at + shift, length);
+            const uint32_t q_pair = lane_pair(q + at * a.q_stride[2], a.head_dim);
+            float largest = -INFINITY, base = 0.0f, sum = 0.0f, x = 0.0f, y = 0.0f;
+            for (int32_t t = begin; t < end; ++t) {
+                const int32_t key = all.first_key(t, kKeyTile);
+                for (int32_t j = key; j < key + kKeyTile; ++j) {
+                    if (!seen(j)) continue;
+                    const uint32_t v_pair = lane_pair(v + j * a.v_stride[2], a.head_dim);
+                    const float score =
+                        factor
+                        * row_product<kHalf>(q_pair, lane_pair(k + j * a.k_stride[2], a.head_dim));
+                    largest = fmaxf(largest, score);
+                    const float next = largest == -INFINITY ? 0.0f : largest;
+                    const float change = sum == 0.0f ? 0.0f : exp2_fast(base - next);
+                    const float weight = exp2_fast(score - next);
+                    base = next;
+                    x = (sum == 0.0f ? 0.0f : x * change) + weight * Element<kHalf>::low(v_pair);
+                    y = (sum == 0.0f ? 0.0f : y * change) + weight * Element<kHalf>::high(v_pair);
+                    sum = sum * change + weight;
+                }
+            }
+            if constexpr (kSplit) {
+                float *part_out =
+                    parts + ((int64_t{bh} * splits + split) * a.queries + at) * (a.head_dim + 2);
+                if (channel < a.head_dim)
+                    *reinterpret_cast<f32x2 *>(part_out + channel) = f32x2{x, y};
+                if (lane == 0) *reinterpret_cast<f32x2 *>(part_out + a.head_dim) = f32x2{base, sum};
+            } else {
+                const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+                if (channel < a.head_dim)
+                    *reinterpret_cast<uint32_t *>(
+                        static_cast<uint16_t *>(a.out) + b * a.out_stride[0] + h * a.out_stride[1]
+                        + at * a.out_stride[2] + channel) =
+                        Element<kHalf>::round_pair(x * inverse, y * inverse);
+                if (a.lse != nullptr && lane == 0)
+                    a.lse[int64_t{bh} * lse_pitch(a.queries) + at] =
+                        sum == 0.0f ? INFINITY : base + __log2f(sum);
+            }
+        }
+        if (!kSplit && a.lse != nullptr && half == 0 && row >= a.queries)
+            a.lse[int64_t{bh} * lse_pitch(a.queries) + row] = INFINITY;
+        return;
+    }
     if constexpr (kSplit) {
         if (row >= a.queries) return;
         float *part_out = parts + ((int64_t{bh} * splits + split) * a.queries + row) * (a.head_dim + 2);
@@ -393,6 +480,41 @@ __global__ __launch_bounds__(kAttentionThreads, 2) void attention_dq_kernel(
         __syncthreads();
         if (t + 2 < all.count) load(t + 2, k_even, v_even);
         step(t + 1, k_odd, v_odd);
+    }
+    if (not_finite(dq)) {
+        const int32_t channel = 2 * lane;
+        const uint16_t *q =
+            static_cast<const uint16_t *>(a.q) + b * a.q_stride[0] + h * a.q_stride[1];
+        const uint16_t *g = static_cast<const uint16_t *>(d.grad) + b * d.grad_stride[0]
+                            + h * d.grad_stride[1];
+        for (int r = 0; r < 32; ++r) {
+            const int32_t at = wave_first + r;
+            if (at >= a.queries) break;
+            const Sight seen = sight_of(a, at + shift, length);
+            const uint32_t q_pair = lane_pair(q + at * a.q_stride[2], a.head_dim);
+            const uint32_t g_pair = lane_pair(g + at * d.grad_stride[2], a.head_dim);
+            const float row_lse = of_lane(lse, r), row_delta = of_lane(delta, r);
+            float x = 0.0f, y = 0.0f;
+            for (int32_t t = 0; t < all.count; ++t) {
+                const int32_t key = all.first_key(t, kKeyTile);
+                for (int32_t j = key; j < key + kKeyTile; ++j) {
+                    if (!seen(j)) continue;
+                    const uint32_t k_pair = lane_pair(k + j * a.k_stride[2], a.head_dim);
+                    const float score = row_product<kHalf>(q_pair, k_pair);
+                    const float dp = row_product<kHalf>(
+                        g_pair, lane_pair(v + j * a.v_stride[2], a.head_dim));
+                    const float ds =
+                        exp2_fast(__builtin_fmaf(score, factor, -row_lse)) * (dp - row_delta);
+                    x += ds * Element<kHalf>::low(k_pair);
+                    y += ds * Element<kHalf>::high(k_pair);
+                }
+            }
+            if (channel < a.head_dim)
+                *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(d.dq) + b * d.dq_stride[0]
+                                              + h * d.dq_stride[1] + at * d.dq_stride[2] + channel) =
+                    Element<kHalf>::round_pair(x * a.scale, y * a.scale);
+        }
+        return;
     }
     if (row >= a.queries) return;
     uint16_t *dst = static_cast<uint16_t *>(d.dq) + b * d.dq_stride[0] + h * d.dq_stride[1]
@@ -648,6 +770,56 @@ __global__ __launch_bounds__(key_block(kDim) * 2, 2) void attention_dkdv_kernel(
         step(t + 1, q_odd, g_odd, stats_odd);
     }
 
+    float *part_out = parts
+                      + (bkv * blocks.parts() + blocks.first_part(block) + split) * 2 * kKeyBlock
+                            * a.head_dim;
+    if (not_finite(dk[0]) || not_finite(dv[0])) {
+        const int32_t channel = 2 * lane;
+        for (int m = 0; m < kWaveKeys; ++m) {
+            const int32_t key = wave_first + m;
+            if (key >= a.keys) break;
+            float kx = 0.0f, ky = 0.0f, vx = 0.0f, vy = 0.0f;
+            const bool there = key < length;
+            const uint32_t k_pair = there ? lane_pair(k + key * a.k_stride[2], a.head_dim) : 0u;
+            const uint32_t v_pair = there ? lane_pair(v + key * a.v_stride[2], a.head_dim) : 0u;
+            for (int32_t t = begin; t < end; ++t) {
+                const int32_t h = kv * group + t / per_query_head;
+                const int32_t query = (low_tile + t % per_query_head) * kQueryStep;
+                const uint16_t *q =
+                    static_cast<const uint16_t *>(a.q) + b * a.q_stride[0] + h * a.q_stride[1];
+                const uint16_t *g = static_cast<const uint16_t *>(d.grad) + b * d.grad_stride[0]
+                                    + h * d.grad_stride[1];
+                const int64_t stats = (int64_t{b} * a.heads + h) * lse_pitch(a.queries);
+                for (int32_t i = query; i < min(query + kQueryStep, live); ++i) {
+                    if (!sight_of(a, i + shift, length)(key)) continue;
+                    const uint32_t q_pair = lane_pair(q + i * a.q_stride[2], a.head_dim);
+                    const uint32_t g_pair = lane_pair(g + i * d.grad_stride[2], a.head_dim);
+                    const float weight = exp2_fast(__builtin_fmaf(
+                        row_product<kHalf>(q_pair, k_pair), factor, -a.lse[stats + i]));
+                    const float ds =
+                        weight * (row_product<kHalf>(g_pair, v_pair) - d.delta[stats + i]);
+                    vx += weight * Element<kHalf>::low(g_pair);
+                    vy += weight * Element<kHalf>::high(g_pair);
+                    kx += ds * Element<kHalf>::low(q_pair);
+                    ky += ds * Element<kHalf>::high(q_pair);
+                }
+            }
+            if (channel >= a.head_dim) continue;
+            if (splits > 1) {
+                float *dst = part_out + int64_t{key - first} * a.head_dim + channel;
+                *reinterpret_cast<f32x2 *>(dst) = f32x2{kx * a.scale, ky * a.scale};
+                *reinterpret_cast<f32x2 *>(dst + kKeyBlock * a.head_dim) = f32x2{vx, vy};
+                continue;
+            }
+            *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(d.dk) + b * d.dk_stride[0]
+                                          + kv * d.dk_stride[1] + key * d.dk_stride[2] + channel) =
+                Element<kHalf>::round_pair(kx * a.scale, ky * a.scale);
+            *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(d.dv) + b * d.dv_stride[0]
+                                          + kv * d.dv_stride[1] + key * d.dv_stride[2] + channel) =
+                Element<kHalf>::round_pair(vx, vy);
+        }
+        return;
+    }
     const float dv_scale = kHalf ? 1.0f / kHalfWeights : 1.0f;
 #pragma unroll
     for (int m = 0; m < kGroups; ++m) {
@@ -662,10 +834,7 @@ __global__ __launch_bounds__(key_block(kDim) * 2, 2) void attention_dkdv_kernel(
                                        dv[m], dv_scale, a.head_dim);
             continue;
         }
-        float *dst = parts
-                     + (bkv * blocks.parts() + blocks.first_part(block) + split) * 2 * kKeyBlock
-                           * a.head_dim
-                     + int64_t{key - first} * a.head_dim;
+        float *dst = part_out + int64_t{key - first} * a.head_dim;
 #pragma unroll
         for (int c = 0; c < kColumns; ++c)
 #pragma unroll

@@ -344,3 +344,45 @@ def test_refusals():
     grad, = torch.autograd.grad(call(leaf, k, k).float().sum(), leaf, create_graph=True)
     with pytest.raises(RuntimeError):
         grad.sum().backward()
+
+
+@pytest.mark.parametrize("dim,splits", [(64, None), (128, None), (64, 3)])
+@pytest.mark.parametrize("where", ["v", "k", "q", "grad"])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_infinities_reach_only_what_sees_them(where, value, dim, splits, monkeypatch):
+    """One token of one tensor is not finite: results that it has no part in keep
+    their bounds, whatever tiles they share with it; those that it has are not
+    finite."""
+    if splits is not None:
+        monkeypatch.setattr(kernels, "forward_splits", lambda *a: splits)
+        monkeypatch.setattr(kernels, "backward_splits", lambda *a: (splits, splits))
+    tokens, window, sinks, at = 260, 40, 2, 100
+    clean = dict(zip("qkv", _inputs(1, 2, 1, tokens, tokens, dim)[:3]),
+                 grad=_inputs(1, 2, 1, tokens, tokens, dim)[3])
+    seen = oracle.sees(tokens, tokens, window, sinks).to(DEV)
+    pairs = seen[0, 0]
+    poisoned = {n: t.clone() for n, t in clean.items()}
+    poisoned[where][:, :, at] = value
+    got = _run(*(poisoned[n] for n in ("q", "k", "v", "grad")), window=window, sinks=sinks)
+    # Rows and keys that the token has a part in, and the results without it.
+    if where in "kv":
+        rows = pairs[:, at]
+        without = seen.clone()
+        without[..., at] = False
+    else:
+        rows = torch.arange(tokens, device=DEV) == at
+        without = seen.clone()
+        without[..., at, :] = False
+    keys = pairs[rows].any(0)
+    for name, (exact, bound) in oracle.attention_with_bounds(
+            *(clean[n] for n in "qkv"), without, dim ** -0.5, clean["grad"]).items():
+        # The output does not depend on the gradient that comes back.
+        if name == "out" and where == "grad":
+            continue
+        clear = ~(rows if name in ("out", "dq") else keys)
+        far = (got[name].double() - exact).abs() - bound
+        assert bool((far[:, :, clear] <= 0).all()), name
+    if where != "grad":
+        assert not bool(got["out"][:, :, rows].isfinite().all(-1).any()) or value == float("inf")
+    assert bool(got["dq"][:, :, ~rows].isfinite().all())
+    assert bool(got["dk"][:, :, ~keys].isfinite().all())
