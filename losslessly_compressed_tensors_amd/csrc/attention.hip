@@ -115,7 +115,9 @@ __global__ __launch_bounds__(kAttentionThreads, 2) void attention_forward_kernel
 #pragma unroll
     for (int s = 0; s < kSteps; ++s)
         q_operand[s] = load_operand(q, a.q_stride[2], row, a.queries, a.head_dim, s);
-    const Sight sight = sight_of(a, row < a.queries ? row + shift : -1, length);
+    const int32_t position =
+        row < a.queries && row + shift >= 0 && row + shift < length ? row + shift : kNowhere;
+    const int32_t tile_sinks = a.window > 0 ? a.sinks : 0;
     const int32_t low_position = wave_first + shift;
     const int32_t high_position = min(wave_first + 31, a.queries - 1) + shift;
 
@@ -158,13 +160,11 @@ __global__ __launch_bounds__(kAttentionThreads, 2) void attention_forward_kernel
                 s[n] = Element<kHalf>::multiply(read_rows<kPitch>(keys, n, d), q_operand[d], s[n]);
         }
         if (!seen_by_all) {
+            const TileSight sight(a, position, key);
 #pragma unroll
             for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int32_t at = key + 32 * n + 8 * (r / 4) + 4 * half + r % 4;
-                    s[n][r] = sight(at) ? s[n][r] : -INFINITY;
-                }
+                sight.each(key, 32 * n, tile_sinks,
+                           [&](int r, bool seen) { s[n][r] = seen ? s[n][r] : -INFINITY; });
         }
         float top = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
@@ -380,11 +380,13 @@ __global__ __launch_bounds__(kAttentionThreads, 2) void attention_dq_kernel(
 
     const int32_t wave_first = first + 32 * wave;
     const int32_t row = wave_first + (lane & 31);
-    const Sight sight = sight_of(a, row < a.queries ? row + shift : -1, length);
+    const int32_t position =
+        row < a.queries && row + shift >= 0 && row + shift < length ? row + shift : kNowhere;
+    const int32_t tile_sinks = a.window > 0 ? a.sinks : 0;
     const int32_t low_position = wave_first + shift;
     const int32_t high_position = min(wave_first + 31, a.queries - 1) + shift;
     // Queries that see nothing take part as zeros.
-    const int32_t rows = sight.limit > 0 ? a.queries : 0;
+    const int32_t rows = position != kNowhere ? a.queries : 0;
 
     u32x4 q_operand[kSteps], g_operand[kSteps];
     float delta = 0.0f;
@@ -451,13 +453,10 @@ __global__ __launch_bounds__(kAttentionThreads, 2) void attention_dq_kernel(
             }
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = exp2_fast(__builtin_fmaf(s[r], factor, -lse)) * e[r];
-            if (!seen_by_all) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int32_t column = key + 32 * n + 8 * (r / 4) + 4 * half + r % 4;
-                    s[r] = sight(column) ? s[r] : 0.0f;
-                }
-            }
+            if (!seen_by_all)
+                TileSight(a, position, key).each(
+                    key, 32 * n, tile_sinks,
+                    [&](int r, bool seen) { s[r] = seen ? s[r] : 0.0f; });
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
                 const u32x4 ds = as_operand<kHalf>(s, p);

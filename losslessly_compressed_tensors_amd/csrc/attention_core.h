@@ -192,6 +192,44 @@ struct Sight {
     }
 };
 
+// What a lane's query sees of a tile of scores, by its place in the registers:
+// register 4 g + i of rows 32 n .. holds key first + 32 n + 8 g + 4 half + i.
+// The gap from that key to the query's position must lie between 0 and the
+// window, one unsigned comparison (a query that sees nothing is at a position
+// before all keys); tiles with sinks (uniform: few) need two more.
+struct TileSight {
+    int32_t gap;            // position - key of register 0
+    uint32_t reach;
+    int32_t sinks;          // sinks from register 0's key on, 0 where the tile has none
+    __device__ __forceinline__ TileSight(const lct_attention &a, int32_t position, int32_t first) {
+        const int32_t key = first + 4 * (wave_lane() >> 5);
+        gap = position - key;
+        reach = a.window > 0 ? static_cast<uint32_t>(a.window) : 0x40000000u;
+        sinks = a.window > 0 && first < a.sinks ? a.sinks - key : 0;
+    }
+    // `offset`: 32 n + 8 g + i.
+    __device__ __forceinline__ bool operator()(int32_t offset) const {
+        return static_cast<uint32_t>(gap - offset) < reach;
+    }
+    __device__ __forceinline__ bool with_sinks(int32_t offset) const {
+        return (*this)(offset) || (offset < sinks && offset <= gap);
+    }
+    template <class Keep>
+    __device__ __forceinline__ void each(int32_t first, int32_t base, int32_t total_sinks,
+                                         Keep keep) const {
+        if (first < total_sinks) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) keep(r, with_sinks(base + 8 * (r / 4) + r % 4));
+        } else {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) keep(r, (*this)(base + 8 * (r / 4) + r % 4));
+        }
+    }
+};
+
+// Before every key: where a query that sees none stands.
+constexpr int32_t kNowhere = -(1 << 30);
+
 // Keys a sequence has, within the tensor's.
 __device__ __forceinline__ int32_t sequence_length(const lct_attention &a, int32_t b) {
     return a.lengths == nullptr ? a.keys : max(0, min(a.lengths[b], a.keys));
