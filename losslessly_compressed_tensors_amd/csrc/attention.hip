@@ -872,6 +872,7 @@ __global__ __launch_bounds__(kAttentionThreads) void attention_sum_parts_kernel(
     const float *src = parts + (bkv * blocks.parts() + blocks.first_part(block)) * step
                        + int64_t{key % per_block} * a.head_dim + channel;
     f32x4 x{}, y{};
+#pragma unroll 8
     for (int32_t s = 0; s < count; ++s) {
         x += *reinterpret_cast<const f32x4 *>(src + s * step);
         y += *reinterpret_cast<const f32x4 *>(src + s * step + per_block * a.head_dim);

@@ -129,8 +129,8 @@ def backward_splits(batch: int, heads: int, kv_heads: int, queries: int, keys: i
     unit takes, and what the parts' sums cost (the traffic of a part's FP32 sums
     is 0.04 steps of one compute unit, over all of them).  With a window all
     blocks see about as many queries, without one the first sees all and the last
-    few.  A block with sinks, which all later queries see, gets parts of an
-    eighth of the others' length, which fill what the others leave."""
+    few.  A block with sinks, which all later queries see, gets parts of a
+    sixteenth of the others' length, which fill what the others leave."""
     per_block = key_block(dim)
     blocks, group = -(-keys // per_block), heads // kv_heads
     slots = _CUS if dim > 64 else 2 * _CUS
@@ -149,7 +149,7 @@ def backward_splits(batch: int, heads: int, kv_heads: int, queries: int, keys: i
     splits = best[1]
     if window == 0 or sinks == 0:
         return splits, 1
-    part = max(4, -(-steps // splits) // 8)
+    part = max(4, -(-steps // splits) // 16)
     return splits, max(1, min(_MAX_SPLITS, -(-(-(-queries // 64) * group) // part)))
 
 
