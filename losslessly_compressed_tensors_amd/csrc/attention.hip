@@ -550,7 +550,7 @@ __host__ __device__ constexpr int key_block(int dim) { return dim > 64 ? 256 : 1
 
 // A wave's 32 or 64 keys, the queries (of all heads that share them) in tiles.
 template <bool kHalf, int kDim>
-__global__ __launch_bounds__(key_block(kDim) * 2, 2) void attention_dkdv_kernel(
+__global__ __launch_bounds__(key_block(kDim) * 2, kDim > 64 ? 2 : 3) void attention_dkdv_kernel(
     lct_attention a, lct_attention_gradients d, KeyBlocks blocks, float *__restrict__ parts) {
     constexpr int kPitch = kPitchOf<kDim>;
     constexpr int kSteps = kDim / 16, kColumns = kDim / 32;
@@ -628,10 +628,16 @@ __global__ __launch_bounds__(key_block(kDim) * 2, 2) void attention_dkdv_kernel(
     TileLoads<kQueryStep, kPitch, kThreads> q_loads, g_loads;
     q_loads.prepare(a.q_stride[2], a.head_dim);
     g_loads.prepare(d.grad_stride[2], a.head_dim);
-    const auto load = [&](int32_t t, uint16_t *q_tile, uint16_t *g_tile, float *stats)
+    // The step that is loaded next: its head and its tile of queries.
+    int32_t next_head = kv * group, next_tile = low_tile;
+    if (begin < end) {
+        next_head += begin / per_query_head;
+        next_tile += begin % per_query_head;
+    }
+    int32_t here_tile = next_tile;           // the tile of the step that is computed next
+    const auto load = [&](uint16_t *q_tile, uint16_t *g_tile, float *stats)
                           __attribute__((always_inline)) {
-        const int32_t h = kv * group + t / per_query_head;
-        const int32_t query = (low_tile + t % per_query_head) * kQueryStep;
+        const int32_t h = next_head, query = next_tile * kQueryStep;
         q_loads.issue(static_cast<const uint16_t *>(a.q) + b * a.q_stride[0] + h * a.q_stride[1]
                           + query * a.q_stride[2],
                       live - query, a.q_stride[2], a.head_dim, q_tile);
@@ -645,6 +651,10 @@ __global__ __launch_bounds__(key_block(kDim) * 2, 2) void attention_dkdv_kernel(
                 make_rsrc(from, kQueryStep * 4),
                 (__attribute__((address_space(3))) void *)(stats + wave * kQueryStep), 4, lane * 4,
                 0, 0, 0);
+        }
+        if (++next_tile == low_tile + per_query_head) {
+            next_tile = low_tile;
+            ++next_head;
         }
     };
 
@@ -686,6 +696,27 @@ __global__ __launch_bounds__(key_block(kDim) * 2, 2) void attention_dkdv_kernel(
                     e[m] = Element<kHalf>::multiply(g_rows, v_operand[m][i], e[m]);
             }
         }
+        if (!all) {
+            // Position - key: from 0 to below what the key's place allows; rows past
+            // the sequence are few tiles' (uniform).
+            const int32_t at = position + 4 * half;
+#pragma unroll
+            for (int m = 0; m < kGroups; ++m) {
+                const int32_t key = wave_first + 32 * m + (lane & 31);
+                const uint32_t reach =
+                    a.window == 0 || key < a.sinks ? kMaxTokens : static_cast<uint32_t>(a.window);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int32_t c = 8 * (r / 4) + r % 4;
+                    s[m][r] = static_cast<uint32_t>(at - key + c) < reach ? s[m][r] : -INFINITY;
+                }
+                if (position + 31 >= length) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        s[m][r] = at < length - (8 * (r / 4) + r % 4) ? s[m][r] : -INFINITY;
+                }
+            }
+        }
         // In FP16 the weights of long rows lie below the normal numbers: they are
         // held 2^8 larger until the sums of dv are stored.
 #pragma unroll
@@ -700,24 +731,6 @@ __global__ __launch_bounds__(key_block(kDim) * 2, 2) void attention_dkdv_kernel(
                     e[m][r] *= s[m][r];
                     if (kHalf) s[m][r] *= kHalfWeights;
                 }
-        }
-        if (!all) {
-            // Query at - key: from 0 to below what the key's place allows.
-            const int32_t at = position + 4 * half;
-#pragma unroll
-            for (int m = 0; m < kGroups; ++m) {
-                const int32_t key = wave_first + 32 * m + (lane & 31);
-                const uint32_t reach =
-                    a.window == 0 || key < a.sinks ? kMaxTokens : static_cast<uint32_t>(a.window);
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int32_t c = 8 * (r / 4) + r % 4;
-                    const bool seen =
-                        static_cast<uint32_t>(at - key + c) < reach && at < length - c;
-                    s[m][r] = seen ? s[m][r] : 0.0f;
-                    e[m][r] = seen ? e[m][r] : 0.0f;
-                }
-            }
         }
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
@@ -739,9 +752,10 @@ __global__ __launch_bounds__(key_block(kDim) * 2, 2) void attention_dkdv_kernel(
             }
         }
     };
-    const auto step = [&](int32_t t, const uint16_t *q_tile, const uint16_t *g_tile,
-                          const float *stats) __attribute__((always_inline)) {
-        const int32_t position = (low_tile + t % per_query_head) * kQueryStep + shift;
+    const auto step = [&](const uint16_t *q_tile, const uint16_t *g_tile, const float *stats)
+                          __attribute__((always_inline)) {
+        const int32_t position = here_tile * kQueryStep + shift;
+        if (++here_tile == low_tile + per_query_head) here_tile = low_tile;
         const int32_t last_here = position + kQueryStep - 1, wave_last = wave_first + kWaveKeys - 1;
         const bool all =
             wave_last <= position && last_here < length
@@ -756,17 +770,17 @@ __global__ __launch_bounds__(key_block(kDim) * 2, 2) void attention_dkdv_kernel(
         }
     };
 
-    if (begin < end) load(begin, q_even, g_even, stats_even);
+    if (begin < end) load(q_even, g_even, stats_even);
     for (int32_t t = begin; t < end; t += 2) {
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
-        if (t + 1 < end) load(t + 1, q_odd, g_odd, stats_odd);
-        step(t, q_even, g_even, stats_even);
+        if (t + 1 < end) load(q_odd, g_odd, stats_odd);
+        step(q_even, g_even, stats_even);
         if (t + 1 >= end) break;
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
-        if (t + 2 < end) load(t + 2, q_even, g_even, stats_even);
-        step(t + 1, q_odd, g_odd, stats_odd);
+        if (t + 2 < end) load(q_even, g_even, stats_even);
+        step(q_odd, g_odd, stats_odd);
     }
 
     float *part_out = parts

@@ -125,9 +125,13 @@ struct TileLoads {
     // Rows [0, rows) from `base`; zeros for the others.
     __device__ __forceinline__ void issue(const uint16_t *base, int32_t rows, int64_t row_stride,
                                           int32_t dim, uint16_t *tile) const {
+        // Below 2^31 bytes: 32 bits hold the product.
         const int32_t valid = min(rows, kRows);
         const __amdgpu_buffer_rsrc_t rsrc = make_rsrc(
-            base, valid > 0 ? static_cast<uint32_t>(((valid - 1) * row_stride + dim) * 2) : 0u);
+            base, valid > 0 ? (static_cast<uint32_t>(valid - 1) * static_cast<uint32_t>(row_stride)
+                               + static_cast<uint32_t>(dim))
+                                  * 2u
+                            : 0u);
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
 #pragma unroll
         for (int i = 0; i < kCount; ++i)

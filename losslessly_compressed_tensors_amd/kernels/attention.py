@@ -133,7 +133,7 @@ def backward_splits(batch: int, heads: int, kv_heads: int, queries: int, keys: i
     sixteenth of the others' length, which fill what the others leave."""
     per_block = key_block(dim)
     blocks, group = -(-keys // per_block), heads // kv_heads
-    slots = _CUS if dim > 64 else 2 * _CUS
+    slots = _CUS if dim > 64 else 3 * _CUS
     steps = -(-min(queries, keys if window == 0 else window + per_block) // 64) * group
     items = batch * kv_heads * blocks
     best = None
