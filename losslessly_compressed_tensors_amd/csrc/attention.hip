@@ -1,4 +1,10 @@
-// Attention with a sliding window and sinks, forward.
+// Attention with a sliding window and sinks, forward and backward.
+//
+// Follows LCT/components/layers.py:225-305, whose causal attention is a library's.
+// out = softmax(scale q k^T) v over the keys that a query sees: the last `window`
+// up to its own and the first `sinks` (attention_core.h).  Only tiles that some
+// query of a workgroup sees are loaded, a wave skips those that none of its own
+// sees, and those that all of them see are computed without masks.
 #include <algorithm>
 #include <type_traits>
 
@@ -78,6 +84,28 @@ __device__ __forceinline__ float of_lane(float v, int lane) {
     return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane));
 }
 
+// A workgroup has 128 queries of a head, a wave 32 of them, and walks its key
+// tiles once: scores with the keys in their rows (a lane's 32 scores of a tile are
+// one query's, so its maximum and sum need one exchange between two lanes), the
+// running maximum and sum of the softmax per lane, and the product with the
+// values.  The next tile's keys and values are on their way to LDS meanwhile.
+//
+// The maximum may lag by 2^kRescale before the sums are scaled to a new one: all
+// are FP32, so the weights' larger values cost no precision, and after the first
+// tiles the 32 to 128 products are rarely due.  The weights are rounded to the
+// tensors' type for the product (BF16 2^-9, FP16 2^-12 of each weight); their sum is
+// taken before.
+//
+// Matrix instructions, LDS reads (one fragment per instruction) and the softmax's
+// vector instructions take about 512, 512 and 450 clocks of a SIMD per 32 x 32
+// scores at heads of 128, at 1.9 to 2.0 GHz under this load; the two waves of a
+// SIMD overlap them in part (matrix instructions busy half of the time).  1560 us
+// for 8191 queries after 8192 keys, 32 heads of 128 over 8 (1057 TFLOP/s); 495 us
+// for 1 x 16384, 16 heads over 4, window 4096 (970); 22 us for 8 x 1024, 12 heads
+// of 64, window 256.  Tried: 32-key halves of a tile with the second half's scores
+// issued between the first's exponentials 1650 us at the first of these; matrix
+// phases at a higher wave priority 1560; column reads without the wait that the
+// compiler puts before them 1645; 64 queries per wave did not fit the registers.
 template <bool kHalf, int kDim, bool kSplit>
 __global__ __launch_bounds__(kAttentionThreads, 2) void attention_forward_kernel(
     lct_attention a, int32_t tiles, int32_t splits, float *__restrict__ parts) {
@@ -126,12 +154,11 @@ __global__ __launch_bounds__(kAttentionThreads, 2) void attention_forward_kernel
     TileLoads<kKeyTile, kPitch> k_loads, v_loads;
     k_loads.prepare(a.k_stride[2], a.head_dim);
     v_loads.prepare(a.v_stride[2], a.head_dim);
-    const auto load = [&](int32_t t, uint16_t *keys, uint16_t *values) __attribute__((always_inline)) {
+    const auto load = [&](int32_t t, uint16_t *keys, uint16_t *values)
+                          __attribute__((always_inline)) {
         const int32_t key = all.first_key(t, kKeyTile);
-        k_loads.issue(k + key * a.k_stride[2], length - key, a.k_stride[2], a.head_dim,
-                      keys);
-        v_loads.issue(v + key * a.v_stride[2], length - key, a.v_stride[2], a.head_dim,
-                      values);
+        k_loads.issue(k + key * a.k_stride[2], length - key, a.k_stride[2], a.head_dim, keys);
+        v_loads.issue(v + key * a.v_stride[2], length - key, a.v_stride[2], a.head_dim, values);
     };
 
     const float factor = a.scale * kLog2e;
@@ -142,7 +169,8 @@ __global__ __launch_bounds__(kAttentionThreads, 2) void attention_forward_kernel
     float shifted = 0.0f;       // its product with factor, 0 while no key was seen
     float total = 0.0f;         // this lane's keys' weights
 
-    const auto step = [&](int32_t t, const uint16_t *keys, const uint16_t *values) __attribute__((always_inline)) {
+    const auto step = [&](int32_t t, const uint16_t *keys, const uint16_t *values)
+                          __attribute__((always_inline)) {
         const int32_t key = all.first_key(t, kKeyTile);
         const bool seen_by_some =
             key <= high_position
@@ -265,7 +293,8 @@ __global__ __launch_bounds__(kAttentionThreads, 2) void attention_forward_kernel
     }
     if constexpr (kSplit) {
         if (row >= a.queries) return;
-        float *part_out = parts + ((int64_t{bh} * splits + split) * a.queries + row) * (a.head_dim + 2);
+        float *part_out =
+            parts + ((int64_t{bh} * splits + split) * a.queries + row) * (a.head_dim + 2);
 #pragma unroll
         for (int c = 0; c < kColumns; ++c)
 #pragma unroll
@@ -294,7 +323,9 @@ __global__ __launch_bounds__(kAttentionThreads, 2) void attention_forward_kernel
 
 // Joins the parts of a query's keys: sum of 2^(shift - largest) out, over the
 // same sum of the weights.  A workgroup per query, two channels per lane, a
-// quarter of the parts per wave; lane s holds part s's shift and weight.
+// quarter of the parts per wave; lane s holds part s's shift and weight, so the
+// parts' loads do not wait for each other (64 queries of 16 parts: 5.5 us; a wave
+// per query that read part after part: 18).
 template <bool kHalf>
 __global__ __launch_bounds__(kAttentionThreads) void attention_join_kernel(
     lct_attention a, int64_t pitch, int32_t splits, const float *__restrict__ parts) {
@@ -352,7 +383,11 @@ __global__ __launch_bounds__(kAttentionThreads) void attention_join_kernel(
 // again: seven products in place of five, but no sum is shared between
 // workgroups, so results do not depend on timing.
 
-// A wave's 32 queries, the keys in tiles.  delta is stored for the other kernel.
+// A wave's 32 queries, the keys in tiles of 64: as in the forward kernel, with dP
+// beside the scores (its sums begin at -delta) and the keys' columns for the last
+// product.  delta is taken from the operands on their way in, and stored for the
+// other kernel.  685 us for 1 x 16384, 16 heads of 128 over 4, window 4096 (1055
+// TFLOP/s), 30 us for 8 x 1024, 12 heads of 64, window 256.
 template <bool kHalf, int kDim>
 __global__ __launch_bounds__(kAttentionThreads, 2) void attention_dq_kernel(
     lct_attention a, lct_attention_gradients d, int32_t tiles) {
@@ -452,7 +487,8 @@ __global__ __launch_bounds__(kAttentionThreads, 2) void attention_dq_kernel(
                 e = Element<kHalf>::multiply(read_rows<kPitch>(values, n, i), g_operand[i], e);
             }
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = exp2_fast(__builtin_fmaf(s[r], factor, -lse)) * e[r];
+            for (int r = 0; r < 16; ++r)
+                s[r] = exp2_fast(__builtin_fmaf(s[r], factor, -lse)) * e[r];
             if (!seen_by_all)
                 TileSight(a, position, key).each(
                     key, 32 * n, tile_sinks,
@@ -510,7 +546,8 @@ __global__ __launch_bounds__(kAttentionThreads, 2) void attention_dq_kernel(
             }
             if (channel < a.head_dim)
                 *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(d.dq) + b * d.dq_stride[0]
-                                              + h * d.dq_stride[1] + at * d.dq_stride[2] + channel) =
+                                              + h * d.dq_stride[1] + at * d.dq_stride[2]
+                                              + channel) =
                     Element<kHalf>::round_pair(x * a.scale, y * a.scale);
         }
         return;
@@ -548,14 +585,26 @@ constexpr int kQueryStep = 64;       // queries per step
 // Keys of a workgroup of the kernel below.
 __host__ __device__ constexpr int key_block(int dim) { return dim > 64 ? 256 : 128; }
 
-// A wave's 32 or 64 keys, the queries (of all heads that share them) in tiles.
+// A wave's 32 keys, the queries (of all heads that share them) in tiles of 64;
+// S and dP have the queries in their rows, so that P and dS are the operands of
+// dv and dk, whose other operands are the columns of the tiles that S and dP read
+// by rows.
+//
+// Four products per tile, each fragment of LDS read for one of them: LDS (128
+// bytes a clock, what four SIMDs' matrix instructions use) and the matrix
+// instructions are busy alike.  Heads wider than 64 hold 128 registers of sums and
+// 32 of the keys' operands; the values' stay in LDS (64 KB for 256 keys, read
+// again for each tile), so that two waves share a SIMD.  1111 us for 1 x 16384, 16
+// heads of 128 over 4, window 4096 (870 TFLOP/s); 64 keys per wave at one wave
+// per SIMD, which read half as much: 1420; 32 with all operands in registers at
+// one wave per SIMD: 2200.  8 x 1024, 12 heads of 64, window 256: 38 us, bound by
+// the exponentials, masks and conversions of three waves per SIMD (two: 42).
 template <bool kHalf, int kDim>
 __global__ __launch_bounds__(key_block(kDim) * 2, kDim > 64 ? 2 : 3) void attention_dkdv_kernel(
     lct_attention a, lct_attention_gradients d, KeyBlocks blocks, float *__restrict__ parts) {
     constexpr int kPitch = kPitchOf<kDim>;
     constexpr int kSteps = kDim / 16, kColumns = kDim / 32;
     constexpr int kKeyBlock = key_block(kDim), kWaveKeys = 32, kThreads = kKeyBlock * 2;
-    constexpr int kGroups = kWaveKeys / 32;
     __shared__ __attribute__((aligned(1024))) uint16_t q_even[kQueryStep * kPitch];
     __shared__ __attribute__((aligned(1024))) uint16_t g_even[kQueryStep * kPitch];
     __shared__ __attribute__((aligned(1024))) uint16_t q_odd[kQueryStep * kPitch];
@@ -569,11 +618,11 @@ __global__ __launch_bounds__(key_block(kDim) * 2, kDim > 64 ? 2 : 3) void attent
     // The blocks without sinks, then those with: each kind dealt out over the
     // XCDs by itself, since their parts are of unequal length.
     const int64_t heads = int64_t{a.batch} * a.kv_heads;
-    const int64_t other_items = blocks.other_parts() * heads, sink_items = blocks.sink_parts() * heads;
-    const bool sinks = blockIdx.x >= xcd_grid(other_items);
-    const int64_t items = sinks ? sink_items : other_items;
-    const int64_t item =
-        xcd_item(items, sinks ? blockIdx.x - static_cast<uint32_t>(xcd_grid(other_items)) : blockIdx.x);
+    const int64_t other_items = blocks.other_parts() * heads;
+    const uint32_t other_grid = static_cast<uint32_t>(xcd_grid(other_items));
+    const bool sinks = blockIdx.x >= other_grid;
+    const int64_t items = sinks ? blocks.sink_parts() * heads : other_items;
+    const int64_t item = xcd_item(items, sinks ? blockIdx.x - other_grid : blockIdx.x);
     if (item >= items) return;
     const int64_t per_head = sinks ? blocks.sink_parts() : blocks.other_parts();
     const int32_t bkv = static_cast<int32_t>(item / per_head);
@@ -606,7 +655,8 @@ __global__ __launch_bounds__(key_block(kDim) * 2, kDim > 64 ? 2 : 3) void attent
     const int32_t wave_first = first + kWaveKeys * wave;
     const uint16_t *k = static_cast<const uint16_t *>(a.k) + b * a.k_stride[0] + kv * a.k_stride[1];
     const uint16_t *v = static_cast<const uint16_t *>(a.v) + b * a.v_stride[0] + kv * a.v_stride[1];
-    u32x4 k_operand[kGroups][kSteps], v_operand[kStaged ? 1 : kGroups][kStaged ? 1 : kSteps];
+    const int32_t key = wave_first + (lane & 31);
+    u32x4 k_operand[kSteps], v_operand[kStaged ? 1 : kSteps];
     if constexpr (kStaged) {
         TileLoads<kQueryStep, kPitch, kThreads> v_loads;
         v_loads.prepare(a.v_stride[2], a.head_dim);
@@ -616,14 +666,11 @@ __global__ __launch_bounds__(key_block(kDim) * 2, kDim > 64 ? 2 : 3) void attent
                           a.head_dim, v_block + i * kPitch);
     }
 #pragma unroll
-    for (int m = 0; m < kGroups; ++m)
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            const int32_t key = wave_first + 32 * m + (lane & 31);
-            k_operand[m][s] = load_operand(k, a.k_stride[2], key, length, a.head_dim, s);
-            if constexpr (!kStaged)
-                v_operand[m][s] = load_operand(v, a.v_stride[2], key, length, a.head_dim, s);
-        }
+    for (int s = 0; s < kSteps; ++s) {
+        k_operand[s] = load_operand(k, a.k_stride[2], key, length, a.head_dim, s);
+        if constexpr (!kStaged)
+            v_operand[s] = load_operand(v, a.v_stride[2], key, length, a.head_dim, s);
+    }
 
     TileLoads<kQueryStep, kPitch, kThreads> q_loads, g_loads;
     q_loads.prepare(a.q_stride[2], a.head_dim);
@@ -659,62 +706,44 @@ __global__ __launch_bounds__(key_block(kDim) * 2, kDim > 64 ? 2 : 3) void attent
     };
 
     const float factor = a.scale * kLog2e;
-    f32x16 dk[kGroups][kColumns], dv[kGroups][kColumns];
+    const uint32_t reach =
+        a.window == 0 || key < a.sinks ? kMaxTokens : static_cast<uint32_t>(a.window);
+    f32x16 dk[kColumns], dv[kColumns];
 #pragma unroll
-    for (int m = 0; m < kGroups; ++m)
-#pragma unroll
-        for (int c = 0; c < kColumns; ++c) dk[m][c] = dv[m][c] = f32x16{};
+    for (int c = 0; c < kColumns; ++c) dk[c] = dv[c] = f32x16{};
 
     // 32 of the step's queries, at `position`; `all`: each sees all the wave's keys.
     const auto rows = [&](int n, bool all, int32_t position, const uint16_t *q_tile,
                           const uint16_t *g_tile, const float *stats)
                           __attribute__((always_inline)) {
-        f32x16 s[kGroups], e[kGroups];
+        f32x16 s{}, e;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const f32x4 delta = *reinterpret_cast<const f32x4 *>(stats + kQueryStep + 32 * n + 8 * g
                                                                  + 4 * half);
 #pragma unroll
-            for (int m = 0; m < kGroups; ++m)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    s[m][4 * g + i] = 0.0f;
-                    e[m][4 * g + i] = -delta[i];
-                }
+            for (int i = 0; i < 4; ++i) e[4 * g + i] = -delta[i];
         }
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
-            const u32x4 q_rows = read_rows<kPitch>(q_tile, n, i);
-            const u32x4 g_rows = read_rows<kPitch>(g_tile, n, i);
-#pragma unroll
-            for (int m = 0; m < kGroups; ++m) {
-                s[m] = Element<kHalf>::multiply(q_rows, k_operand[m][i], s[m]);
-                if constexpr (kStaged)
-                    e[m] = Element<kHalf>::multiply(
-                        g_rows, read_rows<kPitch>(v_block, kGroups * wave + m, i), e[m]);
-                else
-                    e[m] = Element<kHalf>::multiply(g_rows, v_operand[m][i], e[m]);
-            }
+            s = Element<kHalf>::multiply(read_rows<kPitch>(q_tile, n, i), k_operand[i], s);
+            const u32x4 v_rows =
+                kStaged ? read_rows<kPitch>(v_block, wave, i) : v_operand[kStaged ? 0 : i];
+            e = Element<kHalf>::multiply(read_rows<kPitch>(g_tile, n, i), v_rows, e);
         }
         if (!all) {
             // Position - key: from 0 to below what the key's place allows; rows past
             // the sequence are few tiles' (uniform).
             const int32_t at = position + 4 * half;
 #pragma unroll
-            for (int m = 0; m < kGroups; ++m) {
-                const int32_t key = wave_first + 32 * m + (lane & 31);
-                const uint32_t reach =
-                    a.window == 0 || key < a.sinks ? kMaxTokens : static_cast<uint32_t>(a.window);
+            for (int r = 0; r < 16; ++r) {
+                const int32_t c = 8 * (r / 4) + r % 4;
+                s[r] = static_cast<uint32_t>(at - key + c) < reach ? s[r] : -INFINITY;
+            }
+            if (position + 31 >= length) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int32_t c = 8 * (r / 4) + r % 4;
-                    s[m][r] = static_cast<uint32_t>(at - key + c) < reach ? s[m][r] : -INFINITY;
-                }
-                if (position + 31 >= length) {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        s[m][r] = at < length - (8 * (r / 4) + r % 4) ? s[m][r] : -INFINITY;
-                }
+                for (int r = 0; r < 16; ++r)
+                    s[r] = at < length - (8 * (r / 4) + r % 4) ? s[r] : -INFINITY;
             }
         }
         // In FP16 the weights of long rows lie below the normal numbers: they are
@@ -723,32 +752,22 @@ __global__ __launch_bounds__(key_block(kDim) * 2, kDim > 64 ? 2 : 3) void attent
         for (int g = 0; g < 4; ++g) {
             const f32x4 lse = *reinterpret_cast<const f32x4 *>(stats + 32 * n + 8 * g + 4 * half);
 #pragma unroll
-            for (int m = 0; m < kGroups; ++m)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int r = 4 * g + i;
-                    s[m][r] = exp2_fast(__builtin_fmaf(s[m][r], factor, -lse[i]));
-                    e[m][r] *= s[m][r];
-                    if (kHalf) s[m][r] *= kHalfWeights;
-                }
+            for (int i = 0; i < 4; ++i) {
+                const int r = 4 * g + i;
+                s[r] = exp2_fast(__builtin_fmaf(s[r], factor, -lse[i]));
+                e[r] *= s[r];
+                if (kHalf) s[r] *= kHalfWeights;
+            }
         }
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
-            u32x4 weights[kGroups], ds[kGroups];
-#pragma unroll
-            for (int m = 0; m < kGroups; ++m) {
-                weights[m] = as_operand<kHalf>(s[m], p);
-                ds[m] = as_operand<kHalf>(e[m], p);
-            }
+            const u32x4 weights = as_operand<kHalf>(s, p), ds = as_operand<kHalf>(e, p);
 #pragma unroll
             for (int c = 0; c < kColumns; ++c) {
-                const u32x4 g_columns = read_columns<kPitch>(g_tile, 32 * n + 16 * p, c);
-                const u32x4 q_columns = read_columns<kPitch>(q_tile, 32 * n + 16 * p, c);
-#pragma unroll
-                for (int m = 0; m < kGroups; ++m) {
-                    dv[m][c] = Element<kHalf>::multiply(g_columns, weights[m], dv[m][c]);
-                    dk[m][c] = Element<kHalf>::multiply(q_columns, ds[m], dk[m][c]);
-                }
+                dv[c] = Element<kHalf>::multiply(
+                    read_columns<kPitch>(g_tile, 32 * n + 16 * p, c), weights, dv[c]);
+                dk[c] = Element<kHalf>::multiply(
+                    read_columns<kPitch>(q_tile, 32 * n + 16 * p, c), ds, dk[c]);
             }
         }
     };
@@ -786,15 +805,13 @@ __global__ __launch_bounds__(key_block(kDim) * 2, kDim > 64 ? 2 : 3) void attent
     float *part_out = parts
                       + (bkv * blocks.parts() + blocks.first_part(block) + split) * 2 * kKeyBlock
                             * a.head_dim;
-    if (not_finite(dk[0]) || not_finite(dv[0])) {
+    if (not_finite(dk) || not_finite(dv)) {
         const int32_t channel = 2 * lane;
-        for (int m = 0; m < kWaveKeys; ++m) {
-            const int32_t key = wave_first + m;
-            if (key >= a.keys) break;
+        for (int32_t j = wave_first; j < min(wave_first + kWaveKeys, a.keys); ++j) {
             float kx = 0.0f, ky = 0.0f, vx = 0.0f, vy = 0.0f;
-            const bool there = key < length;
-            const uint32_t k_pair = there ? lane_pair(k + key * a.k_stride[2], a.head_dim) : 0u;
-            const uint32_t v_pair = there ? lane_pair(v + key * a.v_stride[2], a.head_dim) : 0u;
+            const bool there = j < length;
+            const uint32_t k_pair = there ? lane_pair(k + j * a.k_stride[2], a.head_dim) : 0u;
+            const uint32_t v_pair = there ? lane_pair(v + j * a.v_stride[2], a.head_dim) : 0u;
             for (int32_t t = begin; t < end; ++t) {
                 const int32_t h = kv * group + t / per_query_head;
                 const int32_t query = (low_tile + t % per_query_head) * kQueryStep;
@@ -804,7 +821,7 @@ __global__ __launch_bounds__(key_block(kDim) * 2, kDim > 64 ? 2 : 3) void attent
                                     + h * d.grad_stride[1];
                 const int64_t stats = (int64_t{b} * a.heads + h) * lse_pitch(a.queries);
                 for (int32_t i = query; i < min(query + kQueryStep, live); ++i) {
-                    if (!sight_of(a, i + shift, length)(key)) continue;
+                    if (!sight_of(a, i + shift, length)(j)) continue;
                     const uint32_t q_pair = lane_pair(q + i * a.q_stride[2], a.head_dim);
                     const uint32_t g_pair = lane_pair(g + i * d.grad_stride[2], a.head_dim);
                     const float weight = exp2_fast(__builtin_fmaf(
@@ -819,51 +836,47 @@ __global__ __launch_bounds__(key_block(kDim) * 2, kDim > 64 ? 2 : 3) void attent
             }
             if (channel >= a.head_dim) continue;
             if (splits > 1) {
-                float *dst = part_out + int64_t{key - first} * a.head_dim + channel;
+                float *dst = part_out + int64_t{j - first} * a.head_dim + channel;
                 *reinterpret_cast<f32x2 *>(dst) = f32x2{kx * a.scale, ky * a.scale};
                 *reinterpret_cast<f32x2 *>(dst + kKeyBlock * a.head_dim) = f32x2{vx, vy};
                 continue;
             }
             *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(d.dk) + b * d.dk_stride[0]
-                                          + kv * d.dk_stride[1] + key * d.dk_stride[2] + channel) =
+                                          + kv * d.dk_stride[1] + j * d.dk_stride[2] + channel) =
                 Element<kHalf>::round_pair(kx * a.scale, ky * a.scale);
             *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(d.dv) + b * d.dv_stride[0]
-                                          + kv * d.dv_stride[1] + key * d.dv_stride[2] + channel) =
+                                          + kv * d.dv_stride[1] + j * d.dv_stride[2] + channel) =
                 Element<kHalf>::round_pair(vx, vy);
         }
         return;
     }
     const float dv_scale = kHalf ? 1.0f / kHalfWeights : 1.0f;
-#pragma unroll
-    for (int m = 0; m < kGroups; ++m) {
-        const int32_t key = wave_first + 32 * m + (lane & 31);
-        if (key >= a.keys) continue;
-        if (splits == 1) {
-            store_row<kHalf, kColumns>(static_cast<uint16_t *>(d.dk) + b * d.dk_stride[0]
-                                           + kv * d.dk_stride[1] + key * d.dk_stride[2],
-                                       dk[m], a.scale, a.head_dim);
-            store_row<kHalf, kColumns>(static_cast<uint16_t *>(d.dv) + b * d.dv_stride[0]
-                                           + kv * d.dv_stride[1] + key * d.dv_stride[2],
-                                       dv[m], dv_scale, a.head_dim);
-            continue;
-        }
-        float *dst = part_out + int64_t{key - first} * a.head_dim;
-#pragma unroll
-        for (int c = 0; c < kColumns; ++c)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int32_t channel = 32 * c + 8 * g + 4 * half;
-                if (channel >= a.head_dim) continue;
-                f32x4 x, y;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    x[i] = dk[m][c][4 * g + i] * a.scale;
-                    y[i] = dv[m][c][4 * g + i] * dv_scale;
-                }
-                *reinterpret_cast<f32x4 *>(dst + channel) = x;
-                *reinterpret_cast<f32x4 *>(dst + kKeyBlock * a.head_dim + channel) = y;
-            }
+    if (key >= a.keys) return;
+    if (splits == 1) {
+        store_row<kHalf, kColumns>(static_cast<uint16_t *>(d.dk) + b * d.dk_stride[0]
+                                       + kv * d.dk_stride[1] + key * d.dk_stride[2],
+                                   dk, a.scale, a.head_dim);
+        store_row<kHalf, kColumns>(static_cast<uint16_t *>(d.dv) + b * d.dv_stride[0]
+                                       + kv * d.dv_stride[1] + key * d.dv_stride[2],
+                                   dv, dv_scale, a.head_dim);
+        return;
     }
+    float *dst = part_out + int64_t{key - first} * a.head_dim;
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int32_t channel = 32 * c + 8 * g + 4 * half;
+            if (channel >= a.head_dim) continue;
+            f32x4 x, y;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[i] = dk[c][4 * g + i] * a.scale;
+                y[i] = dv[c][4 * g + i] * dv_scale;
+            }
+            *reinterpret_cast<f32x4 *>(dst + channel) = x;
+            *reinterpret_cast<f32x4 *>(dst + kKeyBlock * a.head_dim + channel) = y;
+        }
 }
 
 // Adds the parts of the blocks from `first_block` on that have several, in
@@ -1037,7 +1050,8 @@ extern "C" int32_t lct_attention_backward(const lct_attention *a, const lct_atte
     blocks.sink_splits = sink_splits;
     const int64_t parts = blocks.parts() * a->batch * a->kv_heads;
     if (parts > kMaxAttentionItems
-        || int64_t{(a->queries + kQueryTile - 1) / kQueryTile} * a->batch * a->heads > kMaxAttentionItems
+        || int64_t{(a->queries + kQueryTile - 1) / kQueryTile} * a->batch * a->heads
+               > kMaxAttentionItems
         || int64_t{a->keys} * (a->head_dim / 4) * a->batch * a->kv_heads
                > kMaxAttentionItems * kAttentionThreads)
         return LCT_E_SIZE;

@@ -289,7 +289,8 @@ int32_t decode(const lct_attention &a, int32_t splits, float *workspace, hipStre
                                 decltype(cache)::value>
             <<<grid, kAttentionThreads, 0, stream>>>(a, splits, workspace);
     };
-    const int64_t seen = a.window > 0 ? std::min<int64_t>(a.keys, int64_t{a.window} + a.sinks) : a.keys;
+    const int64_t seen =
+        a.window > 0 ? std::min<int64_t>(a.keys, int64_t{a.window} + a.sinks) : a.keys;
     const bool stream_once = 4 * seen * a.batch * a.kv_heads * a.head_dim > kCacheBytes;
     by_width(a.head_dim, [&](auto width) {
         if (splits > 1 && stream_once)

@@ -229,8 +229,8 @@ int32_t launch(const lct_rotary &r, hipStream_t stream) {
     double best = 0.0;
     for (int64_t per = 1; per <= most; ++per) {
         const int64_t units = per * n.per_token;
-        const double used =
-            static_cast<double>(units) / static_cast<double>((units + kRound - 1) / kRound * kRound);
+        const double used = static_cast<double>(units)
+                            / static_cast<double>((units + kRound - 1) / kRound * kRound);
         if (used > best + 1e-9) {
             best = used;
             n.per_group = static_cast<int32_t>(per);
