@@ -105,7 +105,8 @@ __device__ __forceinline__ float of_lane(float v, int lane) {
 // of 64, window 256.  Tried: 32-key halves of a tile with the second half's scores
 // issued between the first's exponentials 1650 us at the first of these; matrix
 // phases at a higher wave priority 1560; column reads without the wait that the
-// compiler puts before them 1645; 64 queries per wave did not fit the registers.
+// compiler puts before them 1645; 64 queries per wave, which halve the LDS reads but
+// leave one wave per SIMD, 2020 with the instructions interleaved by hand.
 template <bool kHalf, int kDim, bool kSplit>
 __global__ __launch_bounds__(kAttentionThreads, 2) void attention_forward_kernel(
     lct_attention a, int32_t tiles, int32_t splits, float *__restrict__ parts) {

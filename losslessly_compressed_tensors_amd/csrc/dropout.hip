@@ -6,6 +6,9 @@
 // 2011), at counter (index / 8, offset) under the key `seed`; a value is kept
 // where its 16 bits are at least `below`.  The mask is a function of these
 // alone: it is never stored, and the gradient's pass draws it again.
+//
+// Bound by memory where the launch is not what counts (the ten rounds' products
+// take about half of the time that the values' bytes do): a thread has one draw.
 #include <type_traits>
 
 #include "attention_core.h"

@@ -73,7 +73,10 @@ struct Places {
 
 // A workgroup takes a few tokens: it computes their angles' sines and cosines
 // once, into LDS, for all of their heads, then moves its units, kAhead of a
-// thread's in flight.
+// thread's in flight.  Bound by memory: 127 us for 32767 tokens of 40 heads of 128
+// in FP16, half of each turned (5.3 TB/s; one unit at a time with the token's place
+// computed for each: 195), 10.9 us for 8 x 1024 tokens of 24 heads of 64, 4.4 us for
+// one token of 64 sequences, most of it the launch.
 template <int kType, int kVector, bool kInterleaved>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(lct_rotary r, Counts n) {
     using V = Value<kType>;

@@ -238,6 +238,9 @@ def rotate(plan, q: Tensor, k, positions, start: int, inverse: bool):
         k_in_stride, k_out_stride = k.stride()[:3], k_out.stride()[:3]
     at = b = t = 0
     if positions is not None:
+        if positions.ndim == 2 and positions.stride(1) == 0:
+            # A stride of 0 would mean that the sequence's tokens follow each other.
+            positions = positions.contiguous()
         at, b = positions.data_ptr(), positions.stride(0)
         t = positions.stride(1) if positions.ndim == 2 else 0
     _launch("lct_rotate", q.get_device(), hip.ROTARY.pack(

@@ -87,6 +87,20 @@ def test_positions(kind):
         assert bool(((y.cpu().double() - exact).abs() <= bound).all())
 
 
+def test_broadcast_positions():
+    """One position for all tokens of a sequence, or one row for all sequences."""
+    q = _values(3, 6, 2, 64, dtype=FP32)
+    plan = attention.Rotary(attention.rotary_frequencies(64))
+    for given in (torch.tensor([[7], [1], [0]], dtype=torch.int32, device=DEV).expand(3, 6),
+                  torch.arange(6, dtype=torch.int32, device=DEV).expand(3, 6),
+                  torch.tensor([9], dtype=torch.int32, device=DEV).expand(3)):
+        assert torch.equal(attention.apply_rotary(plan, q, positions=given),
+                           attention.apply_rotary(plan, q, positions=given.contiguous()))
+    same = torch.tensor([[7], [1], [0]], dtype=torch.int32, device=DEV).expand(3, 6)
+    _near(attention.apply_rotary(plan, q, positions=same), q, same,
+          attention.rotary_frequencies(64), FP32)
+
+
 def test_the_trainers_rotation():
     """The frequencies of the trainer's eager form, and its sense."""
     from examples.nanogpt.train_gpt_lct import Rotary
