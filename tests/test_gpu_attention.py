@@ -386,3 +386,38 @@ def test_infinities_reach_only_what_sees_them(where, value, dim, splits, monkeyp
         assert not bool(got["out"][:, :, rows].isfinite().all(-1).any()) or value == float("inf")
     assert bool(got["dq"][:, :, ~rows].isfinite().all())
     assert bool(got["dk"][:, :, ~keys].isfinite().all())
+
+
+def test_offsets_past_32_bits():
+    """A cache of over 2^31 bytes per tensor: its last tokens through the append,
+    the single-token and the chunk form, and the chunk's gradients."""
+    tokens, kv_heads, dim, window, sinks = 1_100_000, 8, 128, 300, 3
+    assert tokens * kv_heads * dim * 2 > 2 ** 31
+    caches = [torch.zeros(1, tokens, kv_heads, dim, dtype=BF16, device=DEV) for _ in range(2)]
+    near = 1000
+    for i, cache in enumerate(caches):
+        cache[:, :sinks] = _values(1, sinks, kv_heads, dim, seed=10 + i)
+        cache[:, -near:] = _values(1, near, kv_heads, dim, seed=20 + i)
+    plan = attention.Rotary(attention.rotary_frequencies(dim))
+    q, k, v = (_values(1, h, dim, seed=h) for h in (16, 8, 8))
+    at = torch.tensor([tokens - 1], dtype=torch.int32, device=DEV)
+    q = attention.rotary_append(plan, q, k, v, *caches, at)
+    assert torch.equal(caches[1][:, -1], v)
+    assert torch.equal(caches[0][:, -1:], attention.apply_rotary(plan, k.unsqueeze(1),
+                                                                 positions=at))
+    got = attention.decode_attention(q, *caches, at + 1, window=window, sinks=sinks)
+    # The same keys next to each other: sinks, then the last 1000.
+    small = [torch.cat([c[:, :sinks], c[:, -near:]], 1).transpose(1, 2) for c in caches]
+    seen = oracle.sees(1, sinks + near, window, sinks).to(DEV)
+    _check({"out": got.unsqueeze(2)},
+           oracle.attention_with_bounds(q.unsqueeze(2), *small, seen, dim ** -0.5))
+
+    queries = 70
+    chunk, grad = (_values(1, queries, 16, dim, seed=s).transpose(1, 2) for s in (31, 32))
+    result = _run(chunk, *(c.transpose(1, 2) for c in caches), grad, window=window, sinks=sinks)
+    seen = oracle.sees(queries, sinks + near, window, sinks).to(DEV)
+    for name in ("dk", "dv"):
+        full = result[name]
+        assert bool((full[:, :, sinks:-near] == 0).all())
+        result[name] = torch.cat([full[:, :, :sinks], full[:, :, -near:]], 2)
+    _check(result, oracle.attention_with_bounds(chunk, *small, seen, dim ** -0.5, grad))
