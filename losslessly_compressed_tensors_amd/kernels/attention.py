@@ -53,6 +53,17 @@ def _readable(t: Tensor) -> Tensor:
     return t.clone(memory_format=torch.contiguous_format)
 
 
+def _cache(t: Tensor) -> tuple:
+    """A [batch, token, head, channel] cache as :func:`_readable` would have it, and
+    its strides of batch, head and token."""
+    b, n, h, c = t.stride()
+    if c == 1 and not (b | h | n) & 7 and n < 1 << 24 and not t.data_ptr() & 15:
+        return t, (b, h, n)
+    t = _readable(t.transpose(1, 2)).transpose(1, 2)
+    b, n, h, _ = t.stride()
+    return t, (b, h, n)
+
+
 def _token_major(like: Tensor) -> Tensor:
     """A new [batch, head, token, channel] tensor in token-major storage."""
     b, h, t, d = like.shape
@@ -200,20 +211,23 @@ def attention_decode(q: Tensor, k_cache: Tensor, v_cache: Tensor, window: int, s
                      scale: float, lengths) -> Tensor:
     """[batch, head, channel] of queries of that shape over [batch, token, head,
     channel] caches."""
-    if (q.stride(2) != 1 or (q.stride(0) | q.stride(1)) & 7 or q.data_ptr() & 15):
+    qb, qh, qc = q.stride()
+    if qc != 1 or (qb | qh) & 7 or q.data_ptr() & 15:
         q = q.clone(memory_format=torch.contiguous_format)
-    k, v = (_readable(t.transpose(1, 2)) for t in (k_cache, v_cache))
+        qb, qh, _ = q.stride()
+    k_cache, k_stride = _cache(k_cache)
+    v_cache, v_stride = _cache(v_cache)
     batch, heads, dim = q.shape
+    _, capacity, kv_heads, _ = k_cache.shape
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    _, kv_heads, capacity, _ = k.shape
     splits = decode_splits(batch, heads, kv_heads, capacity, window, sinks)
     floats = batch * heads * splits * (dim + 2) if splits > 1 else 0
     workspace, address = _workspace(q, floats)
     _launch("lct_attention_decode", q.get_device(), hip.ATTENTION.pack(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0,
-        0 if lengths is None else lengths.data_ptr(), *q.stride()[:2], 0, *k.stride()[:3],
-        *v.stride()[:3], heads * dim, dim, 0, batch, heads, kv_heads, 1, capacity, dim, window,
-        sinks, q.dtype == torch.float16, scale), splits, address, floats)
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), 0,
+        0 if lengths is None else lengths.data_ptr(), qb, qh, 0, *k_stride, *v_stride, heads * dim,
+        dim, 0, batch, heads, kv_heads, 1, capacity, dim, window, sinks, q.dtype == torch.float16,
+        scale), splits, address, floats)
     return out
 
 
