@@ -233,6 +233,32 @@ def test_decode_parts_and_head_major_caches(splits, monkeypatch):
             oracle.sees(1, n, 300, 9).to(DEV), 0.3))
 
 
+def test_decode_of_strided_and_misaligned_tensors():
+    """Results of plain copies: a query and caches at odd addresses, channels not
+    adjacent, slices of wider tensors."""
+    q = _values(2, 4, 64)
+    k, v = (_values(2, 90, 2, 64, seed=s) for s in (1, 2))
+    lengths = torch.tensor([90, 31], device=DEV)
+    want = attention.decode_attention(q, k, v, lengths, window=20, sinks=1)
+
+    def odd(t):
+        out = torch.zeros(t.numel() + 1, dtype=BF16, device=DEV)[1:].view(t.shape)
+        out.copy_(t)
+        return out
+
+    def turned(t):
+        return t.transpose(-1, -2).contiguous().transpose(-1, -2)
+
+    def slice_of_wider(t):
+        wide = torch.zeros(*t.shape[:-1], 72, dtype=BF16, device=DEV)
+        wide[..., :64] = t
+        return wide[..., :64]
+
+    for other in (odd, turned, slice_of_wider):
+        got = attention.decode_attention(other(q), other(k), other(v), lengths, window=20, sinks=1)
+        assert torch.equal(got, want)
+
+
 def test_decode_is_the_last_row_of_attention():
     """The cache's path and the prompt's agree within their bounds."""
     plan = attention.Rotary(attention.rotary_frequencies(64))
