@@ -100,14 +100,16 @@ __device__ __forceinline__ float of_lane(float v, int lane) {
 // Matrix instructions, LDS reads (one fragment per instruction) and the softmax's
 // vector instructions take about 512, 512 and 450 clocks of a SIMD per 32 x 32
 // scores at heads of 128, at 1.9 to 2.0 GHz under this load; the two waves of a
-// SIMD overlap them in part (matrix instructions busy half of the time).  1560 us
-// for 8191 queries after 8192 keys, 32 heads of 128 over 8 (1057 TFLOP/s); 495 us
-// for 1 x 16384, 16 heads over 4, window 4096 (970); 22 us for 8 x 1024, 12 heads
-// of 64, window 256.  Tried: 32-key halves of a tile with the second half's scores
-// issued between the first's exponentials 1650 us at the first of these; matrix
-// phases at a higher wave priority 1560; column reads without the wait that the
-// compiler puts before them 1645; 64 queries per wave, which halve the LDS reads but
-// leave one wave per SIMD, 2020 with the instructions interleaved by hand.
+// SIMD overlap them in part (matrix instructions busy half of the time).  1525 us
+// for 8191 queries after 8192 keys, 32 heads of 128 over 8 (1080 TFLOP/s; 1580
+// with the compiler's order of LDS reads in place of read_ahead); 485 us for 1 x
+// 16384, 16 heads over 4, window 4096 (990); 22 us for 8 x 1024, 12 heads of 64,
+// window 256.  Tried: 32-key halves of a tile with the second half's scores issued
+// between the first's exponentials 1650 us at the first of these; matrix phases at
+// a higher wave priority 1560; column reads without the wait that the compiler puts
+// before them 1645; 64 queries per wave, which halve the LDS reads but leave one
+// wave per SIMD, 2020 with the instructions interleaved by hand; 8 waves per
+// workgroup, 4 in their products while the other 4 are in their softmax, 1605.
 template <bool kHalf, int kDim, bool kSplit>
 __global__ __launch_bounds__(kAttentionThreads, 2) void attention_forward_kernel(
     lct_attention a, int32_t tiles, int32_t splits, float *__restrict__ parts) {
@@ -189,6 +191,7 @@ __global__ __launch_bounds__(kAttentionThreads, 2) void attention_forward_kernel
             for (int d = 0; d < kSteps; ++d)
                 s[n] = Element<kHalf>::multiply(read_rows<kPitch>(keys, n, d), q_operand[d], s[n]);
         }
+        read_ahead<2 * kSteps, 1, 2>();
         if (!seen_by_all) {
             const TileSight sight(a, position, key);
 #pragma unroll
@@ -229,6 +232,7 @@ __global__ __launch_bounds__(kAttentionThreads, 2) void attention_forward_kernel
                     out[c] = Element<kHalf>::multiply(
                         read_columns<kPitch>(values, 32 * n + 16 * p, c), weights, out[c]);
             }
+        read_ahead<4 * kColumns, 2, 6>();
     };
 
     if (begin < end) load(begin, k_even, v_even);
@@ -388,8 +392,9 @@ __global__ __launch_bounds__(kAttentionThreads) void attention_join_kernel(
 // A wave's 32 queries, the keys in tiles of 64: as in the forward kernel, with dP
 // beside the scores (its sums begin at -delta) and the keys' columns for the last
 // product.  delta is taken from the operands on their way in, and stored for the
-// other kernel.  685 us for 1 x 16384, 16 heads of 128 over 4, window 4096 (1055
-// TFLOP/s), 30 us for 8 x 1024, 12 heads of 64, window 256.
+// other kernel.  650 us for 1 x 16384, 16 heads of 128 over 4, window 4096 (1110
+// TFLOP/s; 690 with the compiler's order of LDS reads), 29 us for 8 x 1024, 12
+// heads of 64, window 256.
 template <bool kHalf, int kDim>
 __global__ __launch_bounds__(kAttentionThreads, 2) void attention_dq_kernel(
     lct_attention a, lct_attention_gradients d, int32_t tiles) {
@@ -485,6 +490,7 @@ __global__ __launch_bounds__(kAttentionThreads, 2) void attention_dq_kernel(
                 s = Element<kHalf>::multiply(read_rows<kPitch>(keys, n, i), q_operand[i], s);
                 e = Element<kHalf>::multiply(read_rows<kPitch>(values, n, i), g_operand[i], e);
             }
+            read_ahead<2 * kSteps, 1, 4>();
 #pragma unroll
             for (int r = 0; r < 16; ++r)
                 s[r] = exp2_fast(__builtin_fmaf(s[r], factor, -lse)) * e[r];
@@ -504,6 +510,7 @@ __global__ __launch_bounds__(kAttentionThreads, 2) void attention_dq_kernel(
                         dq[c] = Element<kHalf>::multiply(
                             read_columns<kPitch>(keys, 32 * n + 16 * p, c), ds, dq[c]);
                 }
+                read_ahead<2 * kColumns, 2, 6>();
             }
         }
     };
@@ -616,10 +623,12 @@ __host__ __device__ constexpr int key_block(int dim) { return dim > 64 ? 256 : 1
 // bytes a clock, what four SIMDs' matrix instructions use) and the matrix
 // instructions are busy alike.  Heads wider than 64 hold 128 registers of sums and
 // 32 of the keys' operands; the values' stay in LDS (64 KB for 256 keys, read
-// again for each tile), so that two waves share a SIMD.  1111 us for 1 x 16384, 16
-// heads of 128 over 4, window 4096 (870 TFLOP/s); 64 keys per wave at one wave
-// per SIMD, which read half as much: 1420; 32 with all operands in registers at
-// one wave per SIMD: 2200.  8 x 1024, 12 heads of 64, window 256: 38 us, bound by
+// again for each tile), so that two waves share a SIMD.  1080 us for 1 x 16384, 16
+// heads of 128 over 4, window 4096 (890 TFLOP/s; 1110 with the compiler's order of
+// LDS reads; 0.16 of it the end, when the workgroups of the last keys, which fewer
+// queries see, are done: parts of equal work would cost as much to add); 64 keys
+// per wave at one wave per SIMD, which read half as much: 1420; 32 with all
+// operands in registers at one wave per SIMD: 2200.  8 x 1024, 12 heads of 64, window 256: 38 us, bound by
 // the exponentials, masks and conversions of three waves per SIMD (two: 42).
 template <bool kHalf, int kDim>
 __global__ __launch_bounds__(key_block(kDim) * 2, kDim > 64 ? 2 : 3) void attention_dkdv_kernel(
@@ -753,6 +762,17 @@ __global__ __launch_bounds__(key_block(kDim) * 2, kDim > 64 ? 2 : 3) void attent
                 kStaged ? read_rows<kPitch>(v_block, wave, i) : v_operand[kStaged ? 0 : i];
             e = Element<kHalf>::multiply(read_rows<kPitch>(g_tile, n, i), v_rows, e);
         }
+        if constexpr (kStaged) {
+            // delta's reads and 4 more, then 3 reads for every 2 products.
+            __builtin_amdgcn_sched_group_barrier(kLdsReadGroup, 8, 0);
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                __builtin_amdgcn_sched_group_barrier(kMatrixGroup, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(kLdsReadGroup, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(kMatrixGroup, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(kLdsReadGroup, 2, 0);
+            }
+        }
         if (!all) {
             // Position - key: from 0 to below what the key's place allows; rows past
             // the sequence are few tiles' (uniform).
@@ -792,6 +812,7 @@ __global__ __launch_bounds__(key_block(kDim) * 2, kDim > 64 ? 2 : 3) void attent
                     read_columns<kPitch>(q_tile, 32 * n + 16 * p, c), ds, dk[c]);
             }
         }
+        if constexpr (kStaged) read_ahead<4 * kColumns, 2, 4>();
     };
     const auto step = [&](const uint16_t *q_tile, const uint16_t *g_tile, const float *stats)
                           __attribute__((always_inline)) {

@@ -163,6 +163,23 @@ __device__ __forceinline__ u32x4 read_columns(const uint16_t *tile, int first, i
     return u32x4{lo[0], lo[1], hi[0], hi[1]};
 }
 
+// The order of the matrix products since the last branch and of the LDS reads that
+// feed them: kFirst reads, then a product and the next kReads reads in turn.  (Left
+// alone, the compiler reads an operand just before its product, which then waits
+// for LDS.)
+constexpr int kMatrixGroup = 0x008, kLdsReadGroup = 0x100;    // sched_group_barrier's masks
+template <int kProducts, int kReads, int kFirst>
+__device__ __forceinline__ void read_ahead() {
+    constexpr int kLeft = kProducts - kFirst / kReads;
+    __builtin_amdgcn_sched_group_barrier(kLdsReadGroup, kFirst, 0);
+#pragma unroll
+    for (int i = 0; i < kLeft; ++i) {
+        __builtin_amdgcn_sched_group_barrier(kMatrixGroup, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(kLdsReadGroup, kReads, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(kMatrixGroup, kFirst / kReads, 0);
+}
+
 // Two groups (8 registers) of a tile of scores as the next operand.
 template <bool kHalf>
 __device__ __forceinline__ u32x4 as_operand(const f32x16 &s, int pair) {
