@@ -628,8 +628,9 @@ __host__ __device__ constexpr int key_block(int dim) { return dim > 64 ? 256 : 1
 // LDS reads; 0.16 of it the end, when the workgroups of the last keys, which fewer
 // queries see, are done: parts of equal work would cost as much to add); 64 keys
 // per wave at one wave per SIMD, which read half as much: 1420; 32 with all
-// operands in registers at one wave per SIMD: 2200.  8 x 1024, 12 heads of 64, window 256: 38 us, bound by
-// the exponentials, masks and conversions of three waves per SIMD (two: 42).
+// operands in registers at one wave per SIMD: 2200.  8 x 1024, 12 heads of 64,
+// window 256: 38 us, bound by the exponentials, masks and conversions of three
+// waves per SIMD (two: 42).
 template <bool kHalf, int kDim>
 __global__ __launch_bounds__(key_block(kDim) * 2, kDim > 64 ? 2 : 3) void attention_dkdv_kernel(
     lct_attention a, lct_attention_gradients d, KeyBlocks blocks, float *__restrict__ parts) {
