@@ -365,8 +365,9 @@ def window_attention(q: Tensor, k: Tensor, v: Tensor, *, window: int | None = No
     do not depend on timing."""
     window, sinks, scale, lengths = check_attention(q, k, v, window, sinks, scale, lengths)
     if q.numel() == 0 or k.shape[2] == 0:
-        # Nothing to compute, or nothing to see: zero, with zero gradients.
-        return q * 0 + (k.sum() + v.sum()) * 0
+        # Nothing to compute, or nothing to see: zero whatever q holds, with zero
+        # gradients.
+        return torch.zeros_like(q) + sum(t[..., :0].sum() for t in (q, k, v))
     if _recorded(q, k, v):
         return _WindowAttention.apply(q, k, v, lengths, window, sinks, scale)
     return kernels.attention_forward(q, k, v, window, sinks, scale, lengths, False)[0]

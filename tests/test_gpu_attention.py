@@ -329,6 +329,17 @@ def test_a_captured_step_replays():
             assert torch.equal(result, want)
 
 
+def test_nothing_to_see_is_zero_whatever_the_query_holds():
+    q = _values(1, 2, 3, 64)
+    q[0, 0, 0, 0], q[0, 1, 2, 3] = float("inf"), float("nan")
+    q.requires_grad_()
+    none = _values(1, 2, 0, 64)
+    out = attention.window_attention(q, none, none)
+    assert bool((out == 0).all())
+    out.sum().backward()
+    assert bool((q.grad == 0).all())
+
+
 def test_refusals():
     q, k = _values(1, 4, 5, 64), _values(1, 2, 5, 64)
     call = attention.window_attention
