@@ -88,7 +88,8 @@ def _indices(t, name: str, shapes, device) -> Tensor:
                          f"got {tuple(t.shape)}")
     if t.device != device:
         raise ValueError(f"{name} must be on {device}")
-    return t if t.dtype == torch.int32 else t.to(torch.int32)
+    # Not modulo 2^32: a length or place that INT32 does not hold is past the end.
+    return t if t.dtype == torch.int32 else t.clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32)
 
 
 # ---- rotary positions
@@ -217,7 +218,7 @@ def apply_rotary(plan: Rotary, q: Tensor, k: Tensor | None = None, positions=Non
     """``q`` and ``k``, [batch, token, head, channel] of BF16, FP16 or FP32, turned
     by their positions: ``(q, k)``, or ``q`` alone.  ``positions``: None (0, 1, ..),
     the first token's as an integer or per sequence as [batch], or each token's
-    as [batch, token] (INT32; INT64 is converted).  Angles and products are FP32,
+    as [batch, token] (INT32; INT64 is held to INT32's range).  Angles and products are FP32,
     rounded once.  Differentiable in ``q`` and ``k``."""
     _check_tensor(q, "q", 4, _ROTARY_TYPES)
     _check_rotary(plan, q)

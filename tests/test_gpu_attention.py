@@ -340,6 +340,20 @@ def test_nothing_to_see_is_zero_whatever_the_query_holds():
     assert bool((q.grad == 0).all())
 
 
+def test_lengths_past_32_bits_count_as_the_capacity():
+    q, cache = _values(3, 4, 64), _values(3, 20, 2, 64, seed=1)
+    got = attention.decode_attention(
+        q, cache, cache, torch.tensor([2 ** 32 + 5, 20, -2 ** 32 + 20], device=DEV))
+    want = attention.decode_attention(q, cache, cache, torch.tensor([20, 20, 0], device=DEV))
+    assert torch.equal(got, want)
+    # A place past the cache is not written.
+    plan = attention.Rotary(attention.rotary_frequencies(64))
+    before = cache.clone()
+    attention.rotary_append(plan, q, q[:, :2], q[:, 2:], cache, cache.clone(),
+                            torch.tensor([2 ** 32, 2 ** 33 + 1, -2 ** 32], device=DEV))
+    assert torch.equal(cache, before)
+
+
 def test_refusals():
     q, k = _values(1, 4, 5, 64), _values(1, 2, 5, 64)
     call = attention.window_attention
