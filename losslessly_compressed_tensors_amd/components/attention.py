@@ -413,6 +413,8 @@ class KVCache:
                            for n, name in ((batch, "batch"), (capacity, "capacity")))
         if dtype not in _ATTENTION_TYPES:
             raise TypeError("the cache holds BF16 or FP16")
+        kv_heads = _whole(kv_heads, "kv_heads", 1, _MAX_HEADS)
+        head_dim = _whole(head_dim, "head_dim", 8, kernels.MAX_HEAD_DIM)
         _check_heads(kv_heads, kv_heads, head_dim)
         shape = (batch, capacity, kv_heads, head_dim)
         self.k = torch.zeros(shape, dtype=dtype, device=device)
@@ -429,30 +431,42 @@ class KVCache:
         self.lengths.zero_()
         self._most = 0
 
-    def _grow(self, tokens: int) -> None:
+    def _check_room(self, tokens: int) -> None:
         if self._most + tokens > self.capacity:
             raise ValueError(f"the cache holds {self.capacity} tokens, {self._most + tokens} asked")
+
+    def _grow(self, tokens: int) -> None:
+        self._check_room(tokens)
         self._most += tokens
 
     def append(self, plan: Rotary, q: Tensor, k: Tensor, v: Tensor) -> Tensor:
         """One new token for every sequence: ``q``, ``k``, ``v`` [batch, head, channel].
         Returns ``q`` turned; ``k`` (turned) and ``v`` are in the cache."""
-        self._grow(1)
+        self._check_room(1)
         out = rotary_append(plan, q, k, v, self.k, self.v, self.lengths)
         self.lengths += 1
+        self._grow(1)
         return out
 
     def fill(self, plan: Rotary, q: Tensor, k: Tensor, v: Tensor) -> tuple:
         """The prompts of an empty cache, [batch, token, head, channel], all of one
-        length: returns ``q`` and ``k`` turned; ``k`` (turned) and ``v`` are in the cache."""
+        length: returns ``q`` and ``k`` turned; ``k`` (turned) and ``v`` are in the cache.
+        Not differentiable."""
         if self._most:
             raise ValueError("fill() takes an empty cache")
+        _check_like(k, "k", self.k, 4)
+        _check_like(v, "v", self.k, 4)
+        batch, tokens, *heads = k.shape
+        if v.shape != k.shape or batch != self.k.shape[0] or tuple(heads) != self.k.shape[2:]:
+            raise ValueError("k and v must be [batch, token, head, channel] of the cache's heads")
+        if _recorded(q, k, v):
+            raise ValueError(_NO_GRADIENT)
+        self._check_room(tokens)
         q, k = apply_rotary(plan, q, k)
-        tokens = k.shape[1]
-        self._grow(tokens)
         self.k[:, :tokens] = k
         self.v[:, :tokens] = v
         self.lengths.fill_(tokens)
+        self._grow(tokens)
         return q, k
 
     def attend(self, q: Tensor, *, window: int | None = None, sinks: int = 0,

@@ -354,6 +354,31 @@ def test_lengths_past_32_bits_count_as_the_capacity():
     assert torch.equal(cache, before)
 
 
+def test_a_refused_call_leaves_the_cache_as_it_was():
+    plan = attention.Rotary(attention.rotary_frequencies(64))
+    cache = attention.KVCache(2, 4, 2, 64)
+    q, k = _values(2, 3, 4, 64), _values(2, 3, 2, 64)
+    for bad, error, match in (
+            (lambda: cache.fill(plan, q, k, k[:1]), ValueError, "cache's heads"),
+            (lambda: cache.fill(plan, q, k[:, :, :1], k[:, :, :1]), ValueError, "cache's heads"),
+            (lambda: cache.fill(plan, q, k, k.half()), TypeError, "one type"),
+            (lambda: cache.fill(plan, q.half(), k, k), TypeError, "one type"),
+            (lambda: cache.fill(plan, q, k.clone().requires_grad_(), k), ValueError, "gradient"),
+            (lambda: cache.fill(plan, *[torch.cat([t, t], 1) for t in (q, k, k)]), ValueError,
+             "holds 4 tokens"),
+            (lambda: cache.append(plan, q[:, 0], k[:, 0], k[:1, 0]), ValueError, "agree"),
+            (lambda: attention.KVCache(1, 4, 0, 64), ValueError, "kv_heads"),
+            (lambda: attention.KVCache(1, 4, 2.0, 64), TypeError, "kv_heads")):
+        with pytest.raises(error, match=match):
+            bad()
+    cache.fill(plan, q, k, k)
+    cache.append(plan, q[:, 0], k[:, 0], k[:, 0])
+    assert cache.lengths.tolist() == [4, 4]
+    with pytest.raises(ValueError, match="holds 4 tokens"):
+        cache.append(plan, q[:, 0], k[:, 0], k[:, 0])
+    assert cache.lengths.tolist() == [4, 4]
+
+
 def test_refusals():
     q, k = _values(1, 4, 5, 64), _values(1, 2, 5, 64)
     call = attention.window_attention
