@@ -267,6 +267,10 @@ def rotary_append(plan: Rotary, q: Tensor, k: Tensor, v: Tensor, k_cache: Tensor
         raise ValueError("the caches must be [batch, capacity, head, channel] of k's heads")
     if k_cache.stride(3) != 1 or v_cache.stride(3) != 1:
         raise ValueError("the caches' channels must be adjacent")
+    for cache in (k_cache, v_cache):
+        if 0 in cache.stride() and any(s == 0 and n > 1
+                                       for s, n in zip(cache.stride(), cache.shape)):
+            raise ValueError("the caches must not be expanded: tokens would overwrite each other")
     if _recorded(q, k, v, k_cache, v_cache):
         raise ValueError(_NO_GRADIENT)
     if kv_heads > _MAX_HEADS or k_cache.shape[1] > kernels.MAX_TOKENS:
@@ -274,7 +278,10 @@ def rotary_append(plan: Rotary, q: Tensor, k: Tensor, v: Tensor, k_cache: Tensor
     positions = _indices(positions, "positions", ((batch,),), q.device)
     if q.numel() == 0 or k_cache.numel() == 0:
         raise ValueError("rotary_append needs a token and a cache")
-    return kernels.rotate_into(plan, q, k, v, k_cache, v_cache, positions)
+    q = kernels.rotate_into(plan, q, k, v, k_cache, v_cache, positions)
+    # Written: a graph that has saved them must notice.
+    torch.autograd.graph.increment_version((k_cache, v_cache))
+    return q
 
 
 # ---- attention

@@ -379,6 +379,21 @@ def test_a_refused_call_leaves_the_cache_as_it_was():
     assert cache.lengths.tolist() == [4, 4]
 
 
+def test_append_writes_to_its_caches_alone():
+    plan = attention.Rotary(attention.rotary_frequencies(64))
+    q, k = _values(2, 4, 64), _values(2, 2, 64)
+    cache, at = _values(2, 5, 2, 64), torch.zeros(2, dtype=torch.int32, device=DEV)
+    for shared in (cache[:1].expand(2, 5, 2, 64), cache[:, :1].expand(2, 5, 2, 64)):
+        with pytest.raises(ValueError, match="expanded"):
+            attention.rotary_append(plan, q, k, k, shared, cache, at)
+    # A graph that has saved a cache refuses to go on with other values.
+    weights = torch.ones(64, dtype=BF16, device=DEV, requires_grad=True)
+    out = (cache * weights).sum()
+    attention.rotary_append(plan, q, k, k, cache, cache.clone(), at)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.backward()
+
+
 def test_refusals():
     q, k = _values(1, 4, 5, 64), _values(1, 2, 5, 64)
     call = attention.window_attention
