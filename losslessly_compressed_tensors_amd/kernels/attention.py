@@ -198,7 +198,7 @@ def decode_splits(batch: int, heads: int, kv_heads: int, capacity: int, window: 
     257 keys, 7.6 | 7.4 at 1024, two and four parts); above, three workgroups per
     compute unit (8 heads of 8192 keys: 73 in one part, 20 in 6, 13.4 in 24, 16 in
     64; 128 of 4096: 75, 40 in 6, 43 in 8, 59 in 32), with 256 keys each at least,
-    and of long caches parts of 3072 keys at most, so that sequences of unequal
+    and of long caches parts of 24 tiles at most, so that sequences of unequal
     length even out (32 heads of 131072: 316 in 16 parts, 275 in 64)."""
     items = batch * kv_heads * -(-(heads // kv_heads) // 16)
     tiles = -(-_seen(capacity, window, sinks, 1) // _DECODE_TILE)
