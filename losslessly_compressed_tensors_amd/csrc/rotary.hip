@@ -68,15 +68,16 @@ __device__ __forceinline__ int64_t position_of(const lct_rotary &r, int64_t b, i
 
 // Where a token's q, k and v are and go (elements; k's and v's place -1: nowhere).
 struct Places {
-    int64_t in[3], out[3];
+    int64_t position, in[3], out[3];
 };
 
 // A workgroup takes a few tokens: it computes their angles' sines and cosines
-// once, into LDS, for all of their heads, then moves its units, kAhead of a
-// thread's in flight.  Bound by memory: 127 us for 32767 tokens of 40 heads of 128
-// in FP16, half of each turned (5.3 TB/s; one unit at a time with the token's place
-// computed for each: 195), 10.9 us for 8 x 1024 tokens of 24 heads of 64, 4.4 us for
-// one token of 64 sequences, most of it the launch.
+// once, into LDS, for all of their heads, while its first units are on their way,
+// then moves its units, kAhead of a thread's in flight.  Bound by memory: 127 us
+// for 32767 tokens of 40 heads of 128 in FP16, half of each turned (5.3 TB/s; one
+// unit at a time with the token's place computed for each: 195), 10.3 us for 8 x
+// 1024 tokens of 24 heads of 64 (the angles before the first loads: 10.9), 4.3 us
+// for one token of 64 sequences, most of it the launch.
 template <int kType, int kVector, bool kInterleaved>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(lct_rotary r, Counts n) {
     using V = Value<kType>;
@@ -91,17 +92,12 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(lct_rotary r, Counts n
     const int64_t first = int64_t{blockIdx.x} * n.per_group;
     const int32_t here = static_cast<int32_t>(min(int64_t{n.per_group}, tokens - first));
     const int32_t pairs = r.rotary_dim / 2;
-    for (int32_t i = threadIdx.x; i < here * pairs; i += kThreads) {
-        const int32_t token = i / pairs, pair = i % pairs;
-        const int64_t b = (first + token) / r.tokens, t = (first + token) % r.tokens;
+    if (static_cast<int32_t>(threadIdx.x) < here) {
+        static_assert(kMaxTokens <= kThreads, "a thread per token");
+        const int64_t token = first + threadIdx.x, b = token / r.tokens, t = token % r.tokens;
         const int64_t p = position_of(r, b, t);
-        const int64_t angle = static_cast<int64_t>(static_cast<uint64_t>(p)
-                                                   * static_cast<uint64_t>(r.turns[pair]));
-        float sine, cosine;
-        sincospif(static_cast<float>(angle) * 0x1p-63f, &sine, &cosine);
-        turn[i] = f32x2{cosine * r.magnitude, (r.inverse ? -sine : sine) * r.magnitude};
-        if (pair != 0) continue;
-        Places &at = places[token];
+        Places &at = places[threadIdx.x];
+        at.position = p;
         at.in[0] = b * r.q_in_stride[0] + t * r.q_in_stride[1];
         at.in[1] = b * r.k_in_stride[0] + t * r.k_in_stride[1];
         at.in[2] = b * r.v_in_stride[0] + t * r.v_in_stride[1];
@@ -114,11 +110,11 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(lct_rotary r, Counts n
     __syncthreads();
 
     const int32_t items = here * n.per_token;
-    for (int32_t base = threadIdx.x; base < items; base += kAhead * kThreads) {
-        Pack x[kAhead], y[kAhead];
-        Bits *dst[kAhead];           // null: nothing to store
-        int32_t angles[kAhead];      // first of the unit's in `turn`, or -1: a copy
-        int32_t gap[kAhead];         // from x's channels to y's, or 0: no y
+    Pack x[kAhead], y[kAhead];
+    Bits *dst[kAhead];           // null: nothing to store
+    int32_t angles[kAhead];      // first of the unit's in `turn`, or -1: a copy
+    int32_t gap[kAhead];         // from x's channels to y's, or 0: no y
+    const auto load = [&](int32_t base) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
             dst[u] = nullptr;
@@ -164,6 +160,8 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(lct_rotary r, Counts n
             x[u] = *reinterpret_cast<const Pack *>(src);
             if (gap[u] != 0) y[u] = *reinterpret_cast<const Pack *>(src + gap[u]);
         }
+    };
+    const auto store = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
             if (dst[u] == nullptr) continue;
@@ -192,6 +190,23 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(lct_rotary r, Counts n
             *reinterpret_cast<Pack *>(dst[u]) = x[u];
             if (gap[u] != 0) *reinterpret_cast<Pack *>(dst[u] + gap[u]) = y[u];
         }
+    };
+
+    load(threadIdx.x);
+    for (int32_t i = threadIdx.x; i < here * pairs; i += kThreads) {
+        const int32_t token = i / pairs;
+        const int64_t angle =
+            static_cast<int64_t>(static_cast<uint64_t>(places[token].position)
+                                 * static_cast<uint64_t>(r.turns[i - token * pairs]));
+        float sine, cosine;
+        sincospif(static_cast<float>(angle) * 0x1p-63f, &sine, &cosine);
+        turn[i] = f32x2{cosine * r.magnitude, (r.inverse ? -sine : sine) * r.magnitude};
+    }
+    __syncthreads();
+    for (int32_t base = threadIdx.x; base < items;) {
+        store();
+        base += kAhead * kThreads;
+        if (base < items) load(base);
     }
 }
 
