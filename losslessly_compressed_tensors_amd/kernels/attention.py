@@ -14,6 +14,7 @@ from functools import lru_cache
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import hip
 
@@ -37,6 +38,17 @@ def _launch(name: str, device: int, *args) -> None:
     else:
         with torch.cuda.device(device):
             hip.call(name, *args, torch._C._cuda_getCurrentRawStream(device))
+
+
+def _check_unrecorded(*tensors) -> None:
+    """A launch is no operation of torch's, and has none to fall back to: what records
+    or differentiates operations as they run would go on with an unwritten result."""
+    if torch._C._get_tracing_state() is not None or torch._C._len_torch_dispatch_stack():
+        raise RuntimeError("this operator cannot be recorded: a trace or a dispatch mode is active")
+    if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled():
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("this operator has no forward-mode derivative")
 
 
 def _readable(t: Tensor) -> Tensor:
@@ -114,6 +126,7 @@ def forward_splits(batch: int, heads: int, queries: int, keys: int, window: int,
 def attention_forward(q: Tensor, k: Tensor, v: Tensor, window: int, sinks: int, scale: float,
                       lengths, need_lse: bool):
     """``(out, lse)``; ``lse`` is what :func:`attention_backward` needs, or None."""
+    _check_unrecorded(q, k, v)
     q, k, v = _readable(q), _readable(k), _readable(v)
     batch, heads, queries, dim = q.shape
     out = _token_major(q)
@@ -167,6 +180,7 @@ def backward_splits(batch: int, heads: int, kv_heads: int, queries: int, keys: i
 def attention_backward(grad: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor,
                        window: int, sinks: int, scale: float, lengths):
     """``(dq, dk, dv)``."""
+    _check_unrecorded(grad, q, k, v)
     q, k, v, out, grad = (_readable(t) for t in (q, k, v, out, grad))
     batch, heads, queries, dim = q.shape
     kv_heads, keys = k.shape[1], k.shape[2]
@@ -211,6 +225,7 @@ def attention_decode(q: Tensor, k_cache: Tensor, v_cache: Tensor, window: int, s
                      scale: float, lengths) -> Tensor:
     """[batch, head, channel] of queries of that shape over [batch, token, head,
     channel] caches."""
+    _check_unrecorded(q, k_cache, v_cache)
     qb, qh, qc = q.stride()
     if qc != 1 or (qb | qh) & 7 or q.data_ptr() & 15:
         q = q.clone(memory_format=torch.contiguous_format)
@@ -237,6 +252,7 @@ _NO_STRIDES = (0, 0, 0)
 def rotate(plan, q: Tensor, k, positions, start: int, inverse: bool):
     """The rotated ``(q, k)`` of [batch, token, head, channel] tensors; ``k`` may be
     None."""
+    _check_unrecorded(q, k)
     if q.stride(3) != 1:
         q = q.contiguous()
     batch, tokens, heads, dim = q.shape
@@ -269,6 +285,7 @@ def rotate_into(plan, q: Tensor, k: Tensor, v: Tensor, k_cache: Tensor, v_cache:
                 positions: Tensor) -> Tensor:
     """The rotated ``q`` [batch, head, channel]; ``k``, rotated, and ``v`` go to the
     [batch, token, head, channel] caches at ``positions``."""
+    _check_unrecorded(q, k, v, k_cache, v_cache)
     q, k, v = (t if t.stride(2) == 1 else t.contiguous() for t in (q, k, v))
     batch, heads, dim = q.shape
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
@@ -284,6 +301,7 @@ def rotate_into(plan, q: Tensor, k: Tensor, v: Tensor, k_cache: Tensor, v_cache:
 
 def dropout(x: Tensor, residual, below: int, seed: int, offset: int, more) -> Tensor:
     """``residual + dropout(x)`` of contiguous, 16-byte aligned tensors."""
+    _check_unrecorded(x, residual)
     out = torch.empty_like(x)
     _launch("lct_dropout", x.get_device(), x.data_ptr(),
             None if residual is None else residual.data_ptr(), out.data_ptr(), x.numel(),
