@@ -77,10 +77,18 @@ def _recorded(*tensors) -> bool:
     return False
 
 
-def _indices(t, name: str, shapes, device) -> Tensor:
-    """An index tensor as INT32 of one of ``shapes``."""
+def _check_memory(t, name: str) -> None:
+    """Tensors that the kernels may do without: an address of zero, which those
+    without memory have, would mean that there is none."""
     if not isinstance(t, Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
+    if type(t) not in _PLAIN or _wrapped(t) or t._is_zerotensor():
+        raise TypeError(f"{name} must be a plain torch.Tensor")
+
+
+def _indices(t, name: str, shapes, device) -> Tensor:
+    """An index tensor as INT32 of one of ``shapes``."""
+    _check_memory(t, name)
     if t.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"{name} must be int32 or int64, got {t.dtype}")
     if tuple(t.shape) not in shapes:

@@ -12,7 +12,7 @@ from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from ..kernels import attention as kernels
-from .attention import _check_like, _check_tensor, _recorded, _whole
+from .attention import _check_like, _check_memory, _check_tensor, _recorded, _whole
 
 __all__ = ["dropout_add"]
 
@@ -75,6 +75,7 @@ def dropout_add(x: Tensor, residual: Tensor | None, p: float, seed: int, offset=
     seed = _whole(seed, "seed", -2 ** 63, 2 ** 64 - 1) % 2 ** 64
     more = None
     if isinstance(offset, Tensor):
+        _check_memory(offset, "offset")
         if offset.dtype != torch.int64 or offset.numel() != 1 or offset.device != x.device:
             raise ValueError("an offset tensor must be one int64 on x's device")
         offset, more = 0, offset

@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import pytest
 import torch
+from torch._subclasses import FakeTensorMode
 from torch.autograd import forward_ad
 from torch.fx.experimental.proxy_tensor import make_fx
 from torch.utils._python_dispatch import TorchDispatchMode
@@ -98,3 +99,22 @@ def test_a_tangent_is_refused(launch):
             with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
                 call(dual)
     assert not done
+
+
+def test_index_tensors_without_memory_are_refused():
+    """Their address of zero would mean that there are none."""
+    fake = FakeTensorMode().from_tensor(LENGTHS)
+    zero = torch._efficientzerotensor((1,), dtype=torch.int32)
+    for t in (fake, zero):
+        with pytest.raises(TypeError, match="plain"):
+            attention._indices(t, "lengths", ((1,),), t.device)
+    assert attention._indices(LENGTHS, "lengths", ((1,),), LENGTHS.device) is LENGTHS
+    with pytest.raises(TypeError, match="Tensor"):
+        attention._indices(3, "lengths", ((1,),), LENGTHS.device)
+    torch.func.vmap(lambda t: _wrapped_is_refused(t))(torch.zeros(2, 1, dtype=torch.int32))
+
+
+def _wrapped_is_refused(t):
+    with pytest.raises(TypeError, match="plain"):
+        attention._indices(t, "lengths", ((1,),), t.device)
+    return t
