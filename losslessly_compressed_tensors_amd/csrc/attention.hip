@@ -588,7 +588,8 @@ __global__ __launch_bounds__(kAttentionThreads, 2) void attention_dq_kernel(
 }
 
 // How a key block's queries are shared: blocks that hold sinks are seen by all
-// later queries and have parts of their own number.
+// later queries and have parts of their own number.  A kind of one part stores its
+// gradients itself and has no place in the workspace.
 struct KeyBlocks {
     int32_t blocks, sink_blocks, splits, sink_splits;
     __host__ __device__ __forceinline__ int64_t sink_parts() const {
@@ -597,12 +598,17 @@ struct KeyBlocks {
     __host__ __device__ __forceinline__ int64_t other_parts() const {
         return int64_t{blocks - sink_blocks} * splits;
     }
-    __host__ __device__ __forceinline__ int64_t parts() const {
-        return sink_parts() + other_parts();
+    __host__ __device__ __forceinline__ int64_t stored_sink_parts() const {
+        return sink_splits > 1 ? sink_parts() : 0;
     }
+    // Of a head, in the workspace.
+    __host__ __device__ __forceinline__ int64_t stored_parts() const {
+        return stored_sink_parts() + (splits > 1 ? other_parts() : 0);
+    }
+    // Of a block of several parts.
     __host__ __device__ __forceinline__ int64_t first_part(int32_t block) const {
         return block < sink_blocks ? int64_t{block} * sink_splits
-                                   : sink_parts() + int64_t{block - sink_blocks} * splits;
+                                   : stored_sink_parts() + int64_t{block - sink_blocks} * splits;
     }
     __host__ __device__ __forceinline__ int32_t parts_of(int32_t block) const {
         return block < sink_blocks ? sink_splits : splits;
@@ -846,9 +852,11 @@ __global__ __launch_bounds__(key_block(kDim) * 2, kDim > 64 ? 2 : 3) void attent
         step(q_odd, g_odd, stats_odd);
     }
 
-    float *part_out = parts
-                      + (bkv * blocks.parts() + blocks.first_part(block) + split) * 2 * kKeyBlock
-                            * a.head_dim;
+    float *part_out =             // read where there are several parts
+        splits == 1 ? nullptr
+                    : parts
+                          + (bkv * blocks.stored_parts() + blocks.first_part(block) + split) * 2
+                                * kKeyBlock * a.head_dim;
     if (not_finite(dk) || not_finite(dv)) {
         const int32_t channel = 2 * lane;
         for (int32_t j = wave_first; j < min(wave_first + kWaveKeys, a.keys); ++j) {
@@ -940,7 +948,7 @@ __global__ __launch_bounds__(kAttentionThreads) void attention_sum_parts_kernel(
     const int32_t count = blocks.parts_of(block);
     if (count == 1) return;
     const int64_t step = int64_t{2} * per_block * a.head_dim;
-    const float *src = parts + (bkv * blocks.parts() + blocks.first_part(block)) * step
+    const float *src = parts + (bkv * blocks.stored_parts() + blocks.first_part(block)) * step
                        + int64_t{key % per_block} * a.head_dim + channel;
     f32x4 x{}, y{};
 #pragma unroll 8
@@ -1040,10 +1048,8 @@ int32_t backward(const lct_attention &a, const lct_attention_gradients &d, const
     });
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return static_cast<int32_t>(err);
-    const int32_t end_block = blocks.splits > 1        ? blocks.blocks
-                              : blocks.sink_splits > 1 ? blocks.sink_blocks
-                                                       : 0;
-    if (end_block == 0) return LCT_OK;
+    if (blocks.stored_parts() == 0) return LCT_OK;
+    const int32_t end_block = blocks.splits > 1 ? blocks.blocks : blocks.sink_blocks;
     const int64_t keys = std::min<int64_t>(a.keys, int64_t{end_block} * key_block(a.head_dim));
     const int64_t threads = keys * (a.head_dim / 4) * a.batch * a.kv_heads;
     attention_sum_parts_kernel<kHalf>
@@ -1092,16 +1098,17 @@ extern "C" int32_t lct_attention_backward(const lct_attention *a, const lct_atte
         a->window > 0 ? (std::min(a->sinks, a->keys) + per_block - 1) / per_block : 0;
     blocks.splits = splits;
     blocks.sink_splits = sink_splits;
-    const int64_t parts = blocks.parts() * a->batch * a->kv_heads;
-    if (parts > kMaxAttentionItems
+    const int64_t heads = int64_t{a->batch} * a->kv_heads;
+    if ((blocks.sink_parts() + blocks.other_parts()) * heads > kMaxAttentionItems
         || int64_t{(a->queries + kQueryTile - 1) / kQueryTile} * a->batch * a->heads
                > kMaxAttentionItems
         || int64_t{a->keys} * (a->head_dim / 4) * a->batch * a->kv_heads
                > kMaxAttentionItems * kAttentionThreads)
         return LCT_E_SIZE;
-    if (splits > 1 || (sink_splits > 1 && blocks.sink_blocks > 0)) {
+    if (blocks.stored_parts() > 0) {
         if (!workspace) return LCT_E_NULL;
-        if (workspace_floats < parts * 2 * per_block * a->head_dim) return LCT_E_SIZE;
+        if (workspace_floats < blocks.stored_parts() * heads * 2 * per_block * a->head_dim)
+            return LCT_E_SIZE;
     }
     return a->fp16 ? backward<true>(*a, *d, blocks, workspace, stream)
                    : backward<false>(*a, *d, blocks, workspace, stream);

@@ -177,6 +177,17 @@ def backward_splits(batch: int, heads: int, kv_heads: int, queries: int, keys: i
     return splits, max(1, min(_MAX_SPLITS, -(-(-(-queries // 64) * group) // part)))
 
 
+def backward_workspace(batch: int, kv_heads: int, keys: int, dim: int, window: int, sinks: int,
+                       splits: int, sink_splits: int) -> int:
+    """Floats of the parts of dk and dv: of the key blocks that have several."""
+    per_block = key_block(dim)
+    sink_blocks = -(-min(sinks, keys) // per_block) if window else 0
+    parts = sink_blocks * sink_splits if sink_splits > 1 else 0
+    if splits > 1:
+        parts += (-(-keys // per_block) - sink_blocks) * splits
+    return batch * kv_heads * parts * 2 * per_block * dim
+
+
 def attention_backward(grad: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor,
                        window: int, sinks: int, scale: float, lengths):
     """``(dq, dk, dv)``."""
@@ -188,12 +199,7 @@ def attention_backward(grad: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tenso
     delta = _lse(q)
     splits, sink_splits = backward_splits(batch, heads, kv_heads, queries, keys, dim, window,
                                           sinks)
-    per_block = key_block(dim)
-    blocks = -(-keys // per_block)
-    sink_blocks = -(-min(sinks, keys) // per_block) if window else 0
-    parts = sink_blocks * sink_splits + (blocks - sink_blocks) * splits
-    floats = (batch * kv_heads * parts * 2 * per_block * dim
-              if splits > 1 or (sink_splits > 1 and sink_blocks) else 0)
+    floats = backward_workspace(batch, kv_heads, keys, dim, window, sinks, splits, sink_splits)
     workspace, address = _workspace(q, floats)
     _launch("lct_attention_backward", q.get_device(),
             _record(q, k, v, out, lse, lengths, window, sinks, scale),

@@ -220,3 +220,31 @@ def test_the_oracle_itself():
     assert int(oracle.sees(5, 3).sum()) == 6 and int(oracle.sees(4, 4, 1, 2).sum()) == 1 + 2 + 3 + 3
     assert [hex(int(w)) for w in oracle.philox_words(1, 0, 0)[0]] == [
         "0x6627e8d5", "0xe169c58d", "0xbc57ac4c", "0x9b00dbd8"]
+
+
+@pytest.mark.parametrize("dim,block", [(64, 128), (128, 256)])
+def test_the_workspace_holds_parts_of_blocks_that_have_several(lib, dim, block):
+    """1000 keys of 2 key heads, 300 sinks: no more is asked than parts that are
+    written, by the entry point and by its caller."""
+    blocks, sink_blocks = -(-1000 // block), -(-300 // block)
+    gradients = hip.ATTENTION_GRADIENTS.pack(*(FAKE,) * 5, *(512, 64, 128) * 4)
+    fake = ctypes.c_void_p(FAKE)
+    for window, sinks, splits, sink_splits, parts in (
+            (50, 300, 1, 5, sink_blocks * 5), (50, 300, 3, 1, (blocks - sink_blocks) * 3),
+            (50, 300, 3, 5, sink_blocks * 5 + (blocks - sink_blocks) * 3), (0, 300, 1, 5, 0),
+            (0, 300, 3, 5, blocks * 3), (50, 1000, 3, 1, 0), (50, 300, 1, 1, 0)):
+        floats = 2 * parts * 2 * block * dim
+        assert kernels.backward_workspace(1, 2, 1000, dim, window, sinks, splits,
+                                          sink_splits) == floats
+        record = _attention(heads=4, kv_heads=2, queries=1000, keys=1000, dim=dim, window=window,
+                            sinks=sinks)
+        if parts:
+            assert lib.lct_attention_backward(record, gradients, splits, sink_splits, fake,
+                                              floats - 1, None) == LCT_E_SIZE
+            assert lib.lct_attention_backward(record, gradients, splits, sink_splits, None, floats,
+                                              None) == LCT_E_NULL
+    # One long sequence under a window: its blocks without sinks are stored whole.
+    splits, sink_splits = kernels.backward_splits(1, 16, 4, 16384, 16384, 128, 4096, 4)
+    assert splits == 1 and sink_splits > 1
+    assert kernels.backward_workspace(1, 4, 16384, 128, 4096, 4, splits, sink_splits) == (
+        4 * sink_splits * 2 * 256 * 128)

@@ -512,3 +512,37 @@ def test_offsets_past_32_bits():
         assert bool((full[:, :, sinks:-near] == 0).all())
         result[name] = torch.cat([full[:, :, :sinks], full[:, :, -near:]], 2)
     _check(result, oracle.attention_with_bounds(chunk, *small, seen, dim ** -0.5, grad))
+
+
+@pytest.mark.parametrize("splits,sink_splits", [(1, 5), (3, 1), (3, 5), (1, 1)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_parts_of_one_kind_of_key_block(dim, splits, sink_splits, monkeypatch):
+    """Blocks with sinks in parts and the others whole, the other way round, both:
+    the parts fill the workspace that is asked for, and no more."""
+    sizes = []
+    monkeypatch.setattr(kernels, "backward_splits", lambda *a: (splits, sink_splits))
+    plain = kernels._workspace
+
+    def guarded(q, floats):
+        sizes.append(floats)
+        if not floats:
+            return plain(q, floats)
+        memory = torch.full((floats + 1024,), float("nan"), device=DEV)
+        guarded.memory = memory
+        return memory, memory.data_ptr()
+
+    q, k, v, grad = _inputs(2, 4, 2, 900, 900, dim)
+    seen = oracle.sees(900, 900, 100, 300, None, 2).to(DEV)
+    out, lse = kernels.attention_forward(q, k, v, 100, 300, 0.1, None, True)
+    monkeypatch.setattr(kernels, "_workspace", guarded)
+    got = dict(zip(("out", "dq", "dk", "dv"), (out, *kernels.attention_backward(
+        grad, q, k, v, out, lse, 100, 300, 0.1, None))))
+    torch.cuda.synchronize()
+    _check(got, oracle.attention_with_bounds(q, k, v, seen, 0.1, grad))
+    if splits == sink_splits == 1:
+        assert sizes == [0]
+    else:
+        floats, = sizes
+        assert bool(guarded.memory[floats:].isnan().all())
+        # Every part's keys that exist are written: the last block's others are not.
+        assert int(guarded.memory[:floats].isnan().sum()) <= floats // 2
