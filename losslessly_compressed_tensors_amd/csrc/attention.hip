@@ -389,14 +389,51 @@ __global__ __launch_bounds__(kAttentionThreads) void attention_join_kernel(
 // again: seven products in place of five, but no sum is shared between
 // workgroups, so results do not depend on timing.
 
+// dS is the product of a weight and an incoming gradient, often far below FP16's
+// normal numbers (and now and then above its largest): 4096 keys under gradients of
+// 1e-4 left a fifth of them zero.  In FP16 a lane, whose sums are of one query or
+// key, holds them and each dS times a power of two that begins at 2^60 (FP16's
+// least products are 2^-48) and goes down to put the largest dS so far between 2^8
+// and 2^15.  What is 2^22 smaller is still rounded to FP16's 11 bits.  A lane's
+// maximum of 16 numbers per 32 x 32 scores: at 1 x 16384, 16 heads of 128 over 4,
+// window 4096, dq takes 720 us where it took 690, dk and dv 1230 as before; at 8 x
+// 1024, 12 heads of 64, window 256, 32.8 for 29.7 and 41.4 for 40.3.
+constexpr float kHalfPower = 60.0f, kHalfFirst = 0x1p60f;
+constexpr float kHalfMost = 0x1p15f;
+
+template <int kColumns>
+__device__ __forceinline__ void multiply_all(f32x16 (&x)[kColumns], float factor) {
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[c][r] *= factor;
+}
+
+// Multiplies `ds` and `sums` by a power of two, lowered(factor), where `ds` is too large.
+template <int kColumns, class Lowered>
+__device__ __forceinline__ void lower_half(f32x16 &ds, f32x16 (&sums)[kColumns], Lowered lowered) {
+    float top = fmaxf(fabsf(ds[0]), fabsf(ds[1]));
+#pragma unroll
+    for (int r = 2; r < 16; ++r) top = fmaxf(top, fabsf(ds[r]));
+    if (!__any(top > kHalfMost)) return;
+    top = across_max(top);                   // of both lanes that share the sums
+    const float factor =
+        top > kHalfMost ? __uint_as_float((262u << 23) - (__float_as_uint(top) & 0x7F800000u))
+                        : 1.0f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) ds[r] *= factor;
+    multiply_all(sums, factor);
+    lowered(factor);
+}
+
 // A wave's 32 queries, the keys in tiles of 64: as in the forward kernel, with dP
 // beside the scores (its sums begin at -delta) and the keys' columns for the last
 // product.  delta is taken from the operands on their way in, and stored for the
 // other kernel.  650 us for 1 x 16384, 16 heads of 128 over 4, window 4096 (1110
 // TFLOP/s; 690 with the compiler's order of LDS reads), 29 us for 8 x 1024, 12
-// heads of 64, window 256.
+// heads of 64, window 256, three waves per SIMD (in FP16 32.8; two waves 38.5).
 template <bool kHalf, int kDim>
-__global__ __launch_bounds__(kAttentionThreads, 2) void attention_dq_kernel(
+__global__ __launch_bounds__(kAttentionThreads, kDim > 64 ? 2 : 3) void attention_dq_kernel(
     lct_attention a, lct_attention_gradients d, int32_t tiles) {
     constexpr int kPitch = kPitchOf<kDim>;
     constexpr int kSteps = kDim / 16, kColumns = kDim / 32;
@@ -453,7 +490,6 @@ __global__ __launch_bounds__(kAttentionThreads, 2) void attention_dq_kernel(
     }
     delta = across_sum(delta);
     const int64_t at = int64_t{bh} * lse_pitch(a.queries) + row;
-    const float lse = a.lse[at];
 
     const uint16_t *k = static_cast<const uint16_t *>(a.k) + b * a.k_stride[0] + kv * a.k_stride[1];
     const uint16_t *v = static_cast<const uint16_t *>(a.v) + b * a.v_stride[0] + kv * a.v_stride[1];
@@ -469,6 +505,7 @@ __global__ __launch_bounds__(kAttentionThreads, 2) void attention_dq_kernel(
 
     const float factor = a.scale * kLog2e;
     f32x16 dq[kColumns];
+    float base = -a.lse[at]; // what exponents begin at; in FP16 with dS's power of two
     float rest = 0.0f;       // this lane's keys' sum of dS
     const auto step = [&](auto sums, int32_t t, const uint16_t *keys, const uint16_t *values)
                           __attribute__((always_inline)) {
@@ -493,7 +530,7 @@ __global__ __launch_bounds__(kAttentionThreads, 2) void attention_dq_kernel(
             read_ahead<2 * kSteps, 1, 4>();
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-                s[r] = exp2_fast(__builtin_fmaf(s[r], factor, -lse)) * e[r];
+                s[r] = exp2_fast(__builtin_fmaf(s[r], factor, base)) * e[r];
             if (!seen_by_all)
                 TileSight(a, position, key).each(
                     key, 32 * n, tile_sinks,
@@ -502,6 +539,11 @@ __global__ __launch_bounds__(kAttentionThreads, 2) void attention_dq_kernel(
 #pragma unroll
                 for (int r = 0; r < 16; ++r) rest += s[r];
             } else {
+                if constexpr (kHalf)
+                    lower_half(s, dq, [&](float factor) {
+                        base += static_cast<float>(
+                            static_cast<int32_t>(__float_as_uint(factor) >> 23) - 127);
+                    });
 #pragma unroll
                 for (int p = 0; p < 2; ++p) {
                     const u32x4 ds = as_operand<kHalf>(s, p);
@@ -544,7 +586,13 @@ __global__ __launch_bounds__(kAttentionThreads, 2) void attention_dq_kernel(
     if (half == 0) d.delta[at] = delta;
 #pragma unroll
     for (int c = 0; c < kColumns; ++c) dq[c] = f32x16{};
+    if constexpr (kHalf) base += kHalfPower;
     walk(std::false_type{});
+    if constexpr (kHalf) {
+        // A row that sees nothing has no power, and zeros.
+        const float power = base + a.lse[at];
+        multiply_all(dq, power == power ? exp2_fast(-power) : 1.0f);
+    }
     if (not_finite(dq)) {
         const int32_t channel = 2 * lane;
         const uint16_t *q =
@@ -557,7 +605,8 @@ __global__ __launch_bounds__(kAttentionThreads, 2) void attention_dq_kernel(
             const Sight seen = sight_of(a, at + shift, length);
             const uint32_t q_pair = lane_pair(q + at * a.q_stride[2], a.head_dim);
             const uint32_t g_pair = lane_pair(g + at * d.grad_stride[2], a.head_dim);
-            const float row_lse = of_lane(lse, r), row_delta = of_lane(delta, r);
+            const float row_lse = a.lse[int64_t{bh} * lse_pitch(a.queries) + at];
+            const float row_delta = of_lane(delta, r);
             float x = 0.0f, y = 0.0f;
             for (int32_t t = 0; t < all.count; ++t) {
                 const int32_t key = all.first_key(t, kKeyTile);
@@ -749,6 +798,7 @@ __global__ __launch_bounds__(key_block(kDim) * 2, kDim > 64 ? 2 : 3) void attent
     f32x16 dk[kColumns], dv[kColumns];
 #pragma unroll
     for (int c = 0; c < kColumns; ++c) dk[c] = dv[c] = f32x16{};
+    float up = kHalfFirst;   // of dS and dk in FP16
 
     // 32 of the step's queries, at `position`; `all`: each sees all the wave's keys.
     const auto rows = [&](int n, bool all, int32_t position, const uint16_t *q_tile,
@@ -804,9 +854,12 @@ __global__ __launch_bounds__(key_block(kDim) * 2, kDim > 64 ? 2 : 3) void attent
             for (int i = 0; i < 4; ++i) {
                 const int r = 4 * g + i;
                 s[r] = exp2_fast(__builtin_fmaf(s[r], factor, -lse[i]));
-                e[r] *= s[r];
+                e[r] *= kHalf ? s[r] * up : s[r];
                 if (kHalf) s[r] *= kHalfWeights;
             }
+        }
+        if constexpr (kHalf) {
+            lower_half(e, dk, [&](float factor) { up *= factor; });
         }
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
@@ -857,6 +910,7 @@ __global__ __launch_bounds__(key_block(kDim) * 2, kDim > 64 ? 2 : 3) void attent
                     : parts
                           + (bkv * blocks.stored_parts() + blocks.first_part(block) + split) * 2
                                 * kKeyBlock * a.head_dim;
+    if constexpr (kHalf) multiply_all(dk, 1.0f / up);
     if (not_finite(dk) || not_finite(dv)) {
         const int32_t channel = 2 * lane;
         for (int32_t j = wave_first; j < min(wave_first + kWaveKeys, a.keys); ++j) {
