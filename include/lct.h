@@ -845,9 +845,11 @@ int32_t lct_attention_forward(const lct_attention *a, int32_t splits, float *wor
  * their sum.  delta: working array of lse's size.  The queries that see a block
  * of n keys (128, 256 where head_dim > 64) are shared among `splits` workgroups,
  * among `sink_splits` where the block holds sinks (and window > 0).  `workspace`
- * holds batch * kv_heads * parts * 2 n * head_dim floats, added by a further launch
- * in their order: parts are sink blocks * sink_splits, if sink_splits > 1, and other
- * blocks * splits, if splits > 1 (none: workspace may be NULL). */
+ * holds batch * kv_heads * parts * (2 n * head_dim + LCT_ATTENTION_PART_GAP) floats,
+ * added by a further launch in their order: parts are sink blocks * sink_splits, if
+ * sink_splits > 1, and other blocks * splits, if splits > 1 (none: workspace may be
+ * NULL). */
+#define LCT_ATTENTION_PART_GAP 64
 typedef struct {
     const void *grad;
     void *dq, *dk, *dv;

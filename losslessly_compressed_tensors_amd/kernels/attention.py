@@ -26,6 +26,7 @@ _QUERY_TILE, _KEY_TILE = 128, 64
 _DECODE_TILE = 4 * 32    # keys that a workgroup's waves take at a time
 _MAX_SPLITS = 64        # LCT_MAX_ATTENTION_SPLITS
 _MAX_PARTS = 8          # of dk and dv: FP32 copies of both in the workspace
+_PART_GAP = 64          # LCT_ATTENTION_PART_GAP
 _CUS = 256
 
 TYPES = {torch.bfloat16: hip.BF16, torch.float16: hip.FP16, torch.float32: hip.FP32}
@@ -185,7 +186,7 @@ def backward_workspace(batch: int, kv_heads: int, keys: int, dim: int, window: i
     parts = sink_blocks * sink_splits if sink_splits > 1 else 0
     if splits > 1:
         parts += (-(-keys // per_block) - sink_blocks) * splits
-    return batch * kv_heads * parts * 2 * per_block * dim
+    return batch * kv_heads * parts * (2 * per_block * dim + _PART_GAP)
 
 
 def attention_backward(grad: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor,

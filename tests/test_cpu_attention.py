@@ -233,7 +233,7 @@ def test_the_workspace_holds_parts_of_blocks_that_have_several(lib, dim, block):
             (50, 300, 1, 5, sink_blocks * 5), (50, 300, 3, 1, (blocks - sink_blocks) * 3),
             (50, 300, 3, 5, sink_blocks * 5 + (blocks - sink_blocks) * 3), (0, 300, 1, 5, 0),
             (0, 300, 3, 5, blocks * 3), (50, 1000, 3, 1, 0), (50, 300, 1, 1, 0)):
-        floats = 2 * parts * 2 * block * dim
+        floats = 2 * parts * (2 * block * dim + 64)
         assert kernels.backward_workspace(1, 2, 1000, dim, window, sinks, splits,
                                           sink_splits) == floats
         record = _attention(heads=4, kv_heads=2, queries=1000, keys=1000, dim=dim, window=window,
@@ -247,4 +247,4 @@ def test_the_workspace_holds_parts_of_blocks_that_have_several(lib, dim, block):
     splits, sink_splits = kernels.backward_splits(1, 16, 4, 16384, 16384, 128, 4096, 4)
     assert splits == 1 and sink_splits > 1
     assert kernels.backward_workspace(1, 4, 16384, 128, 4096, 4, splits, sink_splits) == (
-        4 * sink_splits * 2 * 256 * 128)
+        4 * sink_splits * (2 * 256 * 128 + 64))
