@@ -667,6 +667,10 @@ struct KeyBlocks {
         return block < sink_blocks ? int64_t{block} * sink_splits
                                    : stored_sink_parts() + int64_t{block - sink_blocks} * splits;
     }
+    // One past the last block that may have several.
+    __host__ __device__ __forceinline__ int32_t end_of_parts() const {
+        return splits > 1 ? blocks : sink_blocks;
+    }
     __host__ __device__ __forceinline__ int32_t parts_of(int32_t block) const {
         return block < sink_blocks ? sink_splits : splits;
     }
@@ -1093,6 +1097,14 @@ int32_t forward(const lct_attention &a, int32_t splits, float *workspace, hipStr
     return join_parts(a, splits, workspace, stream);
 }
 
+// Workgroups of the launch that adds parts: four channels of a key per thread.
+int64_t sum_groups(const lct_attention &a, const KeyBlocks &blocks) {
+    const int64_t keys =
+        std::min<int64_t>(a.keys, int64_t{blocks.end_of_parts()} * key_block(a.head_dim));
+    const int64_t threads = keys * (a.head_dim / 4) * a.batch * a.kv_heads;
+    return (threads + kAttentionThreads - 1) / kAttentionThreads;
+}
+
 template <bool kHalf>
 int32_t backward(const lct_attention &a, const lct_attention_gradients &d, const KeyBlocks &blocks,
                  float *workspace, hipStream_t stream) {
@@ -1111,12 +1123,9 @@ int32_t backward(const lct_attention &a, const lct_attention_gradients &d, const
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return static_cast<int32_t>(err);
     if (blocks.stored_parts() == 0) return LCT_OK;
-    const int32_t end_block = blocks.splits > 1 ? blocks.blocks : blocks.sink_blocks;
-    const int64_t keys = std::min<int64_t>(a.keys, int64_t{end_block} * key_block(a.head_dim));
-    const int64_t threads = keys * (a.head_dim / 4) * a.batch * a.kv_heads;
     attention_sum_parts_kernel<kHalf>
-        <<<static_cast<uint32_t>((threads + kAttentionThreads - 1) / kAttentionThreads),
-           kAttentionThreads, 0, stream>>>(a, d, blocks, workspace, end_block);
+        <<<static_cast<uint32_t>(sum_groups(a, blocks)), kAttentionThreads, 0, stream>>>(
+            a, d, blocks, workspace, blocks.end_of_parts());
     return static_cast<int32_t>(hipGetLastError());
 }
 
@@ -1164,8 +1173,7 @@ extern "C" int32_t lct_attention_backward(const lct_attention *a, const lct_atte
     if ((blocks.sink_parts() + blocks.other_parts()) * heads > kMaxAttentionItems
         || int64_t{(a->queries + kQueryTile - 1) / kQueryTile} * a->batch * a->heads
                > kMaxAttentionItems
-        || int64_t{a->keys} * (a->head_dim / 4) * a->batch * a->kv_heads
-               > kMaxAttentionItems * kAttentionThreads)
+        || (blocks.stored_parts() > 0 && sum_groups(*a, blocks) > kMaxAttentionItems))
         return LCT_E_SIZE;
     if (blocks.stored_parts() > 0) {
         if (!workspace) return LCT_E_NULL;

@@ -248,3 +248,12 @@ def test_the_workspace_holds_parts_of_blocks_that_have_several(lib, dim, block):
     assert splits == 1 and sink_splits > 1
     assert kernels.backward_workspace(1, 4, 16384, 128, 4096, 4, splits, sink_splits) == (
         4 * sink_splits * (2 * 256 * 128 + 64))
+
+
+def test_long_caches_are_only_bound_by_what_is_launched(lib):
+    """2^28 keys: the launch that adds parts is as large as the blocks that have any."""
+    gradients = hip.ATTENTION_GRADIENTS.pack(*(FAKE,) * 5, *(512, 64, 128) * 4)
+    long = _attention(keys=2 ** 28, window=5, sinks=3)
+    call = lib.lct_attention_backward
+    assert call(long, gradients, 1, 2, None, 0, None) == LCT_E_NULL      # the workspace
+    assert call(long, gradients, 2, 1, None, 0, None) == LCT_E_SIZE      # parts of all keys
