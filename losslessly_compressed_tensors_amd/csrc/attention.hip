@@ -16,7 +16,6 @@ namespace {
 constexpr int kQueryTile = 128;      // queries of a workgroup, 32 per wave
 constexpr int kKeyTile = 64;         // keys per step
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kRescale = 8.0f;     // how far (log2) a running maximum may lag
 constexpr float kHalfWeights = 256.0f;
 constexpr int32_t kFewKeys = 64;     // rows of up to so many keys get an exact delta
 constexpr int32_t kMaxTokens = 1 << 30;
@@ -208,7 +207,7 @@ __global__ __launch_bounds__(kAttentionThreads, 2) void attention_forward_kernel
             const float scaled = next == -INFINITY ? 0.0f : next * factor;
             const float change = exp2_fast(most * factor - scaled);
             most = next;
-            shifted = scaled;
+            shifted = scaled - (kHalf ? kHalfLift : 0.0f);
             total *= change;
 #pragma unroll
             for (int c = 0; c < kColumns; ++c)

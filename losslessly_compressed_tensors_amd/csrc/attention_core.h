@@ -69,6 +69,11 @@ struct Element {
     }
 };
 
+// How far (log2) a running maximum may lag.  In FP16 the weights are held 2^kHalfLift
+// larger, up to 2^15: one below 2^-25 of the largest would be lost, and a cache has
+// enough keys for those to count.
+constexpr float kRescale = 8.0f, kHalfLift = 7.0f;
+
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Both halves of a wave: f(lane's value, the value of the lane 32 further).

@@ -27,7 +27,6 @@ namespace {
 constexpr int kDecodeKeys = 32;      // keys per tile
 constexpr int kQueries = 16;         // query heads per workgroup
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kRescale = 8.0f;
 
 // Keys and values of more bytes than half the memory side's cache (256 MiB) are
 // read past it: 263 us in place of 292 for 4 sequences of up to 131072 keys, 188
@@ -197,7 +196,7 @@ __global__ __launch_bounds__(kAttentionThreads, 2) void attention_decode_kernel(
             const float scaled = next == -INFINITY ? 0.0f : next * factor;
             const float change = exp2_fast(most * factor - scaled);
             most = next;
-            shifted = scaled;
+            shifted = scaled - (kHalf ? kHalfLift : 0.0f);
             total *= change;
 #pragma unroll
             for (int c = 0; c < kColumns; ++c) out[c] *= change;

@@ -13,6 +13,7 @@ import pytest
 import torch
 
 from losslessly_compressed_tensors_amd.components import attention
+from losslessly_compressed_tensors_amd.kernels import attention as kernels
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -94,3 +95,30 @@ def test_large_gradients(dim):
     """dS beyond FP16's largest number."""
     q, k, v, grad = (_values(1, 2, 700, dim, seed=i) for i in range(4))
     _check(*(t.to(FP16) for t in (q, k, v, 5e3 * grad)), scale=0.02)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("sink", [0, 39_999])
+def test_many_small_weights_beside_a_large_one(sink, dtype, monkeypatch):
+    """40000 keys of which one outscores the others by 18: their weights are e^-18 =
+    2^-26 of its own, and the result is theirs alone, its value being 0."""
+    for name in ("forward_splits", "decode_splits"):     # all weights beside the largest
+        monkeypatch.setattr(kernels, name, lambda *a: 1)
+    keys, dim, gap = 40_000, 64, 18.0
+    q = torch.ones(1, 1, 1, dim, dtype=dtype, device=DEV)
+    k = torch.zeros(1, 1, keys, dim, dtype=dtype, device=DEV)
+    k[:, :, sink] = gap / dim
+    v = torch.ones(1, 1, keys, dim, dtype=dtype, device=DEV)
+    v[:, :, sink] = 0.0
+    exact, _ = oracle.attention(q, k, v, oracle.sees(1, keys).to(DEV), 1.0)
+    # Each weight's rounding, of FP16's least step where it is held 2^7 larger than its
+    # share of the largest; the sums' FP32 steps; the result's rounding.
+    unit = oracle.UNIT[dtype]
+    bound = (2 * unit + keys * oracle.STEP) * exact + (keys * 2.0 ** -32 if dtype == FP16 else 0.0)
+    lengths = torch.tensor([keys], device=DEV)
+    got = attention.window_attention(q, k, v, scale=1.0)
+    one = attention.decode_attention(q[:, :, 0], k.transpose(1, 2), v.transpose(1, 2), lengths,
+                                     scale=1.0)
+    for value in (got[:, :, 0], one):
+        assert bool(((value.double() - exact[:, :, 0]).abs() <= bound[:, :, 0]).all()), (
+            float(value.flatten()[0]), float(exact.flatten()[0]))
