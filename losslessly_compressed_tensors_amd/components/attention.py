@@ -21,6 +21,7 @@ from __future__ import annotations
 
 import math
 import numbers
+from fractions import Fraction
 
 import torch
 from torch import Tensor
@@ -155,7 +156,8 @@ class Rotary:
 
     Pair i is channels (i, i + n) of n frequencies or, if ``interleaved``,
     (2 i, 2 i + 1); channels from 2 n on are left as they are.  Frequencies are
-    kept as 64-bit fractions of a turn, so positions of any size turn exactly."""
+    kept as the nearest 64-bit fractions of FP64's turn (2^-54 of its value from the
+    turn): up to 2^31 radians an angle is off by less than its rounding to FP32."""
 
     def __init__(self, frequencies, *, interleaved: bool = False, magnitude: float = 1.0,
                  device="cuda"):
@@ -167,7 +169,8 @@ class Rotary:
         if not math.isfinite(magnitude):
             raise ValueError("magnitude must be finite")
         self.interleaved, self.magnitude = bool(interleaved), float(magnitude)
-        turns = [int(math.ldexp(f / (2 * math.pi), 64)) % 2 ** 64 for f in values]
+        turn = Fraction(2 * math.pi)
+        turns = [round(Fraction(f) * 2 ** 64 / turn) % 2 ** 64 for f in values]
         self.turns = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in turns],
                                   dtype=torch.int64).to(device)
 
@@ -190,6 +193,10 @@ def _check_rotary(plan, q) -> None:
                          f"got {q.shape[-1]}")
     if q.shape[-2] > _MAX_HEADS:
         raise ValueError(f"at most {_MAX_HEADS} heads")
+
+
+def _first_position(value) -> int:
+    return _whole(value, "positions", -2 ** 31, 2 ** 31)
 
 
 class _ApplyRotary(torch.autograd.Function):
@@ -225,8 +232,8 @@ _rotary_backward_once = once_differentiable(_rotary_backward)
 def apply_rotary(plan: Rotary, q: Tensor, k: Tensor | None = None, positions=None):
     """``q`` and ``k``, [batch, token, head, channel] of BF16, FP16 or FP32, turned
     by their positions: ``(q, k)``, or ``q`` alone.  ``positions``: None (0, 1, ..),
-    the first token's as an integer or per sequence as [batch], or each token's
-    as [batch, token] (INT32; INT64 is held to INT32's range).  Angles and products are FP32,
+    the first token's as an integer up to 2^31 or per sequence as [batch], or each
+    token's as [batch, token] (INT32; INT64 is held to INT32's range).  Angles and products are FP32,
     rounded once.  Differentiable in ``q`` and ``k``."""
     _check_tensor(q, "q", 4, _ROTARY_TYPES)
     _check_rotary(plan, q)
@@ -240,7 +247,7 @@ def apply_rotary(plan: Rotary, q: Tensor, k: Tensor | None = None, positions=Non
     if isinstance(positions, Tensor):
         positions = _indices(positions, "positions", ((q.shape[0],), tuple(q.shape[:2])), q.device)
     elif positions is not None:
-        start, positions = _whole(positions, "positions", -2 ** 62, 2 ** 62), None
+        start, positions = _first_position(positions), None
     if q.numel() == 0 or (k is not None and k.numel() == 0):
         if k is None:
             return q.clone()

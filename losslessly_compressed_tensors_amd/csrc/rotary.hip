@@ -3,8 +3,9 @@
 // A pair (x, y) of channels at position p turns by the angle p f of its
 // frequency: (x cos - y sin, y cos + x sin), times a magnitude.  Frequencies are
 // fractions of a turn per position in 64-bit fixed point, so the product with
-// the position wraps modulo one turn exactly, whatever the position: no table
-// bounds the context, and the angle's only rounding is to FP32 in [-1/2, 1/2].
+// the position wraps modulo one turn exactly: no table bounds the context.  A
+// position p multiplies the frequency's rounding, 2^-65 of a turn; for any that 32
+// bits hold the product is less than the angle's rounding to FP32 in [-1/2, 1/2].
 //
 // Follows examples/nanogpt/train_gpt_lct.py:150-165 (whose rotation has the
 // other sense: negative frequencies).

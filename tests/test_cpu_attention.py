@@ -6,6 +6,7 @@ import ctypes
 import math
 import shutil
 import subprocess
+from fractions import Fraction
 
 import attention_oracle as oracle
 import pytest
@@ -257,3 +258,29 @@ def test_long_caches_are_only_bound_by_what_is_launched(lib):
     call = lib.lct_attention_backward
     assert call(long, gradients, 1, 2, None, 0, None) == LCT_E_NULL      # the workspace
     assert call(long, gradients, 2, 1, None, 0, None) == LCT_E_SIZE      # parts of all keys
+
+
+# To 60 digits.
+PI = Fraction("3.14159265358979323846264338327950288419716939937510582097494")
+
+
+@pytest.mark.parametrize("frequency", [1.0, 0.01, 1e-6, -0.3333333333333333, 5e-324, 1e300, 12345.678,
+                                       *attention.rotary_frequencies(16).tolist()])
+def test_frequencies_are_the_nearest_fractions_of_a_turn(frequency):
+    """Half of the last place, and the 2^-54 that FP64's turn is off."""
+    turns, = attention.Rotary([frequency], device="cpu").turns.tolist()
+    exact = Fraction(frequency) * 2 ** 64 / (2 * PI)
+    off = (turns - exact) % 2 ** 64
+    assert min(off, 2 ** 64 - off) <= Fraction(1, 2) + abs(exact) / 2 ** 54
+
+
+def test_positions_are_held_to_where_angles_are_right():
+    for position in (2 ** 31, -2 ** 31, 0):
+        assert attention._first_position(position) == position
+    for position in (2 ** 31 + 1, -2 ** 31 - 1, 2 ** 62):
+        with pytest.raises(ValueError, match="positions"):
+            attention._first_position(position)
+    # The fastest pair there: less than FP32's 2^-26 of a turn off.
+    turns, = attention.Rotary([1.0], device="cpu").turns.tolist()
+    off = (Fraction(turns, 2 ** 64) - 1 / (2 * PI)) * 2 ** 31 % 1
+    assert min(off, 1 - off) < Fraction(1, 2 ** 26)

@@ -2,6 +2,8 @@
 bits (``attention_oracle``)."""
 from __future__ import annotations
 
+from fractions import Fraction
+
 import attention_oracle as oracle
 import pytest
 import torch
@@ -192,3 +194,18 @@ def test_refusals():
             (lambda: attention.rotary_frequencies(8, scaling="other"), ValueError, "scaling")):
         with pytest.raises(error, match=match):
             bad()
+
+
+@pytest.mark.parametrize("start", [2 ** 31, -2 ** 31, 1234567890])
+def test_far_positions_have_exact_angles(start):
+    """Against angles reduced in whole numbers."""
+    tokens, dim = 4, 64
+    x = _values(1, tokens, 2, dim, dtype=FP32)
+    frequencies = attention.rotary_frequencies(dim)
+    got = attention.apply_rotary(attention.Rotary(frequencies), x, positions=start)
+    turn = 2 * Fraction("3.14159265358979323846264338327950288419716939937510582097494")
+    for t in range(tokens):
+        angles = [float((Fraction(f) * (start + t)) % turn) for f in frequencies.tolist()]
+        _near(got[:, t:t + 1], x[:, t:t + 1], torch.ones(1, 1), angles, FP32)
+    with pytest.raises(ValueError, match="positions"):
+        attention.apply_rotary(attention.Rotary(frequencies), x, positions=2 ** 31 + 1)
