@@ -8,7 +8,7 @@ import torch
 
 from examples.nanogpt import train_gpt_lct as trainer
 from examples.nanogpt.generate import Generator
-from losslessly_compressed_tensors_amd.components import layers
+from losslessly_compressed_tensors_amd.components import attention, layers
 from losslessly_compressed_tensors_amd.tensor_buffer import TensorBuffer
 
 pytestmark = pytest.mark.gpu
@@ -99,3 +99,69 @@ def test_generation_follows_the_whole_prompt():
     assert float((whole - last).abs().amax()) <= 2 * 12 * 2.0 ** -8 * float(whole.abs().amax())
     out = Generator(model, 3, 48, window=16, sinks=2).generate(tokens, 8)
     assert out.shape == (3, 8) and bool(((out >= 0) & (out < 512)).all())
+
+
+# The trainer starts from projections of zero, under which nothing of the attention
+# reaches a loss: these start from others.
+
+
+def _started(**how):
+    model, optimizers = trainer.build(DEV, compress_weights=False, **SHAPE, **how)
+    with torch.no_grad():
+        for i, (name, p) in enumerate(model.named_parameters()):
+            if name.endswith("proj.weight"):
+                p.copy_(0.05 * _values(*p.shape, seed=100 + i))
+    return model, optimizers
+
+
+def _loss_and_gradients(plan=None, **how):
+    model, _ = _started(compress_activations=False, compress_optimizer=False, **how)
+    if plan is not None:
+        for block in model.blocks:
+            block.attn.rotary_plan = plan
+    inputs, targets = trainer.random_tokens(2, 256, DEV, seed=0, token_ids=512)
+    loss = model(inputs, targets)
+    loss.backward()
+    return float(loss.detach()), {name: p.grad.double() for name, p in model.named_parameters()
+                         if ".attn." in name and name.endswith("weight")}
+
+
+# BF16 rounds a value by 2^-9.8 of it in the mean square; a pass through 2 layers and back
+# has some 24 roundings on a path to a gradient, two paths are compared, and twice that.
+FAR = 2 * (2 * 2 * 24) ** 0.5 * 2.0 ** -9.8
+
+
+def test_the_windowed_path_is_the_default_path_under_a_window_of_everything():
+    """Loss and the gradients of all of the attention's weights."""
+    loss, gradients = _loss_and_gradients()
+    same, window = _loss_and_gradients(window=256)
+    assert len(gradients) == 2 * 4 and abs(same - loss) <= FAR * abs(loss)
+    for name, grad in gradients.items():
+        assert float((window[name] - grad).norm()) <= FAR * float(grad.norm()), name
+    # What the comparison would not miss: another window, the other sense of rotation,
+    # no rotation.
+    frequencies = attention.trainer_frequencies(trainer.HEAD_DIM)
+    for how in (dict(window=8), dict(window=256, plan=attention.Rotary(-frequencies)),
+                dict(window=256, plan=attention.Rotary(0 * frequencies))):
+        _, other = _loss_and_gradients(**how)
+        assert any(float((other[name] - grad).norm()) > 2 * FAR * float(grad.norm())
+                   for name, grad in gradients.items()), how
+
+
+def test_windowed_training_is_lossless_in_every_parameter():
+    """Three steps whose attention gradients are not zero, dense and compressed."""
+    results = []
+    for compressed in (False, True):
+        model, optimizers = _started(compress_activations=compressed,
+                                     compress_optimizer=compressed, window=64, sinks=2,
+                                     dropout=0.1)
+        before = [p.detach().clone() for _, p in model.named_parameters()]
+        losses = []
+        for i in range(3):
+            inputs, targets = trainer.random_tokens(2, 256, DEV, seed=i, token_ids=512)
+            losses.append(trainer.train_step(model, optimizers, inputs, targets))
+        named = list(model.named_parameters())
+        moved = {name for (name, p), old in zip(named, before) if not torch.equal(p, old)}
+        assert {name for name, _ in named if ".attn." in name and name.endswith("weight")} <= moved
+        results.append(losses + [p.detach() for _, p in named])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
