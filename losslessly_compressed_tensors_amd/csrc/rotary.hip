@@ -53,7 +53,7 @@ struct Value<LCT_FP32> {
 struct Counts {
     int32_t per_group;      // tokens of a workgroup
     int32_t pair_units, units, per_token;
-    uint32_t units_inverse, per_token_inverse;   // ceil(2^32 / .), 0 for 1
+    uint32_t units_inverse, per_token_inverse;   // ceil(2^32 / .), 0 for 1, 1 for all
 };
 
 __device__ __forceinline__ int32_t divide(int32_t x, uint32_t inverse) {
@@ -211,7 +211,8 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(lct_rotary r, Counts n
     }
 }
 
-// x / d is the high half of x ceil(2^32 / d) for x and d up to 2^16.
+// x / d is the high half of x ceil(2^32 / d) where x d is up to 2^32: for the items
+// of several tokens, up to 2^16, and for those of one (3 x 4096 heads of 128 units).
 constexpr int32_t kMaxItems = 1 << 16;
 
 uint32_t inverse_of(int32_t x) {
@@ -237,7 +238,6 @@ int32_t launch(const lct_rotary &r, hipStream_t stream) {
     n.pair_units = r.interleaved && kVector > 1 ? r.rotary_dim / kVector : pairs / kVector;
     n.units = n.pair_units + (r.head_dim - r.rotary_dim) / kVector;
     n.per_token = (r.heads + (r.k_in ? r.kv_heads : 0) + (r.v_in ? r.kv_heads : 0)) * n.units;
-    if (n.per_token > kMaxItems) return LCT_E_SIZE;
     const int64_t tokens = int64_t{r.batch} * r.tokens;
     // Whole rounds of the threads' units (to a tenth), while there are workgroups
     // for every compute unit.
@@ -257,7 +257,8 @@ int32_t launch(const lct_rotary &r, hipStream_t stream) {
         if (best >= 0.9) break;
     }
     n.units_inverse = inverse_of(n.units);
-    n.per_token_inverse = inverse_of(n.per_token);
+    // Of one token all items are: more than kMaxItems may be its own.
+    n.per_token_inverse = n.per_group == 1 ? 1u : inverse_of(n.per_token);
     const int64_t grid = (tokens + n.per_group - 1) / n.per_group;
     if (grid >= int64_t{1} << 24) return LCT_E_SIZE;
     if (r.interleaved)

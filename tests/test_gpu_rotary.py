@@ -209,3 +209,23 @@ def test_far_positions_have_exact_angles(start):
         _near(got[:, t:t + 1], x[:, t:t + 1], torch.ones(1, 1), angles, FP32)
     with pytest.raises(ValueError, match="positions"):
         attention.apply_rotary(attention.Rotary(frequencies), x, positions=2 ** 31 + 1)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dim,turned", [(256, 256), (10, 6)])
+def test_as_many_heads_as_are_allowed(dim, turned, interleaved):
+    """4096 query and key heads: more units per token than 2^16."""
+    frequencies = attention.rotary_frequencies(turned)
+    plan = attention.Rotary(frequencies, interleaved=interleaved)
+    q, k = (_values(1, 2, 4096, dim, dtype=FP32, seed=s) for s in (0, 1))
+    at = _positions(1, 2, 3)
+    for x, got in zip((q, k), attention.apply_rotary(plan, q, k, positions=3)):
+        _near(got, x, at, frequencies, FP32, interleaved=interleaved)
+    caches = [torch.zeros(1, 5, 4096, dim, device=DEV) for _ in range(2)]
+    where = torch.tensor([4], device=DEV)
+    got = attention.rotary_append(plan, q[:, 0], k[:, 0], k[:, 1], *caches, where)
+    one = torch.tensor([[4]])
+    _near(got.unsqueeze(1), q[:, :1], one, frequencies, FP32, interleaved=interleaved)
+    _near(caches[0][:, 4:], k[:, :1], one, frequencies, FP32, interleaved=interleaved)
+    assert torch.equal(caches[1][:, 4], k[:, 1])
+    assert not bool(caches[0][:, :4].any()) and not bool(caches[1][:, :4].any())
