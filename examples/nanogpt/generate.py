@@ -93,6 +93,10 @@ class Generator:
 
     def generate(self, prompts: Tensor, steps: int) -> Tensor:
         """The ``steps`` likeliest tokens after each prompt, [batch, steps]."""
+        if steps < 1:
+            raise ValueError("steps must be at least 1")
+        for cache in self.caches:
+            cache.reset()
         token = self.logits(prompts).argmax(-1)
         out = [token]
         for _ in range(steps - 1):

@@ -165,3 +165,16 @@ def test_windowed_training_is_lossless_in_every_parameter():
         assert {name for name, _ in named if ".attn." in name and name.endswith("weight")} <= moved
         results.append(losses + [p.detach() for _, p in named])
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+def test_generation_begins_with_its_prompts():
+    """Again with the same generator, of one token, of none."""
+    model, _ = _started(compress_activations=False, compress_optimizer=False)
+    prompts = torch.randint(0, 512, (2, 5), generator=torch.Generator().manual_seed(1)).to(DEV)
+    generator = Generator(model, 2, 16, window=8)
+    for tokens in (prompts, prompts[:, :1]):
+        want = Generator(model, 2, 16, window=8).generate(tokens, 4)
+        for _ in range(2):
+            assert torch.equal(generator.generate(tokens, 4), want)
+    with pytest.raises(ValueError, match="steps"):
+        generator.generate(prompts, 0)
