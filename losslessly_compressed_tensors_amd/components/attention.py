@@ -233,8 +233,8 @@ def apply_rotary(plan: Rotary, q: Tensor, k: Tensor | None = None, positions=Non
     """``q`` and ``k``, [batch, token, head, channel] of BF16, FP16 or FP32, turned
     by their positions: ``(q, k)``, or ``q`` alone.  ``positions``: None (0, 1, ..),
     the first token's as an integer up to 2^31 or per sequence as [batch], or each
-    token's as [batch, token] (INT32; INT64 is held to INT32's range).  Angles and products are FP32,
-    rounded once.  Differentiable in ``q`` and ``k``."""
+    token's as [batch, token] (INT32; INT64 is held to INT32's range).  Angles and
+    products are FP32, rounded once.  Differentiable in ``q`` and ``k``."""
     _check_tensor(q, "q", 4, _ROTARY_TYPES)
     _check_rotary(plan, q)
     if k is not None:
@@ -403,8 +403,9 @@ def decode_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, lengths: Tenso
     """Attention of one query per sequence, ``q`` [batch, head, channel], over
     caches [batch, capacity, head, channel] that hold ``lengths`` [batch] tokens,
     the query's own last: :func:`window_attention` of that token.  A length of 0
-    gives zeros; lengths above the capacity count as the capacity.  Only keys
-    that are seen are read.  Not differentiable."""
+    gives zeros; lengths above the capacity count as the capacity.  Of the keys,
+    tiles of 32 that hold some that are seen are read; what is not seen has no
+    effect, whatever it holds.  Not differentiable."""
     _check_tensor(q, "q", 3, _ATTENTION_TYPES)
     _check_like(k_cache, "k_cache", q, 4)
     _check_like(v_cache, "v_cache", q, 4)

@@ -99,16 +99,19 @@ __device__ __forceinline__ float of_lane(float v, int lane) {
 // Matrix instructions, LDS reads (one fragment per instruction) and the softmax's
 // vector instructions take about 512, 512 and 450 clocks of a SIMD per 32 x 32
 // scores at heads of 128, at 1.9 to 2.0 GHz under this load; the two waves of a
-// SIMD overlap them in part (matrix instructions busy half of the time).  1525 us
-// for 8191 queries after 8192 keys, 32 heads of 128 over 8 (1080 TFLOP/s; 1580
-// with the compiler's order of LDS reads in place of read_ahead); 485 us for 1 x
-// 16384, 16 heads over 4, window 4096 (990); 22 us for 8 x 1024, 12 heads of 64,
-// window 256.  Tried: 32-key halves of a tile with the second half's scores issued
-// between the first's exponentials 1650 us at the first of these; matrix phases at
-// a higher wave priority 1560; column reads without the wait that the compiler puts
-// before them 1645; 64 queries per wave, which halve the LDS reads but leave one
-// wave per SIMD, 2020 with the instructions interleaved by hand; 8 waves per
-// workgroup, 4 in their products while the other 4 are in their softmax, 1605.
+// SIMD overlap them in part (matrix instructions busy half of the time).  1500 to
+// 1580 us for 8191 queries after 8192 keys, 32 heads of 128 over 8 (1045 to 1100
+// TFLOP/s; 1580 where 1525 with the compiler's order of LDS reads in place of
+// read_ahead; in FP16 1680 to 1750); 485 to 500 us for 1 x 16384, 16 heads over 4,
+// window 4096 (960 to 990); 22 to 23 us for 8 x 1024, 12 heads of 64, window 256, whose
+// few steps per wave leave it to latency (while a CU has work, 0.56 of the launch,
+// its vector units are 0.55 busy, its matrix units 0.21).  Tried at the first of these,
+// then 1525: 32-key halves of a tile with the second half's scores issued between the
+// first's exponentials 1650 us; matrix phases at a higher wave priority 1560; column
+// reads without the wait that the compiler puts before them 1645; 64 queries per wave,
+// which halve the LDS reads but leave one wave per SIMD, 2020 with the instructions
+// interleaved by hand; 8 waves per workgroup, 4 in their products while the other 4
+// are in their softmax, 1605.
 template <bool kHalf, int kDim, bool kSplit>
 __global__ __launch_bounds__(kAttentionThreads, 2) void attention_forward_kernel(
     lct_attention a, int32_t tiles, int32_t splits, float *__restrict__ parts) {
@@ -428,9 +431,10 @@ __device__ __forceinline__ void lower_half(f32x16 &ds, f32x16 (&sums)[kColumns],
 // A wave's 32 queries, the keys in tiles of 64: as in the forward kernel, with dP
 // beside the scores (its sums begin at -delta) and the keys' columns for the last
 // product.  delta is taken from the operands on their way in, and stored for the
-// other kernel.  650 us for 1 x 16384, 16 heads of 128 over 4, window 4096 (1110
-// TFLOP/s; 690 with the compiler's order of LDS reads), 29 us for 8 x 1024, 12
-// heads of 64, window 256, three waves per SIMD (in FP16 32.8; two waves 38.5).
+// other kernel.  650 to 670 us for 1 x 16384, 16 heads of 128 over 4, window 4096 (1080
+// to 1110 TFLOP/s; 690 with the compiler's order of LDS reads), 29 to 30 us for 8 x
+// 1024, 12 heads of 64, window 256, three waves per SIMD (in FP16 32.8; two waves 38.5),
+// by latency: CUs have work in 0.63 of it, vector units then 0.42 busy, matrix 0.23.
 template <bool kHalf, int kDim>
 __global__ __launch_bounds__(kAttentionThreads, kDim > 64 ? 2 : 3) void attention_dq_kernel(
     lct_attention a, lct_attention_gradients d, int32_t tiles) {
@@ -575,6 +579,8 @@ __global__ __launch_bounds__(kAttentionThreads, kDim > 64 ? 2 : 3) void attentio
     // of dS does (their error against FP64 is 1.48 and 1.47 times that of one
     // rounding without this, 1.43 and 1.42 with it, at 515 tokens under a window of
     // 127; rows of 16 keys and less make the difference), so it is taken out first.
+    // Where the window makes all rows such ones, every workgroup walks twice: 26.4 us
+    // at 8 x 1024, 12 heads of 64, window 64, for 21.9 at window 65.
     const bool few = first + shift < kFewKeys
                      || (a.window > 0 && a.window <= kFewKeys && a.sinks <= kFewKeys - a.window);
     if (few) {
@@ -689,14 +695,14 @@ __host__ __device__ constexpr int key_block(int dim) { return dim > 64 ? 256 : 1
 // bytes a clock, what four SIMDs' matrix instructions use) and the matrix
 // instructions are busy alike.  Heads wider than 64 hold 128 registers of sums and
 // 32 of the keys' operands; the values' stay in LDS (64 KB for 256 keys, read
-// again for each tile), so that two waves share a SIMD.  1080 us for 1 x 16384, 16
-// heads of 128 over 4, window 4096 (890 TFLOP/s; 1110 with the compiler's order of
-// LDS reads; 0.16 of it the end, when the workgroups of the last keys, which fewer
-// queries see, are done: parts of equal work would cost as much to add); 64 keys
-// per wave at one wave per SIMD, which read half as much: 1420; 32 with all
-// operands in registers at one wave per SIMD: 2200.  8 x 1024, 12 heads of 64,
-// window 256: 38 us, bound by the exponentials, masks and conversions of three
-// waves per SIMD (two: 42).
+// again for each tile), so that two waves share a SIMD.  1060 to 1200 us for 1 x 16384,
+// 16 heads of 128 over 4, window 4096 (800 to 910 TFLOP/s; 1110 where 1080 with the
+// compiler's order of LDS reads; 0.16 of it the end, when the workgroups of the last
+// keys, which fewer queries see, are done: parts of equal work would cost as much to
+// add); 64 keys per wave at one wave per SIMD, which read half as much: 1420; 32 with
+// all operands in registers at one wave per SIMD: 2200.  8 x 1024, 12 heads of 64,
+// window 256: 38 to 39 us at three waves per SIMD (two: 42), by latency: CUs have work
+// in 0.65 of it, vector units then 0.34 busy, matrix 0.19.
 template <bool kHalf, int kDim>
 __global__ __launch_bounds__(key_block(kDim) * 2, kDim > 64 ? 2 : 3) void attention_dkdv_kernel(
     lct_attention a, lct_attention_gradients d, KeyBlocks blocks, float *__restrict__ parts) {

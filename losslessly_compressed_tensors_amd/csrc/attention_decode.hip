@@ -11,7 +11,7 @@
 //
 // Bound by the read of the keys and values that the query sees: 5.8 TB/s for 64
 // sequences under a window of 4096 (32 heads of 128 over 8, 187 us), 6.6 TB/s for 4
-// of up to 131072 keys (263 us, and 12 for the join of 64 parts), where a plain
+// of up to 131072 keys (263 to 272 us, and 6 for the join of 42 parts), where a plain
 // read reaches 6.9.  The loads are issued whether or not there is a next tile, by
 // range-checked resources: with branches around them the wait for one tile also
 // waited for the next (200 and 322 us).  One sequence of 257 keys: 5.1 us, a

@@ -116,7 +116,11 @@ def _seen(keys: int, window: int, sinks: int, rows: int) -> int:
 def forward_splits(batch: int, heads: int, queries: int, keys: int, window: int,
                    sinks: int) -> int:
     """Workgroups that share a query tile's keys: as many as fill the compute
-    units twice where the tiles alone do not, with 4 key tiles each at least."""
+    units twice where there is no tile for each, with 4 key tiles each at least.
+    us in one part | two, of a few queries after 16384 keys: 32 tiles of heads of 128
+    282 | 153 (84 in four), 256 338 | 288; above the line 300 388 | 400, 384 423 | 426,
+    512 491 | 536; of heads of 64 300 278 | 244, 512 314 | 352, 640 407 | 427; 300 of 128
+    after 4096 keys 101 | 128."""
     items = batch * heads * -(-queries // _QUERY_TILE)
     if items > _CUS:
         return 1
@@ -217,10 +221,11 @@ def decode_splits(batch: int, heads: int, kv_heads: int, capacity: int, window: 
     """Workgroups that share a sequence's keys.  Up to 1024 keys one is as fast as
     several with the launch that joins their parts (us at 12 heads: 5.1 | 7.1 at
     257 keys, 7.6 | 7.4 at 1024, two and four parts); above, three workgroups per
-    compute unit (8 heads of 8192 keys: 73 in one part, 20 in 6, 13.4 in 24, 16 in
-    64; 128 of 4096: 75, 40 in 6, 43 in 8, 59 in 32), with 256 keys each at least,
-    and of long caches parts of 24 tiles at most, so that sequences of unequal
-    length even out (32 heads of 131072: 316 in 16 parts, 275 in 64)."""
+    compute unit (8 heads of 8192 keys: 74 in one part, 21 in 6, 13.8 in 24, 16 in
+    48; 128 of 4096: 75, 40 in 6, 44 in 8, 60 in 32), with 256 keys each at least,
+    and of long caches one part per 24 tiles, if more, up to 64, so that sequences of
+    unequal length even out (32 heads of up to 131072: 311 in 16 parts, 278 to 283 in
+    24, 275 to 278 in the 42 that they get, 268 to 275 in 64)."""
     items = batch * kv_heads * -(-(heads // kv_heads) // 16)
     tiles = -(-_seen(capacity, window, sinks, 1) // _DECODE_TILE)
     if tiles <= 8:

@@ -264,8 +264,8 @@ def test_long_caches_are_only_bound_by_what_is_launched(lib):
 PI = Fraction("3.14159265358979323846264338327950288419716939937510582097494")
 
 
-@pytest.mark.parametrize("frequency", [1.0, 0.01, 1e-6, -0.3333333333333333, 5e-324, 1e300, 12345.678,
-                                       *attention.rotary_frequencies(16).tolist()])
+@pytest.mark.parametrize("frequency", [1.0, 0.01, 1e-6, -0.3333333333333333, 5e-324, 1e300,
+                                       12345.678, *attention.rotary_frequencies(16).tolist()])
 def test_frequencies_are_the_nearest_fractions_of_a_turn(frequency):
     """Half of the last place, and the 2^-54 that FP64's turn is off."""
     turns, = attention.Rotary([frequency], device="cpu").turns.tolist()

@@ -28,8 +28,8 @@ def _calls():
                                                          None, 0, 3), heads),
         "decode": (lambda t: attention.decode_attention(t, cache, cache, at), token),
         "rotary": (lambda t: attention.apply_rotary(plan, t), cache),
-        "append": (lambda t: attention.rotary_append(plan, t, token, token, cache, cache.clone(), at),
-                   token),
+        "append": (lambda t: attention.rotary_append(plan, t, token, token, cache, cache.clone(),
+                                                     at), token),
         "dropout": (lambda t: dropout_add(t, heads, 0.5, 3), heads)}, cache
 
 
