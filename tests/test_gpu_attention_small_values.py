@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import attention_oracle as oracle
 import pytest
+import test_gpu_attention as plain
 import torch
 
 from losslessly_compressed_tensors_amd.components import attention
@@ -122,3 +123,17 @@ def test_many_small_weights_beside_a_large_one(sink, dtype, monkeypatch):
     for value in (got[:, :, 0], one):
         assert bool(((value.double() - exact[:, :, 0]).abs() <= bound[:, :, 0]).all()), (
             float(value.flatten()[0]), float(exact.flatten()[0]))
+
+
+@pytest.mark.parametrize("dim,splits", [(64, None), (128, None), (64, 3)])
+@pytest.mark.parametrize("where", ["v", "k", "q", "grad"])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_infinities_in_fp16(where, value, dim, splits, monkeypatch):
+    """The power of two that dS is held at follows finite values alone."""
+    monkeypatch.setattr(plain._inputs, "__defaults__", (FP16,))
+    plain.test_infinities_reach_only_what_sees_them(where, value, dim, splits, monkeypatch)
+
+
+def test_padding_in_fp16(monkeypatch):
+    monkeypatch.setattr(plain._inputs, "__defaults__", (FP16,))
+    plain.test_padding_may_hold_anything()
