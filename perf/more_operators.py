@@ -213,23 +213,25 @@ def _plain_loss(state: dict) -> dict:
     if case["softcap"]:
         slope = (1 + (logits / case["softcap"]).square()).rsqrt()
         logits = logits * slope
-    most = logits.amax(1, keepdim=True)
-    weights = (logits - most).exp()
-    lse = most + weights.sum(1, keepdim=True).log()
+    # The loss is log(1 + the others' weights over the target's), in 64 bits: of a well
+    # predicted token it is far smaller than the logits that it is the difference of.
     counted = targets != _IGNORED
     at = targets.clamp(min=0).unsqueeze(1)
-    losses = torch.where(counted, (lse - logits.gather(1, at)).squeeze(1), 0.0)
+    hit = logits.gather(1, at)
+    most = logits.amax(1, keepdim=True)
+    others = (logits - most).exp().scatter(1, at, 0.0).sum(1, keepdim=True).double()
+    loss = (others * (most - hit).double().exp()).log1p()
+    losses = torch.where(counted, loss.squeeze(1), 0.0)
     if case["kind"] == "score":
-        return {"losses": losses}
+        return {"losses": losses.float()}
     factor = counted.float()
     if case["reduction"] == "mean":
         factor = factor / counted.sum().clamp(min=1)
-    grad = (logits - lse).exp()
-    grad.scatter_add_(1, at, torch.full_like(at, -1.0, dtype=torch.float32))
-    grad = grad * factor.unsqueeze(1)
+    grad = (logits - (hit.double() + loss).float()).exp()
+    grad = grad.scatter(1, at, torch.expm1(-loss).float()) * factor.unsqueeze(1)
     if slope is not None:
         grad = grad * slope * slope * slope
-    out = {"loss": (losses.double() * factor.double()).sum().float(),
+    out = {"loss": (losses * factor.double()).sum().float(),
            "grad_x": (grad @ weight).to(state["x"].dtype),
            "grad_weight": (grad.T @ x).to(state["weight"].dtype)}
     if bias is not None:
