@@ -915,6 +915,64 @@ int32_t lct_dropout(const void *x, const void *residual, void *out, int64_t n, i
                     int32_t below, uint64_t seed, uint64_t offset, const int64_t *offset_more,
                     hipStream_t stream);
 
+/* ---- softmax cross entropy of a projection onto a vocabulary, in pieces of the
+ * vocabulary (examples/nanogpt/train_gpt_lct.py:88-140, which keeps the logits of a
+ * chunk of tokens): z = x W^T + bias, l = z / sqrt(1 + (z / softcap)^2) (softcap 0: z),
+ * losses[n] = log(sum_v exp(l[n][v])) - l[n][targets[n]].
+ *
+ * x [tokens, dim] and weight [vocab, dim]: BF16, or FP16 where fp16 != 0, rows by
+ * strides in elements, 16-byte aligned; dim and the strides: multiples of 8 up to
+ * LCT_MAX_CROSS_ENTROPY_DIM.  bias: FP32 or NULL.  targets: INT64 (targets_64 != 0) or
+ * INT32; tokens whose target is ignore_index have loss 0 and no gradients, and what
+ * their x holds reaches nothing; others outside [0, vocab) give NaN.  Logits,
+ * softmax statistics and sums are FP32. */
+#define LCT_MAX_CROSS_ENTROPY_TOKENS (1 << 22)
+#define LCT_MAX_CROSS_ENTROPY_VOCAB (1 << 24)
+#define LCT_MAX_CROSS_ENTROPY_DIM (1 << 16)
+#define LCT_MAX_CROSS_ENTROPY_SPLITS 16
+typedef struct {
+    const void *x, *weight;
+    const float *bias;
+    const void *targets;
+    int64_t x_stride, weight_stride, ignore_index;
+    int32_t tokens, vocab, dim, fp16, targets_64;
+    float softcap;
+} lct_cross_entropy;
+
+/* losses[n], and lse[n] for the backward call: log2 of sum_v exp(l[n][v]).  total: the
+ * losses' sum, or with mean != 0 that over the number of tokens that count (one at
+ * least); NULL: not written.  parts: working array of part_floats >= 4 * tokens *
+ * ceil(vocab / 256), 8-byte aligned.  index (1 + 2 * tokens values) and gathered (tokens *
+ * dim values, 16-byte aligned): working arrays for multiplying the tokens that count
+ * alone; NULL index: all are multiplied. */
+int32_t lct_cross_entropy_forward(const lct_cross_entropy *c, int32_t *index, int64_t index_size,
+                                  void *gathered, int64_t gathered_size, float *parts,
+                                  int64_t part_floats, float *lse, float *losses, float *total,
+                                  int32_t mean, hipStream_t stream);
+
+/* The gradients of x and weight (contiguous, of their type) and of the bias from those of
+ * the losses (grad_per_token != 0: grad[tokens]) or of their sum or mean (grad[1]).  Those
+ * that are NULL are not computed.  `piece`: how much of the vocabulary is worked on at a
+ * time (a multiple of 128); `splits`: into how many parts its sum for grad_x is divided.
+ * Working arrays: index (1 + 2 * tokens), values (1 + 3 * tokens), gathered (tokens * dim
+ * 16-bit values), dz (min(piece, vocab) * (tokens rounded up to 8) 16-bit values),
+ * hidden_parts (splits * tokens * dim), bias_parts (2 * ceil(tokens / 256) * vocab); those
+ * of 16 bits and hidden_parts 16-byte aligned. */
+typedef struct {
+    const float *grad, *lse, *losses;
+    void *grad_x, *grad_weight;
+    float *grad_bias;
+    int32_t *index;
+    float *values;
+    void *gathered, *dz;
+    float *hidden_parts, *bias_parts;
+    int64_t index_size, value_floats, gathered_size, dz_size, hidden_floats, bias_floats;
+    int32_t grad_per_token, mean, piece, splits;
+} lct_cross_entropy_gradients;
+
+int32_t lct_cross_entropy_backward(const lct_cross_entropy *c,
+                                   const lct_cross_entropy_gradients *d, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

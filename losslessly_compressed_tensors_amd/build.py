@@ -34,6 +34,7 @@ SOURCES = [
     "attention_decode.hip",
     "rotary.hip",
     "dropout.hip",
+    "cross_entropy.hip",
     "bandwidth.hip",
 ]
 

@@ -1,0 +1,844 @@
+// Softmax cross entropy of a projection onto a vocabulary, and its gradients, in
+// pieces of the vocabulary: the logits are never kept.
+//
+// Follows examples/nanogpt/train_gpt_lct.py:88-140, whose head keeps a chunk of
+// tokens' logits.  With z = x W^T + bias and, under a soft cap s, l = z / sqrt(1 + (z /
+// s)^2) (else l = z):
+//     loss = log(sum_v exp(l_v)) - l_t = log(1 + sum_{v != t} exp(l_v - l_t)),
+//     dz_v = g (exp(l_v) / sum - [v = t]) (1 + (z / s)^2)^(-3/2),
+//     dx = dz W,  dW = dz^T x,  dbias = the columns' sums of dz.
+// The second form of the loss keeps its precision where the target is likely:
+// the target is left out of the sums, and its own gradient is exp(-loss) - 1.
+//
+// Tokens that do not count (target ignore_index) are not multiplied: `rows` lists the
+// others, the products run over those, and what an ignored token's x holds reaches
+// nothing.
+#include <algorithm>
+
+#include "product_core.h"
+
+namespace lct {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+// dz in FP16 is held 2^14 larger: |dz| <= 1, and a probability is lost below 2^-38.
+constexpr float kHalfGradient = 16384.0f;
+// Where |z / s| may be squared in FP32; the cap is reached far below.
+constexpr float kCapped = 1e18f;
+
+template <bool kHalf>
+using LogitProduct = Product<kHalf, Lie::kRows, Lie::kRows, 256, 128, 2, 2, 32, 3>;
+template <bool kHalf>
+using HiddenProduct = Product<kHalf, Lie::kColumns, Lie::kColumns, 256, 128, 2, 2, 32, 3>;
+template <bool kHalf>
+using WeightProduct = Product<kHalf, Lie::kColumns, Lie::kRows, 256, 128, 2, 2, 32, 3>;
+
+#define LCT_PRODUCT_STAGES(P)                                                             \
+    __shared__ __attribute__((aligned(1024))) uint16_t stage0[P::kStage];                 \
+    __shared__ __attribute__((aligned(1024))) uint16_t stage1[P::kStage];                 \
+    __shared__ __attribute__((aligned(1024))) uint16_t stage2[P::kStage];                 \
+    uint16_t *const stages[3] = {stage0, stage1, stage2}
+
+// The counted tokens, as prepare_kernel found them.
+struct Counted {
+    const int32_t *count;      // how many
+    const int32_t *rows;       // int32[count]: which tokens
+    const int32_t *targets;    // their targets, -1 for none of the vocabulary
+    const float *lse, *losses, *factor;   // backward: of those
+    const float *scale;        // backward: what gradients are multiplied by at the end
+    const void *gathered;      // their x, where not all count
+};
+
+__device__ __forceinline__ const void *hidden_of(const lct_cross_entropy &c, const Counted &t,
+                                                 int32_t count, int64_t *stride) {
+    const bool all = count == c.tokens;
+    *stride = all ? c.x_stride : c.dim;
+    return all ? c.x : t.gathered;
+}
+
+__device__ __forceinline__ int64_t target_of(const lct_cross_entropy &c, int64_t n) {
+    return c.targets_64 ? static_cast<const int64_t *>(c.targets)[n]
+                        : static_cast<const int32_t *>(c.targets)[n];
+}
+
+// ---- the counted tokens, in order
+
+constexpr int kPrepareThreads = 1024;
+
+__device__ __forceinline__ float block_max(float v, float *scratch) {
+#pragma unroll
+    for (int d = kWave / 2; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor(v, d, kWave));
+    if (wave_lane() == 0) scratch[threadIdx.x / kWave] = v;
+    __syncthreads();
+    v = scratch[0];
+    for (int w = 1; w < kPrepareThreads / kWave; ++w) v = fmaxf(v, scratch[w]);
+    __syncthreads();
+    return v;
+}
+
+// One workgroup.  Forward (grad NULL): which tokens count, and lse and losses of the
+// others.  Backward: also the factor of each token's dz and what all gradients are
+// multiplied by at the end: a token's incoming gradient over the power of two above the
+// largest, and that power, so that dz lies within [-1, 1] whatever the incoming gradients
+// are.  (All infinite or NaN ones go to their tokens' factors.)
+__global__ __launch_bounds__(kPrepareThreads) void prepare_kernel(
+    lct_cross_entropy c, int32_t *count_out, int32_t *rows, int32_t *targets, float *lse,
+    float *losses, const float *grad, int32_t grad_per_token, int32_t mean, float *lse_of,
+    float *losses_of, float *factor, float *scale) {
+    __shared__ float scratch[kPrepareThreads / kWave];
+    __shared__ int32_t counts[kPrepareThreads / kWave];
+    float largest = 0.0f;
+    if (grad != nullptr && grad_per_token)
+        for (int32_t n = threadIdx.x; n < c.tokens; n += kPrepareThreads)
+            if (target_of(c, n) != c.ignore_index) {
+                const float g = fabsf(grad[n]);
+                if (g < INFINITY) largest = fmaxf(largest, g);
+            }
+    float power = 1.0f;
+    if (grad != nullptr && grad_per_token) {
+        largest = block_max(largest, scratch);
+        // 2^e >= largest, within FP32's normal numbers.
+        if (largest > 0.0f) power = ldexpf(1.0f, min(max(ilogbf(largest) + 1, -126), 127));
+    }
+    const float hold = c.fp16 ? kHalfGradient : 1.0f;
+    int32_t done = 0;
+    for (int32_t first = 0; first < c.tokens; first += kPrepareThreads) {
+        const int32_t n = first + threadIdx.x;
+        const int64_t target = n < c.tokens ? target_of(c, n) : c.ignore_index;
+        const bool counts_here = n < c.tokens && target != c.ignore_index;
+        const uint64_t ballot = __ballot(counts_here);
+        if (wave_lane() == 0) counts[threadIdx.x / kWave] = __popcll(ballot);
+        __syncthreads();
+        int32_t before = done, total = 0;
+        for (int w = 0; w < kPrepareThreads / kWave; ++w) {
+            before += w < static_cast<int>(threadIdx.x / kWave) ? counts[w] : 0;
+            total += counts[w];
+        }
+        __syncthreads();
+        if (counts_here) {
+            const int32_t i = before + __popcll(ballot & ((uint64_t{1} << wave_lane()) - 1));
+            const bool inside = target >= 0 && target < c.vocab;
+            rows[i] = n;
+            targets[i] = inside ? static_cast<int32_t>(target) : -1;
+            if (grad != nullptr) {
+                lse_of[i] = lse[n];
+                losses_of[i] = losses[n];
+                factor[i] = inside ? (grad_per_token ? grad[n] / power : 1.0f) * hold : NAN;
+            }
+        } else if (grad == nullptr && n < c.tokens) {
+            lse[n] = 0.0f;
+            losses[n] = 0.0f;
+        }
+        done += total;
+    }
+    if (threadIdx.x == 0) {
+        *count_out = done;
+        if (grad != nullptr)
+            *scale = (grad_per_token ? power : *grad / (mean ? fmaxf(1.0f, done) : 1.0f)) / hold;
+    }
+}
+
+// The counted tokens' x next to each other, 16 bytes a thread, where not all count.
+__global__ __launch_bounds__(256) void gather_kernel(lct_cross_entropy c, Counted t, void *out) {
+    const int32_t count = *t.count, chunks = c.dim / 8;
+    if (count == c.tokens) return;
+    const int64_t all = int64_t{count} * chunks;
+    for (int64_t at = int64_t{blockIdx.x} * 256 + threadIdx.x; at < all;
+         at += int64_t{gridDim.x} * 256) {
+        const int32_t i = static_cast<int32_t>(at / chunks), chunk = static_cast<int32_t>(at % chunks);
+        static_cast<u32x4 *>(out)[at] = *reinterpret_cast<const u32x4 *>(
+            static_cast<const uint16_t *>(c.x) + t.rows[i] * c.x_stride + chunk * 8);
+    }
+}
+
+// ---- forward
+
+// The sums under way of one token over part of the vocabulary, the target left out:
+// the largest logit and the sum of exponentials from there, in powers of two.
+struct Part {
+    float most, total;
+};
+
+__device__ __forceinline__ Part joined(Part a, Part b) {
+    const float most = fmaxf(a.most, b.most);
+    const float base = most == -INFINITY ? 0.0f : most;
+    return {most, a.total * exp2_fast(a.most - base) + b.total * exp2_fast(b.most - base)};
+}
+
+// z / sqrt(1 + (z / s)^2) and, if wanted, (1 + (z / s)^2)^(-1/2).
+struct Cap {
+    float cap, inverse;
+    __device__ __forceinline__ float root(float z) const {
+        const float u = z * inverse;
+        return __builtin_amdgcn_rsqf(__builtin_fmaf(u, u, 1.0f));
+    }
+    // z, or the largest of its sign that root() takes; NaN stays.
+    __device__ __forceinline__ float within(float z) const {
+        const float most = kCapped * cap;
+        return fabsf(z) > most ? copysignf(most, z) : z;
+    }
+};
+
+// 256 of the vocabulary (rows, in a lane's registers) by 128 tokens (columns, a lane
+// each): a token's maximum and sum need one exchange between two lanes.
+template <bool kHalf, bool kCap, bool kBias>
+__global__ __launch_bounds__(256, 2) void logits_kernel(lct_cross_entropy c, Counted t,
+                                                        int32_t vocab_tiles, int32_t token_tiles,
+                                                        Part *__restrict__ parts) {
+    using P = LogitProduct<kHalf>;
+    LCT_PRODUCT_STAGES(P);
+    const int32_t count = t.count == nullptr ? c.tokens : *t.count;
+    const int64_t item = xcd_item(int64_t{vocab_tiles} * token_tiles, blockIdx.x);
+    if (item >= int64_t{vocab_tiles} * token_tiles) return;
+    // Eight vocabulary tiles against all tokens, then the next eight.
+    const int32_t group = static_cast<int32_t>(item / (8 * int64_t{token_tiles}));
+    const int32_t in_group = static_cast<int32_t>(item % (8 * int64_t{token_tiles}));
+    const int32_t width = min(8, vocab_tiles - 8 * group);
+    const int32_t vocab_tile = 8 * group + in_group % width, token_tile = in_group / width;
+    if (int64_t{token_tile} * P::kN >= count) return;
+
+    int64_t x_stride;
+    const void *x = t.count == nullptr ? c.x : hidden_of(c, t, count, &x_stride);
+    if (t.count == nullptr) x_stride = c.x_stride;
+    typename P::A a;
+    typename P::B b;
+    a.prepare(c.weight, c.weight_stride, int64_t{vocab_tile} * P::kM, c.vocab);
+    b.prepare(x, x_stride, int64_t{token_tile} * P::kN, count);
+    P p;
+    p.run(a, b, c.dim, stages);
+
+    const int half = wave_lane() >> 5;
+    const int32_t first = vocab_tile * P::kM + p.first_row();
+    const Cap cap{c.softcap, 1.0f / c.softcap};
+    int32_t token[P::kColumnTiles], target[P::kColumnTiles];
+#pragma unroll
+    for (int n = 0; n < P::kColumnTiles; ++n) {
+        token[n] = token_tile * P::kN + p.first_column() + 32 * n + (wave_lane() & 31);
+        target[n] = -1;
+        if (token[n] < count)
+            target[n] = t.count != nullptr ? t.targets[token[n]]
+                                           : static_cast<int32_t>(std::min<int64_t>(
+                                                 std::max<int64_t>(target_of(c, token[n]), -1),
+                                                 c.vocab));
+        target[n] -= first;
+    }
+    if constexpr (kBias) {
+#pragma unroll
+        for (int m = 0; m < P::kRowTiles; ++m)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int32_t row = first + 32 * m + 8 * (r / 4) + 4 * half + r % 4;
+                const float bias = row < c.vocab ? c.bias[row] : 0.0f;
+#pragma unroll
+                for (int n = 0; n < P::kColumnTiles; ++n) p.sum[m][n][r] += bias;
+            }
+    }
+    if constexpr (kCap) {
+        float largest = 0.0f;
+#pragma unroll
+        for (int m = 0; m < P::kRowTiles; ++m)
+#pragma unroll
+            for (int n = 0; n < P::kColumnTiles; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) largest = fmaxf(largest, fabsf(p.sum[m][n][r]));
+        const bool far = __any(largest > kCapped * c.softcap);
+#pragma unroll
+        for (int m = 0; m < P::kRowTiles; ++m)
+#pragma unroll
+            for (int n = 0; n < P::kColumnTiles; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    float z = p.sum[m][n][r];
+                    if (far) z = cap.within(z);
+                    p.sum[m][n][r] = z * cap.root(z);
+                }
+    }
+    if (first + P::kWaveM > c.vocab) {
+#pragma unroll
+        for (int m = 0; m < P::kRowTiles; ++m)
+#pragma unroll
+            for (int n = 0; n < P::kColumnTiles; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (first + 32 * m + 8 * (r / 4) + 4 * half + r % 4 >= c.vocab)
+                        p.sum[m][n][r] = -INFINITY;
+    }
+    const int32_t entries = 2 * vocab_tiles;
+#pragma unroll
+    for (int n = 0; n < P::kColumnTiles; ++n) {
+        if (__any(target[n] >= 0 && target[n] < P::kWaveM)) {
+#pragma unroll
+            for (int m = 0; m < P::kRowTiles; ++m)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (32 * m + 8 * (r / 4) + 4 * half + r % 4 == target[n])
+                        p.sum[m][n][r] = -INFINITY;
+        }
+        float most = p.sum[0][n][0];
+#pragma unroll
+        for (int m = 0; m < P::kRowTiles; ++m)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) most = fmaxf(most, p.sum[m][n][r]);
+        most = across_max(most) * kLog2e;
+        const float base = most == -INFINITY ? 0.0f : most;
+        float total = 0.0f;
+#pragma unroll
+        for (int m = 0; m < P::kRowTiles; ++m)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                total += exp2_fast(__builtin_fmaf(p.sum[m][n][r], kLog2e, -base));
+        total = across_sum(total);
+        if (half == 0 && token[n] < count)
+            parts[int64_t{token[n]} * entries + 2 * vocab_tile + p.wave() % 2] = Part{most, total};
+    }
+}
+
+// A wave joins one token's parts and computes its target's logit: the loss and lse (in
+// powers of two).
+template <bool kHalf>
+__global__ __launch_bounds__(256) void join_kernel(lct_cross_entropy c, Counted t, int32_t entries,
+                                                   const Part *__restrict__ parts,
+                                                   float *__restrict__ lse,
+                                                   float *__restrict__ losses) {
+    using E = Element<kHalf>;
+    const int32_t count = t.count == nullptr ? c.tokens : *t.count;
+    const int32_t i = blockIdx.x * 4 + threadIdx.x / kWave;
+    if (i >= count) return;
+    const int lane = wave_lane();
+    const int32_t n = t.count == nullptr ? i : t.rows[i];
+    const int64_t target = target_of(c, n);
+    if (target == c.ignore_index) {
+        if (lane == 0) lse[n] = losses[n] = 0.0f;
+        return;
+    }
+    const bool inside = target >= 0 && target < c.vocab;
+    Part part{-INFINITY, 0.0f};
+    for (int32_t e = lane; e < entries; e += kWave)
+        part = joined(part, parts[int64_t{i} * entries + e]);
+    float logit = 0.0f;
+    if (inside) {
+        const uint16_t *x = static_cast<const uint16_t *>(c.x) + n * c.x_stride;
+        const uint16_t *w = static_cast<const uint16_t *>(c.weight) + target * c.weight_stride;
+        for (int32_t d = 8 * lane; d < c.dim; d += 8 * kWave) {
+            const u32x4 p = *reinterpret_cast<const u32x4 *>(x + d);
+            const u32x4 q = *reinterpret_cast<const u32x4 *>(w + d);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                logit = __builtin_fmaf(E::low(p[k]), E::low(q[k]), logit);
+                logit = __builtin_fmaf(E::high(p[k]), E::high(q[k]), logit);
+            }
+        }
+    }
+#pragma unroll
+    for (int d = kWave / 2; d > 0; d >>= 1) {
+        logit += __shfl_xor(logit, d, kWave);
+        part = joined(part, Part{__shfl_xor(part.most, d, kWave), __shfl_xor(part.total, d, kWave)});
+    }
+    if (lane != 0) return;
+    if (!inside) {
+        lse[n] = losses[n] = NAN;
+        return;
+    }
+    if (c.bias != nullptr) logit += c.bias[target];
+    if (c.softcap > 0.0f) {
+        const Cap cap{c.softcap, 1.0f / c.softcap};
+        logit = cap.within(logit);
+        const float u = logit * cap.inverse;
+        logit = logit / sqrtf(__builtin_fmaf(u, u, 1.0f));
+    }
+    // The others' weight over the target's, or that one's inverse.
+    const float own = logit * kLog2e;
+    const float above = part.most - own + log2f(part.total);
+    const float rest = log1pf(above > 0.0f ? exp2f(-above) : part.total * exp2f(part.most - own));
+    float loss = above > 0.0f ? __builtin_fmaf(above, kLn2, rest) : rest;
+    float sum = above > 0.0f ? part.most + log2f(part.total) + rest * kLog2e : own + rest * kLog2e;
+    if (part.total == 0.0f || logit == INFINITY) {    // no others, or nothing but the target
+        loss = logit - logit;
+        sum = own + loss;
+    }
+    losses[n] = loss;
+    lse[n] = sum;
+}
+
+// The losses' sum or mean; one workgroup, in a fixed order.
+__global__ __launch_bounds__(kPrepareThreads) void total_kernel(lct_cross_entropy c,
+                                                                const float *__restrict__ losses,
+                                                                int32_t mean, float *out) {
+    __shared__ double sums[kPrepareThreads / kWave];
+    __shared__ int32_t counts[kPrepareThreads / kWave];
+    double sum = 0.0;
+    int32_t count = 0;
+    for (int32_t n = threadIdx.x; n < c.tokens; n += kPrepareThreads) {
+        sum += losses[n];
+        count += target_of(c, n) != c.ignore_index;
+    }
+#pragma unroll
+    for (int d = kWave / 2; d > 0; d >>= 1) {
+        sum += __shfl_xor(sum, d, kWave);
+        count += __shfl_xor(count, d, kWave);
+    }
+    if (wave_lane() == 0) {
+        sums[threadIdx.x / kWave] = sum;
+        counts[threadIdx.x / kWave] = count;
+    }
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    for (int w = 1; w < kPrepareThreads / kWave; ++w) {
+        sum += sums[w];
+        count += counts[w];
+    }
+    *out = static_cast<float>(mean ? sum / max(1, count) : sum);
+}
+
+// ---- backward
+
+// Writes a wave's tile (rows m, columns n; round(m, n, r, pair) gives two adjacent rows'
+// values) with a column's 128 rows next to each other: 8 bytes a lane into the wave's
+// 8 KB of LDS, 16 bytes a lane out of it, so that the stores are of 256 bytes.
+// `rows`: how many there are from the wave's first on, a multiple of 8.
+template <class P, class Pair>
+__device__ __forceinline__ void store_columns(uint16_t *out, int64_t stride, int32_t columns,
+                                              int32_t rows, uint16_t *mine, Pair pair) {
+    static_assert(P::kWaveM == 128);
+    const int lane = wave_lane(), column = lane & 31, half = lane >> 5;
+#pragma unroll
+    for (int n = 0; n < P::kColumnTiles; ++n) {
+#pragma unroll
+        for (int m = 0; m < P::kRowTiles; ++m)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int chunk = (4 * m + g) ^ (column & 15);
+                *reinterpret_cast<u32x2 *>(mine + column * 128 + chunk * 8
+                                           + (half ^ (column >> 3 & 1)) * 4) =
+                    u32x2{pair(m, n, 4 * g), pair(m, n, 4 * g + 2)};
+            }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int at = 4 * i + (lane >> 4), chunk = lane & 15;
+            u32x4 v = *reinterpret_cast<const u32x4 *>(mine + at * 128 + (chunk ^ (at & 15)) * 8);
+            if (at >> 3 & 1) v = u32x4{v[2], v[3], v[0], v[1]};
+            if (32 * n + at < columns && chunk * 8 < rows)
+                *reinterpret_cast<u32x4 *>(out + (32 * n + at) * stride + chunk * 8) = v;
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+__device__ __forceinline__ uint16_t *wave_store(uint16_t *const (&stages)[3]) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    return (wave < 2 ? stages[0] : stages[1]) + (wave & 1) * 4096;
+}
+
+// dz of 256 tokens (rows) by 128 of a piece of the vocabulary (columns, a lane each), the
+// logits computed again: written by columns, [vocabulary][token], which both products
+// that follow read, and its sums over these tokens.
+template <bool kHalf, bool kCap, bool kBias>
+__global__ __launch_bounds__(256, 2) void gradient_kernel(lct_cross_entropy c, Counted t,
+                                                          int32_t first_vocab, int32_t piece,
+                                                          int32_t vocab_tiles,
+                                                          int32_t token_tiles, uint16_t *dz,
+                                                          int64_t dz_stride, float *bias_parts) {
+    using P = LogitProduct<kHalf>;
+    LCT_PRODUCT_STAGES(P);
+    __shared__ float4 row_values[P::kM];
+    const int32_t count = *t.count;
+    const int64_t item = xcd_item(int64_t{vocab_tiles} * token_tiles, blockIdx.x);
+    if (item >= int64_t{vocab_tiles} * token_tiles) return;
+    const int32_t group = static_cast<int32_t>(item / (8 * int64_t{vocab_tiles}));
+    const int32_t in_group = static_cast<int32_t>(item % (8 * int64_t{vocab_tiles}));
+    const int32_t width = min(8, token_tiles - 8 * group);
+    const int32_t token_tile = 8 * group + in_group % width, vocab_tile = in_group / width;
+    if (int64_t{token_tile} * P::kM >= count) return;
+
+    int64_t x_stride;
+    const void *x = hidden_of(c, t, count, &x_stride);
+    const int32_t last_vocab = first_vocab + piece;
+    typename P::A a;
+    typename P::B b;
+    a.prepare(x, x_stride, int64_t{token_tile} * P::kM, count);
+    b.prepare(c.weight, c.weight_stride, first_vocab + int64_t{vocab_tile} * P::kN, last_vocab);
+    // Each token's lse, factor, target and its dz there; tokens past the last have
+    // factor 0.
+    {
+        const int32_t i = token_tile * P::kM + threadIdx.x;
+        float4 v{INFINITY, 0.0f, __int_as_float(-1), 0.0f};
+        if (i < count)
+            v = float4{t.lse[i], t.factor[i], __int_as_float(t.targets[i]), expm1f(-t.losses[i])};
+        row_values[threadIdx.x] = v;
+    }
+    P p;
+    p.run(a, b, c.dim, stages);
+
+    const int lane = wave_lane(), half = lane >> 5;
+    const int32_t first = first_vocab + vocab_tile * P::kN + p.first_column();
+    const Cap cap{c.softcap, 1.0f / c.softcap};
+    float bias[P::kColumnTiles], column_sum[P::kColumnTiles];
+#pragma unroll
+    for (int n = 0; n < P::kColumnTiles; ++n) {
+        const int32_t column = first + 32 * n + (lane & 31);
+        bias[n] = kBias && column < last_vocab ? c.bias[column] : 0.0f;
+        column_sum[n] = 0.0f;
+    }
+#pragma unroll
+    for (int m = 0; m < P::kRowTiles; ++m) {
+        const float4 *values = row_values + p.first_row() + 32 * m;
+        const int32_t target = __float_as_int(values[lane & 31].z) - first;
+        const bool hit = __any(target >= 0 && target < P::kWaveN);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float4 v = values[8 * (r / 4) + 4 * half + r % 4];
+            const int32_t at = __float_as_int(v.z) - first - (lane & 31);
+#pragma unroll
+            for (int n = 0; n < P::kColumnTiles; ++n) {
+                float z = p.sum[m][n][r] + bias[n], slope = 1.0f;
+                if constexpr (kCap) {
+                    z = cap.within(z);
+                    const float root = cap.root(z);
+                    z *= root;
+                    slope = root * root * root;
+                }
+                float d = exp2_fast(__builtin_fmaf(z, kLog2e, -v.x));
+                if (hit) d = at == 32 * n ? v.w : d;
+                d = v.y == 0.0f ? 0.0f : d * v.y * slope;
+                p.sum[m][n][r] = d;
+                column_sum[n] += d;
+            }
+        }
+    }
+    if (first + P::kWaveN > last_vocab) {
+#pragma unroll
+        for (int n = 0; n < P::kColumnTiles; ++n)
+            if (first + 32 * n + (lane & 31) >= last_vocab) {
+#pragma unroll
+                for (int m = 0; m < P::kRowTiles; ++m)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) p.sum[m][n][r] = 0.0f;
+            }
+    }
+    if (bias_parts != nullptr) {
+#pragma unroll
+        for (int n = 0; n < P::kColumnTiles; ++n) {
+            const float sum = across_sum(column_sum[n]);
+            const int32_t column = first + 32 * n + (lane & 31);
+            if (half == 0 && column < last_vocab)
+                bias_parts[(int64_t{token_tile} * 2 + p.wave() % 2) * c.vocab + column] = sum;
+        }
+    }
+    if (dz == nullptr) return;
+    const int32_t column = vocab_tile * P::kN + p.first_column();
+    const int32_t row = token_tile * P::kM + p.first_row();
+    store_columns<P>(dz + column * dz_stride + row, dz_stride, piece - column,
+                     static_cast<int32_t>(dz_stride) - row, wave_store(stages),
+                     [&](int m, int n, int r) {
+                         return Element<kHalf>::round_pair(p.sum[m][n][r], p.sum[m][n][r + 1]);
+                     });
+}
+
+// dx of a piece of the vocabulary, or of one of its `splits` parts: 256 channels (rows)
+// by 128 tokens (columns), added to the earlier pieces' in FP32.
+template <bool kHalf>
+__global__ __launch_bounds__(256, 2) void hidden_gradient_kernel(
+    lct_cross_entropy c, Counted t, int32_t first_vocab, int32_t piece, int32_t splits,
+    int32_t dim_tiles, int32_t token_tiles, const uint16_t *dz, int64_t dz_stride, float *parts) {
+    using P = HiddenProduct<kHalf>;
+    LCT_PRODUCT_STAGES(P);
+    const int32_t count = *t.count;
+    const int64_t items = int64_t{dim_tiles} * token_tiles * splits;
+    const int64_t item = xcd_item(items, blockIdx.x);
+    if (item >= items) return;
+    const int32_t dim_tile = static_cast<int32_t>(item % dim_tiles);
+    const int32_t token_tile = static_cast<int32_t>(item / dim_tiles % token_tiles);
+    const int32_t split = static_cast<int32_t>(item / dim_tiles / token_tiles);
+    if (int64_t{token_tile} * P::kN >= count) return;
+    const int32_t per = ((piece + splits - 1) / splits + 31) / 32 * 32;
+    const int32_t begin = min(piece, split * per), end = min(piece, begin + per);
+
+    typename P::A a;
+    typename P::B b;
+    a.prepare(static_cast<const uint16_t *>(c.weight) + (first_vocab + begin) * c.weight_stride,
+              c.weight_stride, int64_t{dim_tile} * P::kM, c.dim);
+    b.prepare(dz + begin * dz_stride, dz_stride, int64_t{token_tile} * P::kN,
+              (int64_t{count} + 7) / 8 * 8);
+    P p;
+    p.run(a, b, end - begin, stages);
+
+    const int lane = wave_lane();
+#pragma unroll
+    for (int n = 0; n < P::kColumnTiles; ++n) {
+        const int32_t token = token_tile * P::kN + p.first_column() + 32 * n + (lane & 31);
+        if (token >= count) continue;
+        float *out = parts + (int64_t{split} * c.tokens + token) * c.dim;
+#pragma unroll
+        for (int m = 0; m < P::kRowTiles; ++m)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int32_t d =
+                    dim_tile * P::kM + p.first_row() + 32 * m + 8 * g + 4 * (lane >> 5);
+                if (d >= c.dim) continue;
+                f32x4 v{p.sum[m][n][4 * g], p.sum[m][n][4 * g + 1], p.sum[m][n][4 * g + 2],
+                        p.sum[m][n][4 * g + 3]};
+                if (first_vocab > 0) v += *reinterpret_cast<const f32x4 *>(out + d);
+                *reinterpret_cast<f32x4 *>(out + d) = v;
+            }
+    }
+}
+
+// dW of a piece: 256 channels (rows) by 128 of the vocabulary (columns).
+template <bool kHalf>
+__global__ __launch_bounds__(256, 2) void weight_gradient_kernel(
+    lct_cross_entropy c, Counted t, int32_t first_vocab, int32_t piece, int32_t dim_tiles,
+    int32_t vocab_tiles, const uint16_t *dz, int64_t dz_stride, uint16_t *grad_weight) {
+    using P = WeightProduct<kHalf>;
+    LCT_PRODUCT_STAGES(P);
+    const int32_t count = *t.count;
+    const int64_t item = xcd_item(int64_t{dim_tiles} * vocab_tiles, blockIdx.x);
+    if (item >= int64_t{dim_tiles} * vocab_tiles) return;
+    const int32_t dim_tile = static_cast<int32_t>(item % dim_tiles);
+    const int32_t vocab_tile = static_cast<int32_t>(item / dim_tiles);
+    int64_t x_stride;
+    const void *x = hidden_of(c, t, count, &x_stride);
+    typename P::A a;
+    typename P::B b;
+    a.prepare(x, x_stride, int64_t{dim_tile} * P::kM, c.dim);
+    b.prepare(dz, dz_stride, int64_t{vocab_tile} * P::kN, piece);
+    P p;
+    // Tokens past the last: zeros of dz (up to 7) against zeros of x.
+    p.run(a, b, count, stages);
+
+    const float scale = *t.scale;
+    const int32_t column = vocab_tile * P::kN + p.first_column();
+    const int32_t row = dim_tile * P::kM + p.first_row();
+    store_columns<P>(grad_weight + (int64_t{first_vocab} + column) * c.dim + row, c.dim,
+                     piece - column, c.dim - row, wave_store(stages), [&](int m, int n, int r) {
+                         return Element<kHalf>::round_pair(p.sum[m][n][r] * scale,
+                                                           p.sum[m][n][r + 1] * scale);
+                     });
+}
+
+// dx from its parts, 8 values a thread; zeros for tokens that do not count.
+template <bool kHalf>
+__global__ __launch_bounds__(256) void join_hidden_kernel(lct_cross_entropy c, Counted t,
+                                                          int32_t splits,
+                                                          const float *__restrict__ parts,
+                                                          uint16_t *__restrict__ grad_x) {
+    const int32_t count = *t.count, chunks = c.dim / 8;
+    const float scale = *t.scale;
+    const int64_t all = int64_t{count} * chunks;
+    for (int64_t at = int64_t{blockIdx.x} * 256 + threadIdx.x; at < all;
+         at += int64_t{gridDim.x} * 256) {
+        const int32_t i = static_cast<int32_t>(at / chunks);
+        const int32_t d = static_cast<int32_t>(at % chunks) * 8;
+        f32x4 lo{}, hi{};
+        for (int32_t s = 0; s < splits; ++s) {
+            const float *from = parts + (int64_t{s} * c.tokens + i) * c.dim + d;
+            lo += *reinterpret_cast<const f32x4 *>(from);
+            hi += *reinterpret_cast<const f32x4 *>(from + 4);
+        }
+        lo *= scale;
+        hi *= scale;
+        using E = Element<kHalf>;
+        *reinterpret_cast<u32x4 *>(grad_x + int64_t{t.rows[i]} * c.dim + d) =
+            u32x4{E::round_pair(lo[0], lo[1]), E::round_pair(lo[2], lo[3]),
+                  E::round_pair(hi[0], hi[1]), E::round_pair(hi[2], hi[3])};
+    }
+    if (count == c.tokens) return;
+    for (int64_t at = int64_t{blockIdx.x} * 256 + threadIdx.x; at < int64_t{c.tokens} * chunks;
+         at += int64_t{gridDim.x} * 256) {
+        const int64_t n = at / chunks;
+        if (target_of(c, n) == c.ignore_index)
+            *reinterpret_cast<u32x4 *>(grad_x + at * 8) = u32x4{0u, 0u, 0u, 0u};
+    }
+}
+
+__global__ __launch_bounds__(256) void join_bias_kernel(lct_cross_entropy c, Counted t,
+                                                        const float *__restrict__ parts,
+                                                        float *__restrict__ grad_bias) {
+    const int32_t v = blockIdx.x * 256 + threadIdx.x;
+    if (v >= c.vocab) return;
+    const int32_t tiles = (*t.count + 255) / 256;
+    float sum = 0.0f;
+    for (int32_t i = 0; i < 2 * tiles; ++i) sum += parts[int64_t{i} * c.vocab + v];
+    grad_bias[v] = sum * *t.scale;
+}
+
+// ---- entry points
+
+bool aligned(const void *p, uintptr_t bytes) { return !(reinterpret_cast<uintptr_t>(p) % bytes); }
+
+int32_t check(const lct_cross_entropy *c) {
+    if (c == nullptr || c->x == nullptr || c->weight == nullptr || c->targets == nullptr)
+        return LCT_E_NULL;
+    // Tiles are addressed by 32-bit byte offsets: 256 rows of up to 2^22 values.
+    if (c->tokens < 1 || c->tokens > LCT_MAX_CROSS_ENTROPY_TOKENS || c->vocab < 1
+        || c->vocab > LCT_MAX_CROSS_ENTROPY_VOCAB || c->dim < 8 || c->dim % 8
+        || c->dim > LCT_MAX_CROSS_ENTROPY_DIM)
+        return LCT_E_SIZE;
+    if (c->x_stride < c->dim || c->x_stride % 8 || c->x_stride > LCT_MAX_CROSS_ENTROPY_DIM
+        || c->weight_stride < c->dim || c->weight_stride % 8
+        || c->weight_stride > LCT_MAX_CROSS_ENTROPY_DIM || !aligned(c->x, 16)
+        || !aligned(c->weight, 16) || !aligned(c->bias, 4)
+        || !aligned(c->targets, c->targets_64 ? 8 : 4) || !(c->softcap >= 0.0f)
+        || !(c->softcap < 1e19f))
+        return LCT_E_ARG;
+    return 0;
+}
+
+int32_t tiles_of(int64_t n, int32_t tile) { return static_cast<int32_t>((n + tile - 1) / tile); }
+
+constexpr int32_t kMaxStrideGrid = 1 << 16;
+
+template <class Launch>
+void by_form(const lct_cross_entropy &c, Launch launch) {
+    const auto with = [&](auto half) {
+        const auto capped = [&](auto cap) {
+            if (c.bias != nullptr) launch(half, cap, std::true_type{});
+            else launch(half, cap, std::false_type{});
+        };
+        if (c.softcap > 0.0f) capped(std::true_type{});
+        else capped(std::false_type{});
+    };
+    if (c.fp16) with(std::true_type{});
+    else with(std::false_type{});
+}
+
+}  // namespace
+}  // namespace lct
+
+using namespace lct;
+
+extern "C" int32_t lct_cross_entropy_forward(const lct_cross_entropy *c, int32_t *index,
+                                             int64_t index_size, void *gathered,
+                                             int64_t gathered_size, float *parts,
+                                             int64_t part_floats, float *lse, float *losses,
+                                             float *total, int32_t mean, hipStream_t stream) {
+    if (const int32_t bad = check(c)) return bad;
+    if (parts == nullptr || lse == nullptr || losses == nullptr) return LCT_E_NULL;
+    const int32_t vocab_tiles = tiles_of(c->vocab, 256), token_tiles = tiles_of(c->tokens, 128);
+    if (part_floats < int64_t{4} * vocab_tiles * c->tokens || !aligned(parts, 8)) return LCT_E_SIZE;
+    Counted t{};
+    if (index != nullptr) {
+        if (gathered == nullptr) return LCT_E_NULL;
+        if (index_size < 1 + 2 * int64_t{c->tokens}
+            || gathered_size < int64_t{c->tokens} * c->dim || !aligned(gathered, 16))
+            return LCT_E_SIZE;
+        t.count = index;
+        t.rows = index + 1;
+        t.targets = index + 1 + c->tokens;
+        t.gathered = gathered;
+        prepare_kernel<<<1, kPrepareThreads, 0, stream>>>(
+            *c, index, index + 1, index + 1 + c->tokens, lse, losses, nullptr, 0, 0, nullptr,
+            nullptr, nullptr, nullptr);
+        gather_kernel<<<std::min<int64_t>(kMaxStrideGrid,
+                                          (int64_t{c->tokens} * (c->dim / 8) + 255) / 256),
+                        256, 0, stream>>>(*c, t, gathered);
+    }
+    const uint32_t grid = static_cast<uint32_t>(xcd_grid(int64_t{vocab_tiles} * token_tiles));
+    by_form(*c, [&](auto half, auto cap, auto bias) {
+        logits_kernel<decltype(half)::value, decltype(cap)::value, decltype(bias)::value>
+            <<<grid, 256, 0, stream>>>(*c, t, vocab_tiles, token_tiles,
+                                       reinterpret_cast<Part *>(parts));
+    });
+    const uint32_t waves = static_cast<uint32_t>((c->tokens + 3) / 4);
+    if (c->fp16)
+        join_kernel<true><<<waves, 256, 0, stream>>>(*c, t, 2 * vocab_tiles,
+                                                     reinterpret_cast<const Part *>(parts), lse,
+                                                     losses);
+    else
+        join_kernel<false><<<waves, 256, 0, stream>>>(*c, t, 2 * vocab_tiles,
+                                                      reinterpret_cast<const Part *>(parts), lse,
+                                                      losses);
+    if (total != nullptr)
+        total_kernel<<<1, kPrepareThreads, 0, stream>>>(*c, losses, mean, total);
+    return static_cast<int32_t>(hipGetLastError());
+}
+
+extern "C" int32_t lct_cross_entropy_backward(const lct_cross_entropy *c,
+                                              const lct_cross_entropy_gradients *d,
+                                              hipStream_t stream) {
+    if (const int32_t bad = check(c)) return bad;
+    if (d == nullptr || d->grad == nullptr || d->lse == nullptr || d->losses == nullptr
+        || d->index == nullptr || d->values == nullptr || d->gathered == nullptr)
+        return LCT_E_NULL;
+    const bool products = d->grad_x != nullptr || d->grad_weight != nullptr;
+    if ((products && d->dz == nullptr) || (d->grad_x != nullptr && d->hidden_parts == nullptr)
+        || (d->grad_bias != nullptr && (d->bias_parts == nullptr || c->bias == nullptr)))
+        return LCT_E_NULL;
+    const int64_t tokens = c->tokens, pitch = (tokens + 7) / 8 * 8;
+    const int32_t token_tiles = tiles_of(tokens, 256);
+    if (d->piece < 1 || d->piece % 128 || d->splits < 1 || d->splits > LCT_MAX_CROSS_ENTROPY_SPLITS
+        || d->index_size < 1 + 2 * tokens || d->value_floats < 1 + 3 * tokens
+        || d->gathered_size < tokens * c->dim
+        || (products && d->dz_size < std::min(d->piece, c->vocab) * pitch)
+        || (d->grad_x != nullptr && d->hidden_floats < d->splits * tokens * c->dim)
+        || (d->grad_bias != nullptr && d->bias_floats < int64_t{2} * token_tiles * c->vocab))
+        return LCT_E_SIZE;
+    if (!aligned(d->gathered, 16) || !aligned(d->dz, 16) || !aligned(d->hidden_parts, 16)
+        || !aligned(d->grad_x, 16) || !aligned(d->grad_weight, 16))
+        return LCT_E_ARG;
+    Counted t{};
+    int32_t *rows = d->index + 1, *targets = rows + tokens;
+    float *lse = d->values + 1, *losses = lse + tokens, *factor = losses + tokens;
+    t.count = d->index;
+    t.rows = rows;
+    t.targets = targets;
+    t.scale = d->values;
+    t.lse = lse;
+    t.losses = losses;
+    t.factor = factor;
+    t.gathered = d->gathered;
+    prepare_kernel<<<1, kPrepareThreads, 0, stream>>>(
+        *c, d->index, rows, targets, const_cast<float *>(d->lse), const_cast<float *>(d->losses),
+        d->grad, d->grad_per_token, d->mean, lse, losses, factor, d->values);
+    const uint32_t chunk_grid = static_cast<uint32_t>(
+        std::min<int64_t>(kMaxStrideGrid, (tokens * (c->dim / 8) + 255) / 256));
+    gather_kernel<<<chunk_grid, 256, 0, stream>>>(*c, t, d->gathered);
+    auto *dz = static_cast<uint16_t *>(d->dz);
+    const int32_t dim_tiles = tiles_of(c->dim, 256), hidden_tiles = tiles_of(tokens, 128);
+    for (int32_t first = 0; first < c->vocab; first += d->piece) {
+        const int32_t piece = std::min(d->piece, c->vocab - first);
+        const int32_t vocab_tiles = tiles_of(piece, 128);
+        const uint32_t grid = static_cast<uint32_t>(xcd_grid(int64_t{vocab_tiles} * token_tiles));
+        by_form(*c, [&](auto half, auto cap, auto bias) {
+            gradient_kernel<decltype(half)::value, decltype(cap)::value, decltype(bias)::value>
+                <<<grid, 256, 0, stream>>>(*c, t, first, piece, vocab_tiles, token_tiles,
+                                           products ? dz : nullptr, pitch,
+                                           d->grad_bias != nullptr ? d->bias_parts : nullptr);
+        });
+        if (d->grad_x != nullptr) {
+            const uint32_t items = static_cast<uint32_t>(
+                xcd_grid(int64_t{dim_tiles} * hidden_tiles * d->splits));
+            if (c->fp16)
+                hidden_gradient_kernel<true><<<items, 256, 0, stream>>>(
+                    *c, t, first, piece, d->splits, dim_tiles, hidden_tiles, dz, pitch,
+                    d->hidden_parts);
+            else
+                hidden_gradient_kernel<false><<<items, 256, 0, stream>>>(
+                    *c, t, first, piece, d->splits, dim_tiles, hidden_tiles, dz, pitch,
+                    d->hidden_parts);
+        }
+        if (d->grad_weight != nullptr) {
+            const uint32_t items = static_cast<uint32_t>(xcd_grid(int64_t{dim_tiles} * vocab_tiles));
+            auto *out = static_cast<uint16_t *>(d->grad_weight);
+            if (c->fp16)
+                weight_gradient_kernel<true><<<items, 256, 0, stream>>>(
+                    *c, t, first, piece, dim_tiles, vocab_tiles, dz, pitch, out);
+            else
+                weight_gradient_kernel<false><<<items, 256, 0, stream>>>(
+                    *c, t, first, piece, dim_tiles, vocab_tiles, dz, pitch, out);
+        }
+    }
+    if (d->grad_x != nullptr) {
+        auto *out = static_cast<uint16_t *>(d->grad_x);
+        if (c->fp16)
+            join_hidden_kernel<true>
+                <<<chunk_grid, 256, 0, stream>>>(*c, t, d->splits, d->hidden_parts, out);
+        else
+            join_hidden_kernel<false>
+                <<<chunk_grid, 256, 0, stream>>>(*c, t, d->splits, d->hidden_parts, out);
+    }
+    if (d->grad_bias != nullptr)
+        join_bias_kernel<<<tiles_of(c->vocab, 256), 256, 0, stream>>>(*c, t, d->bias_parts,
+                                                                      d->grad_bias);
+    return static_cast<int32_t>(hipGetLastError());
+}

@@ -164,12 +164,14 @@ class UpdateJob(ctypes.Structure):
     ]
 
 
-# lct_attention, lct_attention_gradients and lct_rotary, packed in one step (a
+# lct_attention, lct_attention_gradients, lct_rotary and those of the cross entropy, packed in one step (a
 # ctypes.Structure's field writes took 12 us of a 20 us call); entry points take
 # the bytes.  Fields as include/lct.h declares them.
 ATTENTION = struct.Struct("@6P12q9if")
 ATTENTION_GRADIENTS = struct.Struct("@5P12q")
 ROTARY = struct.Struct("@8P21q10if4x")
+CROSS_ENTROPY = struct.Struct("@4P3q5if")
+CROSS_ENTROPY_GRADIENTS = struct.Struct("@12P6q4i")
 
 # Value types (LCT_BF16, LCT_FP16, LCT_FP32).
 BF16, FP16, FP32 = 0, 1, 2
@@ -268,6 +270,9 @@ _SIGNATURES = {
     "lct_rotate": [_ptr, _ptr],
     "lct_dropout": [_ptr, _ptr, _ptr, _c_int64, _c_int32, _c_int32, ctypes.c_uint64,
                     ctypes.c_uint64, _ptr, _ptr],
+    "lct_cross_entropy_forward": [_ptr, _ptr, _c_int64, _ptr, _c_int64, _ptr, _c_int64, _ptr, _ptr,
+                                  _ptr, _c_int32, _ptr],
+    "lct_cross_entropy_backward": [_ptr, _ptr, _ptr],
     "lct_bandwidth_probe": [_c_int32, _ptr, _c_int64, _ptr, _c_int64, _c_int32, _ptr],
     "lct_compress_buffered_noalloc": [_ptr, _c_int64, _c_int64, Geometry, _ptr, _ptr, _ptr, _ptr,
                                       _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int32, _ptr,

@@ -1,0 +1,131 @@
+"""Launches of the kernels that are made of matrix products: the cross entropy of a
+projection onto a vocabulary (``csrc/cross_entropy.hip``) and the orthogonalisation
+(``csrc/orthogonal.hip``).
+
+The callers (``components/losses.py``, ``components/orthogonal.py``,
+``components/layers.py``) have checked types and shapes; here tensors get the
+strides and alignment that the kernels read, outputs and workspaces are
+allocated on the current stream, and the work is shared out.
+"""
+from __future__ import annotations
+
+from functools import lru_cache
+
+import torch
+from torch import Tensor
+
+from . import hip
+from .attention import _check_unrecorded, _launch
+
+MAX_TOKENS = 1 << 22    # LCT_MAX_CROSS_ENTROPY_TOKENS
+MAX_VOCAB = 1 << 24     # LCT_MAX_CROSS_ENTROPY_VOCAB
+MAX_DIM = 1 << 16       # LCT_MAX_CROSS_ENTROPY_DIM
+
+_CUS = 256
+_SLOTS = 2 * _CUS       # workgroups of a product's kernel that run at once
+_MAX_SPLITS = 16        # LCT_MAX_CROSS_ENTROPY_SPLITS
+_PIECE_BYTES = 256 << 20
+
+
+def _whole_rows(t: Tensor) -> Tensor:
+    """``t``, or a copy, as a matrix whose rows are whole 16-byte pieces at strides and
+    an address that the kernels read; zeros where it has to be widened."""
+    rows, cols = t.shape
+    if cols % 8:
+        out = t.new_zeros(rows, -(-cols // 8) * 8)
+        out[:, :cols] = t
+        return out
+    stride = t.stride(0) if rows > 1 else cols
+    if (t.stride(1) == 1 and cols <= stride <= MAX_DIM and not stride & 7
+            and not t.data_ptr() & 15):
+        return t if t.stride(0) == stride else t.as_strided(t.shape, (stride, 1))
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _cross_entropy(x: Tensor, weight: Tensor, bias, targets: Tensor, softcap: float,
+                   ignore_index: int) -> bytes:
+    return hip.CROSS_ENTROPY.pack(
+        x.data_ptr(), weight.data_ptr(), 0 if bias is None else bias.data_ptr(),
+        targets.data_ptr(), x.stride(0), weight.stride(0), ignore_index, x.shape[0],
+        weight.shape[0], x.shape[1], x.dtype == torch.float16, targets.dtype == torch.int64,
+        softcap)
+
+
+def cross_entropy_forward(x: Tensor, weight: Tensor, bias, targets: Tensor, softcap: float,
+                          ignore_index: int, reduction: str):
+    """``(losses, lse, total)`` of [token, channel] and [vocabulary, channel] matrices,
+    an FP32 bias or None and contiguous targets; ``total`` is the losses' sum or mean,
+    None for the reduction "none"."""
+    _check_unrecorded(x, weight, bias)
+    x, weight = _whole_rows(x), _whole_rows(weight)
+    tokens, dim = x.shape
+    losses = x.new_empty(tokens, dtype=torch.float32)
+    lse = torch.empty_like(losses)
+    total = None if reduction == "none" else x.new_empty((), dtype=torch.float32)
+    floats = 4 * tokens * -(-weight.shape[0] // 256)
+    parts = x.new_empty(floats, dtype=torch.float32)
+    index = x.new_empty(1 + 2 * tokens, dtype=torch.int32)
+    gathered = x.new_empty(tokens * dim)
+    _launch("lct_cross_entropy_forward", x.get_device(),
+            _cross_entropy(x, weight, bias, targets, softcap, ignore_index), index.data_ptr(),
+            index.numel(), gathered.data_ptr(), gathered.numel(), parts.data_ptr(), floats,
+            lse.data_ptr(), losses.data_ptr(), None if total is None else total.data_ptr(),
+            reduction == "mean")
+    return losses, lse, total
+
+
+@lru_cache(maxsize=1024)
+def vocabulary_pieces(tokens: int, vocab: int, dim: int) -> tuple:
+    """The size of a piece and the parts of its sum for the gradient of x."""
+    pieces = -(-2 * vocab * tokens // _PIECE_BYTES)
+    piece = -(-vocab // (256 * pieces)) * 256
+    tiles = -(-dim // 256) * -(-tokens // 128)
+    best = None
+    for splits in range(1, min(_MAX_SPLITS, max(1, piece // 512)) + 1):
+        time = -(-tiles * splits // _SLOTS) * (piece / 32 / splits + 8) + 2 * splits * tiles / 32
+        if best is None or time < best[0]:
+            best = time, splits
+    return piece, best[1]
+
+
+def cross_entropy_backward(grad: Tensor, x: Tensor, weight: Tensor, bias, targets: Tensor,
+                           losses: Tensor, lse: Tensor, softcap: float, ignore_index: int,
+                           reduction: str, needed: tuple):
+    """``(grad_x, grad_weight, grad_bias)``, None where not ``needed``; the bias's in
+    FP32."""
+    _check_unrecorded(grad, x, weight, bias)
+    dim = x.shape[1]
+    x, weight = _whole_rows(x), _whole_rows(weight)
+    tokens, width = x.shape
+    vocab = weight.shape[0]
+    piece, splits = vocabulary_pieces(tokens, vocab, width)
+    need_x, need_weight, need_bias = needed
+    grad_x = x.new_empty(tokens, width) if need_x else None
+    grad_weight = x.new_empty(vocab, width) if need_weight else None
+    grad_bias = x.new_empty(vocab, dtype=torch.float32) if need_bias else None
+    index = x.new_empty(1 + 2 * tokens, dtype=torch.int32)
+    values = x.new_empty(1 + 3 * tokens, dtype=torch.float32)
+    gathered = x.new_empty(tokens * width)
+    dz = (x.new_empty(min(piece, vocab) * (-(-tokens // 8) * 8)) if need_x or need_weight
+          else None)
+    hidden = x.new_empty(splits * tokens * width, dtype=torch.float32) if need_x else None
+    columns = (x.new_empty(2 * -(-tokens // 256) * vocab, dtype=torch.float32) if need_bias
+               else None)
+
+    def at(t):
+        return 0 if t is None else t.data_ptr()
+
+    def size(t):
+        return 0 if t is None else t.numel()
+
+    _launch("lct_cross_entropy_backward", x.get_device(),
+            _cross_entropy(x, weight, bias, targets, softcap, ignore_index),
+            hip.CROSS_ENTROPY_GRADIENTS.pack(
+                grad.data_ptr(), lse.data_ptr(), losses.data_ptr(), at(grad_x), at(grad_weight),
+                at(grad_bias), at(index), at(values), at(gathered), at(dz), at(hidden),
+                at(columns), size(index), size(values), size(gathered), size(dz), size(hidden),
+                size(columns), reduction == "none", reduction == "mean", piece, splits))
+    if width != dim:
+        grad_x, grad_weight = (None if g is None else g[:, :dim].contiguous()
+                               for g in (grad_x, grad_weight))
+    return grad_x, grad_weight, grad_bias

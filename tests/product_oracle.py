@@ -1,0 +1,104 @@
+"""The product operators' definitions in 64 bits on the CPU, and how far a kernel may
+be from them.
+
+Bounds count roundings: u = eps / 2 of a type is the most that one rounding to it
+moves a value, relative to it; FP32 sums of n products are off by n 2^-24 of the sum of
+the products' magnitudes at most.
+"""
+from __future__ import annotations
+
+import torch
+
+U32 = 2.0 ** -24
+
+
+def half_step(dtype) -> float:
+    return torch.finfo(dtype).eps / 2
+
+
+def smallest(dtype) -> float:
+    """Half of the spacing of the subnormal numbers."""
+    return torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
+
+
+class CrossEntropy:
+    """Losses and gradients of one call, from the definition, and their bounds."""
+
+    def __init__(self, x, weight, targets, bias=None, softcap=None, ignore_index=-100,
+                 reduction="mean", grad=None):
+        self.dtype = weight.dtype
+        dim = x.shape[-1]
+        x = x.reshape(-1, dim).double()
+        weight, targets = weight.double(), targets.reshape(-1)
+        counted = targets != ignore_index
+        x = torch.where(counted[:, None], x, 0.0)
+        vocab = weight.shape[0]
+        z = x @ weight.T
+        # FP32 sums of dim products, the bias's addition.
+        spread = x.abs() @ weight.abs().T
+        if bias is not None:
+            z = z + bias.double()
+            spread = spread + bias.double().abs()
+        z_off = (dim + 2) * U32 * spread
+        slope = torch.ones_like(z)
+        if softcap:
+            root = (1 + (z / softcap).square()).rsqrt()
+            z, slope = z * root, root ** 3
+        z_off = z_off + 4 * U32 * z.abs()
+        z_off = torch.where(z_off.isfinite(), z_off, 0.0)
+        at = targets.clamp(0, vocab - 1)
+        log_p = torch.log_softmax(z, 1)
+        hit = torch.arange(len(at))
+        bad = counted & ((targets < 0) | (targets >= vocab))
+        losses = torch.where(counted, -log_p[hit, at], 0.0)
+        self.losses = torch.where(bad, torch.nan, losses)
+        # A loss moves by at most twice what a logit does; its own few roundings.
+        most = z_off.amax(1)
+        self.losses_off = 2 * most + 16 * U32 * (self.losses.abs() + losses.abs() + 1e-3)
+        count = max(1, int(counted.sum()))
+        share = counted.double()
+        if reduction == "mean":
+            share = share / count
+        self.total = (self.losses * share).sum()
+        self.total_off = (self.losses_off * share).sum() + 2 * U32 * self.total.abs()
+        g = torch.ones((), dtype=torch.float64) if grad is None else grad.double().reshape(-1)
+        share = share * g
+        p = log_p.exp()
+        dz = p.clone()
+        dz[hit, at] = torch.where(counted, torch.expm1(-losses), 0.0)
+        dz = dz * share[:, None] * slope
+        dz = torch.where((share == 0)[:, None], 0.0, dz)
+        dz = torch.where(bad[:, None], torch.nan, dz)
+        # exp turns a difference into a relative one; the slope's cube triples its root's.
+        relative = (2 * most + 32 * U32)[:, None] + (8 * z_off if softcap else 0.0)
+        dz_off = dz.abs() * relative
+        # The target's: exp(-loss) - 1 moves by the loss's difference.
+        dz_off[hit, at] += (share.abs() * self.losses_off * p[hit, at]).nan_to_num(0.0)
+        self.dz = dz
+        self.grad_bias = dz.sum(0)
+        self.grad_bias_off = dz_off.sum(0) + (len(at) + 4) * U32 * dz.abs().sum(0) + 1e-37
+        u = half_step(self.dtype)
+        # Rounded for the products; what FP16 holds 2^14 larger ends at 2^-25 of it, of the
+        # largest factor.
+        rounded = dz_off + u * dz.abs()
+        if self.dtype == torch.float16:
+            rounded = rounded + 2.0 ** -38 * share.abs().max()
+        self.grad_x = dz @ weight
+        off = rounded @ weight.abs() + (vocab + 4) * U32 * (dz.abs() @ weight.abs())
+        self.grad_x_off = off * (1 + u) + u * self.grad_x.abs() + smallest(self.dtype)
+        self.grad_weight = dz.T @ x
+        off = rounded.T @ x.abs() + (len(at) + 4) * U32 * (dz.abs().T @ x.abs())
+        self.grad_weight_off = off * (1 + u) + u * self.grad_weight.abs() + smallest(self.dtype)
+
+
+def assert_within(got, exact, off, name=""):
+    got = got.detach().cpu().double().reshape(exact.shape)
+    assert torch.equal(got.isnan(), exact.isnan()), f"{name}: NaN in other places"
+    infinite = exact.isinf()
+    assert torch.equal(got[infinite], exact[infinite]), f"{name}: infinities"
+    sure = exact.isfinite()
+    far = (got - exact).abs()
+    excess = torch.where(far == 0, 0.0, far / off)[sure]
+    if excess.numel():
+        worst = float(excess.max())
+        assert worst <= 1, f"{name}: {worst:.3g} times its bound"
