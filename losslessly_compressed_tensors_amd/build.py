@@ -35,6 +35,7 @@ SOURCES = [
     "rotary.hip",
     "dropout.hip",
     "cross_entropy.hip",
+    "orthogonal.hip",
     "bandwidth.hip",
 ]
 

@@ -1,0 +1,47 @@
+"""The Newton-Schulz iteration of Muon as kernels of its own.
+
+``components/sparse_utils.py``'s ``zeropower_via_newtonschulz5`` (the reference's,
+``LCT/components/sparse_utils.py:71-86``) iterates in BF16 on the library's products.
+:func:`orthogonalize` computes the same polynomial with the symmetric products by
+half and the iterate in FP32; ``SparseMuon(fused=True)`` steps with it.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+from torch import Tensor
+
+from ..kernels import products as kernels
+from .attention import _check_tensor, _whole
+
+__all__ = ["orthogonalize"]
+
+_EPS = 1e-7
+
+
+@torch.compiler.disable
+@torch.no_grad()
+def orthogonalize(G: Tensor, steps: int = 5, *, scale: float = 1.0) -> Tensor:
+    """``scale`` times the Newton-Schulz approximation of the polar factor of ``G``, a
+    matrix or a batch of them in its last two dimensions, of BF16, FP16 or FP32 and any
+    strides; BF16, contiguous, in ``G``'s orientation.
+
+    Each matrix is divided by its Frobenius norm plus 1e-7, then ``steps`` times ``X <- 2 X
+    + (-1.5 A + 0.5 A A) X`` with ``A = X X^T`` (of a tall one: transposed).  X stays in
+    FP32 between steps, and the products' operands are FP16 at fixed powers of two:
+    results are within 1e-3 of the exact iteration's norm, the rounding to BF16 (1.7e-3)
+    aside.  Not differentiable."""
+    if not isinstance(G, Tensor) or G.ndim < 2:
+        raise TypeError("G must be a torch.Tensor of at least two dimensions")
+    _check_tensor(G, "G", G.ndim, tuple(kernels.TYPES))
+    steps = _whole(steps, "steps", 0, 1000)
+    if not math.isfinite(scale):
+        raise ValueError("scale must be finite")
+    rows, cols = G.shape[-2:]
+    if max(rows, cols) > kernels.MAX_MATRIX_DIM:
+        raise ValueError(f"at most {kernels.MAX_MATRIX_DIM} rows and columns")
+    if G.numel() == 0:
+        return torch.empty(G.shape, dtype=torch.bfloat16, device=G.device)
+    out = kernels.orthogonalize(G.reshape(-1, rows, cols), steps, float(scale), _EPS)
+    return out.view(G.shape)

@@ -164,7 +164,8 @@ class UpdateJob(ctypes.Structure):
     ]
 
 
-# lct_attention, lct_attention_gradients, lct_rotary and those of the cross entropy, packed in one step (a
+# lct_attention, lct_attention_gradients, lct_rotary, lct_cross_entropy,
+# lct_cross_entropy_gradients and lct_orthogonal, packed in one step (a
 # ctypes.Structure's field writes took 12 us of a 20 us call); entry points take
 # the bytes.  Fields as include/lct.h declares them.
 ATTENTION = struct.Struct("@6P12q9if")
@@ -172,6 +173,7 @@ ATTENTION_GRADIENTS = struct.Struct("@5P12q")
 ROTARY = struct.Struct("@8P21q10if4x")
 CROSS_ENTROPY = struct.Struct("@4P3q5if")
 CROSS_ENTROPY_GRADIENTS = struct.Struct("@12P6q4i")
+ORTHOGONAL = struct.Struct("@2P6q5i2f4x")
 
 # Value types (LCT_BF16, LCT_FP16, LCT_FP32).
 BF16, FP16, FP32 = 0, 1, 2
@@ -273,6 +275,7 @@ _SIGNATURES = {
     "lct_cross_entropy_forward": [_ptr, _ptr, _c_int64, _ptr, _c_int64, _ptr, _c_int64, _ptr, _ptr,
                                   _ptr, _c_int32, _ptr],
     "lct_cross_entropy_backward": [_ptr, _ptr, _ptr],
+    "lct_orthogonalize": [_ptr, _ptr, _c_int64, _ptr],
     "lct_bandwidth_probe": [_c_int32, _ptr, _c_int64, _ptr, _c_int64, _c_int32, _ptr],
     "lct_compress_buffered_noalloc": [_ptr, _c_int64, _c_int64, Geometry, _ptr, _ptr, _ptr, _ptr,
                                       _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int32, _ptr,

@@ -1,5 +1,5 @@
 """Launches of the kernels that are made of matrix products: the cross entropy of a
-projection onto a vocabulary (``csrc/cross_entropy.hip``) and the orthogonalisation
+projection onto a vocabulary (``csrc/cross_entropy.hip``) and Muon's orthogonalisation
 (``csrc/orthogonal.hip``).
 
 The callers (``components/losses.py``, ``components/orthogonal.py``,
@@ -15,7 +15,7 @@ import torch
 from torch import Tensor
 
 from . import hip
-from .attention import _check_unrecorded, _launch
+from .attention import TYPES, _check_unrecorded, _launch
 
 MAX_TOKENS = 1 << 22    # LCT_MAX_CROSS_ENTROPY_TOKENS
 MAX_VOCAB = 1 << 24     # LCT_MAX_CROSS_ENTROPY_VOCAB
@@ -25,6 +25,9 @@ _CUS = 256
 _SLOTS = 2 * _CUS       # workgroups of a product's kernel that run at once
 _MAX_SPLITS = 16        # LCT_MAX_CROSS_ENTROPY_SPLITS
 _PIECE_BYTES = 256 << 20
+
+MAX_MATRIX_DIM = 1 << 16    # LCT_MAX_ORTHOGONAL_DIM
+_NORM_PARTS = 64            # LCT_ORTHOGONAL_NORM_PARTS
 
 
 def _whole_rows(t: Tensor) -> Tensor:
@@ -129,3 +132,26 @@ def cross_entropy_backward(grad: Tensor, x: Tensor, weight: Tensor, bias, target
         grad_x, grad_weight = (None if g is None else g[:, :dim].contiguous()
                                for g in (grad_x, grad_weight))
     return grad_x, grad_weight, grad_bias
+
+
+def _up8(n: int) -> int:
+    return -(-n // 8) * 8
+
+
+def orthogonalize(g: Tensor, steps: int, scale: float, eps: float) -> Tensor:
+    """BF16 matrices of [matrix, row, column] ones."""
+    _check_unrecorded(g)
+    out = torch.empty(g.shape, dtype=torch.bfloat16, device=g.device)
+    count, rows, cols = g.shape
+    stride, out_stride = g.stride(), out.stride()
+    if rows > cols:
+        rows, cols = cols, rows
+        stride = stride[0], stride[2], stride[1]
+        out_stride = out_stride[0], out_stride[2], out_stride[1]
+    r, c = _up8(rows), _up8(cols)
+    size = -(-count * 8 * _NORM_PARTS // 16) * 16 + count * (8 * r * c + 4 * r * r)
+    workspace = torch.empty(size, dtype=torch.uint8, device=g.device)
+    _launch("lct_orthogonalize", g.get_device(), hip.ORTHOGONAL.pack(
+        g.data_ptr(), out.data_ptr(), *stride, *out_stride, count, rows, cols, steps,
+        TYPES[g.dtype], scale, eps), workspace.data_ptr(), size)
+    return out

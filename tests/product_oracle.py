@@ -102,3 +102,28 @@ def assert_within(got, exact, off, name=""):
     if excess.numel():
         worst = float(excess.max())
         assert worst <= 1, f"{name}: {worst:.3g} times its bound"
+
+
+def polar(g, steps, scale=1.0, eps=1e-7):
+    """The Newton-Schulz iteration of a matrix or a batch of them, in 64 bits."""
+    g = g.double()
+    tall = g.shape[-2] > g.shape[-1]
+    x = g.mT if tall else g
+    x = x / (x.square().sum((-2, -1), keepdim=True).sqrt() + eps)
+    for _ in range(steps):
+        a = x @ x.mT
+        x = 2.0 * x + (-1.5 * a + 0.5 * (a @ a)) @ x
+    return scale * (x.mT if tall else x)
+
+
+def polar_off(steps) -> float:
+    """How far a result may be, relative to the exact one's Frobenius norm.
+
+    The result is rounded to BF16: 2^-8 of a value at most, evenly spread below that.  A
+    step rounds X, A and P to FP16 (u = 2^-11 at most) for its products: with |X|, |A|,
+    |P| <= 1 and |dP/dA| <= 1.5 they move it by u of X's norm through P X, by 1.5 u
+    through each X of A, 1.5 u through A and 1.5 u through P; evenly spread and
+    independent, sqrt(1 + 4 * 1.5^2) u / sqrt(3) together, and later steps do not let it
+    grow faster than X.  A half more, since small matrices have few roundings."""
+    step = (10.0 / 3) ** 0.5 * 2.0 ** -11
+    return 1.5 * ((2.0 ** -8) ** 2 / 3 + steps * step ** 2) ** 0.5
