@@ -942,7 +942,7 @@ typedef struct {
 /* losses[n], and lse[n] for the backward call: log2 of sum_v exp(l[n][v]).  total: the
  * losses' sum, or with mean != 0 that over the number of tokens that count (one at
  * least); NULL: not written.  parts: working array of part_floats >= 4 * tokens *
- * ceil(vocab / 256), 8-byte aligned.  index (1 + 2 * tokens values) and gathered (tokens *
+ * ceil(vocab / 128), 8-byte aligned.  index (1 + 2 * tokens values) and gathered (tokens *
  * dim values, 16-byte aligned): working arrays for multiplying the tokens that count
  * alone; NULL index: all are multiplied. */
 int32_t lct_cross_entropy_forward(const lct_cross_entropy *c, int32_t *index, int64_t index_size,
@@ -956,7 +956,7 @@ int32_t lct_cross_entropy_forward(const lct_cross_entropy *c, int32_t *index, in
  * time (a multiple of 128); `splits`: into how many parts its sum for grad_x is divided.
  * Working arrays: index (1 + 2 * tokens), values (1 + 3 * tokens), gathered (tokens * dim
  * 16-bit values), dz (min(piece, vocab) * (tokens rounded up to 8) 16-bit values),
- * hidden_parts (splits * tokens * dim), bias_parts (2 * ceil(tokens / 256) * vocab); those
+ * hidden_parts (splits * tokens * dim), bias_parts (2 * ceil(tokens / 128) * vocab); those
  * of 16 bits and hidden_parts 16-byte aligned. */
 typedef struct {
     const float *grad, *lse, *losses;

@@ -26,18 +26,13 @@ constexpr float kHalfGradient = 16384.0f;
 // Where |z / s| may be squared in FP32; the cap is reached far below.
 constexpr float kCapped = 1e18f;
 
+constexpr int kLogitRows = 192;
 template <bool kHalf>
-using LogitProduct = Product<kHalf, Lie::kRows, Lie::kRows, 256, 128, 2, 2, 32, 3>;
+using LogitProduct = Product<kHalf, Lie::kRows, Lie::kRows, kLogitRows, 128, 2, 2, 64, 2>;
 template <bool kHalf>
 using HiddenProduct = Product<kHalf, Lie::kColumns, Lie::kColumns, 256, 128, 2, 2, 32, 3>;
 template <bool kHalf>
 using WeightProduct = Product<kHalf, Lie::kColumns, Lie::kRows, 256, 128, 2, 2, 32, 3>;
-
-#define LCT_PRODUCT_STAGES(P)                                                             \
-    __shared__ __attribute__((aligned(1024))) uint16_t stage0[P::kStage];                 \
-    __shared__ __attribute__((aligned(1024))) uint16_t stage1[P::kStage];                 \
-    __shared__ __attribute__((aligned(1024))) uint16_t stage2[P::kStage];                 \
-    uint16_t *const stages[3] = {stage0, stage1, stage2}
 
 // The counted tokens, as prepare_kernel found them.
 struct Counted {
@@ -165,7 +160,7 @@ __device__ __forceinline__ Part joined(Part a, Part b) {
     return {most, a.total * exp2_fast(a.most - base) + b.total * exp2_fast(b.most - base)};
 }
 
-// z / sqrt(1 + (z / s)^2) and, if wanted, (1 + (z / s)^2)^(-1/2).
+// l = z root(z), root(z) = (1 + (z / s)^2)^(-1/2).
 struct Cap {
     float cap, inverse;
     __device__ __forceinline__ float root(float z) const {
@@ -179,13 +174,26 @@ struct Cap {
     }
 };
 
-// 256 of the vocabulary (rows, in a lane's registers) by 128 tokens (columns, a lane
+// Whether some |z| of the wave's is larger than root() takes: then all go through within().
+template <class P>
+__device__ __forceinline__ bool far_of(const P &p, const Cap &cap) {
+    float largest = 0.0f;
+#pragma unroll
+    for (int m = 0; m < P::kRowTiles; ++m)
+#pragma unroll
+        for (int n = 0; n < P::kColumnTiles; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) largest = fmaxf(largest, fabsf(p.sum[m][n][r]));
+    return __any(largest > kCapped * cap.cap);
+}
+
+// P::kM of the vocabulary (rows, in a lane's registers) by P::kN tokens (columns, a lane
 // each): a token's maximum and sum need one exchange between two lanes.
-template <bool kHalf, bool kCap, bool kBias>
-__global__ __launch_bounds__(256, 2) void logits_kernel(lct_cross_entropy c, Counted t,
-                                                        int32_t vocab_tiles, int32_t token_tiles,
-                                                        Part *__restrict__ parts) {
-    using P = LogitProduct<kHalf>;
+template <class P, bool kHalf, bool kCap, bool kBias>
+__global__ __launch_bounds__(P::kThreads, 2) void logits_kernel(lct_cross_entropy c, Counted t,
+                                                                int32_t vocab_tiles,
+                                                                int32_t token_tiles,
+                                                                Part *__restrict__ parts) {
     LCT_PRODUCT_STAGES(P);
     const int32_t count = t.count == nullptr ? c.tokens : *t.count;
     const int64_t item = xcd_item(int64_t{vocab_tiles} * token_tiles, blockIdx.x);
@@ -197,61 +205,47 @@ __global__ __launch_bounds__(256, 2) void logits_kernel(lct_cross_entropy c, Cou
     const int32_t vocab_tile = 8 * group + in_group % width, token_tile = in_group / width;
     if (int64_t{token_tile} * P::kN >= count) return;
 
-    int64_t x_stride;
-    const void *x = t.count == nullptr ? c.x : hidden_of(c, t, count, &x_stride);
-    if (t.count == nullptr) x_stride = c.x_stride;
+    int64_t x_stride = c.x_stride;
+    const void *x = c.x;
+    if (t.count != nullptr) x = hidden_of(c, t, count, &x_stride);
     typename P::A a;
     typename P::B b;
     a.prepare(c.weight, c.weight_stride, int64_t{vocab_tile} * P::kM, c.vocab);
     b.prepare(x, x_stride, int64_t{token_tile} * P::kN, count);
-    P p;
-    p.run(a, b, c.dim, stages);
-
     const int half = wave_lane() >> 5;
-    const int32_t first = vocab_tile * P::kM + p.first_row();
-    const Cap cap{c.softcap, 1.0f / c.softcap};
-    int32_t token[P::kColumnTiles], target[P::kColumnTiles];
-#pragma unroll
-    for (int n = 0; n < P::kColumnTiles; ++n) {
-        token[n] = token_tile * P::kN + p.first_column() + 32 * n + (wave_lane() & 31);
-        target[n] = -1;
-        if (token[n] < count)
-            target[n] = t.count != nullptr ? t.targets[token[n]]
-                                           : static_cast<int32_t>(std::min<int64_t>(
-                                                 std::max<int64_t>(target_of(c, token[n]), -1),
-                                                 c.vocab));
-        target[n] -= first;
-    }
+    const int32_t first = vocab_tile * P::kM + P::first_row();
+    P p;
     if constexpr (kBias) {
+        const __amdgpu_buffer_rsrc_t bias = make_rsrc(c.bias, static_cast<uint32_t>(c.vocab) * 4u);
+        p.begin([&](int m, int) {
+            f32x16 v;
 #pragma unroll
-        for (int m = 0; m < P::kRowTiles; ++m)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int32_t row = first + 32 * m + 8 * (r / 4) + 4 * half + r % 4;
-                const float bias = row < c.vocab ? c.bias[row] : 0.0f;
-#pragma unroll
-                for (int n = 0; n < P::kColumnTiles; ++n) p.sum[m][n][r] += bias;
-            }
+            for (int r = 0; r < 16; ++r)
+                v[r] = __builtin_bit_cast(
+                    float, __builtin_amdgcn_raw_buffer_load_b32(
+                               bias, (first + 32 * m + 8 * (r / 4) + 4 * half + r % 4) * 4, 0, 0));
+            return v;
+        });
+    } else {
+        p.begin();
     }
+    p.run(a, b, c.dim, stage0, stage1, stage2, stage3);
     if constexpr (kCap) {
-        float largest = 0.0f;
+        const Cap cap{c.softcap, 1.0f / c.softcap};
+        if (far_of(p, cap)) {
+#pragma unroll
+            for (int m = 0; m < P::kRowTiles; ++m)
+#pragma unroll
+                for (int n = 0; n < P::kColumnTiles; ++n)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) p.sum[m][n][r] = cap.within(p.sum[m][n][r]);
+        }
 #pragma unroll
         for (int m = 0; m < P::kRowTiles; ++m)
 #pragma unroll
             for (int n = 0; n < P::kColumnTiles; ++n)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) largest = fmaxf(largest, fabsf(p.sum[m][n][r]));
-        const bool far = __any(largest > kCapped * c.softcap);
-#pragma unroll
-        for (int m = 0; m < P::kRowTiles; ++m)
-#pragma unroll
-            for (int n = 0; n < P::kColumnTiles; ++n)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    float z = p.sum[m][n][r];
-                    if (far) z = cap.within(z);
-                    p.sum[m][n][r] = z * cap.root(z);
-                }
+                for (int r = 0; r < 16; ++r) p.sum[m][n][r] *= cap.root(p.sum[m][n][r]);
     }
     if (first + P::kWaveM > c.vocab) {
 #pragma unroll
@@ -266,12 +260,20 @@ __global__ __launch_bounds__(256, 2) void logits_kernel(lct_cross_entropy c, Cou
     const int32_t entries = 2 * vocab_tiles;
 #pragma unroll
     for (int n = 0; n < P::kColumnTiles; ++n) {
-        if (__any(target[n] >= 0 && target[n] < P::kWaveM)) {
+        const int32_t token = token_tile * P::kN + p.first_column() + 32 * n + (wave_lane() & 31);
+        int32_t target = -1;
+        if (token < count) {
+            if (t.count != nullptr) target = t.targets[token];
+            else target = static_cast<int32_t>(std::min<int64_t>(
+                     std::max<int64_t>(target_of(c, token), -1), c.vocab));
+        }
+        target -= first;
+        if (__any(target >= 0 && target < P::kWaveM)) {
 #pragma unroll
             for (int m = 0; m < P::kRowTiles; ++m)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    if (32 * m + 8 * (r / 4) + 4 * half + r % 4 == target[n])
+                    if (32 * m + 8 * (r / 4) + 4 * half + r % 4 == target)
                         p.sum[m][n][r] = -INFINITY;
         }
         float most = p.sum[0][n][0];
@@ -288,8 +290,8 @@ __global__ __launch_bounds__(256, 2) void logits_kernel(lct_cross_entropy c, Cou
             for (int r = 0; r < 16; ++r)
                 total += exp2_fast(__builtin_fmaf(p.sum[m][n][r], kLog2e, -base));
         total = across_sum(total);
-        if (half == 0 && token[n] < count)
-            parts[int64_t{token[n]} * entries + 2 * vocab_tile + p.wave() % 2] = Part{most, total};
+        if (half == 0 && token < count)
+            parts[int64_t{token} * entries + 2 * vocab_tile + p.wave() % 2] = Part{most, total};
     }
 }
 
@@ -392,56 +394,14 @@ __global__ __launch_bounds__(kPrepareThreads) void total_kernel(lct_cross_entrop
 
 // ---- backward
 
-// Writes a wave's tile (rows m, columns n; round(m, n, r, pair) gives two adjacent rows'
-// values) with a column's 128 rows next to each other: 8 bytes a lane into the wave's
-// 8 KB of LDS, 16 bytes a lane out of it, so that the stores are of 256 bytes.
-// `rows`: how many there are from the wave's first on, a multiple of 8.
-template <class P, class Pair>
-__device__ __forceinline__ void store_columns(uint16_t *out, int64_t stride, int32_t columns,
-                                              int32_t rows, uint16_t *mine, Pair pair) {
-    static_assert(P::kWaveM == 128);
-    const int lane = wave_lane(), column = lane & 31, half = lane >> 5;
-#pragma unroll
-    for (int n = 0; n < P::kColumnTiles; ++n) {
-#pragma unroll
-        for (int m = 0; m < P::kRowTiles; ++m)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int chunk = (4 * m + g) ^ (column & 15);
-                *reinterpret_cast<u32x2 *>(mine + column * 128 + chunk * 8
-                                           + (half ^ (column >> 3 & 1)) * 4) =
-                    u32x2{pair(m, n, 4 * g), pair(m, n, 4 * g + 2)};
-            }
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int at = 4 * i + (lane >> 4), chunk = lane & 15;
-            u32x4 v = *reinterpret_cast<const u32x4 *>(mine + at * 128 + (chunk ^ (at & 15)) * 8);
-            if (at >> 3 & 1) v = u32x4{v[2], v[3], v[0], v[1]};
-            if (32 * n + at < columns && chunk * 8 < rows)
-                *reinterpret_cast<u32x4 *>(out + (32 * n + at) * stride + chunk * 8) = v;
-        }
-        __builtin_amdgcn_wave_barrier();
-    }
-}
-
-__device__ __forceinline__ uint16_t *wave_store(uint16_t *const (&stages)[3]) {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    return (wave < 2 ? stages[0] : stages[1]) + (wave & 1) * 4096;
-}
-
-// dz of 256 tokens (rows) by 128 of a piece of the vocabulary (columns, a lane each), the
+// dz of P::kM tokens (rows) by P::kN of a piece of the vocabulary (columns, a lane each), the
 // logits computed again: written by columns, [vocabulary][token], which both products
 // that follow read, and its sums over these tokens.
-template <bool kHalf, bool kCap, bool kBias>
-__global__ __launch_bounds__(256, 2) void gradient_kernel(lct_cross_entropy c, Counted t,
-                                                          int32_t first_vocab, int32_t piece,
-                                                          int32_t vocab_tiles,
-                                                          int32_t token_tiles, uint16_t *dz,
-                                                          int64_t dz_stride, float *bias_parts) {
-    using P = LogitProduct<kHalf>;
+template <class P, bool kHalf, bool kCap, bool kBias>
+__global__ __launch_bounds__(P::kThreads, 2) void gradient_kernel(
+    lct_cross_entropy c, Counted t, int32_t first_vocab, int32_t piece, int32_t vocab_tiles,
+    int32_t token_tiles, uint16_t *dz, int64_t dz_stride, float *bias_parts) {
     LCT_PRODUCT_STAGES(P);
-    __shared__ float4 row_values[P::kM];
     const int32_t count = *t.count;
     const int64_t item = xcd_item(int64_t{vocab_tiles} * token_tiles, blockIdx.x);
     if (item >= int64_t{vocab_tiles} * token_tiles) return;
@@ -458,54 +418,91 @@ __global__ __launch_bounds__(256, 2) void gradient_kernel(lct_cross_entropy c, C
     typename P::B b;
     a.prepare(x, x_stride, int64_t{token_tile} * P::kM, count);
     b.prepare(c.weight, c.weight_stride, first_vocab + int64_t{vocab_tile} * P::kN, last_vocab);
-    // Each token's lse, factor, target and its dz there; tokens past the last have
-    // factor 0.
+    // Of each token, with its factor f: lse - log2 |f|, so that the exponential from there is
+    // |f| times the probability, f's sign, the target and dz there.  Tokens past the last:
+    // zeros.
+    static_assert(P::kM <= P::kThreads);
+    float4 own{INFINITY, 1.0f, __int_as_float(-1), 0.0f};
     {
         const int32_t i = token_tile * P::kM + threadIdx.x;
-        float4 v{INFINITY, 0.0f, __int_as_float(-1), 0.0f};
-        if (i < count)
-            v = float4{t.lse[i], t.factor[i], __int_as_float(t.targets[i]), expm1f(-t.losses[i])};
-        row_values[threadIdx.x] = v;
+        if (threadIdx.x < P::kM && i < count) {
+            const float f = t.factor[i];
+            own = float4{t.lse[i] - log2f(fabsf(f)), copysignf(1.0f, f),
+                         __int_as_float(t.targets[i]), t.losses[i]};
+            own.w = f * expm1f(-own.w);
+        }
     }
-    P p;
-    p.run(a, b, c.dim, stages);
-
     const int lane = wave_lane(), half = lane >> 5;
-    const int32_t first = first_vocab + vocab_tile * P::kN + p.first_column();
-    const Cap cap{c.softcap, 1.0f / c.softcap};
-    float bias[P::kColumnTiles], column_sum[P::kColumnTiles];
+    const int32_t first = first_vocab + vocab_tile * P::kN + P::first_column();
+    P p;
+    if constexpr (kBias) {
+        float bias[P::kColumnTiles];
 #pragma unroll
-    for (int n = 0; n < P::kColumnTiles; ++n) {
-        const int32_t column = first + 32 * n + (lane & 31);
-        bias[n] = kBias && column < last_vocab ? c.bias[column] : 0.0f;
-        column_sum[n] = 0.0f;
+        for (int n = 0; n < P::kColumnTiles; ++n) {
+            const int32_t column = first + 32 * n + (lane & 31);
+            bias[n] = column < last_vocab ? c.bias[column] : 0.0f;
+        }
+        p.begin([&](int, int n) { return f32x16{} + bias[n]; });
+    } else {
+        p.begin();
     }
+    p.run(a, b, c.dim, stage0, stage1, stage2, stage3);
+
+    auto *row_values = reinterpret_cast<float4 *>(stage0);
+    if (threadIdx.x < P::kM) row_values[threadIdx.x] = own;
+    __syncthreads();
+    const Cap cap{c.softcap, 1.0f / c.softcap};
+    if constexpr (kCap) {
+        if (far_of(p, cap)) {
+#pragma unroll
+            for (int m = 0; m < P::kRowTiles; ++m)
+#pragma unroll
+                for (int n = 0; n < P::kColumnTiles; ++n)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) p.sum[m][n][r] = cap.within(p.sum[m][n][r]);
+        }
+    }
+    float column_sum[P::kColumnTiles] = {};
 #pragma unroll
     for (int m = 0; m < P::kRowTiles; ++m) {
         const float4 *values = row_values + p.first_row() + 32 * m;
-        const int32_t target = __float_as_int(values[lane & 31].z) - first;
-        const bool hit = __any(target >= 0 && target < P::kWaveN);
+        const float4 mine = values[lane & 31];
+        const int32_t target = __float_as_int(mine.z) - first;
+        // Rare: a target, a negative factor, tokens past the last.
+        const bool some = __any((target >= 0 && target < P::kWaveN) || mine.y < 0.0f
+                                || token_tile * P::kM + p.first_row() + 32 * m + 31 >= count);
+        const auto each = [&](auto rare) __attribute__((always_inline)) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const float4 v = values[8 * (r / 4) + 4 * half + r % 4];
-            const int32_t at = __float_as_int(v.z) - first - (lane & 31);
+            for (int r = 0; r < 16; ++r) {
+                const int row = 8 * (r / 4) + 4 * half + r % 4;
+                const float4 v = values[row];
+                const int32_t at = __float_as_int(v.z) - first - (lane & 31);
+                const bool none = token_tile * P::kM + p.first_row() + 32 * m + row >= count;
 #pragma unroll
-            for (int n = 0; n < P::kColumnTiles; ++n) {
-                float z = p.sum[m][n][r] + bias[n], slope = 1.0f;
-                if constexpr (kCap) {
-                    z = cap.within(z);
-                    const float root = cap.root(z);
-                    z *= root;
-                    slope = root * root * root;
+                for (int n = 0; n < P::kColumnTiles; ++n) {
+                    float z = p.sum[m][n][r], slope = 1.0f;
+                    if constexpr (kCap) {
+                        const float root = cap.root(z);
+                        z *= root;
+                        slope = root * root * root;
+                    }
+                    float d = exp2_fast(__builtin_fmaf(z, kLog2e, -v.x));
+                    if constexpr (decltype(rare)::value) {
+                        d = at == 32 * n ? v.w : d * v.y;
+                        d = none ? 0.0f : d;
+                    }
+                    p.sum[m][n][r] = kCap ? d * slope : d;
                 }
-                float d = exp2_fast(__builtin_fmaf(z, kLog2e, -v.x));
-                if (hit) d = at == 32 * n ? v.w : d;
-                d = v.y == 0.0f ? 0.0f : d * v.y * slope;
-                p.sum[m][n][r] = d;
-                column_sum[n] += d;
             }
-        }
+        };
+        if (some) each(std::true_type{});
+        else each(std::false_type{});
+#pragma unroll
+        for (int n = 0; n < P::kColumnTiles; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) column_sum[n] += p.sum[m][n][r];
     }
+    __syncthreads();     // the LDS of row_values is written again
     if (first + P::kWaveN > last_vocab) {
 #pragma unroll
         for (int n = 0; n < P::kColumnTiles; ++n)
@@ -529,46 +526,51 @@ __global__ __launch_bounds__(256, 2) void gradient_kernel(lct_cross_entropy c, C
     const int32_t column = vocab_tile * P::kN + p.first_column();
     const int32_t row = token_tile * P::kM + p.first_row();
     store_columns<P>(dz + column * dz_stride + row, dz_stride, piece - column,
-                     static_cast<int32_t>(dz_stride) - row, wave_store(stages),
+                     static_cast<int32_t>(dz_stride) - row, turn_values<P>(stage0, stage1),
                      [&](int m, int n, int r) {
                          return Element<kHalf>::round_pair(p.sum[m][n][r], p.sum[m][n][r + 1]);
                      });
 }
 
-// dx of a piece of the vocabulary, or of one of its `splits` parts: 256 channels (rows)
-// by 128 tokens (columns), added to the earlier pieces' in FP32.
-template <bool kHalf>
-__global__ __launch_bounds__(256, 2) void hidden_gradient_kernel(
-    lct_cross_entropy c, Counted t, int32_t first_vocab, int32_t piece, int32_t splits,
-    int32_t dim_tiles, int32_t token_tiles, const uint16_t *dz, int64_t dz_stride, float *parts) {
-    using P = HiddenProduct<kHalf>;
-    LCT_PRODUCT_STAGES(P);
-    const int32_t count = *t.count;
-    const int64_t items = int64_t{dim_tiles} * token_tiles * splits;
-    const int64_t item = xcd_item(items, blockIdx.x);
-    if (item >= items) return;
-    const int32_t dim_tile = static_cast<int32_t>(item % dim_tiles);
-    const int32_t token_tile = static_cast<int32_t>(item / dim_tiles % token_tiles);
-    const int32_t split = static_cast<int32_t>(item / dim_tiles / token_tiles);
-    if (int64_t{token_tile} * P::kN >= count) return;
-    const int32_t per = ((piece + splits - 1) / splits + 31) / 32 * 32;
-    const int32_t begin = min(piece, split * per), end = min(piece, begin + per);
+// What both products of a piece with dz need.
+struct PieceProducts {
+    int32_t first_vocab, piece, splits, dim_tiles, token_tiles, vocab_tiles;
+    const uint16_t *dz;
+    int64_t dz_stride;
+    float *hidden_parts;
+    uint16_t *grad_weight;
+};
 
+// dx of a piece of the vocabulary, or of one of its parts: 256 channels (rows) by 128
+// tokens (columns), added to the earlier pieces' in FP32.
+template <bool kHalf>
+__device__ __forceinline__ void hidden_gradient(const lct_cross_entropy &c, int32_t count,
+                                                const PieceProducts &q, int64_t item,
+                                                uint16_t *stage0, uint16_t *stage1,
+                                                uint16_t *stage2, uint16_t *stage3) {
+    using P = HiddenProduct<kHalf>;
+    const int32_t dim_tile = static_cast<int32_t>(item % q.dim_tiles);
+    const int32_t token_tile = static_cast<int32_t>(item / q.dim_tiles % q.token_tiles);
+    const int32_t split = static_cast<int32_t>(item / q.dim_tiles / q.token_tiles);
+    if (int64_t{token_tile} * P::kN >= count) return;
+    const int32_t per = ((q.piece + q.splits - 1) / q.splits + 31) / 32 * 32;
+    const int32_t begin = min(q.piece, split * per), end = min(q.piece, begin + per);
     typename P::A a;
     typename P::B b;
-    a.prepare(static_cast<const uint16_t *>(c.weight) + (first_vocab + begin) * c.weight_stride,
+    a.prepare(static_cast<const uint16_t *>(c.weight) + (q.first_vocab + begin) * c.weight_stride,
               c.weight_stride, int64_t{dim_tile} * P::kM, c.dim);
-    b.prepare(dz + begin * dz_stride, dz_stride, int64_t{token_tile} * P::kN,
+    b.prepare(q.dz + begin * q.dz_stride, q.dz_stride, int64_t{token_tile} * P::kN,
               (int64_t{count} + 7) / 8 * 8);
     P p;
-    p.run(a, b, end - begin, stages);
+    p.begin();
+    p.run(a, b, end - begin, stage0, stage1, stage2, stage3);
 
     const int lane = wave_lane();
 #pragma unroll
     for (int n = 0; n < P::kColumnTiles; ++n) {
         const int32_t token = token_tile * P::kN + p.first_column() + 32 * n + (lane & 31);
         if (token >= count) continue;
-        float *out = parts + (int64_t{split} * c.tokens + token) * c.dim;
+        float *out = q.hidden_parts + (int64_t{split} * c.tokens + token) * c.dim;
 #pragma unroll
         for (int m = 0; m < P::kRowTiles; ++m)
 #pragma unroll
@@ -578,7 +580,7 @@ __global__ __launch_bounds__(256, 2) void hidden_gradient_kernel(
                 if (d >= c.dim) continue;
                 f32x4 v{p.sum[m][n][4 * g], p.sum[m][n][4 * g + 1], p.sum[m][n][4 * g + 2],
                         p.sum[m][n][4 * g + 3]};
-                if (first_vocab > 0) v += *reinterpret_cast<const f32x4 *>(out + d);
+                if (q.first_vocab > 0) v += *reinterpret_cast<const f32x4 *>(out + d);
                 *reinterpret_cast<f32x4 *>(out + d) = v;
             }
     }
@@ -586,34 +588,55 @@ __global__ __launch_bounds__(256, 2) void hidden_gradient_kernel(
 
 // dW of a piece: 256 channels (rows) by 128 of the vocabulary (columns).
 template <bool kHalf>
-__global__ __launch_bounds__(256, 2) void weight_gradient_kernel(
-    lct_cross_entropy c, Counted t, int32_t first_vocab, int32_t piece, int32_t dim_tiles,
-    int32_t vocab_tiles, const uint16_t *dz, int64_t dz_stride, uint16_t *grad_weight) {
+__device__ __forceinline__ void weight_gradient(const lct_cross_entropy &c, const Counted &t,
+                                                int32_t count, const PieceProducts &q,
+                                                int64_t item, uint16_t *stage0, uint16_t *stage1,
+                                                uint16_t *stage2, uint16_t *stage3) {
     using P = WeightProduct<kHalf>;
-    LCT_PRODUCT_STAGES(P);
-    const int32_t count = *t.count;
-    const int64_t item = xcd_item(int64_t{dim_tiles} * vocab_tiles, blockIdx.x);
-    if (item >= int64_t{dim_tiles} * vocab_tiles) return;
-    const int32_t dim_tile = static_cast<int32_t>(item % dim_tiles);
-    const int32_t vocab_tile = static_cast<int32_t>(item / dim_tiles);
+    const int32_t dim_tile = static_cast<int32_t>(item % q.dim_tiles);
+    const int32_t vocab_tile = static_cast<int32_t>(item / q.dim_tiles);
     int64_t x_stride;
     const void *x = hidden_of(c, t, count, &x_stride);
     typename P::A a;
     typename P::B b;
     a.prepare(x, x_stride, int64_t{dim_tile} * P::kM, c.dim);
-    b.prepare(dz, dz_stride, int64_t{vocab_tile} * P::kN, piece);
+    b.prepare(q.dz, q.dz_stride, int64_t{vocab_tile} * P::kN, q.piece);
     P p;
+    p.begin();
     // Tokens past the last: zeros of dz (up to 7) against zeros of x.
-    p.run(a, b, count, stages);
+    p.run(a, b, count, stage0, stage1, stage2, stage3);
 
     const float scale = *t.scale;
     const int32_t column = vocab_tile * P::kN + p.first_column();
     const int32_t row = dim_tile * P::kM + p.first_row();
-    store_columns<P>(grad_weight + (int64_t{first_vocab} + column) * c.dim + row, c.dim,
-                     piece - column, c.dim - row, wave_store(stages), [&](int m, int n, int r) {
+    store_columns<P>(q.grad_weight + (int64_t{q.first_vocab} + column) * c.dim + row, c.dim,
+                     q.piece - column, c.dim - row, turn_values<P>(stage0, stage1),
+                     [&](int m, int n, int r) {
                          return Element<kHalf>::round_pair(p.sum[m][n][r] * scale,
                                                            p.sum[m][n][r + 1] * scale);
                      });
+}
+
+// Both, one launch: neither has as many tiles as fill the compute units evenly.
+template <bool kHalf>
+__global__ __launch_bounds__(256, 2) void products_kernel(lct_cross_entropy c, Counted t,
+                                                          PieceProducts q, uint32_t weight_grid) {
+    using P = HiddenProduct<kHalf>;
+    static_assert(P::kStage == WeightProduct<kHalf>::kStage
+                  && P::kStages == WeightProduct<kHalf>::kStages);
+    LCT_PRODUCT_STAGES(P);
+    const int32_t count = *t.count;
+    if (blockIdx.x < weight_grid) {
+        const int64_t items = int64_t{q.dim_tiles} * q.vocab_tiles;
+        const int64_t item = xcd_item(items, blockIdx.x);
+        if (item < items)
+            weight_gradient<kHalf>(c, t, count, q, item, stage0, stage1, stage2, stage3);
+    } else {
+        const int64_t items = int64_t{q.dim_tiles} * q.token_tiles * q.splits;
+        const int64_t item = xcd_item(items, blockIdx.x - weight_grid);
+        if (item < items)
+            hidden_gradient<kHalf>(c, count, q, item, stage0, stage1, stage2, stage3);
+    }
 }
 
 // dx from its parts, 8 values a thread; zeros for tokens that do not count.
@@ -652,13 +675,13 @@ __global__ __launch_bounds__(256) void join_hidden_kernel(lct_cross_entropy c, C
 }
 
 __global__ __launch_bounds__(256) void join_bias_kernel(lct_cross_entropy c, Counted t,
+                                                        int32_t rows,
                                                         const float *__restrict__ parts,
                                                         float *__restrict__ grad_bias) {
     const int32_t v = blockIdx.x * 256 + threadIdx.x;
     if (v >= c.vocab) return;
-    const int32_t tiles = (*t.count + 255) / 256;
     float sum = 0.0f;
-    for (int32_t i = 0; i < 2 * tiles; ++i) sum += parts[int64_t{i} * c.vocab + v];
+    for (int32_t i = 0; i < 2 * ((*t.count + rows - 1) / rows); ++i) sum += parts[int64_t{i} * c.vocab + v];
     grad_bias[v] = sum * *t.scale;
 }
 
@@ -714,8 +737,10 @@ extern "C" int32_t lct_cross_entropy_forward(const lct_cross_entropy *c, int32_t
                                              float *total, int32_t mean, hipStream_t stream) {
     if (const int32_t bad = check(c)) return bad;
     if (parts == nullptr || lse == nullptr || losses == nullptr) return LCT_E_NULL;
-    const int32_t vocab_tiles = tiles_of(c->vocab, 256), token_tiles = tiles_of(c->tokens, 128);
-    if (part_floats < int64_t{4} * vocab_tiles * c->tokens || !aligned(parts, 8)) return LCT_E_SIZE;
+    const int32_t vocab_tiles = tiles_of(c->vocab, kLogitRows);
+    const int32_t token_tiles = tiles_of(c->tokens, 128);
+    if (part_floats < int64_t{4} * tiles_of(c->vocab, 128) * c->tokens || !aligned(parts, 8))
+        return LCT_E_SIZE;
     Counted t{};
     if (index != nullptr) {
         if (gathered == nullptr) return LCT_E_NULL;
@@ -735,7 +760,8 @@ extern "C" int32_t lct_cross_entropy_forward(const lct_cross_entropy *c, int32_t
     }
     const uint32_t grid = static_cast<uint32_t>(xcd_grid(int64_t{vocab_tiles} * token_tiles));
     by_form(*c, [&](auto half, auto cap, auto bias) {
-        logits_kernel<decltype(half)::value, decltype(cap)::value, decltype(bias)::value>
+        logits_kernel<LogitProduct<decltype(half)::value>, decltype(half)::value,
+                      decltype(cap)::value, decltype(bias)::value>
             <<<grid, 256, 0, stream>>>(*c, t, vocab_tiles, token_tiles,
                                        reinterpret_cast<Part *>(parts));
     });
@@ -765,13 +791,13 @@ extern "C" int32_t lct_cross_entropy_backward(const lct_cross_entropy *c,
         || (d->grad_bias != nullptr && (d->bias_parts == nullptr || c->bias == nullptr)))
         return LCT_E_NULL;
     const int64_t tokens = c->tokens, pitch = (tokens + 7) / 8 * 8;
-    const int32_t token_tiles = tiles_of(tokens, 256);
+    const int32_t token_tiles = tiles_of(tokens, kLogitRows);
     if (d->piece < 1 || d->piece % 128 || d->splits < 1 || d->splits > LCT_MAX_CROSS_ENTROPY_SPLITS
         || d->index_size < 1 + 2 * tokens || d->value_floats < 1 + 3 * tokens
         || d->gathered_size < tokens * c->dim
         || (products && d->dz_size < std::min(d->piece, c->vocab) * pitch)
         || (d->grad_x != nullptr && d->hidden_floats < d->splits * tokens * c->dim)
-        || (d->grad_bias != nullptr && d->bias_floats < int64_t{2} * token_tiles * c->vocab))
+        || (d->grad_bias != nullptr && d->bias_floats < int64_t{2} * tiles_of(tokens, 128) * c->vocab))
         return LCT_E_SIZE;
     if (!aligned(d->gathered, 16) || !aligned(d->dz, 16) || !aligned(d->hidden_parts, 16)
         || !aligned(d->grad_x, 16) || !aligned(d->grad_weight, 16))
@@ -800,33 +826,30 @@ extern "C" int32_t lct_cross_entropy_backward(const lct_cross_entropy *c,
         const int32_t vocab_tiles = tiles_of(piece, 128);
         const uint32_t grid = static_cast<uint32_t>(xcd_grid(int64_t{vocab_tiles} * token_tiles));
         by_form(*c, [&](auto half, auto cap, auto bias) {
-            gradient_kernel<decltype(half)::value, decltype(cap)::value, decltype(bias)::value>
+            gradient_kernel<LogitProduct<decltype(half)::value>, decltype(half)::value,
+                            decltype(cap)::value, decltype(bias)::value>
                 <<<grid, 256, 0, stream>>>(*c, t, first, piece, vocab_tiles, token_tiles,
                                            products ? dz : nullptr, pitch,
                                            d->grad_bias != nullptr ? d->bias_parts : nullptr);
         });
-        if (d->grad_x != nullptr) {
-            const uint32_t items = static_cast<uint32_t>(
-                xcd_grid(int64_t{dim_tiles} * hidden_tiles * d->splits));
-            if (c->fp16)
-                hidden_gradient_kernel<true><<<items, 256, 0, stream>>>(
-                    *c, t, first, piece, d->splits, dim_tiles, hidden_tiles, dz, pitch,
-                    d->hidden_parts);
-            else
-                hidden_gradient_kernel<false><<<items, 256, 0, stream>>>(
-                    *c, t, first, piece, d->splits, dim_tiles, hidden_tiles, dz, pitch,
-                    d->hidden_parts);
-        }
-        if (d->grad_weight != nullptr) {
-            const uint32_t items = static_cast<uint32_t>(xcd_grid(int64_t{dim_tiles} * vocab_tiles));
-            auto *out = static_cast<uint16_t *>(d->grad_weight);
-            if (c->fp16)
-                weight_gradient_kernel<true><<<items, 256, 0, stream>>>(
-                    *c, t, first, piece, dim_tiles, vocab_tiles, dz, pitch, out);
-            else
-                weight_gradient_kernel<false><<<items, 256, 0, stream>>>(
-                    *c, t, first, piece, dim_tiles, vocab_tiles, dz, pitch, out);
-        }
+        const PieceProducts q{first,    piece,       d->splits, dim_tiles,
+                              hidden_tiles, vocab_tiles, dz,        pitch,
+                              d->hidden_parts, static_cast<uint16_t *>(d->grad_weight)};
+        const uint32_t weight_grid =
+            d->grad_weight == nullptr
+                ? 0
+                : static_cast<uint32_t>(xcd_grid(int64_t{dim_tiles} * vocab_tiles));
+        const uint32_t hidden_grid =
+            d->grad_x == nullptr
+                ? 0
+                : static_cast<uint32_t>(xcd_grid(int64_t{dim_tiles} * hidden_tiles * d->splits));
+        if (weight_grid + hidden_grid == 0) continue;
+        if (c->fp16)
+            products_kernel<true>
+                <<<weight_grid + hidden_grid, 256, 0, stream>>>(*c, t, q, weight_grid);
+        else
+            products_kernel<false>
+                <<<weight_grid + hidden_grid, 256, 0, stream>>>(*c, t, q, weight_grid);
     }
     if (d->grad_x != nullptr) {
         auto *out = static_cast<uint16_t *>(d->grad_x);
@@ -838,7 +861,7 @@ extern "C" int32_t lct_cross_entropy_backward(const lct_cross_entropy *c,
                 <<<chunk_grid, 256, 0, stream>>>(*c, t, d->splits, d->hidden_parts, out);
     }
     if (d->grad_bias != nullptr)
-        join_bias_kernel<<<tiles_of(c->vocab, 256), 256, 0, stream>>>(*c, t, d->bias_parts,
-                                                                      d->grad_bias);
+        join_bias_kernel<<<tiles_of(c->vocab, 256), 256, 0, stream>>>(
+            *c, t, kLogitRows, d->bias_parts, d->grad_bias);
     return static_cast<int32_t>(hipGetLastError());
 }

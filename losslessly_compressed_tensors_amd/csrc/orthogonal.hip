@@ -109,12 +109,6 @@ __global__ __launch_bounds__(256) void start_kernel(lct_orthogonal o, int32_t pa
     }
 }
 
-#define LCT_PRODUCT_STAGES(P)                                                             \
-    __shared__ __attribute__((aligned(1024))) uint16_t stage0[P::kStage];                 \
-    __shared__ __attribute__((aligned(1024))) uint16_t stage1[P::kStage];                 \
-    __shared__ __attribute__((aligned(1024))) uint16_t stage2[P::kStage];                 \
-    uint16_t *const stages[3] = {stage0, stage1, stage2}
-
 // Tile `t` of those of a symmetric matrix that touch its lower triangle: 256 rows (block
 // i) by 128 columns (block j <= 2 i + 1), i's 2 i + 2 tiles in turn.
 __device__ __forceinline__ void lower_tile(int32_t t, int32_t *i, int32_t *j) {
@@ -150,7 +144,8 @@ __global__ __launch_bounds__(256, 2) void symmetric_kernel(const uint16_t *opera
     a.prepare(from, depth, int64_t{i} * P::kM, size);
     b.prepare(from, depth, int64_t{j} * P::kN, size);
     P p;
-    p.run(a, b, depth, stages);
+    p.begin();
+    p.run(a, b, depth, stage0, stage1, stage2, stage3);
 
     const int lane = wave_lane(), half = lane >> 5;
     // A block on the diagonal is computed whole, by its two tiles.
@@ -217,7 +212,8 @@ __global__ __launch_bounds__(256, 2) void update_kernel(const uint16_t *poly,
     a.prepare(operand + first, cols, int64_t{j} * P::kM, cols);
     b.prepare(poly + int64_t{matrix} * rows * rows, rows, int64_t{i} * P::kN, rows);
     P p;
-    p.run(a, b, rows, stages);
+    p.begin();
+    p.run(a, b, rows, stage0, stage1, stage2, stage3);
 
     const int lane = wave_lane(), half = lane >> 5;
 #pragma unroll

@@ -2,14 +2,11 @@
 // in registers (cross_entropy.hip, orthogonal.hip).
 //
 // The tile has kM "rows" and kN "columns": out(m, n) = sum over k of A(m, k) B(n, k),
-// with FP32 sums.  Four waves share it, two by two.  Operands are 16-bit matrices in
-// memory either by rows (a row's k adjacent) or by columns (a k's rows adjacent);
-// both go to LDS as they lie, 32 of k at a time, straight from memory and three
-// steps deep, so that the loads of two steps are on their way while one is
-// multiplied.  Operands by columns are turned by gfx950's transposed LDS reads.
-//
-// Two such workgroups fit a compute unit (72 KB of LDS, 128 sums per lane at 256 x
-// 128), so that one's epilogue runs under the other's products.
+// with FP32 sums.  Operands are 16-bit matrices in memory either by rows (a row's k
+// adjacent) or by columns (a k's rows adjacent); both go to LDS as they lie, kStep of k at a
+// time, straight from memory and kStages steps deep.  Operands by columns are turned by
+// gfx950's transposed LDS reads.  A wave reads the next 16 of k from LDS while it multiplies
+// these; the barrier of a step lies between the two, under products.
 //
 // A 32x32x16 instruction leaves lane l with column l & 31 and rows 8 g + 4 (l >> 5) + i
 // (register 4 g + i): four adjacent rows of a column lie in one lane.
@@ -24,10 +21,9 @@ enum class Lie { kRows, kColumns };
 // One operand's tile of kTile rows by 32 of k: how it comes to LDS and how an
 // instruction's 32 rows by 16 of k are read from there.
 //
-// By rows: 4 chunks of 16 bytes per row, permuted by the row's bits 1 and 2, so that 8
-// rows read at one chunk lie in different 16-byte columns of the 128 bytes of a clock.
-// By columns: a line of kTile values per k, permuted by swizzle() as the attention
-// kernels' tiles are.
+// LDS returns 256 bytes a clock: the chunks of 16 bytes that 16 rows are read at (by
+// rows), and the 64 bytes of each of 4 lines (by columns, a line of kTile values per k), are
+// permuted so that they lie in different ones of its 16 columns (counted: no conflicts).
 template <Lie kLie, int kTile, int kStep, int kThreads>
 struct Operand {
     static constexpr int kValues = kTile * kStep;
@@ -41,7 +37,10 @@ struct Operand {
     uint32_t offset[kCount];
 
     static __device__ __forceinline__ int permuted(int line, int chunk) {
-        return chunk ^ (kLie == Lie::kColumns ? swizzle(line) : kStep == 32 ? (line >> 1) & 3 : line & 7);
+        if constexpr (kLie == Lie::kRows)
+            return chunk ^ (kStep == 32 ? (line >> 2) & 3 : (line >> 1) & 7);
+        else    // lines of 1.5 times 256 bytes differ by 128 as they are
+            return chunk ^ (kTile == 192 ? (line & 2) << 1 : (line & 3) << 2);
     }
 
     __device__ __forceinline__ void prepare(const void *matrix, int64_t stride_, int64_t first,
@@ -86,23 +85,46 @@ struct Operand {
         }
     }
 
-    // Rows 32 n .. + 31, values 16 step .. + 15 of k.
-    static __device__ __forceinline__ u32x4 read(const uint16_t *tile, int n, int step) {
+    // Where this lane reads the fragments of 32 rows from `first_row` on by 16 of k, in a
+    // tile: places that differ by more than a constant.  (Held in registers that the
+    // compiler does not look into: left alone, it finds constant addresses in some, whose
+    // reads it then takes for ones of any stage and lets wait for all loads.)
+    static constexpr int kPlaces = kLie == Lie::kRows ? kStep / 16 : 4;   // kColumns: of 4 n
+    struct Places {
+        int at[kPlaces];
+    };
+    static __device__ __forceinline__ Places places(int first_row) {
         const int lane = wave_lane();
+        Places p;
         if constexpr (kLie == Lie::kRows) {
             const int row = lane & 31;
-            const int chunk = permuted(row, 2 * step + (lane >> 5));
-            return *reinterpret_cast<const u32x4 *>(tile + (32 * n + row) * kStep
-                                                    + chunk * 8);
+#pragma unroll
+            for (int s = 0; s < kPlaces; ++s)
+                p.at[s] = (first_row + row) * kStep + permuted(row, 2 * s + (lane >> 5)) * 8;
         } else {
             const int line = 8 * (lane >> 5) + ((lane & 15) >> 2);
-            const int chunk = 4 * n + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
-            const uint16_t *at = tile + (16 * step + line) * kTile + (lane & 1) * 4;
+            const int chunk = first_row / 8 + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
+#pragma unroll
+            for (int n = 0; n < kPlaces; ++n)
+                p.at[n] = line * kTile + permuted(line, chunk + 4 * n) * 8 + (lane & 1) * 4;
+        }
+#pragma unroll
+        for (int i = 0; i < kPlaces; ++i) asm("" : "+v"(p.at[i]));
+        return p;
+    }
+
+    // Fragment n, k 16 step .. + 15.
+    static __device__ __forceinline__ u32x4 read(const uint16_t *tile, const Places &p, int n,
+                                                 int step) {
+        if constexpr (kLie == Lie::kRows) {
+            return *reinterpret_cast<const u32x4 *>(tile + p.at[step] + 32 * n * kStep);
+        } else {
+            // (The permutation moves chunks within 16 of them.)
+            const uint16_t *at = tile + p.at[n & 3] + (n & ~3) * 32 + 16 * step * kTile;
             const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) i16x4 *)(at + permuted(line, chunk) * 8));
+                (__attribute__((address_space(3))) i16x4 *)(at));
             const i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) i16x4 *)(at + 4 * kTile
-                                                            + permuted(line + 4, chunk) * 8));
+                (__attribute__((address_space(3))) i16x4 *)(at + 4 * kTile));
             const u32x2 lo = __builtin_bit_cast(u32x2, a), hi = __builtin_bit_cast(u32x2, b);
             return u32x4{lo[0], lo[1], hi[0], hi[1]};
         }
@@ -122,9 +144,10 @@ __device__ __forceinline__ void loads_barrier() {
 }
 
 template <bool kHalf, Lie kLieA, Lie kLieB, int kM_, int kN_, int kWavesM, int kWavesN, int kStep,
-          int kStages>
+          int kStages_>
 struct Product {
-    static constexpr int kM = kM_, kN = kN_, kThreads = 64 * kWavesM * kWavesN;
+    static constexpr int kM = kM_, kN = kN_, kThreads = kWave * kWavesM * kWavesN;
+    static constexpr int kStages = kStages_;
     using A = Operand<kLieA, kM, kStep, kThreads>;
     using B = Operand<kLieB, kN, kStep, kThreads>;
     static constexpr int kWaveM = kM / kWavesM, kWaveN = kN / kWavesN;
@@ -140,51 +163,132 @@ struct Product {
     static __device__ __forceinline__ int first_row() { return (wave() % kWavesM) * kWaveM; }
     static __device__ __forceinline__ int first_column() { return (wave() / kWavesM) * kWaveN; }
 
-    __device__ __forceinline__ void multiply(const uint16_t *stage) {
-        const uint16_t *a_tile = stage, *b_tile = stage + A::kValues;
-        const int row_tile = first_row() / 32, column_tile = first_column() / 32;
-#pragma unroll
-        for (int s = 0; s < kStep / 16; ++s) {
-            u32x4 b[kColumnTiles];
-#pragma unroll
-            for (int n = 0; n < kColumnTiles; ++n) b[n] = B::read(b_tile, column_tile + n, s);
-#pragma unroll
-            for (int m = 0; m < kRowTiles; ++m) {
-                const u32x4 a = A::read(a_tile, row_tile + m, s);
-#pragma unroll
-                for (int n = 0; n < kColumnTiles; ++n)
-                    sum[m][n] = Element<kHalf>::multiply(a, b[n], sum[m][n]);
-            }
-        }
-    }
+    struct Fragments {
+        u32x4 a[kRowTiles], b[kColumnTiles];
+    };
+    static constexpr int kFragmentReads = kRowTiles * A::kReads + kColumnTiles * B::kReads;
 
-    // All of `depth`; the stages are free afterwards.
-    __device__ __forceinline__ void run(const A &a, const B &b, int32_t depth,
-                                        uint16_t *const (&stages)[kStages]) {
-        constexpr int kLoads = A::kCount + B::kCount;
+    static __device__ __forceinline__ void read(Fragments &f, const uint16_t *stage,
+                                                const typename A::Places &a,
+                                                const typename B::Places &b, int s) {
+#pragma unroll
+        for (int n = 0; n < kColumnTiles; ++n) f.b[n] = B::read(stage + A::kValues, b, n, s);
+#pragma unroll
+        for (int m = 0; m < kRowTiles; ++m) f.a[m] = A::read(stage, a, m, s);
+    }
+    __device__ __forceinline__ void multiply(const Fragments &f) {
 #pragma unroll
         for (int m = 0; m < kRowTiles; ++m)
 #pragma unroll
-            for (int n = 0; n < kColumnTiles; ++n) sum[m][n] = f32x16{};
+            for (int n = 0; n < kColumnTiles; ++n)
+                sum[m][n] = Element<kHalf>::multiply(f.a[m], f.b[n], sum[m][n]);
+    }
+
+    // The sums' first values: start(m, n) gives 16 registers' of a 32 x 32 tile.
+    template <class Start>
+    __device__ __forceinline__ void begin(Start start) {
+#pragma unroll
+        for (int m = 0; m < kRowTiles; ++m)
+#pragma unroll
+            for (int n = 0; n < kColumnTiles; ++n) sum[m][n] = start(m, n);
+    }
+    __device__ __forceinline__ void begin() {
+        begin([](int, int) { return f32x16{}; });
+    }
+
+    // Adds all of `depth` to the sums; the stages are free afterwards.
+    __device__ __forceinline__ void run(const A &a, const B &b, int32_t depth,
+                                        uint16_t *s0, uint16_t *s1, uint16_t *s2, uint16_t *s3) {
+        uint16_t *const stages[4] = {s0, s1, s2, s3};
+        constexpr int kLoads = A::kCount + B::kCount, kParts = kStep / 16;
         const auto load = [&](int32_t k, uint16_t *stage) __attribute__((always_inline)) {
             a.issue(k, depth, stage);
             b.issue(k, depth, stage + A::kValues);
         };
 #pragma unroll
-        for (int s = 0; s + 1 < kStages; ++s) load(s * kStep, stages[s]);
+        for (int s = 0; s < kStages; ++s) load(s * kStep, stages[s]);
+        loads_barrier<kLoads * (kStages - 1)>();
+        // Two sets of fragments: one is read while the other is multiplied.
+        const typename A::Places at_a = A::places(first_row());
+        const typename B::Places at_b = B::places(first_column());
+        Fragments f[2];
+        read(f[0], stages[0], at_a, at_b, 0);
         for (int32_t k = 0; k < depth; k += kStages * kStep) {
 #pragma unroll
             for (int s = 0; s < kStages; ++s) {
-                // Behind the barrier all have the stage's loads, and have read the stage
-                // that is loaded next.
-                loads_barrier<kLoads * (kStages - 2)>();
-                load(k + (s + kStages - 1) * kStep, stages[(s + kStages - 1) % kStages]);
-                multiply(stages[s]);
+#pragma unroll
+                for (int part = 0; part < kParts; ++part) {
+                    const int now = (s * kParts + part) & 1;
+                    if (part + 1 < kParts) {
+                        read(f[now ^ 1], stages[s], at_a, at_b, part + 1);
+                    } else {
+                        // Behind the barrier all have the next stage's loads, and have read
+                        // this one, which is loaded for the step after the others.
+                        loads_barrier<kLoads * (kStages - 2)>();
+                        load(k + (s + kStages) * kStep, stages[s]);
+                        read(f[now ^ 1], stages[(s + 1) % kStages], at_a, at_b, 0);
+                    }
+                    multiply(f[now]);
+                    __builtin_amdgcn_sched_group_barrier(kLdsReadGroup, kFragmentReads, 0);
+                    __builtin_amdgcn_sched_group_barrier(kMatrixGroup, kRowTiles * kColumnTiles, 0);
+                }
             }
         }
         // Loads of steps past the end are still on their way.
         loads_barrier<0>();
     }
 };
+
+// The stages' LDS of product P, as run()'s last arguments.  (Arrays of their own: the compiler
+// then knows which loads a read has to wait for.)
+#define LCT_PRODUCT_STAGES(P)                                                                  \
+    __shared__ __attribute__((aligned(1024))) uint16_t stage0[P::kStage];                      \
+    __shared__ __attribute__((aligned(1024))) uint16_t stage1[P::kStage];                      \
+    __shared__ __attribute__((aligned(1024))) uint16_t stage2[P::kStages > 2 ? P::kStage : 8]; \
+    __shared__ __attribute__((aligned(1024))) uint16_t stage3[P::kStages > 3 ? P::kStage : 8]
+
+// A wave's tile (rows m, columns n; pair(m, n, r) gives two adjacent rows' values) to memory
+// with a column's rows next to each other: 8 bytes a lane into LDS of the wave's own
+// (kTurnValues<P>), 16 bytes a lane out of it, so that a column's rows are stored together.
+// `rows`: how many there are from the wave's first on, a multiple of 8.
+template <class P>
+constexpr int kTurnValues = 32 * (P::kWaveM + 8);
+
+template <class P, class Pair>
+__device__ __forceinline__ void store_columns(uint16_t *out, int64_t stride, int32_t columns,
+                                              int32_t rows, uint16_t *mine, Pair pair) {
+    constexpr int kPitch = P::kWaveM + 8, kChunks = P::kWaveM / 8;
+    const int lane = wave_lane();
+    uint16_t *at = mine + (lane & 31) * kPitch + (lane >> 5) * 4;
+#pragma unroll
+    for (int n = 0; n < P::kColumnTiles; ++n) {
+#pragma unroll
+        for (int m = 0; m < P::kRowTiles; ++m)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<u32x2 *>(at + 32 * m + 8 * g) =
+                    u32x2{pair(m, n, 4 * g), pair(m, n, 4 * g + 2)};
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < 32 * kChunks / kWave; ++i) {
+            const int slot = i * kWave + lane, column = slot / kChunks, chunk = slot % kChunks;
+            const u32x4 v = *reinterpret_cast<const u32x4 *>(mine + column * kPitch + chunk * 8);
+            if (32 * n + column < columns && chunk * 8 < rows)
+                *reinterpret_cast<u32x4 *>(out + (32 * n + column) * stride + chunk * 8) = v;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// That LDS: in the first two stages, which a finished run() leaves free.
+template <class P>
+__device__ __forceinline__ uint16_t *turn_values(uint16_t *stage0, uint16_t *stage1) {
+    constexpr int kWaves = P::kThreads / kWave;
+    static_assert(kWaves / 2 * kTurnValues<P> <= P::kStage);
+    const int wave = P::wave();
+    return (wave < kWaves / 2 ? stage0 : stage1) + wave % (kWaves / 2) * kTurnValues<P>;
+}
 
 }  // namespace lct

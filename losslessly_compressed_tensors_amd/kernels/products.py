@@ -10,6 +10,7 @@ allocated on the current stream, and the work is shared out.
 from __future__ import annotations
 
 from functools import lru_cache
+from heapq import heapreplace
 
 import torch
 from torch import Tensor
@@ -65,7 +66,7 @@ def cross_entropy_forward(x: Tensor, weight: Tensor, bias, targets: Tensor, soft
     losses = x.new_empty(tokens, dtype=torch.float32)
     lse = torch.empty_like(losses)
     total = None if reduction == "none" else x.new_empty((), dtype=torch.float32)
-    floats = 4 * tokens * -(-weight.shape[0] // 256)
+    floats = 4 * tokens * -(-weight.shape[0] // 128)
     parts = x.new_empty(floats, dtype=torch.float32)
     index = x.new_empty(1 + 2 * tokens, dtype=torch.int32)
     gathered = x.new_empty(tokens * dim)
@@ -77,15 +78,32 @@ def cross_entropy_forward(x: Tensor, weight: Tensor, bias, targets: Tensor, soft
     return losses, lse, total
 
 
+def _last_end(lengths) -> float:
+    """When the last of (how many, how long) workgroups ends that start in this order,
+    each as soon as one of the slots is free."""
+    free = [0.0] * _SLOTS
+    for count, length in lengths:
+        rounds, rest = divmod(count, _SLOTS)
+        if rounds:
+            # As many for each slot: they stay as far apart.
+            free = [t + rounds * length for t in free]
+        for _ in range(rest):
+            heapreplace(free, free[0] + length)
+    return max(free)
+
+
 @lru_cache(maxsize=1024)
 def vocabulary_pieces(tokens: int, vocab: int, dim: int) -> tuple:
-    """The size of a piece and the parts of its sum for the gradient of x."""
+    """The size of a piece and the parts of its sum for the gradient of x: those with
+    which the products of a piece end first, by their steps of 32 and what a workgroup's
+    start, epilogue and part cost in those."""
     pieces = -(-2 * vocab * tokens // _PIECE_BYTES)
     piece = -(-vocab // (256 * pieces)) * 256
-    tiles = -(-dim // 256) * -(-tokens // 128)
+    dims = -(-dim // 256)
+    hidden, weight = dims * -(-tokens // 128), dims * -(-piece // 128)
     best = None
     for splits in range(1, min(_MAX_SPLITS, max(1, piece // 512)) + 1):
-        time = -(-tiles * splits // _SLOTS) * (piece / 32 / splits + 8) + 2 * splits * tiles / 32
+        time = _last_end(((weight, tokens / 32 + 8), (hidden * splits, piece / 32 / splits + 16)))
         if best is None or time < best[0]:
             best = time, splits
     return piece, best[1]
@@ -112,7 +130,7 @@ def cross_entropy_backward(grad: Tensor, x: Tensor, weight: Tensor, bias, target
     dz = (x.new_empty(min(piece, vocab) * (-(-tokens // 8) * 8)) if need_x or need_weight
           else None)
     hidden = x.new_empty(splits * tokens * width, dtype=torch.float32) if need_x else None
-    columns = (x.new_empty(2 * -(-tokens // 256) * vocab, dtype=torch.float32) if need_bias
+    columns = (x.new_empty(2 * -(-tokens // 128) * vocab, dtype=torch.float32) if need_bias
                else None)
 
     def at(t):
