@@ -977,12 +977,12 @@ int32_t lct_cross_entropy_backward(const lct_cross_entropy *c,
  * X) after `steps` of X <- 2 X + (-3/2 A + 1/2 A A) X, A = X X^T, from X = G / (|G|_F +
  * eps), for `count` matrices G of rows <= cols <= LCT_MAX_ORTHOGONAL_DIM (a tall one is
  * passed transposed).  input: type LCT_BF16, LCT_FP16 or LCT_FP32; strides in elements of
- * matrix, row and column, out's likewise.  X is FP32, the products' operands FP16 at
- * powers of two, sums FP32, the norm FP64.  workspace (16-byte aligned): with both
- * dimensions rounded up to 8, count * (8 LCT_ORTHOGONAL_NORM_PARTS + 8 rows cols + 4
- * rows^2) bytes, the first term rounded up to 16. */
+ * matrix, row and column, out's likewise.  X is the sum of two FP16 numbers, the products'
+ * operands FP16 at powers of two, sums FP32, the norm FP64.  workspace (16-byte aligned):
+ * with both dimensions rounded up to 8, count * (8 LCT_ORTHOGONAL_NORM_PARTS + 6 rows cols
+ * + 4 rows^2) bytes. */
 #define LCT_MAX_ORTHOGONAL_DIM (1 << 16)
-#define LCT_ORTHOGONAL_NORM_PARTS 64
+#define LCT_ORTHOGONAL_NORM_PARTS 1024
 typedef struct {
     const void *input;
     void *out;

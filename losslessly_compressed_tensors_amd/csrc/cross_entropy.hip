@@ -526,7 +526,7 @@ __global__ __launch_bounds__(P::kThreads, 2) void gradient_kernel(
     const int32_t column = vocab_tile * P::kN + p.first_column();
     const int32_t row = token_tile * P::kM + p.first_row();
     store_columns<P>(dz + column * dz_stride + row, dz_stride, piece - column,
-                     static_cast<int32_t>(dz_stride) - row, turn_values<P>(stage0, stage1),
+                     static_cast<int32_t>(dz_stride) - row, turn_values<P>(stage0, stage1, stage2, stage3),
                      [&](int m, int n, int r) {
                          return Element<kHalf>::round_pair(p.sum[m][n][r], p.sum[m][n][r + 1]);
                      });
@@ -610,7 +610,7 @@ __device__ __forceinline__ void weight_gradient(const lct_cross_entropy &c, cons
     const int32_t column = vocab_tile * P::kN + p.first_column();
     const int32_t row = dim_tile * P::kM + p.first_row();
     store_columns<P>(q.grad_weight + (int64_t{q.first_vocab} + column) * c.dim + row, c.dim,
-                     q.piece - column, c.dim - row, turn_values<P>(stage0, stage1),
+                     q.piece - column, c.dim - row, turn_values<P>(stage0, stage1, stage2, stage3),
                      [&](int m, int n, int r) {
                          return Element<kHalf>::round_pair(p.sum[m][n][r] * scale,
                                                            p.sum[m][n][r + 1] * scale);

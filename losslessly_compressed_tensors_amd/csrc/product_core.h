@@ -247,6 +247,46 @@ struct Product {
     __shared__ __attribute__((aligned(1024))) uint16_t stage2[P::kStages > 2 ? P::kStage : 8]; \
     __shared__ __attribute__((aligned(1024))) uint16_t stage3[P::kStages > 3 ? P::kStage : 8]
 
+// What one wave wrote to LDS can be read by its other lanes.
+__device__ __forceinline__ void wave_fence() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// 16 bytes a lane of `lines` lines of `length` values (a multiple of 8): lane l's of access
+// i are those of slot 64 i + l, kChunks to a line.  What is past either end reads as
+// zeros and is not written.
+template <int kChunks>
+struct Lines {
+    __amdgpu_buffer_rsrc_t rsrc;
+    uint32_t pitch;      // bytes
+    int32_t length;
+
+    __device__ __forceinline__ Lines(const uint16_t *base, int64_t stride, int32_t lines,
+                                     int32_t length_)
+        : pitch(static_cast<uint32_t>(stride) * 2u), length(length_) {
+        rsrc = make_rsrc(base, lines > 0 && length > 0
+                                   ? static_cast<uint32_t>(lines - 1) * pitch
+                                         + static_cast<uint32_t>(length) * 2u
+                                   : 0u);
+    }
+    __device__ __forceinline__ uint32_t at(int first, int slot) const {
+        const int chunk = slot % kChunks;
+        return chunk * 8 < length ? static_cast<uint32_t>(first + slot / kChunks) * pitch
+                                        + static_cast<uint32_t>(chunk) * 16u
+                                  : kOutOfRange;
+    }
+    __device__ __forceinline__ u32x4 load(int first, int slot) const {
+        return __builtin_bit_cast(u32x4,
+                                  __builtin_amdgcn_raw_buffer_load_b128(rsrc, at(first, slot), 0, 0));
+    }
+    __device__ __forceinline__ void store(u32x4 v, int first, int slot) const {
+        store_b128<0>(__builtin_bit_cast(uint4, v), rsrc, at(first, slot));
+    }
+};
+
 // A wave's tile (rows m, columns n; pair(m, n, r) gives two adjacent rows' values) to memory
 // with a column's rows next to each other: 8 bytes a lane into LDS of the wave's own
 // (kTurnValues<P>), 16 bytes a lane out of it, so that a column's rows are stored together.
@@ -259,6 +299,7 @@ __device__ __forceinline__ void store_columns(uint16_t *out, int64_t stride, int
                                               int32_t rows, uint16_t *mine, Pair pair) {
     constexpr int kPitch = P::kWaveM + 8, kChunks = P::kWaveM / 8;
     const int lane = wave_lane();
+    const Lines<kChunks> lines(out, stride, columns, rows);
     uint16_t *at = mine + (lane & 31) * kPitch + (lane >> 5) * 4;
 #pragma unroll
     for (int n = 0; n < P::kColumnTiles; ++n) {
@@ -268,27 +309,95 @@ __device__ __forceinline__ void store_columns(uint16_t *out, int64_t stride, int
             for (int g = 0; g < 4; ++g)
                 *reinterpret_cast<u32x2 *>(at + 32 * m + 8 * g) =
                     u32x2{pair(m, n, 4 * g), pair(m, n, 4 * g + 2)};
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+        wave_fence();
 #pragma unroll
         for (int i = 0; i < 32 * kChunks / kWave; ++i) {
-            const int slot = i * kWave + lane, column = slot / kChunks, chunk = slot % kChunks;
-            const u32x4 v = *reinterpret_cast<const u32x4 *>(mine + column * kPitch + chunk * 8);
-            if (32 * n + column < columns && chunk * 8 < rows)
-                *reinterpret_cast<u32x4 *>(out + (32 * n + column) * stride + chunk * 8) = v;
+            const int slot = i * kWave + lane;
+            lines.store(*reinterpret_cast<const u32x4 *>(mine + slot / kChunks * kPitch
+                                                         + slot % kChunks * 8),
+                        32 * n, slot);
         }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+        wave_fence();
     }
 }
 
-// That LDS: in the first two stages, which a finished run() leaves free.
+// The other way: take(m, n, r, pair) gets each two adjacent rows' values, zeros where there
+// are none.
+template <class P, class Take>
+__device__ __forceinline__ void load_columns(const uint16_t *from, int64_t stride, int32_t columns,
+                                             int32_t rows, uint16_t *mine, Take take) {
+    constexpr int kPitch = P::kWaveM + 8, kChunks = P::kWaveM / 8;
+    constexpr int kCount = 32 * kChunks / kWave;
+    const int lane = wave_lane();
+    const Lines<kChunks> lines(from, stride, columns, rows);
+    const uint16_t *at = mine + (lane & 31) * kPitch + (lane >> 5) * 4;
+#pragma unroll
+    for (int n = 0; n < P::kColumnTiles; ++n) {
+        u32x4 v[kCount];
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) v[i] = lines.load(32 * n, i * kWave + lane);
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) {
+            const int slot = i * kWave + lane;
+            *reinterpret_cast<u32x4 *>(mine + slot / kChunks * kPitch + slot % kChunks * 8) = v[i];
+        }
+        wave_fence();
+#pragma unroll
+        for (int m = 0; m < P::kRowTiles; ++m)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const u32x2 pairs = *reinterpret_cast<const u32x2 *>(at + 32 * m + 8 * g);
+                take(m, n, 4 * g, pairs[0]);
+                take(m, n, 4 * g + 2, pairs[1]);
+            }
+        wave_fence();
+    }
+}
+
+// A wave's tile to memory with a row's columns next to each other, 32 rows at a time.
+// `columns`: how many there are from the wave's first on, a multiple of 8.
+template <class P, class Pair>
+__device__ __forceinline__ void store_rows(uint16_t *out, int64_t stride, int32_t rows,
+                                           int32_t columns, uint16_t *mine, Pair pair) {
+    constexpr int kPitch = P::kWaveN + 8, kChunks = P::kWaveN / 8;
+    static_assert(32 * kPitch <= kTurnValues<P>);
+    const int lane = wave_lane();
+    const Lines<kChunks> lines(out, stride, rows, columns);
+    // Of two rows' values of two adjacent lanes: the even one takes the first row's, the
+    // odd one the second's.
+    const uint32_t select = lane & 1 ? 0x03020706u : 0x05040100u;
+    uint16_t *at = mine + (4 * (lane >> 5) + (lane & 1)) * kPitch + (lane & 30);
+#pragma unroll
+    for (int m = 0; m < P::kRowTiles; ++m) {
+#pragma unroll
+        for (int n = 0; n < P::kColumnTiles; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) {
+                const uint32_t own = pair(m, n, r);
+                const uint32_t other = __builtin_amdgcn_mov_dpp(own, 0xB1, 0xF, 0xF, true);
+                *reinterpret_cast<uint32_t *>(at + (8 * (r / 4) + r % 4) * kPitch + 32 * n) =
+                    __builtin_amdgcn_perm(other, own, select);
+            }
+        wave_fence();
+#pragma unroll
+        for (int i = 0; i < 32 * kChunks / kWave; ++i) {
+            const int slot = i * kWave + lane;
+            lines.store(*reinterpret_cast<const u32x4 *>(mine + slot / kChunks * kPitch
+                                                         + slot % kChunks * 8),
+                        32 * m, slot);
+        }
+        wave_fence();
+    }
+}
+
+// That LDS: in the stages, which a finished run() leaves free.
 template <class P>
-__device__ __forceinline__ uint16_t *turn_values(uint16_t *stage0, uint16_t *stage1) {
-    constexpr int kWaves = P::kThreads / kWave;
-    static_assert(kWaves / 2 * kTurnValues<P> <= P::kStage);
-    const int wave = P::wave();
-    return (wave < kWaves / 2 ? stage0 : stage1) + wave % (kWaves / 2) * kTurnValues<P>;
+__device__ __forceinline__ uint16_t *turn_values(uint16_t *s0, uint16_t *s1, uint16_t *s2,
+                                                 uint16_t *s3) {
+    constexpr int kWaves = P::kThreads / kWave, kPer = (kWaves + P::kStages - 1) / P::kStages;
+    static_assert(kPer * kTurnValues<P> <= P::kStage);
+    const int wave = P::wave(), stage = wave / kPer;
+    return (stage == 0 ? s0 : stage == 1 ? s1 : stage == 2 ? s2 : s3) + wave % kPer * kTurnValues<P>;
 }
 
 }  // namespace lct

@@ -28,7 +28,7 @@ _MAX_SPLITS = 16        # LCT_MAX_CROSS_ENTROPY_SPLITS
 _PIECE_BYTES = 256 << 20
 
 MAX_MATRIX_DIM = 1 << 16    # LCT_MAX_ORTHOGONAL_DIM
-_NORM_PARTS = 64            # LCT_ORTHOGONAL_NORM_PARTS
+_NORM_PARTS = 1024          # LCT_ORTHOGONAL_NORM_PARTS
 
 
 def _whole_rows(t: Tensor) -> Tensor:
@@ -167,7 +167,7 @@ def orthogonalize(g: Tensor, steps: int, scale: float, eps: float) -> Tensor:
         stride = stride[0], stride[2], stride[1]
         out_stride = out_stride[0], out_stride[2], out_stride[1]
     r, c = _up8(rows), _up8(cols)
-    size = -(-count * 8 * _NORM_PARTS // 16) * 16 + count * (8 * r * c + 4 * r * r)
+    size = count * (8 * _NORM_PARTS + 6 * r * c + 4 * r * r)
     workspace = torch.empty(size, dtype=torch.uint8, device=g.device)
     _launch("lct_orthogonalize", g.get_device(), hip.ORTHOGONAL.pack(
         g.data_ptr(), out.data_ptr(), *stride, *out_stride, count, rows, cols, steps,
