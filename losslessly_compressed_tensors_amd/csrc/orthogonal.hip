@@ -200,13 +200,19 @@ __device__ __forceinline__ void lower_tile(int32_t t, int32_t *i, int32_t *j) {
     *j = t - row * (row + 1) / 2;
 }
 
-// A symmetric product of an operand by rows with itself: A (kPoly false; from X) or P
-// (from A).  `size`: rows of the result.
-template <class P, bool kPoly>
-__global__ __launch_bounds__(P::kThreads, 2) void symmetric_kernel(const uint16_t *operand,
-                                                                   int32_t count, int32_t size,
-                                                                   int32_t depth, int32_t tiles,
-                                                                   uint16_t *out) {
+// out = factor L R + share (E + F): a symmetric product (of X and itself, or of two polynomials
+// of one symmetric matrix, which commute) of operands by rows, and up to kMore of the
+// matrices E and F.  `size`: rows of the result.
+struct SymmetricTerms {
+    const uint16_t *left, *right, *more[2];
+    uint16_t *out;
+    float factor, share;
+};
+
+template <class P, int kMore>
+__global__ __launch_bounds__(P::kThreads, 2) void symmetric_kernel(SymmetricTerms s, int32_t count,
+                                                                   int32_t size, int32_t depth,
+                                                                   int32_t tiles) {
     static_assert(P::kM == P::kN);
     LCT_PRODUCT_STAGES(P);
     const int64_t item = xcd_item(int64_t{count} * tiles, blockIdx.x);
@@ -214,46 +220,53 @@ __global__ __launch_bounds__(P::kThreads, 2) void symmetric_kernel(const uint16_
     const int32_t matrix = static_cast<int32_t>(item / tiles);
     int32_t i, j;
     lower_tile(static_cast<int32_t>(item % tiles), &i, &j);
-    const uint16_t *from = operand + int64_t{matrix} * size * depth;
-    out += int64_t{matrix} * size * size;
+    const int64_t of = int64_t{matrix} * size * depth;
     typename P::A a;
     typename P::B b;
-    a.prepare(from, depth, int64_t{i} * P::kM, size);
-    b.prepare(from, depth, int64_t{j} * P::kN, size);
+    a.prepare(s.left + of, depth, int64_t{i} * P::kM, size);
+    b.prepare(s.right + of, depth, int64_t{j} * P::kN, size);
     P p;
     p.begin();
     p.run(a, b, depth, stage0, stage1, stage2, stage3);
 
     const int32_t row = i * P::kM + p.first_row(), column = j * P::kN + p.first_column();
+    const int64_t first = int64_t{matrix} * size * size;
     uint16_t *mine = turn_values<P>(stage0, stage1, stage2, stage3);
-    if constexpr (kPoly) {
-        // A(row, column) is A(column, row).
-        load_columns<P>(from + int64_t{column} * depth + row, depth, size - column, size - row,
-                        mine, [&](int m, int n, int r, uint32_t own) __attribute__((always_inline)) {
+#pragma unroll
+    for (int m = 0; m < P::kRowTiles; ++m)
+#pragma unroll
+        for (int n = 0; n < P::kColumnTiles; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) p.sum[m][n][r] *= s.factor;
+#pragma unroll
+    for (int e = 0; e < kMore; ++e)
+        // Its value at (row, column) is that at (column, row).
+        load_columns<P>(s.more[e] + first + int64_t{column} * size + row, size, size - column,
+                        size - row, mine,
+                        [&](int m, int n, int r, uint32_t own) __attribute__((always_inline)) {
                             p.sum[m][n][r] =
-                                __builtin_fmaf(kC / kHoldA, p.sum[m][n][r], kB * Half::low(own));
-                            p.sum[m][n][r + 1] = __builtin_fmaf(kC / kHoldA, p.sum[m][n][r + 1],
-                                                                kB * Half::high(own));
+                                __builtin_fmaf(s.share, Half::low(own), p.sum[m][n][r]);
+                            p.sum[m][n][r + 1] =
+                                __builtin_fmaf(s.share, Half::high(own), p.sum[m][n][r + 1]);
                         });
-    }
     const auto pair = [&](int m, int n, int r) __attribute__((always_inline)) {
-        constexpr float kFactor = kPoly ? 1.0f : kHoldA / (kHoldX * kHoldX);
-        return Half::round_pair(p.sum[m][n][r] * kFactor, p.sum[m][n][r + 1] * kFactor);
+        return Half::round_pair(p.sum[m][n][r], p.sum[m][n][r + 1]);
     };
-    store_columns<P>(out + int64_t{column} * size + row, size, size - column, size - row, mine,
-                     pair);
+    store_columns<P>(s.out + first + int64_t{column} * size + row, size, size - column, size - row,
+                     mine, pair);
     if (i != j)
-        store_rows<P>(out + int64_t{row} * size + column, size, size - row, size - column, mine,
-                      pair);
+        store_rows<P>(s.out + first + int64_t{row} * size + column, size, size - row, size - column,
+                      mine, pair);
 }
 
-// X <- a X + P X: P::kM columns of X (rows of the tile) by P::kN rows of X (columns, a lane
+// X <- share X + S X: P::kM columns of X (rows of the tile) by P::kN rows of X (columns, a lane
 // each).  The last step writes the result, scaled, in BF16 and G's orientation, if its
 // rows are whole 16-byte pieces.
 template <class P, bool kLast>
 __global__ __launch_bounds__(P::kThreads, P::kThreads == 256 ? 2 : 1) void update_kernel(
     const uint16_t *poly, const uint16_t *x, int32_t count, int32_t rows, int32_t cols,
-    int32_t row_tiles, int32_t column_tiles, uint16_t *x_rest, uint16_t *next, lct_orthogonal o) {
+    int32_t row_tiles, int32_t column_tiles, float share, uint16_t *x_rest, uint16_t *next,
+    lct_orthogonal o) {
     LCT_PRODUCT_STAGES(P);
     const int64_t tiles = int64_t{row_tiles} * column_tiles;
     const int64_t item = xcd_item(count * tiles, blockIdx.x);
@@ -273,19 +286,19 @@ __global__ __launch_bounds__(P::kThreads, P::kThreads == 256 ? 2 : 1) void updat
     const int32_t column = j * P::kM + p.first_row(), row = i * P::kN + p.first_column();
     const int64_t at = first + int64_t{row} * cols + column;
     uint16_t *mine = turn_values<P>(stage0, stage1, stage2, stage3);
-    // 2^10 X: the sums are 2^22 P X.
+    // 2^10 X: the sums are 2^22 S X.
     load_columns<P>(x + at, cols, rows - row, cols - column, mine,
                     [&](int m, int n, int r, uint32_t old) __attribute__((always_inline)) {
                         p.sum[m][n][r] = __builtin_fmaf(1.0f / kHoldA, p.sum[m][n][r],
-                                                        kA * Half::low(old));
+                                                        share * Half::low(old));
                         p.sum[m][n][r + 1] = __builtin_fmaf(1.0f / kHoldA, p.sum[m][n][r + 1],
-                                                            kA * Half::high(old));
+                                                            share * Half::high(old));
                     });
     load_columns<P>(x_rest + at, cols, rows - row, cols - column, mine,
                     [&](int m, int n, int r, uint32_t old) __attribute__((always_inline)) {
-                        p.sum[m][n][r] = __builtin_fmaf(kA, Half::low(old), p.sum[m][n][r]);
+                        p.sum[m][n][r] = __builtin_fmaf(share, Half::low(old), p.sum[m][n][r]);
                         p.sum[m][n][r + 1] =
-                            __builtin_fmaf(kA, Half::high(old), p.sum[m][n][r + 1]);
+                            __builtin_fmaf(share, Half::high(old), p.sum[m][n][r + 1]);
                     });
     if constexpr (kLast) {
         const float factor = o.scale * (1.0f / kHoldX);
@@ -314,33 +327,91 @@ __global__ __launch_bounds__(P::kThreads, P::kThreads == 256 ? 2 : 1) void updat
 
 int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
 
-using Symmetric = Product<true, Lie::kRows, Lie::kRows, 128, 128, 2, 2, 64, 2>;
-#ifndef UP
-#define UP 256, 128, 2, 2, 32, 3
-#endif
-using Update = Product<true, Lie::kColumns, Lie::kRows, UP>;
+// ---- tiles, by how many there are for the 256 compute units
+//
+// us of 5 or 12 steps, with tiles of 64 x 64 | 128 x 128 (and, of the update, 256 x 128 | 256 x
+// 256) in all products, two workgroups per compute unit but of the last.  The products by
+// 128 x 128 have, of one 768 x 768, 21 lower tiles and 36 in the update: 110 | 185; of 3:
+// 282 | 439; of 6 (126, 216): 405 with an update by 128 385 | 447; of 4 x 1024 x 1024 (144,
+// 256): 234 | 238; of 12 x 768 x 768 (252, 432): 589 | 537 | 557; of 48 (1008, 1728): 2188
+// | 1807 | 1779 | 1814; of 4096 x 4096 (528, 1024): 2380 | 1780 | 1698 | 1680; of 4096 x
+// 11008: | 3347 | 3217 | 3112.
+template <int kSize>
+using Symmetric = Product<true, Lie::kRows, Lie::kRows, kSize, kSize, 2, 2, 64, kSize == 64 ? 4 : 2>;
+template <int kM, int kN, int kWavesN, int kStep, int kStages>
+using Update = Product<true, Lie::kColumns, Lie::kRows, kM, kN, 2, kWavesN, kStep, kStages>;
+constexpr int64_t kFewTiles = 160, kManyTiles = 800;   // of 128 x 128
+constexpr int32_t kLongDepth = 1024;
 
 struct Iteration {
     int32_t count, rows, cols;
-    uint16_t *x, *next, *x_rest, *gram, *poly;
+    uint16_t *x, *next, *x_rest, *square[3];
     hipStream_t stream;
 
-    template <class P, bool kPoly>
-    void symmetric() const {
-        const int32_t blocks = (rows + P::kM - 1) / P::kM, tiles = blocks * (blocks + 1) / 2;
-        symmetric_kernel<P, kPoly>
-            <<<static_cast<uint32_t>(xcd_grid(int64_t{count} * tiles)), P::kThreads, 0, stream>>>(
-                kPoly ? gram : x, count, rows, kPoly ? rows : cols, tiles, kPoly ? poly : gram);
+    // Tiles of 128 x 128.
+    int64_t lower_tiles() const {
+        const int64_t blocks = (rows + 127) / 128;
+        return count * (blocks * (blocks + 1) / 2);
+    }
+    int64_t all_tiles() const {
+        return count * int64_t{(rows + 127) / 128} * ((cols + 127) / 128);
+    }
+
+    template <int kSize>
+    void launch_symmetric(const SymmetricTerms &s, int32_t depth) const {
+        using P = Symmetric<kSize>;
+        const int32_t blocks = (rows + kSize - 1) / kSize, tiles = blocks * (blocks + 1) / 2;
+        const uint32_t grid = static_cast<uint32_t>(xcd_grid(int64_t{count} * tiles));
+        if (s.more[1] != nullptr)
+            symmetric_kernel<P, 2><<<grid, P::kThreads, 0, stream>>>(s, count, rows, depth, tiles);
+        else if (s.more[0] != nullptr)
+            symmetric_kernel<P, 1><<<grid, P::kThreads, 0, stream>>>(s, count, rows, depth, tiles);
+        else
+            symmetric_kernel<P, 0><<<grid, P::kThreads, 0, stream>>>(s, count, rows, depth, tiles);
+    }
+    void symmetric(const SymmetricTerms &s, int32_t depth) const {
+        if (lower_tiles() < kFewTiles) launch_symmetric<64>(s, depth);
+        else launch_symmetric<128>(s, depth);
+    }
+    // out = A = X X^T.
+    void gram(uint16_t *out) const {
+        symmetric({x, x, {nullptr, nullptr}, out, kHoldA / (kHoldX * kHoldX), 0.0f}, cols);
+    }
+    // out = b A + c A A.
+    void poly(const uint16_t *a, uint16_t *out) const {
+        symmetric({a, a, {a, nullptr}, out, kC / kHoldA, kB}, rows);
+    }
+    // out = a (E + F) + L R.
+    void sum(const uint16_t *l, const uint16_t *r, const uint16_t *e, const uint16_t *f,
+             uint16_t *out) const {
+        symmetric({l, r, {e, f}, out, 1.0f / kHoldA, kA}, rows);
     }
     template <class P, bool kLast>
-    void update(const lct_orthogonal &o) const {
+    void launch_update(const uint16_t *s, float share, const lct_orthogonal &o) const {
         const int32_t row_tiles = (rows + P::kN - 1) / P::kN;
         const int32_t column_tiles = (cols + P::kM - 1) / P::kM;
         const int64_t items = int64_t{count} * row_tiles * column_tiles;
-        update_kernel<P, kLast>
-            <<<static_cast<uint32_t>(xcd_grid(items)), P::kThreads, 0, stream>>>(
-                poly, x, count, rows, cols, row_tiles, column_tiles, x_rest, next, o);
+        update_kernel<P, kLast><<<static_cast<uint32_t>(xcd_grid(items)), P::kThreads, 0, stream>>>(
+            s, x, count, rows, cols, row_tiles, column_tiles, share, x_rest, next, o);
     }
+    // X <- share X + S X.
+    void update(const uint16_t *s, float share, bool last, const lct_orthogonal &o) {
+        const auto with = [&](auto which) {
+            using P = typename decltype(which)::type;
+            if (last) launch_update<P, true>(s, share, o);
+            else launch_update<P, false>(s, share, o);
+        };
+        const int64_t tiles = all_tiles();
+        if (tiles < kFewTiles) with(Type<Update<64, 64, 2, 64, 4>>{});
+        else if (tiles < kManyTiles) with(Type<Update<128, 128, 2, 64, 2>>{});
+        else if (rows < kLongDepth) with(Type<Update<256, 128, 2, 32, 3>>{});
+        else with(Type<Update<256, 256, 4, 32, 4>>{});
+        std::swap(x, next);
+    }
+    template <class T>
+    struct Type {
+        using type = T;
+    };
 };
 
 }  // namespace
@@ -364,19 +435,19 @@ extern "C" int32_t lct_orthogonalize(const lct_orthogonal *o, void *workspace,
     if (count * tiles >= 1 << 23) return LCT_E_SIZE;
     const int32_t parts =
         static_cast<int32_t>(std::min<int64_t>(LCT_ORTHOGONAL_NORM_PARTS, (tiles + 3) / 4));
-    // Norms, X as it is and to be, what X's rounding leaves, A and P.
+    // Norms, X as it is and to be, what X's rounding leaves, and three square matrices.
     const int64_t norm_bytes = count * LCT_ORTHOGONAL_NORM_PARTS * 8;
-    if (workspace_bytes < norm_bytes + values * 6 + square * 4) return LCT_E_SIZE;
+    if (workspace_bytes < norm_bytes + 6 * (values + square)) return LCT_E_SIZE;
     auto *norms = static_cast<double *>(workspace);
     auto *x = reinterpret_cast<uint16_t *>(static_cast<char *>(workspace) + norm_bytes);
+    uint16_t *const squares = x + 3 * values;
     Iteration it{static_cast<int32_t>(count),
                  static_cast<int32_t>(rows),
                  static_cast<int32_t>(cols),
                  x,
                  x + values,
                  x + 2 * values,
-                 x + 3 * values,
-                 x + 3 * values + square,
+                 {squares, squares + square, squares + 2 * square},
                  stream};
     norm_kernel<<<static_cast<uint32_t>(count * parts), 256, 0, stream>>>(*o, parts, norms);
     start_kernel<<<static_cast<uint32_t>(count * tiles), 256, 0, stream>>>(
@@ -386,12 +457,27 @@ extern "C" int32_t lct_orthogonalize(const lct_orthogonal *o, void *workspace,
     const bool whole = o->out_stride[inner] == 1 && length % 8 == 0
                        && o->out_stride[3 - inner] % 8 == 0 && o->out_stride[0] % 8 == 0
                        && reinterpret_cast<uintptr_t>(o->out) % 16 == 0;
-    for (int32_t s = 0; s < o->steps; ++s) {
-        it.symmetric<Symmetric, false>();
-        it.symmetric<Symmetric, true>();
-        if (s + 1 == o->steps && whole) it.update<Update, true>(*o);
-        else it.update<Update, false>(*o);
-        std::swap(it.x, it.next);
+    // Two steps at once have 3 products with X, of rows^2 cols each, in place of 6 and 5 in
+    // place of 2 of rows^3, the symmetric ones by half.  us of 12 or 5 steps one | two at a time:
+    // 48 x 768 x 768 1765 | 1858; 16 x 4096 x 1024 1907 | 1409; 4096 x 11008 3955 | 3217; of few
+    // tiles, which cost their launches, 768 x 768 138 | 138, 8 x 96 x 160 76 | 81.
+    const bool pairs = 2 * cols >= 3 * rows && it.all_tiles() >= kFewTiles;
+    for (int32_t s = 0; s < o->steps;) {
+        uint16_t *const m = it.square[0], *const p = it.square[1], *const r = it.square[2];
+        it.gram(m);
+        it.poly(m, p);
+        if (pairs && s + 2 <= o->steps) {
+            // Two steps at once, X <- (a + P') (a + P) X: the second's A' = (a + P) A (a + P).
+            it.sum(p, m, m, nullptr, r);
+            it.sum(p, r, r, nullptr, m);
+            it.poly(m, r);
+            it.sum(r, p, r, p, m);
+            s += 2;
+            it.update(m, kA * kA, s == o->steps && whole, *o);
+        } else {
+            s += 1;
+            it.update(p, kA, s == o->steps && whole, *o);
+        }
     }
     if (o->steps == 0 || !whole)
         finish_kernel<<<static_cast<uint32_t>(count * tiles), 256, 0, stream>>>(

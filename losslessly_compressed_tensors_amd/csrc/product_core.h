@@ -39,8 +39,8 @@ struct Operand {
     static __device__ __forceinline__ int permuted(int line, int chunk) {
         if constexpr (kLie == Lie::kRows)
             return chunk ^ (kStep == 32 ? (line >> 2) & 3 : (line >> 1) & 7);
-        else    // lines of 1.5 times 256 bytes differ by 128 as they are
-            return chunk ^ (kTile == 192 ? (line & 2) << 1 : (line & 3) << 2);
+        else    // (every second line of 128 or 384 bytes is 128 further as it is)
+            return chunk ^ (kTile % 128 ? (line & 2) << 1 : (line & 3) << 2);
     }
 
     __device__ __forceinline__ void prepare(const void *matrix, int64_t stride_, int64_t first,
@@ -397,7 +397,9 @@ __device__ __forceinline__ uint16_t *turn_values(uint16_t *s0, uint16_t *s1, uin
     constexpr int kWaves = P::kThreads / kWave, kPer = (kWaves + P::kStages - 1) / P::kStages;
     static_assert(kPer * kTurnValues<P> <= P::kStage);
     const int wave = P::wave(), stage = wave / kPer;
-    return (stage == 0 ? s0 : stage == 1 ? s1 : stage == 2 ? s2 : s3) + wave % kPer * kTurnValues<P>;
+    uint16_t *base = stage == 0 ? s0 : s1;
+    if constexpr (2 * kPer < kWaves) base = stage < 2 ? base : stage == 2 ? s2 : s3;
+    return base + wave % kPer * kTurnValues<P>;
 }
 
 }  // namespace lct

@@ -167,7 +167,7 @@ def orthogonalize(g: Tensor, steps: int, scale: float, eps: float) -> Tensor:
         stride = stride[0], stride[2], stride[1]
         out_stride = out_stride[0], out_stride[2], out_stride[1]
     r, c = _up8(rows), _up8(cols)
-    size = count * (8 * _NORM_PARTS + 6 * r * c + 4 * r * r)
+    size = count * (8 * _NORM_PARTS + 6 * r * (c + r))
     workspace = torch.empty(size, dtype=torch.uint8, device=g.device)
     _launch("lct_orthogonalize", g.get_device(), hip.ORTHOGONAL.pack(
         g.data_ptr(), out.data_ptr(), *stride, *out_stride, count, rows, cols, steps,
