@@ -27,12 +27,13 @@ REDUCTIONS = ("mean", "sum", "none")
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, targets, softcap, ignore_index, reduction):
-        losses, lse, total = kernels.cross_entropy_forward(
+        out, stats = kernels.cross_entropy_forward(
             x, weight, None if bias is None else bias.float(), targets, softcap, ignore_index,
             reduction)
         ctx.how = softcap, ignore_index, reduction
-        ctx.save_for_backward(x, weight, bias, targets, losses, lse)
-        return losses if total is None else total
+        ctx.save_for_backward(x, weight, bias, targets, stats)
+        # The caller's losses are its own to change.
+        return out.clone() if reduction == "none" else out
 
     @staticmethod
     def backward(ctx, grad):
@@ -43,9 +44,9 @@ class _LinearCrossEntropy(torch.autograd.Function):
 
 
 def _backward(ctx, grad):
-    x, weight, bias, targets, losses, lse = ctx.saved_tensors
+    x, weight, bias, targets, stats = ctx.saved_tensors
     grad_x, grad_weight, grad_bias = kernels.cross_entropy_backward(
-        grad.contiguous(), x, weight, None if bias is None else bias.float(), targets, losses, lse,
+        grad.contiguous(), x, weight, None if bias is None else bias.float(), targets, stats,
         *ctx.how, ctx.needs_input_grad[:3])
     if grad_bias is not None:
         grad_bias = grad_bias.to(bias.dtype)
@@ -124,10 +125,9 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, targets: Tensor, bias: Tenso
     if _recorded(x, weight, bias):
         out = _LinearCrossEntropy.apply(x, weight, bias, targets, softcap, ignore_index, reduction)
     else:
-        losses, _, total = kernels.cross_entropy_forward(
+        out, _ = kernels.cross_entropy_forward(
             x, weight, None if bias is None else bias.float(), targets, softcap, ignore_index,
             reduction)
-        out = losses if total is None else total
     return out.view(shape) if reduction == "none" else out
 
 

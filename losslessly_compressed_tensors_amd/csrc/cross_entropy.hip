@@ -29,6 +29,11 @@ constexpr float kCapped = 1e18f;
 constexpr int kLogitRows = 192;
 template <bool kHalf>
 using LogitProduct = Product<kHalf, Lie::kRows, Lie::kRows, kLogitRows, 128, 2, 2, 64, 2>;
+// A few tokens, the vocabulary's rows streamed: us of 1 | 16 | 32 tokens against 50304 x 768
+// FEWNUMBERS
+constexpr int kFewTokens = 32;
+template <bool kHalf>
+using FewProduct = Product<kHalf, Lie::kRows, Lie::kRows, 128, kFewTokens, 4, 1, 64, 4>;
 template <bool kHalf>
 using HiddenProduct = Product<kHalf, Lie::kColumns, Lie::kColumns, 256, 128, 2, 2, 32, 3>;
 template <bool kHalf>
@@ -56,9 +61,31 @@ __device__ __forceinline__ int64_t target_of(const lct_cross_entropy &c, int64_t
                         : static_cast<const int32_t *>(c.targets)[n];
 }
 
+// The counted tokens' x next to each other, 16 bytes a thread, where not all count.
+__device__ __forceinline__ void gather(const lct_cross_entropy &c, int32_t count,
+                                       const int32_t *rows, void *out, int64_t first,
+                                       int64_t step) {
+    if (count == c.tokens) return;
+    const int32_t chunks = c.dim / 8;
+    for (int64_t at = first; at < int64_t{count} * chunks; at += step) {
+        const int32_t i = static_cast<int32_t>(at / chunks), chunk = static_cast<int32_t>(at % chunks);
+        static_cast<u32x4 *>(out)[at] = *reinterpret_cast<const u32x4 *>(
+            static_cast<const uint16_t *>(c.x) + rows[i] * c.x_stride + chunk * 8);
+    }
+}
+
+__global__ __launch_bounds__(256) void gather_kernel(lct_cross_entropy c, Counted t, void *out) {
+    gather(c, *t.count, t.rows, out, int64_t{blockIdx.x} * 256 + threadIdx.x,
+           int64_t{gridDim.x} * 256);
+}
+
+// 16-byte pieces of x up to which the one workgroup of prepare_kernel gathers itself.
+constexpr int64_t kGatherHere = 8192;
+
 // ---- the counted tokens, in order
 
-constexpr int kPrepareThreads = 1024;
+constexpr int kPrepareThreads = 1024, kPrepareEach = 16;
+constexpr int kGroups = kPrepareThreads / kWave * kPrepareEach;
 
 __device__ __forceinline__ float block_max(float v, float *scratch) {
 #pragma unroll
@@ -76,73 +103,98 @@ __device__ __forceinline__ float block_max(float v, float *scratch) {
 // multiplied by at the end: a token's incoming gradient over the power of two above the
 // largest, and that power, so that dz lies within [-1, 1] whatever the incoming gradients
 // are.  (All infinite or NaN ones go to their tokens' factors.)
-__global__ __launch_bounds__(kPrepareThreads) void prepare_kernel(
-    lct_cross_entropy c, int32_t *count_out, int32_t *rows, int32_t *targets, float *lse,
-    float *losses, const float *grad, int32_t grad_per_token, int32_t mean, float *lse_of,
-    float *losses_of, float *factor, float *scale) {
+struct PrepareGradients {
+    const float *grad;       // NULL: forward
+    int32_t per_token, mean;
+};
+
+__global__ __launch_bounds__(kPrepareThreads) void prepare_kernel(lct_cross_entropy c, Counted t,
+                                                                  PrepareGradients g, float *lse,
+                                                                  float *losses, void *gathered) {
+    auto *const rows = const_cast<int32_t *>(t.rows);
+    auto *const targets = const_cast<int32_t *>(t.targets);
+    const float *const grad = g.grad;
     __shared__ float scratch[kPrepareThreads / kWave];
-    __shared__ int32_t counts[kPrepareThreads / kWave];
+    __shared__ int32_t counts[kGroups], ends[kGroups / kWave];
     float largest = 0.0f;
-    if (grad != nullptr && grad_per_token)
+    if (grad != nullptr && g.per_token)
         for (int32_t n = threadIdx.x; n < c.tokens; n += kPrepareThreads)
             if (target_of(c, n) != c.ignore_index) {
-                const float g = fabsf(grad[n]);
-                if (g < INFINITY) largest = fmaxf(largest, g);
+                const float of = fabsf(grad[n]);
+                if (of < INFINITY) largest = fmaxf(largest, of);
             }
     float power = 1.0f;
-    if (grad != nullptr && grad_per_token) {
+    if (grad != nullptr && g.per_token) {
         largest = block_max(largest, scratch);
         // 2^e >= largest, within FP32's normal numbers.
         if (largest > 0.0f) power = ldexpf(1.0f, min(max(ilogbf(largest) + 1, -126), 127));
     }
     const float hold = c.fp16 ? kHalfGradient : 1.0f;
+    // Sixteen tokens a thread, their loads in flight together, between the workgroup's
+    // meetings.
     int32_t done = 0;
-    for (int32_t first = 0; first < c.tokens; first += kPrepareThreads) {
-        const int32_t n = first + threadIdx.x;
-        const int64_t target = n < c.tokens ? target_of(c, n) : c.ignore_index;
-        const bool counts_here = n < c.tokens && target != c.ignore_index;
-        const uint64_t ballot = __ballot(counts_here);
-        if (wave_lane() == 0) counts[threadIdx.x / kWave] = __popcll(ballot);
-        __syncthreads();
-        int32_t before = done, total = 0;
-        for (int w = 0; w < kPrepareThreads / kWave; ++w) {
-            before += w < static_cast<int>(threadIdx.x / kWave) ? counts[w] : 0;
-            total += counts[w];
+    for (int64_t first = 0; first < c.tokens; first += kPrepareThreads * kPrepareEach) {
+        int64_t target[kPrepareEach];
+#pragma unroll
+        for (int k = 0; k < kPrepareEach; ++k) {
+            const int64_t n = first + k * kPrepareThreads + threadIdx.x;
+            target[k] = n < c.tokens ? target_of(c, n) : c.ignore_index;
+        }
+#pragma unroll
+        for (int k = 0; k < kPrepareEach; ++k) {
+            const uint64_t counted = __ballot(target[k] != c.ignore_index);
+            if (wave_lane() == 0)
+                counts[k * (kPrepareThreads / kWave) + threadIdx.x / kWave] = __popcll(counted);
         }
         __syncthreads();
-        if (counts_here) {
-            const int32_t i = before + __popcll(ballot & ((uint64_t{1} << wave_lane()) - 1));
-            const bool inside = target >= 0 && target < c.vocab;
-            rows[i] = n;
-            targets[i] = inside ? static_cast<int32_t>(target) : -1;
-            if (grad != nullptr) {
-                lse_of[i] = lse[n];
-                losses_of[i] = losses[n];
-                factor[i] = inside ? (grad_per_token ? grad[n] / power : 1.0f) * hold : NAN;
+        // Where each wave's group begins, by the first four waves.
+        int32_t own = 0, inclusive = 0;
+        if (threadIdx.x < kGroups) {
+            own = counts[threadIdx.x];
+            inclusive = wave_inclusive_scan(own);
+            if (wave_lane() == kWave - 1) ends[threadIdx.x / kWave] = inclusive;
+        }
+        __syncthreads();
+        int32_t total = 0;
+#pragma unroll
+        for (int w = 0; w < kGroups / kWave; ++w) {
+            if (threadIdx.x < kGroups && w < static_cast<int>(threadIdx.x / kWave))
+                inclusive += ends[w];
+            total += ends[w];
+        }
+        if (threadIdx.x < kGroups) counts[threadIdx.x] = done + inclusive - own;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kPrepareEach; ++k) {
+            const int64_t n = first + k * kPrepareThreads + threadIdx.x;
+            if (n >= c.tokens) continue;
+            const bool counted = target[k] != c.ignore_index;
+            const uint64_t before = __ballot(counted) & ((uint64_t{1} << wave_lane()) - 1);
+            if (counted) {
+                const int32_t i = counts[k * (kPrepareThreads / kWave) + threadIdx.x / kWave]
+                                  + __popcll(before);
+                const bool inside = target[k] >= 0 && target[k] < c.vocab;
+                rows[i] = static_cast<int32_t>(n);
+                targets[i] = inside ? static_cast<int32_t>(target[k]) : -1;
+                if (grad != nullptr) {
+                    const_cast<float *>(t.lse)[i] = lse[n];
+                    const_cast<float *>(t.losses)[i] = losses[n];
+                    const_cast<float *>(t.factor)[i] = inside ? (g.per_token ? grad[n] / power : 1.0f) * hold : NAN;
+                }
+            } else if (grad == nullptr) {
+                lse[n] = 0.0f;
+                losses[n] = 0.0f;
             }
-        } else if (grad == nullptr && n < c.tokens) {
-            lse[n] = 0.0f;
-            losses[n] = 0.0f;
         }
         done += total;
+        __syncthreads();
     }
+    if (gathered != nullptr)      // (behind the last barrier above: the rows are written)
+        gather(c, done, rows, gathered, threadIdx.x, kPrepareThreads);
     if (threadIdx.x == 0) {
-        *count_out = done;
+        *const_cast<int32_t *>(t.count) = done;
         if (grad != nullptr)
-            *scale = (grad_per_token ? power : *grad / (mean ? fmaxf(1.0f, done) : 1.0f)) / hold;
-    }
-}
-
-// The counted tokens' x next to each other, 16 bytes a thread, where not all count.
-__global__ __launch_bounds__(256) void gather_kernel(lct_cross_entropy c, Counted t, void *out) {
-    const int32_t count = *t.count, chunks = c.dim / 8;
-    if (count == c.tokens) return;
-    const int64_t all = int64_t{count} * chunks;
-    for (int64_t at = int64_t{blockIdx.x} * 256 + threadIdx.x; at < all;
-         at += int64_t{gridDim.x} * 256) {
-        const int32_t i = static_cast<int32_t>(at / chunks), chunk = static_cast<int32_t>(at % chunks);
-        static_cast<u32x4 *>(out)[at] = *reinterpret_cast<const u32x4 *>(
-            static_cast<const uint16_t *>(c.x) + t.rows[i] * c.x_stride + chunk * 8);
+            *const_cast<float *>(t.scale) = (g.per_token ? power : *grad / (g.mean ? fmaxf(1.0f, done) : 1.0f)) / hold;
     }
 }
 
@@ -189,7 +241,7 @@ __device__ __forceinline__ bool far_of(const P &p, const Cap &cap) {
 
 // P::kM of the vocabulary (rows, in a lane's registers) by P::kN tokens (columns, a lane
 // each): a token's maximum and sum need one exchange between two lanes.
-template <class P, bool kHalf, bool kCap, bool kBias>
+template <class P, bool kCap, bool kBias>
 __global__ __launch_bounds__(P::kThreads, 2) void logits_kernel(lct_cross_entropy c, Counted t,
                                                                 int32_t vocab_tiles,
                                                                 int32_t token_tiles,
@@ -257,7 +309,7 @@ __global__ __launch_bounds__(P::kThreads, 2) void logits_kernel(lct_cross_entrop
                     if (first + 32 * m + 8 * (r / 4) + 4 * half + r % 4 >= c.vocab)
                         p.sum[m][n][r] = -INFINITY;
     }
-    const int32_t entries = 2 * vocab_tiles;
+    const int32_t entries = P::kWavesM * vocab_tiles;
 #pragma unroll
     for (int n = 0; n < P::kColumnTiles; ++n) {
         const int32_t token = token_tile * P::kN + p.first_column() + 32 * n + (wave_lane() & 31);
@@ -291,37 +343,49 @@ __global__ __launch_bounds__(P::kThreads, 2) void logits_kernel(lct_cross_entrop
                 total += exp2_fast(__builtin_fmaf(p.sum[m][n][r], kLog2e, -base));
         total = across_sum(total);
         if (half == 0 && token < count)
-            parts[int64_t{token} * entries + 2 * vocab_tile + p.wave() % 2] = Part{most, total};
+            parts[int64_t{token} * entries + P::kWavesM * vocab_tile + p.wave() % P::kWavesM] =
+                Part{most, total};
     }
 }
 
-// A wave joins one token's parts and computes its target's logit: the loss and lse (in
-// powers of two).
-template <bool kHalf>
+// kWaves join one token's parts and compute its target's logit: the loss and lse (in powers
+// of two).
+template <bool kHalf, int kWaves>
 __global__ __launch_bounds__(256) void join_kernel(lct_cross_entropy c, Counted t, int32_t entries,
                                                    const Part *__restrict__ parts,
                                                    float *__restrict__ lse,
                                                    float *__restrict__ losses) {
     using E = Element<kHalf>;
+    constexpr int kStep = kWaves * kWave, kAtOnce = 4;
+    __shared__ Part others[4];
+    __shared__ float products[4];
     const int32_t count = t.count == nullptr ? c.tokens : *t.count;
-    const int32_t i = blockIdx.x * 4 + threadIdx.x / kWave;
+    const int32_t i = blockIdx.x * (4 / kWaves) + threadIdx.x / kStep;
     if (i >= count) return;
-    const int lane = wave_lane();
+    const int lane = wave_lane(), place = threadIdx.x % kStep;
     const int32_t n = t.count == nullptr ? i : t.rows[i];
     const int64_t target = target_of(c, n);
     if (target == c.ignore_index) {
-        if (lane == 0) lse[n] = losses[n] = 0.0f;
+        if (place == 0) lse[n] = losses[n] = 0.0f;
         return;
     }
     const bool inside = target >= 0 && target < c.vocab;
     Part part{-INFINITY, 0.0f};
-    for (int32_t e = lane; e < entries; e += kWave)
-        part = joined(part, parts[int64_t{i} * entries + e]);
+    for (int32_t first = place; first < entries; first += kAtOnce * kStep) {
+        Part of[kAtOnce];
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+            const int32_t e = first + k * kStep;
+            of[k] = e < entries ? parts[int64_t{i} * entries + e] : Part{-INFINITY, 0.0f};
+        }
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) part = joined(part, of[k]);
+    }
     float logit = 0.0f;
     if (inside) {
         const uint16_t *x = static_cast<const uint16_t *>(c.x) + n * c.x_stride;
         const uint16_t *w = static_cast<const uint16_t *>(c.weight) + target * c.weight_stride;
-        for (int32_t d = 8 * lane; d < c.dim; d += 8 * kWave) {
+        for (int32_t d = 8 * place; d < c.dim; d += 8 * kStep) {
             const u32x4 p = *reinterpret_cast<const u32x4 *>(x + d);
             const u32x4 q = *reinterpret_cast<const u32x4 *>(w + d);
 #pragma unroll
@@ -335,6 +399,19 @@ __global__ __launch_bounds__(256) void join_kernel(lct_cross_entropy c, Counted 
     for (int d = kWave / 2; d > 0; d >>= 1) {
         logit += __shfl_xor(logit, d, kWave);
         part = joined(part, Part{__shfl_xor(part.most, d, kWave), __shfl_xor(part.total, d, kWave)});
+    }
+    if constexpr (kWaves > 1) {
+        if (lane == 0) {
+            others[threadIdx.x / kWave] = part;
+            products[threadIdx.x / kWave] = logit;
+        }
+        __syncthreads();
+        if (threadIdx.x >= kWave) return;
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) {
+            part = joined(part, others[w]);
+            logit += products[w];
+        }
     }
     if (lane != 0) return;
     if (!inside) {
@@ -519,7 +596,8 @@ __global__ __launch_bounds__(P::kThreads, 2) void gradient_kernel(
             const float sum = across_sum(column_sum[n]);
             const int32_t column = first + 32 * n + (lane & 31);
             if (half == 0 && column < last_vocab)
-                bias_parts[(int64_t{token_tile} * 2 + p.wave() % 2) * c.vocab + column] = sum;
+                bias_parts[(int64_t{token_tile} * P::kWavesM + p.wave() % P::kWavesM) * c.vocab
+                           + column] = sum;
         }
     }
     if (dz == nullptr) return;
@@ -641,15 +719,14 @@ __global__ __launch_bounds__(256, 2) void products_kernel(lct_cross_entropy c, C
 
 // dx from its parts, 8 values a thread; zeros for tokens that do not count.
 template <bool kHalf>
-__global__ __launch_bounds__(256) void join_hidden_kernel(lct_cross_entropy c, Counted t,
-                                                          int32_t splits,
-                                                          const float *__restrict__ parts,
-                                                          uint16_t *__restrict__ grad_x) {
+__device__ __forceinline__ void join_hidden(const lct_cross_entropy &c, const Counted &t,
+                                            int32_t splits, const float *__restrict__ parts,
+                                            uint16_t *__restrict__ grad_x, int64_t first,
+                                            int64_t step) {
+    using E = Element<kHalf>;
     const int32_t count = *t.count, chunks = c.dim / 8;
     const float scale = *t.scale;
-    const int64_t all = int64_t{count} * chunks;
-    for (int64_t at = int64_t{blockIdx.x} * 256 + threadIdx.x; at < all;
-         at += int64_t{gridDim.x} * 256) {
+    for (int64_t at = first; at < int64_t{count} * chunks; at += step) {
         const int32_t i = static_cast<int32_t>(at / chunks);
         const int32_t d = static_cast<int32_t>(at % chunks) * 8;
         f32x4 lo{}, hi{};
@@ -660,29 +737,46 @@ __global__ __launch_bounds__(256) void join_hidden_kernel(lct_cross_entropy c, C
         }
         lo *= scale;
         hi *= scale;
-        using E = Element<kHalf>;
         *reinterpret_cast<u32x4 *>(grad_x + int64_t{t.rows[i]} * c.dim + d) =
             u32x4{E::round_pair(lo[0], lo[1]), E::round_pair(lo[2], lo[3]),
                   E::round_pair(hi[0], hi[1]), E::round_pair(hi[2], hi[3])};
     }
     if (count == c.tokens) return;
-    for (int64_t at = int64_t{blockIdx.x} * 256 + threadIdx.x; at < int64_t{c.tokens} * chunks;
-         at += int64_t{gridDim.x} * 256) {
-        const int64_t n = at / chunks;
-        if (target_of(c, n) == c.ignore_index)
+    for (int64_t at = first; at < int64_t{c.tokens} * chunks; at += step)
+        if (target_of(c, at / chunks) == c.ignore_index)
             *reinterpret_cast<u32x4 *>(grad_x + at * 8) = u32x4{0u, 0u, 0u, 0u};
-    }
 }
 
-__global__ __launch_bounds__(256) void join_bias_kernel(lct_cross_entropy c, Counted t,
-                                                        int32_t rows,
-                                                        const float *__restrict__ parts,
-                                                        float *__restrict__ grad_bias) {
-    const int32_t v = blockIdx.x * 256 + threadIdx.x;
-    if (v >= c.vocab) return;
+// The bias's gradient: 64 of the vocabulary, their parts (one per `rows` / 2 tokens) among the
+// four waves.
+__device__ __forceinline__ void join_bias(const lct_cross_entropy &c, const Counted &t,
+                                          int32_t rows, const float *__restrict__ parts,
+                                          float *__restrict__ grad_bias, int32_t block) {
+    __shared__ float sums[4][kWave];
+    const int32_t v = block * kWave + wave_lane(), wave = threadIdx.x / kWave;
+    const int32_t all = 2 * ((*t.count + rows - 1) / rows);
     float sum = 0.0f;
-    for (int32_t i = 0; i < 2 * ((*t.count + rows - 1) / rows); ++i) sum += parts[int64_t{i} * c.vocab + v];
-    grad_bias[v] = sum * *t.scale;
+    if (v < c.vocab)
+        for (int32_t i = wave; i < all; i += 4) sum += parts[int64_t{i} * c.vocab + v];
+    sums[wave][wave_lane()] = sum;
+    __syncthreads();
+    if (wave == 0 && v < c.vocab)
+        grad_bias[v] = (sum + sums[1][wave_lane()] + (sums[2][wave_lane()] + sums[3][wave_lane()]))
+                       * *t.scale;
+}
+
+template <bool kHalf>
+__global__ __launch_bounds__(256) void join_gradients_kernel(lct_cross_entropy c, Counted t,
+                                                             int32_t splits, const float *hidden,
+                                                             uint16_t *grad_x, int32_t rows,
+                                                             const float *bias, float *grad_bias,
+                                                             uint32_t bias_grid) {
+    if (blockIdx.x < bias_grid)
+        join_bias(c, t, rows, bias, grad_bias, blockIdx.x);
+    else
+        join_hidden<kHalf>(c, t, splits, hidden, grad_x,
+                           int64_t{blockIdx.x - bias_grid} * 256 + threadIdx.x,
+                           int64_t{gridDim.x - bias_grid} * 256);
 }
 
 // ---- entry points
@@ -710,6 +804,20 @@ int32_t check(const lct_cross_entropy *c) {
 int32_t tiles_of(int64_t n, int32_t tile) { return static_cast<int32_t>((n + tile - 1) / tile); }
 
 constexpr int32_t kMaxStrideGrid = 1 << 16;
+constexpr int32_t kWideJoin = 1024;    // tokens up to which four waves join one's parts
+
+uint32_t chunk_grid_of(const lct_cross_entropy &c) {
+    return static_cast<uint32_t>(
+        std::min<int64_t>(kMaxStrideGrid, (int64_t{c.tokens} * (c.dim / 8) + 255) / 256));
+}
+
+void prepare(const lct_cross_entropy &c, const Counted &t, void *gathered,
+             const PrepareGradients &g, float *lse, float *losses, hipStream_t stream) {
+    const bool here = int64_t{c.tokens} * (c.dim / 8) <= kGatherHere;
+    prepare_kernel<<<1, kPrepareThreads, 0, stream>>>(c, t, g, lse, losses,
+                                                      here ? gathered : nullptr);
+    if (!here) gather_kernel<<<chunk_grid_of(c), 256, 0, stream>>>(c, t, gathered);
+}
 
 template <class Launch>
 void by_form(const lct_cross_entropy &c, Launch launch) {
@@ -737,10 +845,11 @@ extern "C" int32_t lct_cross_entropy_forward(const lct_cross_entropy *c, int32_t
                                              float *total, int32_t mean, hipStream_t stream) {
     if (const int32_t bad = check(c)) return bad;
     if (parts == nullptr || lse == nullptr || losses == nullptr) return LCT_E_NULL;
-    const int32_t vocab_tiles = tiles_of(c->vocab, kLogitRows);
-    const int32_t token_tiles = tiles_of(c->tokens, 128);
-    if (part_floats < int64_t{4} * tiles_of(c->vocab, 128) * c->tokens || !aligned(parts, 8))
-        return LCT_E_SIZE;
+    const bool few = c->tokens <= kFewTokens;
+    const int32_t vocab_tiles = tiles_of(c->vocab, few ? 128 : kLogitRows);
+    const int32_t token_tiles = tiles_of(c->tokens, few ? kFewTokens : 128);
+    const int32_t entries = (few ? 4 : 2) * vocab_tiles;
+    if (part_floats < int64_t{2} * entries * c->tokens || !aligned(parts, 8)) return LCT_E_SIZE;
     Counted t{};
     if (index != nullptr) {
         if (gathered == nullptr) return LCT_E_NULL;
@@ -751,29 +860,30 @@ extern "C" int32_t lct_cross_entropy_forward(const lct_cross_entropy *c, int32_t
         t.rows = index + 1;
         t.targets = index + 1 + c->tokens;
         t.gathered = gathered;
-        prepare_kernel<<<1, kPrepareThreads, 0, stream>>>(
-            *c, index, index + 1, index + 1 + c->tokens, lse, losses, nullptr, 0, 0, nullptr,
-            nullptr, nullptr, nullptr);
-        gather_kernel<<<std::min<int64_t>(kMaxStrideGrid,
-                                          (int64_t{c->tokens} * (c->dim / 8) + 255) / 256),
-                        256, 0, stream>>>(*c, t, gathered);
+        prepare(*c, t, gathered, PrepareGradients{}, lse, losses, stream);
     }
     const uint32_t grid = static_cast<uint32_t>(xcd_grid(int64_t{vocab_tiles} * token_tiles));
+    auto *of = reinterpret_cast<Part *>(parts);
     by_form(*c, [&](auto half, auto cap, auto bias) {
-        logits_kernel<LogitProduct<decltype(half)::value>, decltype(half)::value,
-                      decltype(cap)::value, decltype(bias)::value>
-            <<<grid, 256, 0, stream>>>(*c, t, vocab_tiles, token_tiles,
-                                       reinterpret_cast<Part *>(parts));
+        constexpr bool kHalf = decltype(half)::value;
+        if (few)
+            logits_kernel<FewProduct<kHalf>, decltype(cap)::value, decltype(bias)::value>
+                <<<grid, 256, 0, stream>>>(*c, t, vocab_tiles, token_tiles, of);
+        else
+            logits_kernel<LogitProduct<kHalf>, decltype(cap)::value, decltype(bias)::value>
+                <<<grid, 256, 0, stream>>>(*c, t, vocab_tiles, token_tiles, of);
     });
-    const uint32_t waves = static_cast<uint32_t>((c->tokens + 3) / 4);
-    if (c->fp16)
-        join_kernel<true><<<waves, 256, 0, stream>>>(*c, t, 2 * vocab_tiles,
-                                                     reinterpret_cast<const Part *>(parts), lse,
-                                                     losses);
-    else
-        join_kernel<false><<<waves, 256, 0, stream>>>(*c, t, 2 * vocab_tiles,
-                                                      reinterpret_cast<const Part *>(parts), lse,
-                                                      losses);
+    const bool wide = c->tokens <= kWideJoin;
+    const uint32_t joins = static_cast<uint32_t>(wide ? c->tokens : (c->tokens + 3) / 4);
+    const auto join = [&](auto half) {
+        constexpr bool kHalf = decltype(half)::value;
+        if (wide)
+            join_kernel<kHalf, 4><<<joins, 256, 0, stream>>>(*c, t, entries, of, lse, losses);
+        else
+            join_kernel<kHalf, 1><<<joins, 256, 0, stream>>>(*c, t, entries, of, lse, losses);
+    };
+    if (c->fp16) join(std::true_type{});
+    else join(std::false_type{});
     if (total != nullptr)
         total_kernel<<<1, kPrepareThreads, 0, stream>>>(*c, losses, mean, total);
     return static_cast<int32_t>(hipGetLastError());
@@ -813,12 +923,9 @@ extern "C" int32_t lct_cross_entropy_backward(const lct_cross_entropy *c,
     t.losses = losses;
     t.factor = factor;
     t.gathered = d->gathered;
-    prepare_kernel<<<1, kPrepareThreads, 0, stream>>>(
-        *c, d->index, rows, targets, const_cast<float *>(d->lse), const_cast<float *>(d->losses),
-        d->grad, d->grad_per_token, d->mean, lse, losses, factor, d->values);
-    const uint32_t chunk_grid = static_cast<uint32_t>(
-        std::min<int64_t>(kMaxStrideGrid, (tokens * (c->dim / 8) + 255) / 256));
-    gather_kernel<<<chunk_grid, 256, 0, stream>>>(*c, t, d->gathered);
+    prepare(*c, t, d->gathered, PrepareGradients{d->grad, d->grad_per_token, d->mean},
+            const_cast<float *>(d->lse), const_cast<float *>(d->losses), stream);
+    const uint32_t chunk_grid = chunk_grid_of(*c);
     auto *dz = static_cast<uint16_t *>(d->dz);
     const int32_t dim_tiles = tiles_of(c->dim, 256), hidden_tiles = tiles_of(tokens, 128);
     for (int32_t first = 0; first < c->vocab; first += d->piece) {
@@ -832,6 +939,7 @@ extern "C" int32_t lct_cross_entropy_backward(const lct_cross_entropy *c,
                                            products ? dz : nullptr, pitch,
                                            d->grad_bias != nullptr ? d->bias_parts : nullptr);
         });
+        if (!products) continue;
         const PieceProducts q{first,    piece,       d->splits, dim_tiles,
                               hidden_tiles, vocab_tiles, dz,        pitch,
                               d->hidden_parts, static_cast<uint16_t *>(d->grad_weight)};
@@ -843,7 +951,6 @@ extern "C" int32_t lct_cross_entropy_backward(const lct_cross_entropy *c,
             d->grad_x == nullptr
                 ? 0
                 : static_cast<uint32_t>(xcd_grid(int64_t{dim_tiles} * hidden_tiles * d->splits));
-        if (weight_grid + hidden_grid == 0) continue;
         if (c->fp16)
             products_kernel<true>
                 <<<weight_grid + hidden_grid, 256, 0, stream>>>(*c, t, q, weight_grid);
@@ -851,17 +958,19 @@ extern "C" int32_t lct_cross_entropy_backward(const lct_cross_entropy *c,
             products_kernel<false>
                 <<<weight_grid + hidden_grid, 256, 0, stream>>>(*c, t, q, weight_grid);
     }
-    if (d->grad_x != nullptr) {
+    const uint32_t bias_grid =
+        d->grad_bias != nullptr ? static_cast<uint32_t>(tiles_of(c->vocab, kWave)) : 0;
+    const uint32_t hidden_grid = d->grad_x != nullptr ? chunk_grid : 0;
+    if (bias_grid + hidden_grid > 0) {
         auto *out = static_cast<uint16_t *>(d->grad_x);
         if (c->fp16)
-            join_hidden_kernel<true>
-                <<<chunk_grid, 256, 0, stream>>>(*c, t, d->splits, d->hidden_parts, out);
+            join_gradients_kernel<true><<<bias_grid + hidden_grid, 256, 0, stream>>>(
+                *c, t, d->splits, d->hidden_parts, out, kLogitRows, d->bias_parts, d->grad_bias,
+                bias_grid);
         else
-            join_hidden_kernel<false>
-                <<<chunk_grid, 256, 0, stream>>>(*c, t, d->splits, d->hidden_parts, out);
+            join_gradients_kernel<false><<<bias_grid + hidden_grid, 256, 0, stream>>>(
+                *c, t, d->splits, d->hidden_parts, out, kLogitRows, d->bias_parts, d->grad_bias,
+                bias_grid);
     }
-    if (d->grad_bias != nullptr)
-        join_bias_kernel<<<tiles_of(c->vocab, 256), 256, 0, stream>>>(
-            *c, t, kLogitRows, d->bias_parts, d->grad_bias);
     return static_cast<int32_t>(hipGetLastError());
 }

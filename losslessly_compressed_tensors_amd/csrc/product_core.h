@@ -143,11 +143,11 @@ __device__ __forceinline__ void loads_barrier() {
     asm volatile("" ::: "memory");
 }
 
-template <bool kHalf, Lie kLieA, Lie kLieB, int kM_, int kN_, int kWavesM, int kWavesN, int kStep,
+template <bool kHalf, Lie kLieA, Lie kLieB, int kM_, int kN_, int kWavesM_, int kWavesN, int kStep,
           int kStages_>
 struct Product {
-    static constexpr int kM = kM_, kN = kN_, kThreads = kWave * kWavesM * kWavesN;
-    static constexpr int kStages = kStages_;
+    static constexpr int kM = kM_, kN = kN_, kThreads = kWave * kWavesM_ * kWavesN;
+    static constexpr int kStages = kStages_, kWavesM = kWavesM_;
     using A = Operand<kLieA, kM, kStep, kThreads>;
     using B = Operand<kLieB, kN, kStep, kThreads>;
     static constexpr int kWaveM = kM / kWavesM, kWaveN = kN / kWavesN;

@@ -55,27 +55,52 @@ def _cross_entropy(x: Tensor, weight: Tensor, bias, targets: Tensor, softcap: fl
         softcap)
 
 
+class _Workspace:
+    """One allocation for several working arrays, each at a multiple of 256 bytes."""
+
+    def __init__(self, *sizes: int):
+        self.offsets, total = [], 0
+        for size in sizes:
+            self.offsets.append(total)
+            total += -(-size // 256) * 256
+        self.bytes = total
+
+    def on(self, like: Tensor) -> list:
+        """The arrays' addresses; the allocation, which has to live until they are used on
+        the stream, comes last."""
+        memory = torch.empty(self.bytes, dtype=torch.uint8, device=like.device)
+        base = memory.data_ptr()
+        return [base + o for o in self.offsets] + [memory]
+
+
+_FEW_TOKENS = 32        # as many as one tile of the kernel for few tokens has
+
+
 def cross_entropy_forward(x: Tensor, weight: Tensor, bias, targets: Tensor, softcap: float,
                           ignore_index: int, reduction: str):
-    """``(losses, lse, total)`` of [token, channel] and [vocabulary, channel] matrices,
-    an FP32 bias or None and contiguous targets; ``total`` is the losses' sum or mean,
-    None for the reduction "none"."""
+    """``(out, stats)`` of [token, channel] and [vocabulary, channel] matrices, an FP32 bias
+    or None and contiguous targets.  ``out``: the losses or, unless the reduction is
+    "none", their sum or mean; ``stats`` [2, token]: the losses and their softmax's
+    statistics for :func:`cross_entropy_backward`."""
     _check_unrecorded(x, weight, bias)
     x, weight = _whole_rows(x), _whole_rows(weight)
     tokens, dim = x.shape
-    losses = x.new_empty(tokens, dtype=torch.float32)
-    lse = torch.empty_like(losses)
-    total = None if reduction == "none" else x.new_empty((), dtype=torch.float32)
-    floats = 4 * tokens * -(-weight.shape[0] // 128)
-    parts = x.new_empty(floats, dtype=torch.float32)
-    index = x.new_empty(1 + 2 * tokens, dtype=torch.int32)
-    gathered = x.new_empty(tokens * dim)
+    stats = torch.empty((2, tokens), dtype=torch.float32, device=x.device)
+    total = None
+    if reduction != "none":
+        total = torch.empty((), dtype=torch.float32, device=x.device)
+    floats = (8 if tokens <= _FEW_TOKENS else 4) * tokens * -(-weight.shape[0] // 128)
+    # Few tokens cost less than finding out which of them count.
+    ints = 1 + 2 * tokens if tokens > 256 else 0
+    parts, index, gathered, memory = _Workspace(4 * floats, 4 * ints,
+                                                2 * tokens * dim if ints else 0).on(x)
+    losses = stats.data_ptr()
     _launch("lct_cross_entropy_forward", x.get_device(),
-            _cross_entropy(x, weight, bias, targets, softcap, ignore_index), index.data_ptr(),
-            index.numel(), gathered.data_ptr(), gathered.numel(), parts.data_ptr(), floats,
-            lse.data_ptr(), losses.data_ptr(), None if total is None else total.data_ptr(),
+            _cross_entropy(x, weight, bias, targets, softcap, ignore_index),
+            index if ints else None, ints, gathered, tokens * dim if ints else 0, parts, floats,
+            losses + 4 * tokens, losses, None if total is None else total.data_ptr(),
             reduction == "mean")
-    return losses, lse, total
+    return (stats[0] if total is None else total), stats
 
 
 def _last_end(lengths) -> float:
@@ -110,8 +135,8 @@ def vocabulary_pieces(tokens: int, vocab: int, dim: int) -> tuple:
 
 
 def cross_entropy_backward(grad: Tensor, x: Tensor, weight: Tensor, bias, targets: Tensor,
-                           losses: Tensor, lse: Tensor, softcap: float, ignore_index: int,
-                           reduction: str, needed: tuple):
+                           stats: Tensor, softcap: float, ignore_index: int, reduction: str,
+                           needed: tuple):
     """``(grad_x, grad_weight, grad_bias)``, None where not ``needed``; the bias's in
     FP32."""
     _check_unrecorded(grad, x, weight, bias)
@@ -124,28 +149,24 @@ def cross_entropy_backward(grad: Tensor, x: Tensor, weight: Tensor, bias, target
     grad_x = x.new_empty(tokens, width) if need_x else None
     grad_weight = x.new_empty(vocab, width) if need_weight else None
     grad_bias = x.new_empty(vocab, dtype=torch.float32) if need_bias else None
-    index = x.new_empty(1 + 2 * tokens, dtype=torch.int32)
-    values = x.new_empty(1 + 3 * tokens, dtype=torch.float32)
-    gathered = x.new_empty(tokens * width)
-    dz = (x.new_empty(min(piece, vocab) * (-(-tokens // 8) * 8)) if need_x or need_weight
-          else None)
-    hidden = x.new_empty(splits * tokens * width, dtype=torch.float32) if need_x else None
-    columns = (x.new_empty(2 * -(-tokens // 128) * vocab, dtype=torch.float32) if need_bias
-               else None)
+    ints, floats, halves = 1 + 2 * tokens, 1 + 3 * tokens, tokens * width
+    dz_size = min(piece, vocab) * _up8(tokens) if need_x or need_weight else 0
+    hidden_floats = splits * tokens * width if need_x else 0
+    bias_floats = 2 * -(-tokens // 128) * vocab if need_bias else 0
+    index, values, gathered, dz, hidden, columns, memory = _Workspace(
+        4 * ints, 4 * floats, 2 * halves, 2 * dz_size, 4 * hidden_floats, 4 * bias_floats).on(x)
 
     def at(t):
         return 0 if t is None else t.data_ptr()
 
-    def size(t):
-        return 0 if t is None else t.numel()
-
+    losses = stats.data_ptr()
     _launch("lct_cross_entropy_backward", x.get_device(),
             _cross_entropy(x, weight, bias, targets, softcap, ignore_index),
             hip.CROSS_ENTROPY_GRADIENTS.pack(
-                grad.data_ptr(), lse.data_ptr(), losses.data_ptr(), at(grad_x), at(grad_weight),
-                at(grad_bias), at(index), at(values), at(gathered), at(dz), at(hidden),
-                at(columns), size(index), size(values), size(gathered), size(dz), size(hidden),
-                size(columns), reduction == "none", reduction == "mean", piece, splits))
+                grad.data_ptr(), losses + 4 * tokens, losses, at(grad_x), at(grad_weight),
+                at(grad_bias), index, values, gathered, dz, hidden, columns, ints, floats, halves,
+                dz_size, hidden_floats, bias_floats, reduction == "none", reduction == "mean",
+                piece, splits))
     if width != dim:
         grad_x, grad_weight = (None if g is None else g[:, :dim].contiguous()
                                for g in (grad_x, grad_weight))
