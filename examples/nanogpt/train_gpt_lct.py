@@ -18,7 +18,10 @@ tokens per second and peak device memory of the training step.  With ``--window`
 the blocks' rotary embedding and attention are the kernels of
 ``components/attention.py`` (a sliding window with ``--sinks`` first tokens that
 stay visible), and with ``--dropout`` each residual addition drops what it adds
-(``components/dropout.py``); the reference has neither.
+(``components/dropout.py``).  With ``--fused-head`` the head's loss is computed without
+its logits (``components/losses.py``), and with ``--fused-muon`` the updates are
+orthogonalised by the kernels of ``components/orthogonal.py``.  The reference has none
+of these.
 """
 from __future__ import annotations
 
@@ -44,8 +47,8 @@ from losslessly_compressed_tensors_amd.components.attention import (
 )
 from losslessly_compressed_tensors_amd.components.dropout import dropout_add
 from losslessly_compressed_tensors_amd.components.layers import (
-    Embedding, FlashAttention, Linear, RMSLinear, RMSNormFunction, Relu2Linear, WindowAttention,
-    compress_weight, dense_weight, flush_saved, named_trainable_tensors, prefetch_saved,
+    Embedding, FlashAttention, Linear, RMSLinear, RMSLinearCrossEntropy, RMSNormFunction,
+    Relu2Linear, WindowAttention, compress_weight, dense_weight, flush_saved, named_trainable_tensors, prefetch_saved,
     prefetch_weights, queued_saved, rms_norm_qkv,
 )
 from losslessly_compressed_tensors_amd.components.sparse_utils import SparseAdamW, SparseMuon
@@ -284,8 +287,9 @@ class GPT(nn.Module):
     def __init__(self, vocab_size=VOCAB_SIZE, num_layers=NUM_LAYERS, model_dim=MODEL_DIM,
                  head_dim=HEAD_DIM, compress_activations=False,
                  min_compress_elements=MIN_COMPRESS_ELEMENTS, window=None, sinks=0, dropout=0.0,
-                 dropout_seed=0):
+                 dropout_seed=0, fused_head=False):
         super().__init__()
+        self.fused_head = fused_head
         self.embed = nn.Embedding(vocab_size, model_dim, dtype=torch.bfloat16)
         self.blocks = nn.ModuleList([Block(model_dim, head_dim, compress_activations,
                                            min_compress_elements, window, sinks, dropout)
@@ -323,6 +327,10 @@ class GPT(nn.Module):
         for block in self.blocks:
             x = block(x, self.dropout_seed, self.dropout_offset)
             self.dropout_offset += 2
+        if self.fused_head:
+            return RMSLinearCrossEntropy.apply(
+                x, self.proj.weight, self.norm2.gains, self.proj.bias, targets,
+                self.tensor_buffer, compressed, act_dist, self.min_compress_elements, SOFTCAP)
         return SoftcapCrossEntropy.head_loss(x, targets, self.proj.weight, self.norm2.gains,
                                              self.proj.bias, self.tensor_buffer,
                                              self.compress_activations, self.min_compress_elements)
@@ -348,7 +356,7 @@ def initialize_model(model):
                 raise ValueError(f"Uninitialized parameter: {name}")
 
 
-def make_optimizers(model, compressed=False):
+def make_optimizers(model, compressed=False, fused_muon=False):
     """AdamW for the embedding, the head and the vectors; Muon for the block
     matrices (train_gpt_lct.py:333-348)."""
     named = dict(model.named_trainable_tensors())
@@ -360,7 +368,7 @@ def make_optimizers(model, compressed=False):
     muon = SparseMuon([p for name, p in named.items() if name.startswith("blocks.") and p.ndim >= 2],
                       lr=0.035, weight_decay=0.025, compressed=compressed,
                       buffer=model.tensor_buffer, distribution=momentum_dist,
-                      zero_first_step=True, ns_iters=12)
+                      zero_first_step=True, ns_iters=12, fused=fused_muon)
     parameters = [p for g in adam.param_groups for p in g["params"]] + muon.params
     assert len(parameters) == len(named)
     assert {id(p) for p in parameters} == {id(p) for p in named.values()}
@@ -370,18 +378,18 @@ def make_optimizers(model, compressed=False):
 def build(device, *, compress_weights, compress_activations, compress_optimizer,
           use_buffer=True, vocab_size=VOCAB_SIZE, num_layers=NUM_LAYERS, model_dim=MODEL_DIM,
           head_dim=HEAD_DIM, buffer_mib=BUFFER_SIZE_MIB, seed=0, window=None, sinks=0,
-          dropout=0.0):
+          dropout=0.0, fused_head=False, fused_muon=False):
     """Model and optimizers for one mode, initialised from ``seed``."""
     torch.manual_seed(seed)
     model = GPT(vocab_size, num_layers, model_dim, head_dim,
                 compress_activations=compress_activations, window=window, sinks=sinks,
-                dropout=dropout, dropout_seed=seed).to(device)
+                dropout=dropout, dropout_seed=seed, fused_head=fused_head).to(device)
     initialize_model(model)
     if use_buffer and (compress_weights or compress_activations or compress_optimizer):
         model.set_tensor_buffer(TensorBuffer(buffer_mib * 2 ** 20, device=device))
     if compress_weights:
         model.compress_weights()
-    return model, make_optimizers(model, compressed=compress_optimizer)
+    return model, make_optimizers(model, compressed=compress_optimizer, fused_muon=fused_muon)
 
 
 def random_tokens(batch, seq_len, device, seed, token_ids=TOKEN_IDS):
@@ -464,6 +472,10 @@ def main():
     parser.add_argument("--sinks", type=int, default=0,
                         help="first tokens that stay visible under a window")
     parser.add_argument("--dropout", type=float, default=0.0)
+    parser.add_argument("--fused-head", action="store_true",
+                        help="the loss without its logits")
+    parser.add_argument("--fused-muon", action="store_true",
+                        help="the updates orthogonalised by kernels of their own")
     args = parser.parse_args()
     if not torch.cuda.is_available():
         raise RuntimeError("training needs a GPU")
@@ -473,7 +485,8 @@ def main():
     for mode in modes:
         result = measure(device, compressed=mode == "lct", steps=args.steps, warmup=args.warmup,
                          batch=args.batch, num_layers=args.layers, window=args.window,
-                         sinks=args.sinks, dropout=args.dropout)
+                         sinks=args.sinks, dropout=args.dropout, fused_head=args.fused_head,
+                         fused_muon=args.fused_muon)
         print(json.dumps({"mode": mode, **result}), flush=True)
 
 

@@ -25,14 +25,16 @@ from ..LCTensor import LCTTensor
 from ..codec.decode import decode_batch
 from ..kernels import attention as attention_kernels
 from ..kernels import fused
+from ..kernels import products
 from ..operations import compress, compress_batch, decompress
 from .attention import check_attention
 from .dist_configs import act_dist, act_relu_dist, weight_dist
+from .losses import check_cross_entropy
 from .ops import rms_norm, rms_norm_backward
 
 __all__ = [
     "dense_weight", "prefetch_weights", "RMSLinear", "rms_norm_qkv", "RMSNormFunction",
-    "Relu2Linear", "FlashAttention", "WindowAttention", "compress_weight", "Linear", "Embedding",
+    "RMSLinearCrossEntropy", "Relu2Linear", "FlashAttention", "WindowAttention", "compress_weight", "Linear", "Embedding",
     "named_trainable_tensors", "flush_saved", "queued_saved", "prefetch_saved",
     "batch_saved_compression",
 ]
@@ -219,6 +221,48 @@ class RMSLinear(torch.autograd.Function):
         grad_weight = g.T @ normalized
         grad_bias = _bias_grad(g, ctx.bias_dtype)
         return grad_x, grad_weight, grad_gain, grad_bias, None, None, None, None, None
+
+
+class RMSLinearCrossEntropy(torch.autograd.Function):
+    """:class:`RMSLinear` and the cross entropy of its output, whose logits are never kept
+    (``components/losses.py``'s ``linear_cross_entropy``; the reference's head keeps those
+    of a chunk of tokens, ``examples/nanogpt/train_gpt_lct.py:88-140``); saves the norm
+    input.  Returns the FP32 sum, mean or per-token losses."""
+
+    @staticmethod
+    def forward(ctx, x, weight, norm_weight, bias, targets, buffer=None, compressed=False,
+                distribution=None, min_elements=65536, softcap=None, ignore_index=-100,
+                reduction="sum"):
+        W = dense_weight(weight)
+        softcap, ignore_index = check_cross_entropy(x, W, targets, bias, softcap, ignore_index,
+                                                    reduction)
+        if targets.numel() == 0:
+            raise ValueError("the head needs a token")
+        normalized, rstd = _norm(x, norm_weight)
+        flat = targets.reshape(-1).contiguous()
+        out, stats = products.cross_entropy_forward(
+            normalized.reshape(-1, x.shape[-1]), W, bias.float().contiguous(), flat, softcap,
+            ignore_index, reduction)
+        del normalized
+        ctx.saved = _SavedActivation(x, compressed and x.numel() >= min_elements,
+                                     distribution or act_dist, buffer)
+        ctx.save_for_backward(norm_weight, rstd, weight, bias, flat, stats)
+        ctx.how = softcap, ignore_index, reduction
+        return out.clone().view(targets.shape) if reduction == "none" else out
+
+    @staticmethod
+    def backward(ctx, grad):
+        norm_weight, rstd, weight, bias, targets, stats = ctx.saved_tensors
+        x = ctx.saved.take()
+        ctx.saved = None
+        normalized, _ = _norm(x, norm_weight)
+        grad_normalized, grad_weight, grad_bias = products.cross_entropy_backward(
+            grad.contiguous(), normalized.reshape(-1, x.shape[-1]), dense_weight(weight),
+            bias.float().contiguous(), targets, stats, *ctx.how, (True, True, True))
+        grad_x, grad_gain, _ = _norm_backward(grad_normalized.reshape(x.shape), x, rstd,
+                                              norm_weight)
+        return (grad_x, grad_weight, grad_gain, grad_bias.to(bias.dtype), None, None, None, None,
+                None, None, None, None)
 
 
 class _RMSNormQKV(torch.autograd.Function):

@@ -26,7 +26,9 @@ How this build runs them on one MI355X:
   ones transposed to wide) and runs one batched Newton-Schulz per group: three
   batched GEMMs per iteration for the group instead of three per matrix.  A
   GPT-2-small step's 72 block matrices form two groups (48 of 768x768, 24 of
-  768x3072), so 12 iterations take 72 GEMM launches instead of 2592.
+  768x3072), so 12 iterations take 72 GEMM launches instead of 2592.  With
+  ``fused=True`` the iteration is ``components/orthogonal.py``'s kernels, whose
+  iterate is kept in 22 bits.
 * **Multi-tensor AdamW.**  Parameters with the same dtype and step count are
   updated together with ``torch._foreach_*`` operations.
 * **No host synchronisation.**  Scalars that the fused kernels read live on
@@ -50,6 +52,7 @@ from ..codec.decode import decode_batch
 from ..operations import a_compA_add_B
 from ..tensor_buffer import TensorBuffer
 from .dist_configs import momentum_dist, momentum_first_dist
+from .orthogonal import orthogonalize
 
 # Newton-Schulz polynomial p(s) = a s + b s^3 + c s^5 on the singular values:
 # p(1) = 1 and p'(1) = 0, so unit singular values attract quadratically.
@@ -236,7 +239,7 @@ class SparseMuon:
 
     def __init__(self, params: Iterable[LCTTensor | Tensor], lr=0.02, weight_decay=0, mu=0.95,
                  buffer: TensorBuffer | None = None, compressed=True, distribution=None,
-                 zero_first_step=False, ns_iters=5):
+                 zero_first_step=False, ns_iters=5, fused=False):
         self.params = list(params)
         if not all(isinstance(p, (LCTTensor, Tensor)) and p.ndim >= 2 for p in self.params):
             raise AssertionError("Muon requires matrix parameters")
@@ -245,6 +248,7 @@ class SparseMuon:
         self.buffer, self.compressed = buffer, compressed
         self.distribution = distribution or momentum_dist
         self.ns_iters = ns_iters
+        self.fused = fused       # orthogonalize's kernels in place of the library's products
         # The first step's momentum (1 - mu) g of a zero momentum is stored with
         # the half-zero codebook when the caller asks for it.
         self.first_step = zero_first_step
@@ -255,7 +259,7 @@ class SparseMuon:
     @torch.no_grad()
     def step(self):
         dist = momentum_first_dist if self.first_step else self.distribution
-        # Matrices grouped by wide shape: (rows, cols) with rows <= cols.
+        # Matrices grouped by wide shape: (rows, cols) with rows <= cols (fused: by shape).
         groups: dict[tuple, list[tuple[int, Tensor, bool]]] = {}
         active = [(index, param.grad) for index, param in enumerate(self.params)
                   if param.grad is not None]
@@ -267,7 +271,8 @@ class SparseMuon:
             momenta = self.momentums.check_out_many([i for i, _ in part], [g for _, g in part])
             for (index, grad), momentum in zip(part, momenta):
                 direction = _nesterov(grad, momentum, self.mu, nesterov=True)
-                tall = direction.size(-2) > direction.size(-1)
+                # (The kernels turn a tall matrix themselves.)
+                tall = direction.size(-2) > direction.size(-1) and not self.fused
                 wide = direction.transpose(-2, -1) if tall else direction
                 groups.setdefault(tuple(wide.shape), []).append((index, wide, tall))
             # The momenta go back (compressed, one launch for the 16) before
@@ -276,6 +281,11 @@ class SparseMuon:
             del momenta
         for shape, members in groups.items():
             stacked = torch.stack([wide.reshape(-1, *shape[-2:]) for _, wide, _ in members])
+            if self.fused:
+                polar = orthogonalize(stacked, self.ns_iters, scale=_aspect_scale(*shape[-2:]))
+                self._apply_many([self.params[index] for index, _, _ in members],
+                                 list(polar.view(len(members), *shape).unbind(0)))
+                continue
             polar = _orthogonalize_wide(stacked.reshape(-1, *shape[-2:]), self.ns_iters)
             polar = polar.reshape(len(members), *shape)
             params, updates = [], []
