@@ -255,10 +255,10 @@ __device__ __forceinline__ void wave_fence() {
     asm volatile("" ::: "memory");
 }
 
-// 16 bytes a lane of `lines` lines of `length` values (a multiple of 8): lane l's of access
-// i are those of slot 64 i + l, kChunks to a line.  What is past either end reads as
-// zeros and is not written.
-template <int kChunks>
+// 16 bytes a lane of a tile's kLines lines of kChunks pieces: lane l's of access i are those of
+// slot 64 i + l.  What is past the `lines` lines of `length` values (a multiple of 8) that
+// the matrix has from the tile on reads as zeros and is not written.
+template <int kLines, int kChunks>
 struct Lines {
     __amdgpu_buffer_rsrc_t rsrc;
     uint32_t pitch;      // bytes
@@ -267,8 +267,10 @@ struct Lines {
     __device__ __forceinline__ Lines(const uint16_t *base, int64_t stride, int32_t lines,
                                      int32_t length_)
         : pitch(static_cast<uint32_t>(stride) * 2u), length(length_) {
+        // (Of the tile alone: 32 bits hold its size.)
+        length = min(length, kChunks * 8);
         rsrc = make_rsrc(base, lines > 0 && length > 0
-                                   ? static_cast<uint32_t>(lines - 1) * pitch
+                                   ? static_cast<uint32_t>(min(lines, kLines) - 1) * pitch
                                          + static_cast<uint32_t>(length) * 2u
                                    : 0u);
     }
@@ -299,7 +301,7 @@ __device__ __forceinline__ void store_columns(uint16_t *out, int64_t stride, int
                                               int32_t rows, uint16_t *mine, Pair pair) {
     constexpr int kPitch = P::kWaveM + 8, kChunks = P::kWaveM / 8;
     const int lane = wave_lane();
-    const Lines<kChunks> lines(out, stride, columns, rows);
+    const Lines<P::kWaveN, kChunks> lines(out, stride, columns, rows);
     uint16_t *at = mine + (lane & 31) * kPitch + (lane >> 5) * 4;
 #pragma unroll
     for (int n = 0; n < P::kColumnTiles; ++n) {
@@ -329,7 +331,7 @@ __device__ __forceinline__ void load_columns(const uint16_t *from, int64_t strid
     constexpr int kPitch = P::kWaveM + 8, kChunks = P::kWaveM / 8;
     constexpr int kCount = 32 * kChunks / kWave;
     const int lane = wave_lane();
-    const Lines<kChunks> lines(from, stride, columns, rows);
+    const Lines<P::kWaveN, kChunks> lines(from, stride, columns, rows);
     const uint16_t *at = mine + (lane & 31) * kPitch + (lane >> 5) * 4;
 #pragma unroll
     for (int n = 0; n < P::kColumnTiles; ++n) {
@@ -362,7 +364,7 @@ __device__ __forceinline__ void store_rows(uint16_t *out, int64_t stride, int32_
     constexpr int kPitch = P::kWaveN + 8, kChunks = P::kWaveN / 8;
     static_assert(32 * kPitch <= kTurnValues<P>);
     const int lane = wave_lane();
-    const Lines<kChunks> lines(out, stride, rows, columns);
+    const Lines<P::kWaveM, kChunks> lines(out, stride, rows, columns);
     // Of two rows' values of two adjacent lanes: the even one takes the first row's, the
     // odd one the second's.
     const uint32_t select = lane & 1 ? 0x03020706u : 0x05040100u;

@@ -108,11 +108,11 @@ def _last_end(lengths) -> float:
     each as soon as one of the slots is free."""
     free = [0.0] * _SLOTS
     for count, length in lengths:
-        rounds, rest = divmod(count, _SLOTS)
+        rounds = max(0, count // _SLOTS - 2)
         if rounds:
-            # As many for each slot: they stay as far apart.
+            # As many for each slot, about: they stay as far apart.
             free = [t + rounds * length for t in free]
-        for _ in range(rest):
+        for _ in range(count - rounds * _SLOTS):
             heapreplace(free, free[0] + length)
     return max(free)
 

@@ -127,3 +127,10 @@ def polar_off(steps) -> float:
     grow faster than X.  A half more, since small matrices have few roundings."""
     step = (10.0 / 3) ** 0.5 * 2.0 ** -11
     return 1.5 * ((2.0 ** -8) ** 2 / 3 + steps * step ** 2) ** 0.5
+
+
+def polar_floor(steps, values) -> float:
+    """The same in absolute terms, of a matrix so small (against eps) that X's numbers are
+    FP16's smallest: X times 2^10 is held to half of their spacing, 2^-25, and a step at most
+    doubles what the steps before have left: 2^-35 (1 + 2 + .. + 2^steps) a value."""
+    return values ** 0.5 * 2.0 ** (steps + 1 - 35)

@@ -7,7 +7,7 @@ import torch
 
 from gpu_util import require_gpu
 from losslessly_compressed_tensors_amd.components.orthogonal import orthogonalize
-from product_oracle import polar, polar_off
+from product_oracle import polar, polar_floor, polar_off
 
 pytestmark = pytest.mark.gpu
 BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
@@ -36,7 +36,8 @@ def _assert_polar(got, g, steps, scale=1.0):
     assert got.dtype == BF16 and got.shape == g.shape and got.is_contiguous()
     exact = polar(g.cpu(), steps, scale)
     off = (got.cpu().double() - exact).square().sum((-2, -1)).sqrt()
-    bound = polar_off(steps) * exact.square().sum((-2, -1)).sqrt()
+    bound = (polar_off(steps) * exact.square().sum((-2, -1)).sqrt()
+             + abs(scale) * polar_floor(steps, g.shape[-1] * g.shape[-2]))
     assert (off <= bound).all(), f"{(off / bound).max():.3g} times the bound"
 
 
@@ -63,3 +64,128 @@ def test_steps_and_spectra(kind, steps):
 def test_batches(shape):
     g = _matrix(shape).to(BF16)
     _assert_polar(orthogonalize(g.cuda(), 5), g, 5)
+
+
+def _views(g):
+    """The same matrices in other storages."""
+    count, rows, cols = g.shape
+    yield g
+    yield g.mT.contiguous().mT
+    wide = torch.full((count, rows, 2 * cols + 3), 7.0, dtype=g.dtype, device=g.device)
+    wide[:, :, 3:cols + 3] = g
+    yield wide[:, :, 3:cols + 3]
+    steps = torch.full((count, rows, 2 * cols), 7.0, dtype=g.dtype, device=g.device)
+    steps[:, :, ::2] = g
+    yield steps[:, :, ::2]
+    yield g.flip(0).flip(0)
+    by_matrix = g.permute(1, 2, 0).contiguous().permute(2, 0, 1)
+    yield by_matrix
+
+
+@pytest.mark.parametrize("shape", [(3, 40, 72), (2, 130, 67), (1, 200, 200)])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_strides(shape, dtype):
+    g = _matrix(shape).to(dtype).cuda()
+    base = orthogonalize(g, 5)
+    _assert_polar(base, g, 5)
+    for view in _views(g):
+        assert torch.equal(orthogonalize(view, 5), base)
+
+
+def test_wide_and_tall_are_each_others_transposes():
+    for shape in ((64, 136), (200, 512), (1000, 1537)):
+        g = _matrix(shape).to(BF16).cuda()
+        assert torch.equal(orthogonalize(g.mT.contiguous(), 5).mT.contiguous(),
+                           orthogonalize(g, 5))
+
+
+@pytest.mark.parametrize("size", [1e-30, 1e-6, 1.0, 1e30])
+def test_any_size(size):
+    """eps counts below 1e-6; squares do not overflow."""
+    for dtype in (BF16, FP32):
+        g = (_matrix((72, 136)) * size).to(dtype)
+        _assert_polar(orthogonalize(g.cuda(), 5), g, 5)
+
+
+def test_nothing_and_zeros():
+    assert orthogonalize(torch.zeros(0, 5, 7, device="cuda")).shape == (0, 5, 7)
+    assert orthogonalize(torch.zeros(5, 0, device="cuda")).shape == (5, 0)
+    out = orthogonalize(torch.zeros(3, 40, 24, device="cuda"), 12)
+    assert out.shape == (3, 40, 24) and not out.any()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_one_matrix_does_not_reach_another(bad):
+    g = _matrix((3, 130, 200)).to(FP32)
+    clean = orthogonalize(g.cuda(), 5)
+    g[1, 7, 9] = bad
+    out = orthogonalize(g.cuda(), 5)
+    assert out[1].isnan().any()
+    assert torch.equal(out[0], clean[0]) and torch.equal(out[2], clean[2])
+
+
+# Each tile of the products and one and two steps at a time: by the number of 128 x 128 tiles.
+RULES = [(1, 300, 300), (40, 200, 256), (50, 256, 520), (1, 1100, 1100), (90, 300, 400),
+         (210, 256, 384), (14, 1024, 1152), (2, 2048, 3200)]
+
+
+@pytest.mark.parametrize("count,rows,cols", RULES)
+def test_every_tile(count, rows, cols):
+    g = _matrix((1, rows, cols), "falling").to(BF16).cuda().expand(count, rows, cols).clone()
+    signs = torch.where(torch.arange(count, device="cuda") % 2 == 0, 1.0, -1.0).to(BF16)
+    g *= signs[:, None, None]
+    for steps in (4, 5):
+        out = orthogonalize(g, steps)
+        exact = polar(g[0].cpu(), steps)
+        # Equal matrices give equal results; the negatives' differ from them in roundings (the
+        # matrix instructions' are not symmetric about zero).
+        for first in (0, 1)[:count]:
+            off = float((out[first].cpu().double() * float(signs[first]) - exact).norm()
+                        / exact.norm())
+            assert off <= polar_off(steps)
+            assert torch.equal(out[first::2], out[first:first + 1].expand_as(out[first::2]))
+
+
+def test_streams_and_replays():
+    g = _matrix((4, 200, 136)).to(BF16).cuda()
+    eager = orthogonalize(g, 5)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out = orthogonalize(g, 5)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert torch.equal(out, eager)
+    static = g.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = orthogonalize(static, 5)
+    for seed in (1, 2, 3):
+        static.copy_(_matrix((4, 200, 136), seed=seed))
+        graph.replay()
+        expected = orthogonalize(static, 5)
+        torch.cuda.synchronize()
+        assert torch.equal(out, expected)
+
+
+def test_results_do_not_depend_on_the_run():
+    g = _matrix((5, 333, 517)).to(BF16).cuda()
+    first = orthogonalize(g, 12)
+    assert all(torch.equal(first, orthogonalize(g, 12)) for _ in range(3))
+
+
+def test_refusals():
+    g = torch.randn(4, 6, device="cuda")
+    for args, error in (((g.double(),), TypeError), ((g.cpu(),), ValueError),
+                        ((g.to(torch.complex64),), TypeError), ((g, -1), ValueError),
+                        ((g, 2.0), TypeError), ((g, 1001), ValueError)):
+        with pytest.raises(error):
+            orthogonalize(*args)
+    with pytest.raises(ValueError, match="scale"):
+        orthogonalize(g, 5, scale=float("nan"))
+    with pytest.raises(ValueError, match="at most"):
+        orthogonalize(torch.zeros(1, (1 << 16) + 1, device="cuda"))
+    with pytest.raises(RuntimeError, match="recorded"):
+        torch.jit.trace(lambda a: orthogonalize(a), g)
+    # A result has no gradient, whoever asks.
+    assert not orthogonalize(g.requires_grad_()).requires_grad
