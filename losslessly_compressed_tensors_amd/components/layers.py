@@ -255,14 +255,20 @@ class RMSLinearCrossEntropy(torch.autograd.Function):
         norm_weight, rstd, weight, bias, targets, stats = ctx.saved_tensors
         x = ctx.saved.take()
         ctx.saved = None
+        need = ctx.needs_input_grad
         normalized, _ = _norm(x, norm_weight)
         grad_normalized, grad_weight, grad_bias = products.cross_entropy_backward(
             grad.contiguous(), normalized.reshape(-1, x.shape[-1]), dense_weight(weight),
-            bias.float().contiguous(), targets, stats, *ctx.how, (True, True, True))
-        grad_x, grad_gain, _ = _norm_backward(grad_normalized.reshape(x.shape), x, rstd,
-                                              norm_weight)
-        return (grad_x, grad_weight, grad_gain, grad_bias.to(bias.dtype), None, None, None, None,
-                None, None, None, None)
+            bias.float().contiguous(), targets, stats, *ctx.how,
+            (need[0] or need[2], need[1], need[3]))
+        grad_x = grad_gain = None
+        if grad_normalized is not None:
+            grad_x, grad_gain, _ = _norm_backward(grad_normalized.reshape(x.shape), x, rstd,
+                                                  norm_weight)
+        if grad_bias is not None:
+            grad_bias = grad_bias.to(bias.dtype)
+        return (grad_x, grad_weight, grad_gain, grad_bias, None, None, None, None, None, None,
+                None, None)
 
 
 class _RMSNormQKV(torch.autograd.Function):
