@@ -930,6 +930,7 @@ int32_t lct_dropout(const void *x, const void *residual, void *out, int64_t n, i
 #define LCT_MAX_CROSS_ENTROPY_VOCAB (1 << 24)
 #define LCT_MAX_CROSS_ENTROPY_DIM (1 << 16)
 #define LCT_MAX_CROSS_ENTROPY_SPLITS 16
+#define LCT_CROSS_ENTROPY_EXACT_TOKENS 128
 typedef struct {
     const void *x, *weight;
     const float *bias;
@@ -955,9 +956,10 @@ int32_t lct_cross_entropy_forward(const lct_cross_entropy *c, int32_t *index, in
  * that are NULL are not computed.  `piece`: how much of the vocabulary is worked on at a
  * time (a multiple of 128); `splits`: into how many parts its sum for grad_x is divided.
  * Working arrays: index (1 + 2 * tokens), values (1 + 3 * tokens), gathered (tokens * dim
- * 16-bit values), dz (min(piece, vocab) * (tokens rounded up to 8) 16-bit values),
- * hidden_parts (splits * tokens * dim), bias_parts (2 * ceil(tokens / 128) * vocab); those
- * of 16 bits and hidden_parts 16-byte aligned. */
+ * 16-bit values), dz (min(piece, vocab) * (tokens rounded up to 8) 16-bit values,
+ * twice that for up to LCT_CROSS_ENTROPY_EXACT_TOKENS), hidden_parts (splits * tokens *
+ * dim), bias_parts (2 * ceil(tokens / 128) * vocab); those of 16 bits and hidden_parts
+ * 16-byte aligned. */
 typedef struct {
     const float *grad, *lse, *losses;
     void *grad_x, *grad_weight;

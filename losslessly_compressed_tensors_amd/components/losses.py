@@ -109,7 +109,7 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, targets: Tensor, bias: Tenso
     No logits are kept: forward needs 16 bytes per token and 256 of the vocabulary,
     backward their gradient in 16 bits for up to 256 MiB of the vocabulary at a time.
     Logits, softmax and sums are FP32; the logits' gradients are rounded to 16 bits for
-    their products with ``weight`` and ``x``."""
+    their products with ``weight`` and ``x`` (of up to 128 tokens, kept in two numbers)."""
     softcap, ignore_index = check_cross_entropy(x, weight, targets, bias, softcap, ignore_index,
                                                 reduction)
     shape = targets.shape

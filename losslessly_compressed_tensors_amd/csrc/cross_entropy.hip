@@ -7,6 +7,9 @@
 //     loss = log(sum_v exp(l_v)) - l_t = log(1 + sum_{v != t} exp(l_v - l_t)),
 //     dz_v = g (exp(l_v) / sum - [v = t]) (1 + (z / s)^2)^(-3/2),
 //     dx = dz W,  dW = dz^T x,  dbias = the columns' sums of dz.
+// dz is rounded to 16 bits for its products, as far off as their results' own rounding.  Of
+// up to 128 tokens, whose products wait for memory in any case, what the rounding leaves
+// is multiplied too: there a few large values carry the results.
 // The second form of the loss keeps its precision where the target is likely:
 // the target is left out of the sums, and its own gradient is exp(-loss) - 1.
 //
@@ -477,7 +480,7 @@ __global__ __launch_bounds__(kPrepareThreads) void total_kernel(lct_cross_entrop
 template <class P, bool kHalf, bool kCap, bool kBias>
 __global__ __launch_bounds__(P::kThreads, 2) void gradient_kernel(
     lct_cross_entropy c, Counted t, int32_t first_vocab, int32_t piece, int32_t vocab_tiles,
-    int32_t token_tiles, uint16_t *dz, int64_t dz_stride, float *bias_parts) {
+    int32_t token_tiles, uint16_t *dz, uint16_t *dz_rest, int64_t dz_stride, float *bias_parts) {
     LCT_PRODUCT_STAGES(P);
     const int32_t count = *t.count;
     const int64_t item = xcd_item(int64_t{vocab_tiles} * token_tiles, blockIdx.x);
@@ -603,17 +606,25 @@ __global__ __launch_bounds__(P::kThreads, 2) void gradient_kernel(
     if (dz == nullptr) return;
     const int32_t column = vocab_tile * P::kN + p.first_column();
     const int32_t row = token_tile * P::kM + p.first_row();
-    store_columns<P>(dz + column * dz_stride + row, dz_stride, piece - column,
-                     static_cast<int32_t>(dz_stride) - row, turn_values<P>(stage0, stage1, stage2, stage3),
-                     [&](int m, int n, int r) {
-                         return Element<kHalf>::round_pair(p.sum[m][n][r], p.sum[m][n][r + 1]);
-                     });
+    using E = Element<kHalf>;
+    uint16_t *const mine = turn_values<P>(stage0, stage1, stage2, stage3);
+    const int64_t at = column * dz_stride + row;
+    const int32_t rows = static_cast<int32_t>(dz_stride) - row;
+    store_columns<P>(dz + at, dz_stride, piece - column, rows, mine, [&](int m, int n, int r) {
+        return E::round_pair(p.sum[m][n][r], p.sum[m][n][r + 1]);
+    });
+    if (dz_rest == nullptr) return;
+    store_columns<P>(dz_rest + at, dz_stride, piece - column, rows, mine, [&](int m, int n, int r) {
+        const float a = p.sum[m][n][r], b = p.sum[m][n][r + 1];
+        const uint32_t pair = E::round_pair(a, b);
+        return E::round_pair(a - E::low(pair), b - E::high(pair));
+    });
 }
 
 // What both products of a piece with dz need.
 struct PieceProducts {
     int32_t first_vocab, piece, splits, dim_tiles, token_tiles, vocab_tiles;
-    const uint16_t *dz;
+    const uint16_t *dz, *dz_rest;     // dz_rest: what dz's rounding leaves, or NULL
     int64_t dz_stride;
     float *hidden_parts;
     uint16_t *grad_weight;
@@ -621,7 +632,7 @@ struct PieceProducts {
 
 // dx of a piece of the vocabulary, or of one of its parts: 256 channels (rows) by 128
 // tokens (columns), added to the earlier pieces' in FP32.
-template <bool kHalf>
+template <bool kHalf, bool kExact>
 __device__ __forceinline__ void hidden_gradient(const lct_cross_entropy &c, int32_t count,
                                                 const PieceProducts &q, int64_t item,
                                                 uint16_t *stage0, uint16_t *stage1,
@@ -637,11 +648,16 @@ __device__ __forceinline__ void hidden_gradient(const lct_cross_entropy &c, int3
     typename P::B b;
     a.prepare(static_cast<const uint16_t *>(c.weight) + (q.first_vocab + begin) * c.weight_stride,
               c.weight_stride, int64_t{dim_tile} * P::kM, c.dim);
-    b.prepare(q.dz + begin * q.dz_stride, q.dz_stride, int64_t{token_tile} * P::kN,
-              (int64_t{count} + 7) / 8 * 8);
+    const int64_t tokens = (int64_t{count} + 7) / 8 * 8;
+    b.prepare(q.dz + begin * q.dz_stride, q.dz_stride, int64_t{token_tile} * P::kN, tokens);
     P p;
     p.begin();
     p.run(a, b, end - begin, stage0, stage1, stage2, stage3);
+    if constexpr (kExact) {
+        b.prepare(q.dz_rest + begin * q.dz_stride, q.dz_stride, int64_t{token_tile} * P::kN,
+                  tokens);
+        p.run(a, b, end - begin, stage0, stage1, stage2, stage3);
+    }
 
     const int lane = wave_lane();
 #pragma unroll
@@ -665,7 +681,7 @@ __device__ __forceinline__ void hidden_gradient(const lct_cross_entropy &c, int3
 }
 
 // dW of a piece: 256 channels (rows) by 128 of the vocabulary (columns).
-template <bool kHalf>
+template <bool kHalf, bool kExact>
 __device__ __forceinline__ void weight_gradient(const lct_cross_entropy &c, const Counted &t,
                                                 int32_t count, const PieceProducts &q,
                                                 int64_t item, uint16_t *stage0, uint16_t *stage1,
@@ -683,6 +699,10 @@ __device__ __forceinline__ void weight_gradient(const lct_cross_entropy &c, cons
     p.begin();
     // Tokens past the last: zeros of dz (up to 7) against zeros of x.
     p.run(a, b, count, stage0, stage1, stage2, stage3);
+    if constexpr (kExact) {
+        b.prepare(q.dz_rest, q.dz_stride, int64_t{vocab_tile} * P::kN, q.piece);
+        p.run(a, b, count, stage0, stage1, stage2, stage3);
+    }
 
     const float scale = *t.scale;
     const int32_t column = vocab_tile * P::kN + p.first_column();
@@ -696,7 +716,7 @@ __device__ __forceinline__ void weight_gradient(const lct_cross_entropy &c, cons
 }
 
 // Both, one launch: neither has as many tiles as fill the compute units evenly.
-template <bool kHalf>
+template <bool kHalf, bool kExact>
 __global__ __launch_bounds__(256, 2) void products_kernel(lct_cross_entropy c, Counted t,
                                                           PieceProducts q, uint32_t weight_grid) {
     using P = HiddenProduct<kHalf>;
@@ -708,12 +728,12 @@ __global__ __launch_bounds__(256, 2) void products_kernel(lct_cross_entropy c, C
         const int64_t items = int64_t{q.dim_tiles} * q.vocab_tiles;
         const int64_t item = xcd_item(items, blockIdx.x);
         if (item < items)
-            weight_gradient<kHalf>(c, t, count, q, item, stage0, stage1, stage2, stage3);
+            weight_gradient<kHalf, kExact>(c, t, count, q, item, stage0, stage1, stage2, stage3);
     } else {
         const int64_t items = int64_t{q.dim_tiles} * q.token_tiles * q.splits;
         const int64_t item = xcd_item(items, blockIdx.x - weight_grid);
         if (item < items)
-            hidden_gradient<kHalf>(c, count, q, item, stage0, stage1, stage2, stage3);
+            hidden_gradient<kHalf, kExact>(c, count, q, item, stage0, stage1, stage2, stage3);
     }
 }
 
@@ -901,11 +921,12 @@ extern "C" int32_t lct_cross_entropy_backward(const lct_cross_entropy *c,
         || (d->grad_bias != nullptr && (d->bias_parts == nullptr || c->bias == nullptr)))
         return LCT_E_NULL;
     const int64_t tokens = c->tokens, pitch = (tokens + 7) / 8 * 8;
+    const bool exact = tokens <= LCT_CROSS_ENTROPY_EXACT_TOKENS;
     const int32_t token_tiles = tiles_of(tokens, kLogitRows);
     if (d->piece < 1 || d->piece % 128 || d->splits < 1 || d->splits > LCT_MAX_CROSS_ENTROPY_SPLITS
         || d->index_size < 1 + 2 * tokens || d->value_floats < 1 + 3 * tokens
         || d->gathered_size < tokens * c->dim
-        || (products && d->dz_size < std::min(d->piece, c->vocab) * pitch)
+        || (products && d->dz_size < std::min(d->piece, c->vocab) * pitch * (exact ? 2 : 1))
         || (d->grad_x != nullptr && d->hidden_floats < d->splits * tokens * c->dim)
         || (d->grad_bias != nullptr && d->bias_floats < int64_t{2} * tiles_of(tokens, 128) * c->vocab))
         return LCT_E_SIZE;
@@ -927,6 +948,8 @@ extern "C" int32_t lct_cross_entropy_backward(const lct_cross_entropy *c,
             const_cast<float *>(d->lse), const_cast<float *>(d->losses), stream);
     const uint32_t chunk_grid = chunk_grid_of(*c);
     auto *dz = static_cast<uint16_t *>(d->dz);
+    uint16_t *const rest = exact && dz != nullptr ? dz + std::min(d->piece, c->vocab) * pitch
+                                                  : nullptr;
     const int32_t dim_tiles = tiles_of(c->dim, 256), hidden_tiles = tiles_of(tokens, 128);
     for (int32_t first = 0; first < c->vocab; first += d->piece) {
         const int32_t piece = std::min(d->piece, c->vocab - first);
@@ -936,12 +959,13 @@ extern "C" int32_t lct_cross_entropy_backward(const lct_cross_entropy *c,
             gradient_kernel<LogitProduct<decltype(half)::value>, decltype(half)::value,
                             decltype(cap)::value, decltype(bias)::value>
                 <<<grid, 256, 0, stream>>>(*c, t, first, piece, vocab_tiles, token_tiles,
-                                           products ? dz : nullptr, pitch,
+                                           products ? dz : nullptr, products ? rest : nullptr,
+                                           pitch,
                                            d->grad_bias != nullptr ? d->bias_parts : nullptr);
         });
         if (!products) continue;
         const PieceProducts q{first,    piece,       d->splits, dim_tiles,
-                              hidden_tiles, vocab_tiles, dz,        pitch,
+                              hidden_tiles, vocab_tiles, dz, rest, pitch,
                               d->hidden_parts, static_cast<uint16_t *>(d->grad_weight)};
         const uint32_t weight_grid =
             d->grad_weight == nullptr
@@ -951,12 +975,16 @@ extern "C" int32_t lct_cross_entropy_backward(const lct_cross_entropy *c,
             d->grad_x == nullptr
                 ? 0
                 : static_cast<uint32_t>(xcd_grid(int64_t{dim_tiles} * hidden_tiles * d->splits));
-        if (c->fp16)
-            products_kernel<true>
+        const auto multiply = [&](auto half, auto both) {
+            products_kernel<decltype(half)::value, decltype(both)::value>
                 <<<weight_grid + hidden_grid, 256, 0, stream>>>(*c, t, q, weight_grid);
-        else
-            products_kernel<false>
-                <<<weight_grid + hidden_grid, 256, 0, stream>>>(*c, t, q, weight_grid);
+        };
+        const auto with = [&](auto half) {
+            if (exact) multiply(half, std::true_type{});
+            else multiply(half, std::false_type{});
+        };
+        if (c->fp16) with(std::true_type{});
+        else with(std::false_type{});
     }
     const uint32_t bias_grid =
         d->grad_bias != nullptr ? static_cast<uint32_t>(tiles_of(c->vocab, kWave)) : 0;

@@ -25,6 +25,7 @@ MAX_DIM = 1 << 16       # LCT_MAX_CROSS_ENTROPY_DIM
 _CUS = 256
 _SLOTS = 2 * _CUS       # workgroups of a product's kernel that run at once
 _MAX_SPLITS = 16        # LCT_MAX_CROSS_ENTROPY_SPLITS
+_EXACT_TOKENS = 128     # LCT_CROSS_ENTROPY_EXACT_TOKENS
 _PIECE_BYTES = 256 << 20
 
 MAX_MATRIX_DIM = 1 << 16    # LCT_MAX_ORTHOGONAL_DIM
@@ -150,7 +151,9 @@ def cross_entropy_backward(grad: Tensor, x: Tensor, weight: Tensor, bias, target
     grad_weight = x.new_empty(vocab, width) if need_weight else None
     grad_bias = x.new_empty(vocab, dtype=torch.float32) if need_bias else None
     ints, floats, halves = 1 + 2 * tokens, 1 + 3 * tokens, tokens * width
-    dz_size = min(piece, vocab) * _up8(tokens) if need_x or need_weight else 0
+    dz_size = 0
+    if need_x or need_weight:
+        dz_size = min(piece, vocab) * _up8(tokens) * (2 if tokens <= _EXACT_TOKENS else 1)
     hidden_floats = splits * tokens * width if need_x else 0
     bias_floats = 2 * -(-tokens // 128) * vocab if need_bias else 0
     index, values, gathered, dz, hidden, columns, memory = _Workspace(

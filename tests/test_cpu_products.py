@@ -150,7 +150,7 @@ def _gradients(grad=1 << 20, lse=1 << 20, losses=1 << 20, grad_x=1 << 20, grad_w
     (dict(dz=0), E_NULL), (dict(hidden=0), E_NULL), (dict(grad_bias=1 << 20), E_NULL),
     (dict(piece=0), E_SIZE), (dict(piece=100), E_SIZE), (dict(splits=0), E_SIZE),
     (dict(splits=17), E_SIZE), (dict(index_size=6), E_SIZE), (dict(value_floats=9), E_SIZE),
-    (dict(gathered_size=23), E_SIZE), (dict(dz_size=39), E_SIZE), (dict(hidden_floats=23), E_SIZE),
+    (dict(gathered_size=23), E_SIZE), (dict(dz_size=79), E_SIZE), (dict(hidden_floats=23), E_SIZE),
     (dict(gathered=(1 << 20) + 8), E_ARG), (dict(dz=(1 << 20) + 8), E_ARG),
     (dict(grad_x=(1 << 20) + 8), E_ARG), (dict(grad_weight=(1 << 20) + 2), E_ARG),
 ])
