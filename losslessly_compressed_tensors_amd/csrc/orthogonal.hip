@@ -70,6 +70,56 @@ __device__ __forceinline__ void eight(const lct_orthogonal &o, int32_t matrix, i
     for (int k = 0; k < 8; ++k) v[k] = k < left ? element(o, at + k * step) : 0.0f;
 }
 
+// kCount of them, at place(k, &i, &j): where all are whole and aligned, the loads in flight
+// together.
+template <int kCount, class Place>
+__device__ __forceinline__ void load_eights(const lct_orthogonal &o, int32_t matrix, bool turned,
+                                            float (&v)[kCount][8], Place place) {
+    const int32_t size = o.type == LCT_FP32 ? 4 : 2, piece = 16 / size;
+    const int64_t line = turned ? o.stride[2] : o.stride[1];
+    const bool whole = (turned ? o.stride[1] : o.stride[2]) == 1 && line % piece == 0
+                       && o.stride[0] % piece == 0 && (turned ? o.rows : o.cols) % 8 == 0
+                       && reinterpret_cast<uintptr_t>(o.input) % 16 == 0;
+    if (!whole) {
+#pragma unroll
+        for (int k = 0; k < kCount; ++k) {
+            int i, j;
+            place(k, &i, &j);
+            eight(o, matrix, i, j, turned, v[k]);
+        }
+        return;
+    }
+    const char *const from = static_cast<const char *>(o.input) + matrix * o.stride[0] * size;
+    u32x4 raw[kCount], more[kCount];
+#pragma unroll
+    for (int k = 0; k < kCount; ++k) {
+        int i, j;
+        place(k, &i, &j);
+        const bool inside = i < o.rows && j < o.cols;
+        const char *at = from + (inside ? (i * o.stride[1] + j * o.stride[2]) * size : 0);
+        raw[k] = *reinterpret_cast<const u32x4 *>(at);
+        if (o.type == LCT_FP32) more[k] = *reinterpret_cast<const u32x4 *>(at + 16);
+    }
+#pragma unroll
+    for (int k = 0; k < kCount; ++k) {
+        int i, j;
+        place(k, &i, &j);
+        const bool inside = i < o.rows && j < o.cols;
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            const uint32_t pair = raw[k][n / 2];
+            float of;
+            if (o.type == LCT_FP32)
+                of = __uint_as_float(n < 4 ? raw[k][n % 4] : more[k][n % 4]);
+            else if (o.type == LCT_FP16)
+                of = n % 2 ? Half::high(pair) : Half::low(pair);
+            else
+                of = n % 2 ? Element<false>::high(pair) : Element<false>::low(pair);
+            v[k][n] = inside ? of : 0.0f;
+        }
+    }
+}
+
 __device__ __forceinline__ bool is_turned(const lct_orthogonal &o) {
     return o.stride[2] != 1 && o.stride[1] == 1;
 }
@@ -187,6 +237,291 @@ __global__ __launch_bounds__(256) void finish_kernel(lct_orthogonal o, int32_t r
             static_cast<uint16_t *>(o.out)[matrix * o.out_stride[0] + (i0 + i) * o.out_stride[1]
                                            + (j0 + j) * o.out_stride[2]] = tile[i][j];
     }
+}
+
+// ---- small matrices: all steps by one workgroup
+//
+// X as operand, A and P lie in LDS, X itself in FP32 in the registers that the update's
+// products leave it in: a wave has 32 x 32 tiles of it, columns in a lane's registers.  Rows are
+// 80 bytes off a multiple of 256, so that neither 16 rows' chunks nor 4 lines' 64 bytes meet
+// in a clock of LDS.
+
+constexpr int kSmallRows = LCT_ORTHOGONAL_SMALL_ROWS, kSmallCols = LCT_ORTHOGONAL_SMALL_COLS;
+constexpr int kSmallPad = 40;
+
+template <int kPitch>
+__device__ __forceinline__ u32x4 small_rows(const uint16_t *from, int block, int step) {
+    const int lane = wave_lane();
+    return *reinterpret_cast<const u32x4 *>(from + (32 * block + (lane & 31)) * kPitch + 16 * step
+                                            + 8 * (lane >> 5));
+}
+
+template <int kPitch>
+__device__ __forceinline__ u32x4 small_columns(const uint16_t *from, int block, int step) {
+    const int lane = wave_lane();
+    const uint16_t *at = from + (16 * step + 8 * (lane >> 5) + ((lane & 15) >> 2)) * kPitch
+                         + 32 * block + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (__attribute__((address_space(3))) i16x4 *)(at));
+    const i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (__attribute__((address_space(3))) i16x4 *)(at + 4 * kPitch));
+    const u32x2 lo = __builtin_bit_cast(u32x2, a), hi = __builtin_bit_cast(u32x2, b);
+    return u32x4{lo[0], lo[1], hi[0], hi[1]};
+}
+
+// A tile's four adjacent values of a lane, as FP16, to (row, column) of a matrix in LDS.
+template <int kPitch>
+__device__ __forceinline__ void small_store(uint16_t *to, int row_block, int column_block,
+                                            const f32x16 &v, float factor) {
+    uint16_t *at = to + (32 * row_block + (wave_lane() & 31)) * kPitch + 32 * column_block
+                   + 4 * (wave_lane() >> 5);
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<u32x2 *>(at + 8 * g) =
+            u32x2{Half::round_pair(v[4 * g] * factor, v[4 * g + 1] * factor),
+                  Half::round_pair(v[4 * g + 2] * factor, v[4 * g + 3] * factor)};
+}
+
+// kTiles tiles, blocks `first` .. of the right operand's rows against the left one's fragments:
+// the next step's are read while one is multiplied.
+template <int kTiles, class Left, class Right>
+__device__ __forceinline__ void small_product(f32x16 (&sum)[kTiles], int steps, Left left,
+                                              Right right) {
+    u32x4 a = left(0), b[kTiles];
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) {
+        sum[t] = f32x16{};
+        b[t] = right(t, 0);
+    }
+    for (int k = 0; k < steps; ++k) {
+        const int next = min(k + 1, steps - 1);
+        const u32x4 next_a = left(next);
+        u32x4 next_b[kTiles];
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) next_b[t] = right(t, next);
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) sum[t] = Half::multiply(a, b[t], sum[t]);
+        // (The reads stay in this round: the compiler would move them to their use.)
+        a = next_a;
+        asm volatile("" : "+v"(a));
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+            b[t] = next_b[t];
+            asm volatile("" : "+v"(b[t]));
+        }
+    }
+}
+
+template <int kRows, int kCols, int kWaves>
+__global__ __launch_bounds__(kWaves *kWave) void small_kernel(lct_orthogonal o) {
+    constexpr int kThreads = kWaves * kWave, kRowBlocks = kRows / 32;
+    constexpr int kTiles = kRowBlocks * (kCols / 32) / kWaves;
+    // (More waves than squares: the last have none.)
+    constexpr int kSquares = kRowBlocks * kRowBlocks < kWaves ? 1 : kRowBlocks * kRowBlocks / kWaves;
+    constexpr int kPitch = kCols + kSmallPad, kSquarePitch = kRows + kSmallPad;
+    static_assert(kTiles <= kRowBlocks && kSquares <= kRowBlocks);
+    // At the start, what X's rounding leaves lies where A and P will.
+    constexpr int kSquareValues = kRows * kSquarePitch;
+    constexpr int kRest = kRows * kPitch > 2 * kSquareValues ? kRows * kPitch : 2 * kSquareValues;
+    __shared__ __attribute__((aligned(16))) uint16_t operand[kRows * kPitch];
+    __shared__ __attribute__((aligned(16))) uint16_t squares[kRest];
+    __shared__ double sums[kWaves];
+    uint16_t *const gram = squares, *const poly = squares + kSquareValues;
+    const int lane = wave_lane();
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int32_t matrix = blockIdx.x;
+    // Blocks of 32 and steps of 16 that the matrices reach into.
+    const int row_blocks = (o.rows + 31) / 32, column_blocks = (o.cols + 31) / 32;
+    const int row_steps = (o.rows + 15) / 16, column_steps = (o.cols + 15) / 16;
+
+    // X's place in the registers that it is loaded to: pieces of eight along the dimension
+    // whose elements are adjacent.
+    constexpr int kPieces = kRows * kCols / 8 / kThreads;
+    float v[kPieces][8];
+    const bool turned = is_turned(o);
+    const auto place = [&](int k, auto by_rows, int *i, int *j) __attribute__((always_inline)) {
+        constexpr int kAcross = decltype(by_rows)::value ? kRows / 8 : kCols / 8;
+        const int slot = k * kThreads + threadIdx.x, line = slot / kAcross;
+        const int chunk = slot % kAcross * 8;
+        *i = decltype(by_rows)::value ? chunk : line;
+        *j = decltype(by_rows)::value ? line : chunk;
+    };
+    const auto load = [&](auto by_rows) __attribute__((always_inline)) {
+        load_eights<kPieces>(o, matrix, decltype(by_rows)::value, v,
+                             [&](int k, int *i, int *j) { place(k, by_rows, i, j); });
+    };
+    if (turned) load(std::true_type{});
+    else load(std::false_type{});
+    double sum = 0.0;
+#pragma unroll
+    for (int k = 0; k < kPieces; ++k)
+#pragma unroll
+        for (int n = 0; n < 8; ++n) sum += static_cast<double>(v[k][n]) * v[k][n];
+#pragma unroll
+    for (int d = kWave / 2; d > 0; d >>= 1) sum += __shfl_xor(sum, d, kWave);
+    if (lane == 0) sums[wave] = sum;
+    __syncthreads();
+    sum = 0.0;
+    for (int w = 0; w < kWaves; ++w) sum += sums[w];
+    const double inverse = 1.0 / (sqrt(sum) + o.eps);
+#pragma unroll
+    for (int k = 0; k < kPieces; ++k) {
+        u32x4 first, second;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            const float a = static_cast<float>(v[k][2 * n] * inverse) * kHoldX;
+            const float b = static_cast<float>(v[k][2 * n + 1] * inverse) * kHoldX;
+            first[n] = Half::round_pair(a, b);
+            second[n] = rest(a, b, first[n]);
+        }
+        int i, j;
+        if (!turned) {
+            place(k, std::false_type{}, &i, &j);
+            *reinterpret_cast<u32x4 *>(operand + i * kPitch + j) = first;
+            *reinterpret_cast<u32x4 *>(squares + i * kPitch + j) = second;
+        } else {
+            place(k, std::true_type{}, &i, &j);
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                const int at = (i + n) * kPitch + j;
+                operand[at] = static_cast<uint16_t>(first[n / 2] >> (n % 2 * 16));
+                squares[at] = static_cast<uint16_t>(second[n / 2] >> (n % 2 * 16));
+            }
+        }
+    }
+    __syncthreads();
+
+    // A wave's tiles are of one block of columns, whose fragment they share.
+    const int column = wave * kTiles / kRowBlocks, first = wave * kTiles % kRowBlocks;
+    const int square_column = wave * kSquares / kRowBlocks;
+    const int square_first = wave * kSquares % kRowBlocks;
+    const bool has = column < column_blocks;
+    const bool has_square = square_column < row_blocks && square_first < row_blocks;
+    f32x16 x[kTiles];
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) {
+        const int at = (32 * (first + t) + (lane & 31)) * kPitch + 32 * column + 4 * (lane >> 5);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const u32x2 p = *reinterpret_cast<const u32x2 *>(operand + at + 8 * g);
+            const u32x2 q = *reinterpret_cast<const u32x2 *>(squares + at + 8 * g);
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                x[t][4 * g + 2 * r] = (Half::low(p[r]) + Half::low(q[r])) * (1.0f / kHoldX);
+                x[t][4 * g + 2 * r + 1] = (Half::high(p[r]) + Half::high(q[r])) * (1.0f / kHoldX);
+            }
+        }
+    }
+    __syncthreads();
+
+    for (int32_t s = 0; s < o.steps; ++s) {
+        if (has_square) {
+            f32x16 a[kSquares];
+            small_product<kSquares>(
+                a, column_steps,
+                [&](int k) { return small_rows<kPitch>(operand, square_column, k); },
+                [&](int t, int k) { return small_rows<kPitch>(operand, square_first + t, k); });
+#pragma unroll
+            for (int t = 0; t < kSquares; ++t)
+                small_store<kSquarePitch>(gram, square_first + t, square_column, a[t],
+                                          kHoldA / (kHoldX * kHoldX));
+        }
+        __syncthreads();
+        if (has_square) {
+            f32x16 p[kSquares];
+            small_product<kSquares>(
+                p, row_steps,
+                [&](int k) { return small_rows<kSquarePitch>(gram, square_column, k); },
+                [&](int t, int k) { return small_rows<kSquarePitch>(gram, square_first + t, k); });
+#pragma unroll
+            for (int t = 0; t < kSquares; ++t) {
+                const uint16_t *own = gram + (32 * (square_first + t) + (lane & 31)) * kSquarePitch
+                                      + 32 * square_column + 4 * (lane >> 5);
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const u32x2 pairs = *reinterpret_cast<const u32x2 *>(own + 8 * g);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        p[t][4 * g + r] = __builtin_fmaf(
+                            kC / kHoldA, p[t][4 * g + r],
+                            kB * (r % 2 ? Half::high(pairs[r / 2]) : Half::low(pairs[r / 2])));
+                }
+                small_store<kSquarePitch>(poly, square_first + t, square_column, p[t], 1.0f);
+            }
+        }
+        __syncthreads();
+        if (has) {
+            f32x16 v[kTiles];
+            small_product<kTiles>(
+                v, row_steps, [&](int k) { return small_columns<kPitch>(operand, column, k); },
+                [&](int t, int k) { return small_rows<kSquarePitch>(poly, first + t, k); });
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    x[t][r] = __builtin_fmaf(1.0f / (kHoldA * kHoldX), v[t][r], kA * x[t][r]);
+        }
+        __syncthreads();     // all have read the operand
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+            small_store<kPitch>(operand, first + t, column, x[t], kHoldX);
+        __syncthreads();
+    }
+
+    // The result through LDS, to lie as it is written.
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) {
+        uint16_t *at = operand + (32 * (first + t) + (lane & 31)) * kPitch + 32 * column
+                       + 4 * (lane >> 5);
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<u32x2 *>(at + 8 * g) =
+                u32x2{Element<false>::round_pair(x[t][4 * g] * o.scale, x[t][4 * g + 1] * o.scale),
+                      Element<false>::round_pair(x[t][4 * g + 2] * o.scale,
+                                                 x[t][4 * g + 3] * o.scale)};
+    }
+    __syncthreads();
+    auto *const out = static_cast<uint16_t *>(o.out) + matrix * o.out_stride[0];
+    const bool out_turned = o.out_stride[2] != 1;
+    const int64_t step = out_turned ? o.out_stride[1] : 1;
+    const int64_t line_step = out_turned ? o.out_stride[2] : o.out_stride[1];
+    const bool whole = step == 1 && line_step % 8 == 0 && o.out_stride[0] % 8 == 0
+                       && reinterpret_cast<uintptr_t>(o.out) % 16 == 0;
+#pragma unroll
+    for (int k = 0; k < kPieces; ++k) {
+        int i, j;
+        u32x4 of{};
+        if (!out_turned) {
+            place(k, std::false_type{}, &i, &j);
+            of = *reinterpret_cast<const u32x4 *>(operand + i * kPitch + j);
+        } else {
+            place(k, std::true_type{}, &i, &j);
+#pragma unroll
+            for (int n = 0; n < 8; ++n)
+                of[n / 2] |= static_cast<uint32_t>(operand[(i + n) * kPitch + j]) << (n % 2 * 16);
+        }
+        if (i >= o.rows || j >= o.cols) continue;
+        uint16_t *to = out + i * o.out_stride[1] + j * o.out_stride[2];
+        const int32_t left = out_turned ? o.rows - i : o.cols - j;
+        if (whole && left >= 8) {
+            *reinterpret_cast<u32x4 *>(to) = of;
+        } else {
+#pragma unroll
+            for (int n = 0; n < 8; ++n)
+                if (n < left) to[n * step] = static_cast<uint16_t>(of[n / 2] >> (n % 2 * 16));
+        }
+    }
+}
+
+// The smallest that holds the matrices.
+void small(const lct_orthogonal &o, hipStream_t stream) {
+    const uint32_t count = static_cast<uint32_t>(o.count);
+    if (o.rows <= 64 && o.cols <= 64) small_kernel<64, 64, 4><<<count, 256, 0, stream>>>(o);
+    else if (o.rows <= 64 && o.cols <= 128)
+        small_kernel<64, 128, 4><<<count, 256, 0, stream>>>(o);
+    else if (o.rows <= 64) small_kernel<64, 256, 8><<<count, 512, 0, stream>>>(o);
+    else if (o.cols <= 128) small_kernel<128, 128, 8><<<count, 512, 0, stream>>>(o);
+    else small_kernel<128, 256, 8><<<count, 512, 0, stream>>>(o);
 }
 
 // ---- products
@@ -421,13 +756,18 @@ using namespace lct;
 
 extern "C" int32_t lct_orthogonalize(const lct_orthogonal *o, void *workspace,
                                      int64_t workspace_bytes, hipStream_t stream) {
-    if (o == nullptr || o->input == nullptr || o->out == nullptr || workspace == nullptr)
-        return LCT_E_NULL;
+    if (o == nullptr || o->input == nullptr || o->out == nullptr) return LCT_E_NULL;
     if (o->count < 1 || o->rows < 1 || o->cols < o->rows
         || o->cols > LCT_MAX_ORTHOGONAL_DIM || o->steps < 0)
         return LCT_E_SIZE;
-    if (o->type < LCT_BF16 || o->type > LCT_FP32 || reinterpret_cast<uintptr_t>(workspace) % 16)
-        return LCT_E_ARG;
+    if (o->type < LCT_BF16 || o->type > LCT_FP32) return LCT_E_ARG;
+    if (o->rows <= kSmallRows && o->cols <= kSmallCols) {
+        if (o->count >= 1 << 23) return LCT_E_SIZE;
+        small(*o, stream);
+        return static_cast<int32_t>(hipGetLastError());
+    }
+    if (workspace == nullptr) return LCT_E_NULL;
+    if (reinterpret_cast<uintptr_t>(workspace) % 16) return LCT_E_ARG;
     const int64_t rows = up8(o->rows), cols = up8(o->cols), count = o->count;
     const int64_t values = count * rows * cols, square = count * rows * rows;
     const int64_t tiles = ((rows + 63) / 64) * ((cols + 63) / 64);

@@ -30,6 +30,7 @@ _PIECE_BYTES = 256 << 20
 
 MAX_MATRIX_DIM = 1 << 16    # LCT_MAX_ORTHOGONAL_DIM
 _NORM_PARTS = 1024          # LCT_ORTHOGONAL_NORM_PARTS
+_SMALL = 128, 256           # LCT_ORTHOGONAL_SMALL_ROWS, _COLS
 
 
 def _whole_rows(t: Tensor) -> Tensor:
@@ -190,10 +191,12 @@ def orthogonalize(g: Tensor, steps: int, scale: float, eps: float) -> Tensor:
         rows, cols = cols, rows
         stride = stride[0], stride[2], stride[1]
         out_stride = out_stride[0], out_stride[2], out_stride[1]
-    r, c = _up8(rows), _up8(cols)
-    size = count * (8 * _NORM_PARTS + 6 * r * (c + r))
-    workspace = torch.empty(size, dtype=torch.uint8, device=g.device)
+    workspace, size = None, 0
+    if rows > _SMALL[0] or cols > _SMALL[1]:
+        r, c = _up8(rows), _up8(cols)
+        size = count * (8 * _NORM_PARTS + 6 * r * (c + r))
+        workspace = torch.empty(size, dtype=torch.uint8, device=g.device)
     _launch("lct_orthogonalize", g.get_device(), hip.ORTHOGONAL.pack(
         g.data_ptr(), out.data_ptr(), *stride, *out_stride, count, rows, cols, steps,
-        TYPES[g.dtype], scale, eps), workspace.data_ptr(), size)
+        TYPES[g.dtype], scale, eps), None if workspace is None else workspace.data_ptr(), size)
     return out

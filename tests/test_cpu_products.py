@@ -177,16 +177,17 @@ def test_forward_refuses_small_workspaces_before_a_launch(lib):
 
 @pytest.mark.parametrize("changes,code", [
     (dict(input=0), E_NULL), (dict(out=0), E_NULL), (dict(count=0), E_SIZE),
-    (dict(rows=0), E_SIZE), (dict(rows=9), E_SIZE), (dict(cols=(1 << 16) + 1), E_SIZE),
+    (dict(rows=0), E_SIZE), (dict(rows=137), E_SIZE), (dict(cols=(1 << 16) + 1), E_SIZE),
     (dict(steps=-1), E_SIZE), (dict(type=3), E_ARG), (dict(type=-1), E_ARG),
-    (dict(count=1 << 23), E_SIZE), (dict(size=8 * 1024 + 6 * 128 - 1), E_SIZE),
+    (dict(count=1 << 23), E_SIZE), (dict(count=1 << 23, rows=8, cols=8), E_SIZE),
+    (dict(size=8 * 1024 + 12 * 136 * 136 - 1), E_SIZE),
     (dict(workspace=(1 << 20) + 8), E_ARG), (dict(workspace=None), E_NULL),
 ])
 def test_orthogonalize_entry_point_refuses_before_a_launch(lib, changes, code):
-    values = dict(input=1 << 20, out=1 << 20, count=1, rows=8, cols=8, steps=1, type=0,
+    values = dict(input=1 << 20, out=1 << 20, count=1, rows=136, cols=136, steps=1, type=0,
                   workspace=1 << 20, size=1 << 40)
     values.update(changes)
-    record = hip.ORTHOGONAL.pack(values["input"], values["out"], 64, 8, 1, 64, 8, 1,
+    record = hip.ORTHOGONAL.pack(values["input"], values["out"], 136 * 136, 136, 1, 136 * 136, 136, 1,
                                  values["count"], values["rows"], values["cols"], values["steps"],
                                  values["type"], 1.0, 1e-7)
     assert lib.lct_orthogonalize(record, values["workspace"], values["size"], None) == code

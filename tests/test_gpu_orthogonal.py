@@ -66,6 +66,16 @@ def test_batches(shape):
     _assert_polar(orthogonalize(g.cuda(), 5), g, 5)
 
 
+@pytest.mark.parametrize("rows,cols", [(64, 64), (63, 65), (64, 128), (40, 129), (64, 256),
+                                       (65, 65), (128, 128), (127, 130), (128, 256), (100, 255),
+                                       (129, 129), (128, 257)])
+def test_either_side_of_the_small_kernels_sizes(rows, cols):
+    for steps in (0, 1, 5, 12):
+        for shape in ((3, rows, cols), (3, cols, rows)):
+            g = _matrix(shape, "falling").to(BF16)
+            _assert_polar(orthogonalize(g.cuda(), steps, scale=-0.5), g, steps, -0.5)
+
+
 def _views(g):
     """The same matrices in other storages."""
     count, rows, cols = g.shape
