@@ -982,10 +982,13 @@ int32_t lct_cross_entropy_backward(const lct_cross_entropy *c,
  * matrix, row and column, out's likewise.  X is the sum of two FP16 numbers, the products'
  * operands FP16 at powers of two, sums FP32, the norm FP64.  workspace (16-byte aligned):
  * with both dimensions rounded up to 8, count * (8 LCT_ORTHOGONAL_NORM_PARTS + 6 rows cols
- * + 6 rows^2) bytes; none, and NULL, for matrices within LCT_ORTHOGONAL_SMALL_ROWS x
+ * + 6 rows^2) bytes, and LCT_ORTHOGONAL_SPLIT_BYTES where there are
+ * LCT_ORTHOGONAL_SPLIT_DEPTH columns; none, and NULL, for matrices within LCT_ORTHOGONAL_SMALL_ROWS x
  * LCT_ORTHOGONAL_SMALL_COLS, which one workgroup each computes. */
 #define LCT_MAX_ORTHOGONAL_DIM (1 << 16)
 #define LCT_ORTHOGONAL_NORM_PARTS 1024
+#define LCT_ORTHOGONAL_SPLIT_DEPTH 2048
+#define LCT_ORTHOGONAL_SPLIT_BYTES (1 << 25)
 #define LCT_ORTHOGONAL_SMALL_ROWS 128
 #define LCT_ORTHOGONAL_SMALL_COLS 256
 typedef struct {

@@ -544,29 +544,13 @@ struct SymmetricTerms {
     float factor, share;
 };
 
+// What becomes of tile (i, j)'s sums.
 template <class P, int kMore>
-__global__ __launch_bounds__(P::kThreads, 2) void symmetric_kernel(SymmetricTerms s, int32_t count,
-                                                                   int32_t size, int32_t depth,
-                                                                   int32_t tiles) {
-    static_assert(P::kM == P::kN);
-    LCT_PRODUCT_STAGES(P);
-    const int64_t item = xcd_item(int64_t{count} * tiles, blockIdx.x);
-    if (item >= int64_t{count} * tiles) return;
-    const int32_t matrix = static_cast<int32_t>(item / tiles);
-    int32_t i, j;
-    lower_tile(static_cast<int32_t>(item % tiles), &i, &j);
-    const int64_t of = int64_t{matrix} * size * depth;
-    typename P::A a;
-    typename P::B b;
-    a.prepare(s.left + of, depth, int64_t{i} * P::kM, size);
-    b.prepare(s.right + of, depth, int64_t{j} * P::kN, size);
-    P p;
-    p.begin();
-    p.run(a, b, depth, stage0, stage1, stage2, stage3);
-
+__device__ __forceinline__ void finish_symmetric(P &p, const SymmetricTerms &s, int32_t matrix,
+                                                 int32_t i, int32_t j, int32_t size,
+                                                 uint16_t *mine) {
     const int32_t row = i * P::kM + p.first_row(), column = j * P::kN + p.first_column();
     const int64_t first = int64_t{matrix} * size * size;
-    uint16_t *mine = turn_values<P>(stage0, stage1, stage2, stage3);
 #pragma unroll
     for (int m = 0; m < P::kRowTiles; ++m)
 #pragma unroll
@@ -592,6 +576,108 @@ __global__ __launch_bounds__(P::kThreads, 2) void symmetric_kernel(SymmetricTerm
     if (i != j)
         store_rows<P>(s.out + first + int64_t{row} * size + column, size, size - row, size - column,
                       mine, pair);
+}
+
+// Tiles that run at once; the depth from which on the last of them, where they are at most
+// half as many, are split; a part's least depth; parts (that symmetric_join_kernel loads at
+// once).  us with 1 | 2 | 4 | 8 | 16 parts at most: 4096 x 11008 (528 tiles) 3203 | 2892 | 2777 |
+// 2779 | 2804; 4096 x 4096 1707 | 1572 | 1520 | 1545 | 1546; 16 x 4096 x 1024 (576 tiles) 1424 |
+// 1372 | 1359 | 1370 | 1371; 4 x 2048 x 8192 (544) 2304 | 2134 | 2077 | 2067 | 2106.
+constexpr int32_t kSlots = 512, kSplitDepth = LCT_ORTHOGONAL_SPLIT_DEPTH, kPartDepth = 512;
+constexpr int32_t kMostSplits = 4;
+
+// The first `whole` tiles by a workgroup each, the others, which would leave most compute
+// units without one, by `splits` of them with a part of the depth each: their sums go to
+// `parts` as they lie in the registers, and symmetric_join_kernel goes on with them.
+struct SymmetricShare {
+    int32_t tiles, whole, splits;
+    uint32_t whole_grid;
+    f32x4 *parts;
+};
+
+template <class P>
+constexpr int kPartPieces = P::kRowTiles * P::kColumnTiles * 4;
+
+template <class P, int kMore>
+__global__ __launch_bounds__(P::kThreads, 2) void symmetric_kernel(SymmetricTerms s,
+                                                                   SymmetricShare share,
+                                                                   int32_t size, int32_t depth) {
+    static_assert(P::kM == P::kN);
+    LCT_PRODUCT_STAGES(P);
+    int64_t item;
+    int32_t begin = 0, end = depth;
+    const bool part = blockIdx.x >= share.whole_grid;
+    if (part) {
+        const int32_t t = blockIdx.x - share.whole_grid;
+        const int32_t per = ((depth + share.splits - 1) / share.splits + 63) / 64 * 64;
+        item = share.whole + t / share.splits;
+        begin = min(depth, t % share.splits * per);
+        end = min(depth, begin + per);
+    } else {
+        item = xcd_item(share.whole, blockIdx.x);
+        if (item >= share.whole) return;
+    }
+    const int32_t matrix = static_cast<int32_t>(item / share.tiles);
+    int32_t i, j;
+    lower_tile(static_cast<int32_t>(item % share.tiles), &i, &j);
+    const int64_t of = int64_t{matrix} * size * depth + begin;
+    typename P::A a;
+    typename P::B b;
+    a.prepare(s.left + of, depth, int64_t{i} * P::kM, size);
+    b.prepare(s.right + of, depth, int64_t{j} * P::kN, size);
+    P p;
+    p.begin();
+    p.run(a, b, end - begin, stage0, stage1, stage2, stage3);
+    if (part) {
+        f32x4 *to = share.parts + int64_t{blockIdx.x - share.whole_grid} * kPartPieces<P> * P::kThreads
+                    + threadIdx.x;
+#pragma unroll
+        for (int m = 0; m < P::kRowTiles; ++m)
+#pragma unroll
+            for (int n = 0; n < P::kColumnTiles; ++n)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    to[((m * P::kColumnTiles + n) * 4 + g) * P::kThreads] =
+                        f32x4{p.sum[m][n][4 * g], p.sum[m][n][4 * g + 1], p.sum[m][n][4 * g + 2],
+                              p.sum[m][n][4 * g + 3]};
+        return;
+    }
+    finish_symmetric<P, kMore>(p, s, matrix, i, j, size,
+                               turn_values<P>(stage0, stage1, stage2, stage3));
+}
+
+// The parts of a tile, added in order.
+template <class P, int kMore>
+__global__ __launch_bounds__(P::kThreads, 1) void symmetric_join_kernel(SymmetricTerms s,
+                                                                     SymmetricShare share,
+                                                                     int32_t size) {
+    __shared__ __attribute__((aligned(16))) uint16_t turn[P::kThreads / kWave * kTurnValues<P>];
+    const int64_t item = share.whole + blockIdx.x;
+    const int32_t matrix = static_cast<int32_t>(item / share.tiles);
+    int32_t i, j;
+    lower_tile(static_cast<int32_t>(item % share.tiles), &i, &j);
+    P p;
+    p.begin();
+    // All parts' loads in flight together.
+    constexpr int kPieces = kPartPieces<P>;
+    const f32x4 *const from =
+        share.parts + int64_t{blockIdx.x} * share.splits * kPieces * P::kThreads + threadIdx.x;
+    f32x4 v[kMostSplits][kPieces];
+#pragma unroll
+    for (int k = 0; k < kMostSplits; ++k)
+#pragma unroll
+        for (int q = 0; q < kPieces; ++q)
+            v[k][q] = from[(int64_t{min(k, share.splits - 1)} * kPieces + q) * P::kThreads];
+#pragma unroll
+    for (int k = 0; k < kMostSplits; ++k)
+        if (k < share.splits)
+#pragma unroll
+            for (int q = 0; q < kPieces; ++q)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    p.sum[q / 4 / P::kColumnTiles][q / 4 % P::kColumnTiles][4 * (q % 4) + r] +=
+                        v[k][q][r];
+    finish_symmetric<P, kMore>(p, s, matrix, i, j, size, turn + P::wave() * kTurnValues<P>);
 }
 
 // X <- share X + S X: P::kM columns of X (rows of the tile) by P::kN rows of X (columns, a lane
@@ -682,6 +768,7 @@ struct Iteration {
     int32_t count, rows, cols;
     uint16_t *x, *next, *x_rest, *square[3];
     hipStream_t stream;
+    f32x4 *parts;
 
     // Tiles of 128 x 128.
     int64_t lower_tiles() const {
@@ -692,21 +779,33 @@ struct Iteration {
         return count * int64_t{(rows + 127) / 128} * ((cols + 127) / 128);
     }
 
-    template <int kSize>
+    template <int kSize, int kMore>
     void launch_symmetric(const SymmetricTerms &s, int32_t depth) const {
         using P = Symmetric<kSize>;
         const int32_t blocks = (rows + kSize - 1) / kSize, tiles = blocks * (blocks + 1) / 2;
-        const uint32_t grid = static_cast<uint32_t>(xcd_grid(int64_t{count} * tiles));
-        if (s.more[1] != nullptr)
-            symmetric_kernel<P, 2><<<grid, P::kThreads, 0, stream>>>(s, count, rows, depth, tiles);
-        else if (s.more[0] != nullptr)
-            symmetric_kernel<P, 1><<<grid, P::kThreads, 0, stream>>>(s, count, rows, depth, tiles);
-        else
-            symmetric_kernel<P, 0><<<grid, P::kThreads, 0, stream>>>(s, count, rows, depth, tiles);
+        const int32_t all = count * tiles, rest = all % kSlots;
+        SymmetricShare share{tiles, all, 1, 0, parts};
+        if (kSize == 128 && depth >= kSplitDepth && rest > 0 && rest <= kSlots / 2) {
+            share.whole = all - rest;
+            share.splits = std::min(std::min(kSlots / rest, depth / kPartDepth), kMostSplits);
+        }
+        share.whole_grid = static_cast<uint32_t>(xcd_grid(share.whole));
+        const int32_t split = all - share.whole;
+        symmetric_kernel<P, kMore>
+            <<<share.whole_grid + split * share.splits, P::kThreads, 0, stream>>>(s, share, rows,
+                                                                                 depth);
+        if constexpr (kSize == 128)
+            if (split > 0)
+                symmetric_join_kernel<P, kMore><<<split, P::kThreads, 0, stream>>>(s, share, rows);
     }
     void symmetric(const SymmetricTerms &s, int32_t depth) const {
-        if (lower_tiles() < kFewTiles) launch_symmetric<64>(s, depth);
-        else launch_symmetric<128>(s, depth);
+        const auto with = [&](auto more) {
+            if (lower_tiles() < kFewTiles) launch_symmetric<64, decltype(more)::value>(s, depth);
+            else launch_symmetric<128, decltype(more)::value>(s, depth);
+        };
+        if (s.more[1] != nullptr) with(std::integral_constant<int, 2>{});
+        else if (s.more[0] != nullptr) with(std::integral_constant<int, 1>{});
+        else with(std::integral_constant<int, 0>{});
     }
     // out = A = X X^T.
     void gram(uint16_t *out) const {
@@ -777,9 +876,12 @@ extern "C" int32_t lct_orthogonalize(const lct_orthogonal *o, void *workspace,
         static_cast<int32_t>(std::min<int64_t>(LCT_ORTHOGONAL_NORM_PARTS, (tiles + 3) / 4));
     // Norms, X as it is and to be, what X's rounding leaves, and three square matrices.
     const int64_t norm_bytes = count * LCT_ORTHOGONAL_NORM_PARTS * 8;
-    if (workspace_bytes < norm_bytes + 6 * (values + square)) return LCT_E_SIZE;
+    // (Parts of up to kSlots tiles.)
+    const int64_t part_bytes = cols >= kSplitDepth ? LCT_ORTHOGONAL_SPLIT_BYTES : 0;
+    if (workspace_bytes < norm_bytes + part_bytes + 6 * (values + square)) return LCT_E_SIZE;
     auto *norms = static_cast<double *>(workspace);
-    auto *x = reinterpret_cast<uint16_t *>(static_cast<char *>(workspace) + norm_bytes);
+    char *const after = static_cast<char *>(workspace) + norm_bytes;
+    auto *x = reinterpret_cast<uint16_t *>(after + part_bytes);
     uint16_t *const squares = x + 3 * values;
     Iteration it{static_cast<int32_t>(count),
                  static_cast<int32_t>(rows),
@@ -788,7 +890,8 @@ extern "C" int32_t lct_orthogonalize(const lct_orthogonal *o, void *workspace,
                  x + values,
                  x + 2 * values,
                  {squares, squares + square, squares + 2 * square},
-                 stream};
+                 stream,
+                 reinterpret_cast<f32x4 *>(after)};
     norm_kernel<<<static_cast<uint32_t>(count * parts), 256, 0, stream>>>(*o, parts, norms);
     start_kernel<<<static_cast<uint32_t>(count * tiles), 256, 0, stream>>>(
         *o, parts, norms, it.rows, it.cols, it.x, it.x_rest);

@@ -30,6 +30,8 @@ _PIECE_BYTES = 256 << 20
 
 MAX_MATRIX_DIM = 1 << 16    # LCT_MAX_ORTHOGONAL_DIM
 _NORM_PARTS = 1024          # LCT_ORTHOGONAL_NORM_PARTS
+_SPLIT_DEPTH = 2048         # LCT_ORTHOGONAL_SPLIT_DEPTH
+_SPLIT_BYTES = 1 << 25      # LCT_ORTHOGONAL_SPLIT_BYTES
 _SMALL = 128, 256           # LCT_ORTHOGONAL_SMALL_ROWS, _COLS
 
 
@@ -194,7 +196,8 @@ def orthogonalize(g: Tensor, steps: int, scale: float, eps: float) -> Tensor:
     workspace, size = None, 0
     if rows > _SMALL[0] or cols > _SMALL[1]:
         r, c = _up8(rows), _up8(cols)
-        size = count * (8 * _NORM_PARTS + 6 * r * (c + r))
+        size = (count * (8 * _NORM_PARTS + 6 * r * (c + r))
+                + (_SPLIT_BYTES if c >= _SPLIT_DEPTH else 0))
         workspace = torch.empty(size, dtype=torch.uint8, device=g.device)
     _launch("lct_orthogonalize", g.get_device(), hip.ORTHOGONAL.pack(
         g.data_ptr(), out.data_ptr(), *stride, *out_stride, count, rows, cols, steps,
