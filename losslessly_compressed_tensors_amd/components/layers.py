@@ -242,7 +242,7 @@ class RMSLinearCrossEntropy(torch.autograd.Function):
         flat = targets.reshape(-1).contiguous()
         out, stats = products.cross_entropy_forward(
             normalized.reshape(-1, x.shape[-1]), W, bias.float().contiguous(), flat, softcap,
-            ignore_index, reduction)
+            ignore_index, reduction, True)
         del normalized
         ctx.saved = _SavedActivation(x, compressed and x.numel() >= min_elements,
                                      distribution or act_dist, buffer)

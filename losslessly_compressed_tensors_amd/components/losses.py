@@ -16,11 +16,12 @@ from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from ..kernels import products as kernels
-from .attention import _check_memory, _check_tensor, _recorded, _whole
+from .attention import _check_like, _check_memory, _check_tensor, _recorded, _whole
 
 __all__ = ["linear_cross_entropy"]
 
 _TYPES = (torch.bfloat16, torch.float16)
+_INDICES = (torch.int32, torch.int64)
 REDUCTIONS = ("mean", "sum", "none")
 
 
@@ -29,7 +30,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
     def forward(ctx, x, weight, bias, targets, softcap, ignore_index, reduction):
         out, stats = kernels.cross_entropy_forward(
             x, weight, None if bias is None else bias.float(), targets, softcap, ignore_index,
-            reduction)
+            reduction, True)
         ctx.how = softcap, ignore_index, reduction
         ctx.save_for_backward(x, weight, bias, targets, stats)
         # The caller's losses are its own to change.
@@ -61,29 +62,31 @@ def check_cross_entropy(x, weight, targets, bias, softcap, ignore_index, reducti
     if not isinstance(x, Tensor) or x.ndim < 1:
         raise TypeError("x must be a torch.Tensor of at least one dimension")
     _check_tensor(x, "x", x.ndim, _TYPES)
-    _check_tensor(weight, "weight", 2, (x.dtype,))
+    _check_like(weight, "weight", x, 2)
     vocab, dim = weight.shape
-    if x.shape[-1] != dim:
-        raise ValueError(f"x has {x.shape[-1]} channels, weight {dim}")
+    shape, device = x.shape, x.device
+    if shape[-1] != dim:
+        raise ValueError(f"x has {shape[-1]} channels, weight {dim}")
     if not 1 <= dim <= kernels.MAX_DIM - 7:
         raise ValueError(f"channels must lie between 1 and {kernels.MAX_DIM - 7}, got {dim}")
     if not 1 <= vocab <= kernels.MAX_VOCAB:
         raise ValueError(f"the vocabulary must lie between 1 and {kernels.MAX_VOCAB}, got {vocab}")
     _check_memory(targets, "targets")
-    if targets.dtype not in (torch.int32, torch.int64):
+    if targets.dtype not in _INDICES:
         raise TypeError(f"targets must be int32 or int64, got {targets.dtype}")
-    if targets.shape != x.shape[:-1]:
-        raise ValueError(f"targets must have shape {tuple(x.shape[:-1])}, "
+    if targets.shape != shape[:-1]:
+        raise ValueError(f"targets must have shape {tuple(shape[:-1])}, "
                          f"got {tuple(targets.shape)}")
+    if targets.device != device:
+        raise ValueError(f"all tensors must be on {device}, targets is on {targets.device}")
     if targets.numel() > kernels.MAX_TOKENS:
         raise ValueError(f"at most {kernels.MAX_TOKENS} tokens")
     if bias is not None:
         _check_tensor(bias, "bias", 1, (torch.float32, x.dtype))
         if bias.shape[0] != vocab:
             raise ValueError(f"bias must have {vocab} values, got {bias.shape[0]}")
-    for t, name in ((weight, "weight"), (targets, "targets"), (bias, "bias")):
-        if t is not None and t.device != x.device:
-            raise ValueError(f"all tensors must be on {x.device}, {name} is on {t.device}")
+        if bias.device != device:
+            raise ValueError(f"all tensors must be on {device}, bias is on {bias.device}")
     if reduction not in REDUCTIONS:
         raise ValueError(f"reduction must be one of {', '.join(REDUCTIONS)}, got {reduction!r}")
     if softcap is None:
@@ -119,7 +122,9 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, targets: Tensor, bias: Tenso
         if not _recorded(x, weight, bias):
             return zero
         return _Nothing.apply(zero, x, weight, bias)
-    x, targets = x.reshape(-1, x.shape[-1]), targets.reshape(-1).contiguous()
+    if x.ndim != 2:
+        x, targets = x.reshape(-1, x.shape[-1]), targets.reshape(-1)
+    targets = targets.contiguous()
     if bias is not None:
         bias = bias.contiguous()
     if _recorded(x, weight, bias):
@@ -127,8 +132,8 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, targets: Tensor, bias: Tenso
     else:
         out, _ = kernels.cross_entropy_forward(
             x, weight, None if bias is None else bias.float(), targets, softcap, ignore_index,
-            reduction)
-    return out.view(shape) if reduction == "none" else out
+            reduction, False)
+    return out.view(shape) if reduction == "none" and len(shape) != 1 else out
 
 
 class _Nothing(torch.autograd.Function):

@@ -224,8 +224,7 @@ def test_last_end_is_a_list_schedules():
 
 
 def test_workspace_arrays_lie_apart_and_aligned():
-    w = products._Workspace(1, 0, 300, 256)
-    assert w.offsets == [0, 256, 256, 768] and w.bytes == 1024
+    assert products._places(1, 0, 300, 256) == [0, 256, 256, 768, 1024]
 
 
 def test_muon_takes_the_option():
