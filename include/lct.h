@@ -929,6 +929,7 @@ int32_t lct_dropout(const void *x, const void *residual, void *out, int64_t n, i
 #define LCT_MAX_CROSS_ENTROPY_TOKENS (1 << 22)
 #define LCT_MAX_CROSS_ENTROPY_VOCAB (1 << 24)
 #define LCT_MAX_CROSS_ENTROPY_DIM (1 << 16)
+#define LCT_MAX_CROSS_ENTROPY_LOGITS ((int64_t)1 << 37)    /* tokens * vocab */
 #define LCT_MAX_CROSS_ENTROPY_SPLITS 16
 #define LCT_CROSS_ENTROPY_EXACT_TOKENS 128
 typedef struct {
@@ -943,9 +944,9 @@ typedef struct {
 /* losses[n], and lse[n] for the backward call: log2 of sum_v exp(l[n][v]).  total: the
  * losses' sum, or with mean != 0 that over the number of tokens that count (one at
  * least); NULL: not written.  parts: working array of part_floats >= 4 * tokens *
- * ceil(vocab / 128), twice that for up to 32 tokens, 8-byte aligned.  index (1 + 2 * tokens values) and gathered (tokens *
- * dim values, 16-byte aligned): working arrays for multiplying the tokens that count
- * alone; NULL index: all are multiplied. */
+ * ceil(vocab / 128), twice that for up to 32 tokens, 8-byte aligned.  index (1 + 2 *
+ * tokens values) and gathered (tokens * dim values, 16-byte aligned): working arrays for
+ * multiplying the tokens that count alone; NULL index: all are multiplied. */
 int32_t lct_cross_entropy_forward(const lct_cross_entropy *c, int32_t *index, int64_t index_size,
                                   void *gathered, int64_t gathered_size, float *parts,
                                   int64_t part_floats, float *lse, float *losses, float *total,
@@ -983,9 +984,12 @@ int32_t lct_cross_entropy_backward(const lct_cross_entropy *c,
  * operands FP16 at powers of two, sums FP32, the norm FP64.  workspace (16-byte aligned):
  * with both dimensions rounded up to 8, count * (8 LCT_ORTHOGONAL_NORM_PARTS + 6 rows cols
  * + 6 rows^2) bytes, and LCT_ORTHOGONAL_SPLIT_BYTES where there are
- * LCT_ORTHOGONAL_SPLIT_DEPTH columns; none, and NULL, for matrices within LCT_ORTHOGONAL_SMALL_ROWS x
- * LCT_ORTHOGONAL_SMALL_COLS, which one workgroup each computes. */
+ * LCT_ORTHOGONAL_SPLIT_DEPTH columns; none, and NULL, for matrices within
+ * LCT_ORTHOGONAL_SMALL_ROWS x LCT_ORTHOGONAL_SMALL_COLS, which one workgroup each computes.
+ * count, or with larger matrices count * ceil(rows / 64) * ceil(cols / 64), below
+ * LCT_MAX_ORTHOGONAL_TILES. */
 #define LCT_MAX_ORTHOGONAL_DIM (1 << 16)
+#define LCT_MAX_ORTHOGONAL_TILES (1 << 23)
 #define LCT_ORTHOGONAL_NORM_PARTS 1024
 #define LCT_ORTHOGONAL_SPLIT_DEPTH 2048
 #define LCT_ORTHOGONAL_SPLIT_BYTES (1 << 25)

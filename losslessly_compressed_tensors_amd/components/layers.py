@@ -241,8 +241,9 @@ class RMSLinearCrossEntropy(torch.autograd.Function):
         normalized, rstd = _norm(x, norm_weight)
         flat = targets.reshape(-1).contiguous()
         out, stats = products.cross_entropy_forward(
-            normalized.reshape(-1, x.shape[-1]), W, bias.float().contiguous(), flat, softcap,
-            ignore_index, reduction, True)
+            normalized.reshape(-1, x.shape[-1]), W,
+            None if bias is None else bias.float().contiguous(), flat, softcap, ignore_index,
+            reduction, True)
         del normalized
         ctx.saved = _SavedActivation(x, compressed and x.numel() >= min_elements,
                                      distribution or act_dist, buffer)
@@ -259,7 +260,7 @@ class RMSLinearCrossEntropy(torch.autograd.Function):
         normalized, _ = _norm(x, norm_weight)
         grad_normalized, grad_weight, grad_bias = products.cross_entropy_backward(
             grad.contiguous(), normalized.reshape(-1, x.shape[-1]), dense_weight(weight),
-            bias.float().contiguous(), targets, stats, *ctx.how,
+            None if bias is None else bias.float().contiguous(), targets, stats, *ctx.how,
             (need[0] or need[2], need[1], need[3]))
         grad_x = grad_gain = None
         if grad_normalized is not None:

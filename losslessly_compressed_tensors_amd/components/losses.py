@@ -81,6 +81,8 @@ def check_cross_entropy(x, weight, targets, bias, softcap, ignore_index, reducti
         raise ValueError(f"all tensors must be on {device}, targets is on {targets.device}")
     if targets.numel() > kernels.MAX_TOKENS:
         raise ValueError(f"at most {kernels.MAX_TOKENS} tokens")
+    if targets.numel() * vocab > kernels.MAX_LOGITS:
+        raise ValueError(f"tokens times vocabulary must not exceed {kernels.MAX_LOGITS}")
     if bias is not None:
         _check_tensor(bias, "bias", 1, (torch.float32, x.dtype))
         if bias.shape[0] != vocab:
@@ -109,8 +111,8 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, targets: Tensor, bias: Tenso
     NaN.  ``reduction``: "mean" over the tokens that count (0 if none does), "sum", or
     "none" for each token's loss.  Differentiable in ``x``, ``weight`` and ``bias``.
 
-    No logits are kept: forward needs 16 bytes per token and 256 of the vocabulary,
-    backward their gradient in 16 bits for up to 256 MiB of the vocabulary at a time.
+    No logits are kept: forward needs 16 bytes per token and 128 of the vocabulary
+    (of up to 32 tokens: twice that), backward their gradient in 16 bits for up to 256 MiB of the vocabulary at a time.
     Logits, softmax and sums are FP32; the logits' gradients are rounded to 16 bits for
     their products with ``weight`` and ``x`` (of up to 128 tokens, kept in two numbers)."""
     softcap, ignore_index = check_cross_entropy(x, weight, targets, bias, softcap, ignore_index,

@@ -31,7 +31,9 @@ def orthogonalize(G: Tensor, steps: int = 5, *, scale: float = 1.0) -> Tensor:
     + (-1.5 A + 0.5 A A) X`` with ``A = X X^T`` (of a tall one: transposed).  X is kept in
     22 bits between steps, and the products' operands are FP16 at fixed powers of two:
     results are within 1.5e-3 of the exact iteration's norm, the rounding to BF16 (1.7e-3)
-    aside, for matrices of a norm of 1e-11 or more.  Not differentiable."""
+    aside, for matrices of a norm of 1e-11 or more.  A call's results are the same in every
+    run; in another batch, or at another place of it, a matrix's may differ in roundings.
+    Not differentiable."""
     if not isinstance(G, Tensor) or G.ndim < 2:
         raise TypeError("G must be a torch.Tensor of at least two dimensions")
     _check_tensor(G, "G", G.ndim, tuple(kernels.TYPES))
@@ -41,6 +43,9 @@ def orthogonalize(G: Tensor, steps: int = 5, *, scale: float = 1.0) -> Tensor:
     rows, cols = G.shape[-2:]
     if max(rows, cols) > kernels.MAX_MATRIX_DIM:
         raise ValueError(f"at most {kernels.MAX_MATRIX_DIM} rows and columns")
+    count = math.prod(G.shape[:-2])
+    if kernels.orthogonal_tiles(count, rows, cols) >= kernels.MAX_TILES:
+        raise ValueError(f"too many matrices: {count} of {rows} x {cols}")
     if G.numel() == 0:
         return torch.empty(G.shape, dtype=torch.bfloat16, device=G.device)
     out = kernels.orthogonalize(G.reshape(-1, rows, cols), steps, float(scale), _EPS)

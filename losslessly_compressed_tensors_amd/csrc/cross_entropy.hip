@@ -806,10 +806,12 @@ bool aligned(const void *p, uintptr_t bytes) { return !(reinterpret_cast<uintptr
 int32_t check(const lct_cross_entropy *c) {
     if (c == nullptr || c->x == nullptr || c->weight == nullptr || c->targets == nullptr)
         return LCT_E_NULL;
-    // Tiles are addressed by 32-bit byte offsets: 256 rows of up to 2^22 values.
+    // Tiles are addressed by 32-bit byte offsets: 256 rows of up to 2^22 values.  A launch has
+    // fewer than 2^32 threads, 256 for 192 x 128 logits.
     if (c->tokens < 1 || c->tokens > LCT_MAX_CROSS_ENTROPY_TOKENS || c->vocab < 1
         || c->vocab > LCT_MAX_CROSS_ENTROPY_VOCAB || c->dim < 8 || c->dim % 8
-        || c->dim > LCT_MAX_CROSS_ENTROPY_DIM)
+        || c->dim > LCT_MAX_CROSS_ENTROPY_DIM
+        || int64_t{c->tokens} * c->vocab > LCT_MAX_CROSS_ENTROPY_LOGITS)
         return LCT_E_SIZE;
     if (c->x_stride < c->dim || c->x_stride % 8 || c->x_stride > LCT_MAX_CROSS_ENTROPY_DIM
         || c->weight_stride < c->dim || c->weight_stride % 8
@@ -824,6 +826,7 @@ int32_t check(const lct_cross_entropy *c) {
 int32_t tiles_of(int64_t n, int32_t tile) { return static_cast<int32_t>((n + tile - 1) / tile); }
 
 constexpr int32_t kMaxStrideGrid = 1 << 16;
+constexpr int64_t kMaxItems = int64_t{1} << 23;    // 256 threads each: below 2^32
 constexpr int32_t kWideJoin = 1024;    // tokens up to which four waves join one's parts
 
 uint32_t chunk_grid_of(const lct_cross_entropy &c) {
@@ -933,6 +936,10 @@ extern "C" int32_t lct_cross_entropy_backward(const lct_cross_entropy *c,
     if (!aligned(d->gathered, 16) || !aligned(d->dz, 16) || !aligned(d->hidden_parts, 16)
         || !aligned(d->grad_x, 16) || !aligned(d->grad_weight, 16))
         return LCT_E_ARG;
+    const int32_t dim_tiles = tiles_of(c->dim, 256), hidden_tiles = tiles_of(tokens, 128);
+    if (int64_t{dim_tiles} * (int64_t{hidden_tiles} * d->splits
+                              + tiles_of(std::min(d->piece, c->vocab), 128)) > kMaxItems)
+        return LCT_E_SIZE;
     Counted t{};
     int32_t *rows = d->index + 1, *targets = rows + tokens;
     float *lse = d->values + 1, *losses = lse + tokens, *factor = losses + tokens;
@@ -950,7 +957,6 @@ extern "C" int32_t lct_cross_entropy_backward(const lct_cross_entropy *c,
     auto *dz = static_cast<uint16_t *>(d->dz);
     uint16_t *const rest = exact && dz != nullptr ? dz + std::min(d->piece, c->vocab) * pitch
                                                   : nullptr;
-    const int32_t dim_tiles = tiles_of(c->dim, 256), hidden_tiles = tiles_of(tokens, 128);
     for (int32_t first = 0; first < c->vocab; first += d->piece) {
         const int32_t piece = std::min(d->piece, c->vocab - first);
         const int32_t vocab_tiles = tiles_of(piece, 128);

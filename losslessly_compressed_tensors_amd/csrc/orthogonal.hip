@@ -861,7 +861,7 @@ extern "C" int32_t lct_orthogonalize(const lct_orthogonal *o, void *workspace,
         return LCT_E_SIZE;
     if (o->type < LCT_BF16 || o->type > LCT_FP32) return LCT_E_ARG;
     if (o->rows <= kSmallRows && o->cols <= kSmallCols) {
-        if (o->count >= 1 << 23) return LCT_E_SIZE;
+        if (o->count >= LCT_MAX_ORTHOGONAL_TILES) return LCT_E_SIZE;
         small(*o, stream);
         return static_cast<int32_t>(hipGetLastError());
     }
@@ -871,7 +871,7 @@ extern "C" int32_t lct_orthogonalize(const lct_orthogonal *o, void *workspace,
     const int64_t values = count * rows * cols, square = count * rows * rows;
     const int64_t tiles = ((rows + 63) / 64) * ((cols + 63) / 64);
     // A launch has fewer than 2^32 threads; no product's tile is smaller than 64 x 64.
-    if (count * tiles >= 1 << 23) return LCT_E_SIZE;
+    if (count * tiles >= LCT_MAX_ORTHOGONAL_TILES) return LCT_E_SIZE;
     const int32_t parts =
         static_cast<int32_t>(std::min<int64_t>(LCT_ORTHOGONAL_NORM_PARTS, (tiles + 3) / 4));
     // Norms, X as it is and to be, what X's rounding leaves, and three square matrices.

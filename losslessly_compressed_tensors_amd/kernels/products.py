@@ -21,6 +21,7 @@ from .attention import TYPES, _check_unrecorded, _launch
 MAX_TOKENS = 1 << 22    # LCT_MAX_CROSS_ENTROPY_TOKENS
 MAX_VOCAB = 1 << 24     # LCT_MAX_CROSS_ENTROPY_VOCAB
 MAX_DIM = 1 << 16       # LCT_MAX_CROSS_ENTROPY_DIM
+MAX_LOGITS = 1 << 37    # LCT_MAX_CROSS_ENTROPY_LOGITS
 
 _CUS = 256
 _SLOTS = 2 * _CUS       # workgroups of a product's kernel that run at once
@@ -29,6 +30,7 @@ _EXACT_TOKENS = 128     # LCT_CROSS_ENTROPY_EXACT_TOKENS
 _PIECE_BYTES = 256 << 20
 
 MAX_MATRIX_DIM = 1 << 16    # LCT_MAX_ORTHOGONAL_DIM
+MAX_TILES = 1 << 23         # LCT_MAX_ORTHOGONAL_TILES
 _NORM_PARTS = 1024          # LCT_ORTHOGONAL_NORM_PARTS
 _SPLIT_DEPTH = 2048         # LCT_ORTHOGONAL_SPLIT_DEPTH
 _SPLIT_BYTES = 1 << 25      # LCT_ORTHOGONAL_SPLIT_BYTES
@@ -189,6 +191,18 @@ def _up8(n: int) -> int:
     return -(-n // 8) * 8
 
 
+def _is_small(rows: int, cols: int) -> bool:
+    """Whether one workgroup computes such a matrix (rows <= cols)."""
+    return rows <= _SMALL[0] and cols <= _SMALL[1]
+
+
+def orthogonal_tiles(count: int, rows: int, cols: int) -> int:
+    """Workgroups of the largest launch for that many matrices: fewer than MAX_TILES."""
+    if _is_small(min(rows, cols), max(rows, cols)):
+        return count
+    return count * -(-rows // 64) * -(-cols // 64)
+
+
 def orthogonalize(g: Tensor, steps: int, scale: float, eps: float) -> Tensor:
     """BF16 matrices of [matrix, row, column] ones."""
     _check_unrecorded(g)
@@ -200,7 +214,7 @@ def orthogonalize(g: Tensor, steps: int, scale: float, eps: float) -> Tensor:
         stride = stride[0], stride[2], stride[1]
         out_stride = out_stride[0], out_stride[2], out_stride[1]
     workspace, size = None, 0
-    if rows > _SMALL[0] or cols > _SMALL[1]:
+    if not _is_small(rows, cols):
         r, c = _up8(rows), _up8(cols)
         size = (count * (8 * _NORM_PARTS + 6 * r * (c + r))
                 + (_SPLIT_BYTES if c >= _SPLIT_DEPTH else 0))

@@ -115,7 +115,8 @@ def _cross_entropy(x=1 << 20, weight=1 << 20, bias=0, targets=1 << 20, x_stride=
 
 @pytest.mark.parametrize("changes,code", [
     (dict(x=0), E_NULL), (dict(weight=0), E_NULL), (dict(targets=0), E_NULL),
-    (dict(tokens=0), E_SIZE), (dict(tokens=(1 << 22) + 1), E_SIZE), (dict(vocab=0), E_SIZE),
+    (dict(tokens=0), E_SIZE), (dict(tokens=(1 << 22) + 1), E_SIZE),
+    (dict(tokens=1 << 22, vocab=(1 << 15) + 1), E_SIZE), (dict(vocab=0), E_SIZE),
     (dict(vocab=(1 << 24) + 1), E_SIZE), (dict(dim=0), E_SIZE), (dict(dim=12), E_SIZE),
     (dict(dim=(1 << 16) + 8), E_SIZE), (dict(x_stride=0), E_ARG), (dict(x_stride=12), E_ARG),
     (dict(weight_stride=0), E_ARG), (dict(weight_stride=(1 << 16) + 8), E_ARG),
@@ -158,6 +159,18 @@ def test_backward_refuses_small_workspaces_before_a_launch(lib, changes, code):
     assert lib.lct_cross_entropy_backward(_cross_entropy(), _gradients(**changes), None) == code
 
 
+def test_launches_of_too_many_workgroups_are_refused(lib):
+    # 256 tiles of channels by 32768 of tokens, and one of the vocabulary.
+    record = _cross_entropy(tokens=1 << 22, dim=1 << 16, x_stride=1 << 16, weight_stride=1 << 16)
+    assert lib.lct_cross_entropy_backward(record, _gradients(), None) == E_SIZE
+
+
+def test_tiles_of_an_orthogonalisation():
+    assert products.orthogonal_tiles(7, 256, 128) == 7
+    assert products.orthogonal_tiles(7, 129, 129) == 7 * 9
+    assert products.orthogonal_tiles(1, 257, 1) == 5
+
+
 def test_forward_refuses_small_workspaces_before_a_launch(lib):
     at = 1 << 20
 
@@ -181,6 +194,7 @@ def test_forward_refuses_small_workspaces_before_a_launch(lib):
     (dict(steps=-1), E_SIZE), (dict(type=3), E_ARG), (dict(type=-1), E_ARG),
     (dict(count=1 << 23), E_SIZE), (dict(count=1 << 23, rows=8, cols=8), E_SIZE),
     (dict(size=8 * 1024 + 12 * 136 * 136 - 1), E_SIZE),
+    (dict(cols=2048, size=8 * 1024 + 6 * 136 * (2048 + 136) + (1 << 25) - 1), E_SIZE),
     (dict(workspace=(1 << 20) + 8), E_ARG), (dict(workspace=None), E_NULL),
 ])
 def test_orthogonalize_entry_point_refuses_before_a_launch(lib, changes, code):

@@ -382,6 +382,11 @@ def test_refusals():
         args.update(changes)
         with pytest.raises(error):
             linear_cross_entropy(**args)
+    # Nothing is allocated for them.
+    few = torch.zeros(1, 8, dtype=BF16, device="cuda")
+    with pytest.raises(ValueError, match="tokens times vocabulary"):
+        linear_cross_entropy(few.expand(1 << 22, 8), few.expand((1 << 15) + 1, 8),
+                             targets.new_zeros(1).expand(1 << 22))
     with pytest.raises(RuntimeError, match="recorded"):
         torch.jit.trace(lambda a: linear_cross_entropy(a, weight, targets), x)
     with torch.autograd.forward_ad.dual_level():

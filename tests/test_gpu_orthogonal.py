@@ -156,6 +156,20 @@ def test_every_tile(count, rows, cols):
             assert torch.equal(out[first::2], out[first:first + 1].expand_as(out[first::2]))
 
 
+# The symmetric products' last tiles share their depth among workgroups: all 190 by 2, the last
+# 32 of 544 by 4.  A matrix's sums then are of an order that its place decides: each result is
+# near the exact one, but equal matrices' need not be equal.
+@pytest.mark.parametrize("count,rows,cols", [(1, 2432, 2440), (4, 2048, 2056)])
+def test_tiles_whose_depth_is_shared(count, rows, cols):
+    g = _matrix((1, rows, cols), "falling").to(BF16).cuda().expand(count, rows, cols).clone()
+    for steps in (4, 5):
+        out = orthogonalize(g, steps)
+        assert torch.equal(out, orthogonalize(g, steps))
+        exact = polar(g[0].cpu(), steps)
+        for got in out.cpu().double():
+            assert float((got - exact).norm() / exact.norm()) <= polar_off(steps)
+
+
 def test_streams_and_replays():
     g = _matrix((4, 200, 136)).to(BF16).cuda()
     eager = orthogonalize(g, 5)
@@ -195,6 +209,9 @@ def test_refusals():
         orthogonalize(g, 5, scale=float("nan"))
     with pytest.raises(ValueError, match="at most"):
         orthogonalize(torch.zeros(1, (1 << 16) + 1, device="cuda"))
+    for size in (1, 130):
+        with pytest.raises(ValueError, match="too many"):
+            orthogonalize(torch.zeros(1, 1, 1, device="cuda").expand(1 << 23, size, size))
     with pytest.raises(RuntimeError, match="recorded"):
         torch.jit.trace(lambda a: orthogonalize(a), g)
     # A result has no gradient, whoever asks.

@@ -85,6 +85,18 @@ def test_head_with_frozen_inputs(frozen):
         assert leaf.grad is None if i in frozen else torch.equal(leaf.grad, grad)
 
 
+def test_head_without_a_bias():
+    x, weight, gain, _, targets = _head()
+    leaves = [t.requires_grad_() for t in (x, weight, gain)]
+    out = layers.RMSLinearCrossEntropy.apply(*leaves, None, targets)
+    grads = torch.autograd.grad(out, leaves)
+    y, _ = layers._norm(x.detach(), gain.detach())
+    y.requires_grad_()
+    expected = linear_cross_entropy(y, weight, targets, reduction="sum")
+    assert torch.equal(out, expected)
+    assert torch.equal(grads[1], torch.autograd.grad(expected, weight)[0])
+
+
 def test_head_refuses_nothing_and_bad_targets():
     x, weight, gain, bias, targets = _head()
     with pytest.raises(ValueError, match="needs a token"):
