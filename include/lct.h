@@ -930,7 +930,7 @@ int32_t lct_dropout(const void *x, const void *residual, void *out, int64_t n, i
 #define LCT_MAX_CROSS_ENTROPY_VOCAB (1 << 24)
 #define LCT_MAX_CROSS_ENTROPY_DIM (1 << 16)
 #define LCT_MAX_CROSS_ENTROPY_LOGITS ((int64_t)1 << 37)    /* tokens * vocab */
-#define LCT_MAX_CROSS_ENTROPY_SPLITS 16
+#define LCT_MAX_CROSS_ENTROPY_SPLITS 32
 #define LCT_CROSS_ENTROPY_EXACT_TOKENS 128
 typedef struct {
     const void *x, *weight;

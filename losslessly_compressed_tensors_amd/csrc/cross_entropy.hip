@@ -29,11 +29,20 @@ constexpr float kHalfGradient = 16384.0f;
 // Where |z / s| may be squared in FP32; the cap is reached far below.
 constexpr float kCapped = 1e18f;
 
+// The tiles, two workgroups per compute unit.  Of operands by rows a step of 32 of k asks L2
+// for 64 bytes a row, and L2's requests bound the tile (counted: 0.83 of one per clock and
+// channel): a step is 64.  By columns a line is 256 or 512 bytes anyhow, and three steps of 32
+// leave the larger tile.  us of a step of 8192 x 50304 x 768 | 1013 x 50257 x 1024 | 16384 x
+// 100352 x 2048 with these: 2760 | 409 | 21608; logits by 256 x 128, three steps of 32: 2937 |
+// 439 | 23543; by 128 x 128, two of 64: 3065 | 439 | 22403; the products of dz by 128 x 128, two
+// of 64: 2873 | 421 | 23799.
 constexpr int kLogitRows = 192;
 template <bool kHalf>
 using LogitProduct = Product<kHalf, Lie::kRows, Lie::kRows, kLogitRows, 128, 2, 2, 64, 2>;
-// A few tokens, the vocabulary's rows streamed: us of 1 | 16 | 32 tokens against 50304 x 768
-// FEWNUMBERS
+// A few tokens, the vocabulary's rows streamed four steps ahead.  us of a call with this | the
+// wide tile: 50304 x 768, 1 token 26.2 | 26.3, 16 25.0 | 26.7, 32 24.9 | 27.2; 32000 x 4096, 1
+// token 64.8 | 80.3, 32 65.8 | 80.5.  The latter is 4.1 TB/s; of the former 14.6 us are the
+// kernel's (5.3 TB/s).
 constexpr int kFewTokens = 32;
 template <bool kHalf>
 using FewProduct = Product<kHalf, Lie::kRows, Lie::kRows, 128, kFewTokens, 4, 1, 64, 4>;
@@ -71,7 +80,8 @@ __device__ __forceinline__ void gather(const lct_cross_entropy &c, int32_t count
     if (count == c.tokens) return;
     const int32_t chunks = c.dim / 8;
     for (int64_t at = first; at < int64_t{count} * chunks; at += step) {
-        const int32_t i = static_cast<int32_t>(at / chunks), chunk = static_cast<int32_t>(at % chunks);
+        const int32_t i = static_cast<int32_t>(at / chunks);
+        const int32_t chunk = static_cast<int32_t>(at % chunks);
         static_cast<u32x4 *>(out)[at] = *reinterpret_cast<const u32x4 *>(
             static_cast<const uint16_t *>(c.x) + rows[i] * c.x_stride + chunk * 8);
     }
@@ -82,7 +92,9 @@ __global__ __launch_bounds__(256) void gather_kernel(lct_cross_entropy c, Counte
            int64_t{gridDim.x} * 256);
 }
 
-// 16-byte pieces of x up to which the one workgroup of prepare_kernel gathers itself.
+// 16-byte pieces of x up to which the one workgroup of prepare_kernel gathers itself.  us of a
+// call of 300 tokens with that | a launch of its own: 64 channels (2400 pieces) 23.0 | 26.1, 256
+// (9600) 23.2 | 26.0, 768 (28800) 33.6 | 26.5; of 1000 tokens of 256 (32000) 31.3 | 26.2.
 constexpr int64_t kGatherHere = 8192;
 
 // ---- the counted tokens, in order
@@ -182,7 +194,8 @@ __global__ __launch_bounds__(kPrepareThreads) void prepare_kernel(lct_cross_entr
                 if (grad != nullptr) {
                     const_cast<float *>(t.lse)[i] = lse[n];
                     const_cast<float *>(t.losses)[i] = losses[n];
-                    const_cast<float *>(t.factor)[i] = inside ? (g.per_token ? grad[n] / power : 1.0f) * hold : NAN;
+                    const float factor = g.per_token ? grad[n] / power : 1.0f;
+                    const_cast<float *>(t.factor)[i] = inside ? factor * hold : NAN;
                 }
             } else if (grad == nullptr) {
                 lse[n] = 0.0f;
@@ -196,8 +209,10 @@ __global__ __launch_bounds__(kPrepareThreads) void prepare_kernel(lct_cross_entr
         gather(c, done, rows, gathered, threadIdx.x, kPrepareThreads);
     if (threadIdx.x == 0) {
         *const_cast<int32_t *>(t.count) = done;
-        if (grad != nullptr)
-            *const_cast<float *>(t.scale) = (g.per_token ? power : *grad / (g.mean ? fmaxf(1.0f, done) : 1.0f)) / hold;
+        if (grad != nullptr) {
+            const float tokens = g.mean ? fmaxf(1.0f, done) : 1.0f;
+            *const_cast<float *>(t.scale) = (g.per_token ? power : *grad / tokens) / hold;
+        }
     }
 }
 
@@ -244,6 +259,11 @@ __device__ __forceinline__ bool far_of(const P &p, const Cap &cap) {
 
 // P::kM of the vocabulary (rows, in a lane's registers) by P::kN tokens (columns, a lane
 // each): a token's maximum and sum need one exchange between two lanes.
+//
+// Bound by the matrix instructions: 2 * tokens * vocab * dim operations, and the exponentials
+// behind them.  14746 x 100352 x 2048: 5.19 ms, 1170 TFLOP/s; 4095 x 32000 x 4096: 0.88 to 1.0
+// ms, 1220 to 1070; 8192 x 50304 x 768, capped: 640 to 730 us, 990 to 870 (12 steps a tile;
+// matrix instructions busy 0.52 of the time, at 1.84 GHz: the power limit's).
 template <class P, bool kCap, bool kBias>
 __global__ __launch_bounds__(P::kThreads, 2) void logits_kernel(lct_cross_entropy c, Counted t,
                                                                 int32_t vocab_tiles,
@@ -352,7 +372,7 @@ __global__ __launch_bounds__(P::kThreads, 2) void logits_kernel(lct_cross_entrop
 }
 
 // kWaves join one token's parts and compute its target's logit: the loss and lse (in powers
-// of two).
+// of two).  Reads the parts once, in flight together: 8192 x 526 in 16.3 us, 2.1 TB/s.
 template <bool kHalf, int kWaves>
 __global__ __launch_bounds__(256) void join_kernel(lct_cross_entropy c, Counted t, int32_t entries,
                                                    const Part *__restrict__ parts,
@@ -401,7 +421,8 @@ __global__ __launch_bounds__(256) void join_kernel(lct_cross_entropy c, Counted 
 #pragma unroll
     for (int d = kWave / 2; d > 0; d >>= 1) {
         logit += __shfl_xor(logit, d, kWave);
-        part = joined(part, Part{__shfl_xor(part.most, d, kWave), __shfl_xor(part.total, d, kWave)});
+        part = joined(part,
+                      Part{__shfl_xor(part.most, d, kWave), __shfl_xor(part.total, d, kWave)});
     }
     if constexpr (kWaves > 1) {
         if (lane == 0) {
@@ -477,6 +498,12 @@ __global__ __launch_bounds__(kPrepareThreads) void total_kernel(lct_cross_entrop
 // dz of P::kM tokens (rows) by P::kN of a piece of the vocabulary (columns, a lane each), the
 // logits computed again: written by columns, [vocabulary][token], which both products
 // that follow read, and its sums over these tokens.
+//
+// As the logits' kernel, and 2 bytes written a logit: a quarter of 8192 x 50304 x 768, capped,
+// 199 to 220 us, 800 to 710 TFLOP/s (matrix instructions busy 0.38 of the time, at 1.98 GHz; the
+// epilogue's exponential, root and stores take as long as the 12 steps); a thirteenth of 14746
+// x 100352 x 2048 466 us, 1000.  The parts a workgroup works in, of both on a compute unit,
+// overlap: starting half of them late, or stores past the caches, changed nothing.
 template <class P, bool kHalf, bool kCap, bool kBias>
 __global__ __launch_bounds__(P::kThreads, 2) void gradient_kernel(
     lct_cross_entropy c, Counted t, int32_t first_vocab, int32_t piece, int32_t vocab_tiles,
@@ -716,6 +743,9 @@ __device__ __forceinline__ void weight_gradient(const lct_cross_entropy &c, cons
 }
 
 // Both, one launch: neither has as many tiles as fill the compute units evenly.
+//
+// Bound by the matrix instructions: a quarter of 8192 x 50304 x 768 337 to 350 us, 940 to 905
+// TFLOP/s (busy 0.52, at 1.85 GHz); a thirteenth of 14746 x 100352 x 2048 835 us, 1120.
 template <bool kHalf, bool kExact>
 __global__ __launch_bounds__(256, 2) void products_kernel(lct_cross_entropy c, Counted t,
                                                           PieceProducts q, uint32_t weight_grid) {
@@ -827,7 +857,9 @@ int32_t tiles_of(int64_t n, int32_t tile) { return static_cast<int32_t>((n + til
 
 constexpr int32_t kMaxStrideGrid = 1 << 16;
 constexpr int64_t kMaxItems = int64_t{1} << 23;    // 256 threads each: below 2^32
-constexpr int32_t kWideJoin = 1024;    // tokens up to which four waves join one's parts
+// Tokens up to which four waves join one's parts.  us of a call with four | one: 50304 x 768, 64
+// tokens 26.2 | 27.9, 256 35.3 | 36.9, 1024 91.4 | 92.4, 2048 159.2 | 158.7, 4096 297.1 | 294.6.
+constexpr int32_t kWideJoin = 1024;
 
 uint32_t chunk_grid_of(const lct_cross_entropy &c) {
     return static_cast<uint32_t>(
@@ -931,7 +963,8 @@ extern "C" int32_t lct_cross_entropy_backward(const lct_cross_entropy *c,
         || d->gathered_size < tokens * c->dim
         || (products && d->dz_size < std::min(d->piece, c->vocab) * pitch * (exact ? 2 : 1))
         || (d->grad_x != nullptr && d->hidden_floats < d->splits * tokens * c->dim)
-        || (d->grad_bias != nullptr && d->bias_floats < int64_t{2} * tiles_of(tokens, 128) * c->vocab))
+        || (d->grad_bias != nullptr
+            && d->bias_floats < int64_t{2} * tiles_of(tokens, 128) * c->vocab))
         return LCT_E_SIZE;
     if (!aligned(d->gathered, 16) || !aligned(d->dz, 16) || !aligned(d->hidden_parts, 16)
         || !aligned(d->grad_x, 16) || !aligned(d->grad_weight, 16))

@@ -45,7 +45,8 @@ __device__ __forceinline__ void eight(const lct_orthogonal &o, int32_t matrix, i
                                       int32_t j, bool turned, float (&v)[8]) {
     const int64_t at = matrix * o.stride[0] + i * o.stride[1] + j * o.stride[2];
     const int64_t step = turned ? o.stride[1] : o.stride[2];
-    const int32_t left = (turned ? j < o.cols : i < o.rows) ? (turned ? o.rows - i : o.cols - j) : 0;
+    const bool inside = turned ? j < o.cols : i < o.rows;
+    const int32_t left = inside ? (turned ? o.rows - i : o.cols - j) : 0;
     const int32_t size = o.type == LCT_FP32 ? 4 : 2;
     const char *from = static_cast<const char *>(o.input) + at * size;
     if (left >= 8 && step == 1 && reinterpret_cast<uintptr_t>(from) % 16 == 0) {
@@ -317,7 +318,8 @@ __global__ __launch_bounds__(kWaves *kWave) void small_kernel(lct_orthogonal o) 
     constexpr int kThreads = kWaves * kWave, kRowBlocks = kRows / 32;
     constexpr int kTiles = kRowBlocks * (kCols / 32) / kWaves;
     // (More waves than squares: the last have none.)
-    constexpr int kSquares = kRowBlocks * kRowBlocks < kWaves ? 1 : kRowBlocks * kRowBlocks / kWaves;
+    constexpr int kSquares =
+        kRowBlocks * kRowBlocks < kWaves ? 1 : kRowBlocks * kRowBlocks / kWaves;
     constexpr int kPitch = kCols + kSmallPad, kSquarePitch = kRows + kSmallPad;
     static_assert(kTiles <= kRowBlocks && kSquares <= kRowBlocks);
     // At the start, what X's rounding leaves lies where A and P will.
@@ -513,7 +515,10 @@ __global__ __launch_bounds__(kWaves *kWave) void small_kernel(lct_orthogonal o) 
     }
 }
 
-// The smallest that holds the matrices.
+// The smallest that holds the matrices.  Bound by the steps' order: three products, each with
+// its barriers and its reads of LDS, of one compute unit.  Up to 256 of them run at once: 8 of
+// 96 x 160, 5 steps, 30.3 us (of which 12 without a step), where the launches for larger
+// matrices took 68; one of 64 x 64, 12 steps: 25 us.
 void small(const lct_orthogonal &o, hipStream_t stream) {
     const uint32_t count = static_cast<uint32_t>(o.count);
     if (o.rows <= 64 && o.cols <= 64) small_kernel<64, 64, 4><<<count, 256, 0, stream>>>(o);
@@ -598,6 +603,10 @@ struct SymmetricShare {
 template <class P>
 constexpr int kPartPieces = P::kRowTiles * P::kColumnTiles * 4;
 
+// Bound by the matrix instructions, and by what a tile's beginning and end cost beside few steps:
+// 48 x 768 x 768 (1008 tiles of 128 x 128, 12 steps of 64) 42.5 us, 600 TFLOP/s over the 21 of 36
+// tiles that are computed; 4096 x 4096 by 11008 212 us, 900.  One of 768 x 768 (78 tiles of 64 x
+// 64): 6.4 us, the latency of 12 steps and of a launch.
 template <class P, int kMore>
 __global__ __launch_bounds__(P::kThreads, 2) void symmetric_kernel(SymmetricTerms s,
                                                                    SymmetricShare share,
@@ -629,7 +638,8 @@ __global__ __launch_bounds__(P::kThreads, 2) void symmetric_kernel(SymmetricTerm
     p.begin();
     p.run(a, b, end - begin, stage0, stage1, stage2, stage3);
     if (part) {
-        f32x4 *to = share.parts + int64_t{blockIdx.x - share.whole_grid} * kPartPieces<P> * P::kThreads
+        f32x4 *to = share.parts
+                    + int64_t{blockIdx.x - share.whole_grid} * kPartPieces<P> * P::kThreads
                     + threadIdx.x;
 #pragma unroll
         for (int m = 0; m < P::kRowTiles; ++m)
@@ -683,6 +693,10 @@ __global__ __launch_bounds__(P::kThreads, 1) void symmetric_join_kernel(Symmetri
 // X <- share X + S X: P::kM columns of X (rows of the tile) by P::kN rows of X (columns, a lane
 // each).  The last step writes the result, scaled, in BF16 and G's orientation, if its
 // rows are whole 16-byte pieces.
+//
+// Bound by the products and by X's way in and out (4 bytes a value each way, through LDS), which
+// a tile's waves do one after the other: 48 x 768 x 768 82.5 us, 530 TFLOP/s; 4096 x 4096 by
+// 11008 395 us, 935; 16 x 1024 x 4096 221 us, 620.
 template <class P, bool kLast>
 __global__ __launch_bounds__(P::kThreads, P::kThreads == 256 ? 2 : 1) void update_kernel(
     const uint16_t *poly, const uint16_t *x, int32_t count, int32_t rows, int32_t cols,

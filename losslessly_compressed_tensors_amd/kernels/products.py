@@ -25,9 +25,13 @@ MAX_LOGITS = 1 << 37    # LCT_MAX_CROSS_ENTROPY_LOGITS
 
 _CUS = 256
 _SLOTS = 2 * _CUS       # workgroups of a product's kernel that run at once
-_MAX_SPLITS = 16        # LCT_MAX_CROSS_ENTROPY_SPLITS
 _EXACT_TOKENS = 128     # LCT_CROSS_ENTROPY_EXACT_TOKENS
 _PIECE_BYTES = 256 << 20
+# Parts of the sum for the gradient of x at most: 32 (LCT_MAX_CROSS_ENTROPY_SPLITS) where dz is
+# two numbers.  us of a step with 8 | 16 | 32 | 64 parts, 50304 x 768: 1 token 222 | 153 | 147 |
+# 149; 128: 246 | 178 | 152 | 169; 256: 189 | 158 | 165 | 177; 1024: 398 | 371 | 381 | 427.
+# 32000 x 4096: 32: 339 | 338 | 331 | 344; 512: 633 | 649 | 701 | 824.
+_MAX_SPLITS, _MAX_EXACT_SPLITS = 16, 32
 
 MAX_MATRIX_DIM = 1 << 16    # LCT_MAX_ORTHOGONAL_DIM
 MAX_TILES = 1 << 23         # LCT_MAX_ORTHOGONAL_TILES
@@ -135,9 +139,12 @@ def vocabulary_pieces(tokens: int, vocab: int, dim: int) -> tuple:
     piece = -(-vocab // (256 * pieces)) * 256
     dims = -(-dim // 256)
     hidden, weight = dims * -(-tokens // 128), dims * -(-piece // 128)
+    exact = tokens <= _EXACT_TOKENS
+    most, twice = (_MAX_EXACT_SPLITS, 2) if exact else (_MAX_SPLITS, 1)
     best = None
-    for splits in range(1, min(_MAX_SPLITS, max(1, piece // 512)) + 1):
-        time = _last_end(((weight, tokens / 32 + 8), (hidden * splits, piece / 32 / splits + 16)))
+    for splits in range(1, min(most, max(1, piece // 512)) + 1):
+        time = _last_end(((weight, twice * tokens / 32 + 8),
+                          (hidden * splits, twice * piece / 32 / splits + 16)))
         if best is None or time < best[0]:
             best = time, splits
     return piece, best[1]

@@ -150,7 +150,7 @@ def _gradients(grad=1 << 20, lse=1 << 20, losses=1 << 20, grad_x=1 << 20, grad_w
     (dict(index=0), E_NULL), (dict(values=0), E_NULL), (dict(gathered=0), E_NULL),
     (dict(dz=0), E_NULL), (dict(hidden=0), E_NULL), (dict(grad_bias=1 << 20), E_NULL),
     (dict(piece=0), E_SIZE), (dict(piece=100), E_SIZE), (dict(splits=0), E_SIZE),
-    (dict(splits=17), E_SIZE), (dict(index_size=6), E_SIZE), (dict(value_floats=9), E_SIZE),
+    (dict(splits=33), E_SIZE), (dict(index_size=6), E_SIZE), (dict(value_floats=9), E_SIZE),
     (dict(gathered_size=23), E_SIZE), (dict(dz_size=79), E_SIZE), (dict(hidden_floats=23), E_SIZE),
     (dict(gathered=(1 << 20) + 8), E_ARG), (dict(dz=(1 << 20) + 8), E_ARG),
     (dict(grad_x=(1 << 20) + 8), E_ARG), (dict(grad_weight=(1 << 20) + 2), E_ARG),
@@ -223,7 +223,7 @@ def test_records_have_the_headers_sizes():
 @pytest.mark.parametrize("dim", [8, 768, 4096])
 def test_pieces_cover_the_vocabulary_within_their_memory(tokens, vocab, dim):
     piece, splits = products.vocabulary_pieces(tokens, vocab, dim)
-    assert piece % 256 == 0 and piece > 0 and 1 <= splits <= 16
+    assert piece % 256 == 0 and piece > 0 and 1 <= splits <= (32 if tokens <= 128 else 16)
     # One tile's width is the least.
     assert 2 * tokens * (piece - 256) <= products._PIECE_BYTES
     assert piece - 256 < vocab or piece == 256
