@@ -34,8 +34,7 @@ constexpr float kCapped = 1e18f;
 // channel): a step is 64.  By columns a line is 256 or 512 bytes anyhow, and three steps of 32
 // leave the larger tile.  us of a step of 8192 x 50304 x 768 | 1013 x 50257 x 1024 | 16384 x
 // 100352 x 2048 with these: 2760 | 409 | 21608; logits by 256 x 128, three steps of 32: 2937 |
-// 439 | 23543; by 128 x 128, two of 64: 3065 | 439 | 22403; the products of dz by 128 x 128, two
-// of 64: 2873 | 421 | 23799.
+// 439 | 23543; by 128 x 128, two of 64: 3065 | 439 | 22403.
 constexpr int kLogitRows = 192;
 template <bool kHalf>
 using LogitProduct = Product<kHalf, Lie::kRows, Lie::kRows, kLogitRows, 128, 2, 2, 64, 2>;
@@ -46,10 +45,17 @@ using LogitProduct = Product<kHalf, Lie::kRows, Lie::kRows, kLogitRows, 128, 2, 
 constexpr int kFewTokens = 32;
 template <bool kHalf>
 using FewProduct = Product<kHalf, Lie::kRows, Lie::kRows, 128, kFewTokens, 4, 1, 64, 4>;
-template <bool kHalf>
-using HiddenProduct = Product<kHalf, Lie::kColumns, Lie::kColumns, 256, 128, 2, 2, 32, 3>;
-template <bool kHalf>
-using WeightProduct = Product<kHalf, Lie::kColumns, Lie::kRows, 256, 128, 2, 2, 32, 3>;
+// Of up to 128 tokens, with dz in two numbers (kExact), and of more: us of a step of 8192 x 50304
+// x 768 | 1013 x 50257 x 1024 | 16384 x 100352 x 2048 with 256 x 256 2737 | 402 | 21059, with the
+// smaller tile 2763 | 405 | 21708 (both with parts chosen for the latter).
+template <bool kHalf, Lie kLieB, bool kExact>
+using GradientProduct =
+    std::conditional_t<kExact, Product<kHalf, Lie::kColumns, kLieB, 256, 128, 2, 2, 32, 3>,
+                       Product<kHalf, Lie::kColumns, kLieB, 256, 256, 2, 4, 32, 4>>;
+template <bool kHalf, bool kExact>
+using HiddenProduct = GradientProduct<kHalf, Lie::kColumns, kExact>;
+template <bool kHalf, bool kExact>
+using WeightProduct = GradientProduct<kHalf, Lie::kRows, kExact>;
 
 // The counted tokens, as prepare_kernel found them.
 struct Counted {
@@ -657,14 +663,14 @@ struct PieceProducts {
     uint16_t *grad_weight;
 };
 
-// dx of a piece of the vocabulary, or of one of its parts: 256 channels (rows) by 128
-// tokens (columns), added to the earlier pieces' in FP32.
+// dx of a piece of the vocabulary, or of one of its parts: channels (rows) by tokens
+// (columns), added to the earlier pieces' in FP32.
 template <bool kHalf, bool kExact>
 __device__ __forceinline__ void hidden_gradient(const lct_cross_entropy &c, int32_t count,
                                                 const PieceProducts &q, int64_t item,
                                                 uint16_t *stage0, uint16_t *stage1,
                                                 uint16_t *stage2, uint16_t *stage3) {
-    using P = HiddenProduct<kHalf>;
+    using P = HiddenProduct<kHalf, kExact>;
     const int32_t dim_tile = static_cast<int32_t>(item % q.dim_tiles);
     const int32_t token_tile = static_cast<int32_t>(item / q.dim_tiles % q.token_tiles);
     const int32_t split = static_cast<int32_t>(item / q.dim_tiles / q.token_tiles);
@@ -707,13 +713,13 @@ __device__ __forceinline__ void hidden_gradient(const lct_cross_entropy &c, int3
     }
 }
 
-// dW of a piece: 256 channels (rows) by 128 of the vocabulary (columns).
+// dW of a piece: channels (rows) by vocabulary (columns).
 template <bool kHalf, bool kExact>
 __device__ __forceinline__ void weight_gradient(const lct_cross_entropy &c, const Counted &t,
                                                 int32_t count, const PieceProducts &q,
                                                 int64_t item, uint16_t *stage0, uint16_t *stage1,
                                                 uint16_t *stage2, uint16_t *stage3) {
-    using P = WeightProduct<kHalf>;
+    using P = WeightProduct<kHalf, kExact>;
     const int32_t dim_tile = static_cast<int32_t>(item % q.dim_tiles);
     const int32_t vocab_tile = static_cast<int32_t>(item / q.dim_tiles);
     int64_t x_stride;
@@ -747,11 +753,13 @@ __device__ __forceinline__ void weight_gradient(const lct_cross_entropy &c, cons
 // Bound by the matrix instructions: a quarter of 8192 x 50304 x 768 337 to 350 us, 940 to 905
 // TFLOP/s (busy 0.52, at 1.85 GHz); a thirteenth of 14746 x 100352 x 2048 835 us, 1120.
 template <bool kHalf, bool kExact>
-__global__ __launch_bounds__(256, 2) void products_kernel(lct_cross_entropy c, Counted t,
-                                                          PieceProducts q, uint32_t weight_grid) {
-    using P = HiddenProduct<kHalf>;
-    static_assert(P::kStage == WeightProduct<kHalf>::kStage
-                  && P::kStages == WeightProduct<kHalf>::kStages);
+__global__ __launch_bounds__(kExact ? 256 : 512, kExact ? 2 : 1) void products_kernel(
+    lct_cross_entropy c, Counted t, PieceProducts q, uint32_t weight_grid) {
+    using P = HiddenProduct<kHalf, kExact>;
+    static_assert(P::kThreads == (kExact ? 256 : 512)
+                  && P::kThreads == WeightProduct<kHalf, kExact>::kThreads);
+    static_assert(P::kStage == WeightProduct<kHalf, kExact>::kStage
+                  && P::kStages == WeightProduct<kHalf, kExact>::kStages);
     LCT_PRODUCT_STAGES(P);
     const int32_t count = *t.count;
     if (blockIdx.x < weight_grid) {
@@ -856,7 +864,7 @@ int32_t check(const lct_cross_entropy *c) {
 int32_t tiles_of(int64_t n, int32_t tile) { return static_cast<int32_t>((n + tile - 1) / tile); }
 
 constexpr int32_t kMaxStrideGrid = 1 << 16;
-constexpr int64_t kMaxItems = int64_t{1} << 23;    // 256 threads each: below 2^32
+constexpr int64_t kMaxItems = int64_t{1} << 22;    // 512 threads each: below 2^32
 // Tokens up to which four waves join one's parts.  us of a call with four | one: 50304 x 768, 64
 // tokens 26.2 | 27.9, 256 35.3 | 36.9, 1024 91.4 | 92.4, 2048 159.2 | 158.7, 4096 297.1 | 294.6.
 constexpr int32_t kWideJoin = 1024;
@@ -969,9 +977,10 @@ extern "C" int32_t lct_cross_entropy_backward(const lct_cross_entropy *c,
     if (!aligned(d->gathered, 16) || !aligned(d->dz, 16) || !aligned(d->hidden_parts, 16)
         || !aligned(d->grad_x, 16) || !aligned(d->grad_weight, 16))
         return LCT_E_ARG;
-    const int32_t dim_tiles = tiles_of(c->dim, 256), hidden_tiles = tiles_of(tokens, 128);
+    const int32_t tile = exact ? 128 : 256;    // of tokens and of the vocabulary
+    const int32_t dim_tiles = tiles_of(c->dim, 256), hidden_tiles = tiles_of(tokens, tile);
     if (int64_t{dim_tiles} * (int64_t{hidden_tiles} * d->splits
-                              + tiles_of(std::min(d->piece, c->vocab), 128)) > kMaxItems)
+                              + tiles_of(std::min(d->piece, c->vocab), tile)) > kMaxItems)
         return LCT_E_SIZE;
     Counted t{};
     int32_t *rows = d->index + 1, *targets = rows + tokens;
@@ -1003,20 +1012,24 @@ extern "C" int32_t lct_cross_entropy_backward(const lct_cross_entropy *c,
                                            d->grad_bias != nullptr ? d->bias_parts : nullptr);
         });
         if (!products) continue;
-        const PieceProducts q{first,    piece,       d->splits, dim_tiles,
-                              hidden_tiles, vocab_tiles, dz, rest, pitch,
-                              d->hidden_parts, static_cast<uint16_t *>(d->grad_weight)};
+        const int32_t weight_tiles = tiles_of(piece, tile);
+        const PieceProducts q{first,        piece,        d->splits, dim_tiles,
+                              hidden_tiles, weight_tiles, dz,        rest,
+                              pitch,        d->hidden_parts,
+                              static_cast<uint16_t *>(d->grad_weight)};
         const uint32_t weight_grid =
             d->grad_weight == nullptr
                 ? 0
-                : static_cast<uint32_t>(xcd_grid(int64_t{dim_tiles} * vocab_tiles));
+                : static_cast<uint32_t>(xcd_grid(int64_t{dim_tiles} * weight_tiles));
         const uint32_t hidden_grid =
             d->grad_x == nullptr
                 ? 0
                 : static_cast<uint32_t>(xcd_grid(int64_t{dim_tiles} * hidden_tiles * d->splits));
         const auto multiply = [&](auto half, auto both) {
-            products_kernel<decltype(half)::value, decltype(both)::value>
-                <<<weight_grid + hidden_grid, 256, 0, stream>>>(*c, t, q, weight_grid);
+            constexpr bool kHalf = decltype(half)::value, kBoth = decltype(both)::value;
+            products_kernel<kHalf, kBoth>
+                <<<weight_grid + hidden_grid, HiddenProduct<kHalf, kBoth>::kThreads, 0, stream>>>(
+                    *c, t, q, weight_grid);
         };
         const auto with = [&](auto half) {
             if (exact) multiply(half, std::true_type{});

@@ -24,14 +24,14 @@ MAX_DIM = 1 << 16       # LCT_MAX_CROSS_ENTROPY_DIM
 MAX_LOGITS = 1 << 37    # LCT_MAX_CROSS_ENTROPY_LOGITS
 
 _CUS = 256
-_SLOTS = 2 * _CUS       # workgroups of a product's kernel that run at once
 _EXACT_TOKENS = 128     # LCT_CROSS_ENTROPY_EXACT_TOKENS
 _PIECE_BYTES = 256 << 20
-# Parts of the sum for the gradient of x at most: 32 (LCT_MAX_CROSS_ENTROPY_SPLITS) where dz is
-# two numbers.  us of a step with 8 | 16 | 32 | 64 parts, 50304 x 768: 1 token 222 | 153 | 147 |
-# 149; 128: 246 | 178 | 152 | 169; 256: 189 | 158 | 165 | 177; 1024: 398 | 371 | 381 | 427.
-# 32000 x 4096: 32: 339 | 338 | 331 | 344; 512: 633 | 649 | 701 | 824.
-_MAX_SPLITS, _MAX_EXACT_SPLITS = 16, 32
+# Parts of the sum for the gradient of x, of which vocabulary_pieces chooses; 32
+# (LCT_MAX_CROSS_ENTROPY_SPLITS) at most.  us of a step with 1 | 2 | 4 | 8 | 16 | 32 parts,
+# 50304 x 768: 136 tokens 934 | 519 | 309 | 206 | 157 | 139; 1024: 1109 | 695 | 488 | 391 | 374 |
+# 384; 4096: 1750 | 1348 | 1219 | 1268 | 1363 | 1528; 8192: 2449 | 2525 | 2490 | 2643 | 2991 | 3744.
+# 32000 x 4096: 512: 1010 | 754 | 655 | 629 | 645 | 704.
+_SPLITS = 1, 2, 3, 4, 6, 8, 12, 16, 24, 32
 
 MAX_MATRIX_DIM = 1 << 16    # LCT_MAX_ORTHOGONAL_DIM
 MAX_TILES = 1 << 23         # LCT_MAX_ORTHOGONAL_TILES
@@ -116,38 +116,51 @@ def cross_entropy_forward(x: Tensor, weight: Tensor, bias, targets: Tensor, soft
     return out, stats
 
 
-def _last_end(lengths) -> float:
+def _last_end(lengths, slots: int) -> float:
     """When the last of (how many, how long) workgroups ends that start in this order,
     each as soon as one of the slots is free."""
-    free = [0.0] * _SLOTS
+    free = [0.0] * slots
     for count, length in lengths:
-        rounds = max(0, count // _SLOTS - 2)
+        rounds = max(0, count // slots - 2)
         if rounds:
             # As many for each slot, about: they stay as far apart.
             free = [t + rounds * length for t in free]
-        for _ in range(count - rounds * _SLOTS):
+        for _ in range(count - rounds * slots):
             heapreplace(free, free[0] + length)
     return max(free)
 
 
-@lru_cache(maxsize=1024)
-def vocabulary_pieces(tokens: int, vocab: int, dim: int) -> tuple:
-    """The size of a piece and the parts of its sum for the gradient of x: those with
-    which the products of a piece end first, by their steps of 32 and what a workgroup's
-    start, epilogue and part cost in those."""
-    pieces = -(-2 * vocab * tokens // _PIECE_BYTES)
-    piece = -(-vocab // (256 * pieces)) * 256
-    dims = -(-dim // 256)
-    hidden, weight = dims * -(-tokens // 128), dims * -(-piece // 128)
-    exact = tokens <= _EXACT_TOKENS
-    most, twice = (_MAX_EXACT_SPLITS, 2) if exact else (_MAX_SPLITS, 1)
+@lru_cache(maxsize=4096)
+def _parts(tokens: int, piece: int, vocab: int, dims: int) -> int:
+    """Into how many parts the sum for the gradient of x is divided: those with which a
+    piece's products end first, counted in their steps of 32."""
+    # The kernel for up to _EXACT_TOKENS takes tiles of 128, two at once per compute unit,
+    # and multiplies twice; that for more takes tiles of 256, one at once.
+    tile, at_once, twice = (128, 2, 2) if tokens <= _EXACT_TOKENS else (256, 1, 1)
+    hidden, weight = dims * -(-tokens // tile), dims * -(-piece // tile)
+    # A workgroup's start and end take about as long as 8 steps, reading what earlier pieces
+    # left likewise; a value of a part to write and add is 4e-6 of a step.  (Fitted to the
+    # times of 13 sizes: what is chosen is within 0.4 % of the best of each.)
+    ends = 8 * (2 - piece / max(piece, vocab))
     best = None
-    for splits in range(1, min(most, max(1, piece // 512)) + 1):
-        time = _last_end(((weight, twice * tokens / 32 + 8),
-                          (hidden * splits, twice * piece / 32 / splits + 16)))
+    for splits in _SPLITS:
+        if splits > max(1, piece // 512):
+            break
+        time = 4e-6 * splits * tokens * dims * 256 + _last_end(
+            ((weight, twice * tokens / 32 + 8),
+             (hidden * splits, twice * piece / 32 / splits + ends)),
+            at_once * _CUS)
         if best is None or time < best[0]:
             best = time, splits
-    return piece, best[1]
+    return best[1]
+
+
+def vocabulary_pieces(tokens: int, vocab: int, dim: int) -> tuple:
+    """The size of a piece and the parts of its sum for the gradient of x."""
+    pieces = -(-2 * vocab * tokens // _PIECE_BYTES)
+    piece = -(-vocab // (256 * pieces)) * 256
+    # (By whole tiles: choosing takes milliseconds.)
+    return piece, _parts(-(-tokens // 128) * 128, piece, vocab, -(-dim // 256))
 
 
 def cross_entropy_backward(grad: Tensor, x: Tensor, weight: Tensor, bias, targets: Tensor,

@@ -223,18 +223,18 @@ def test_records_have_the_headers_sizes():
 @pytest.mark.parametrize("dim", [8, 768, 4096])
 def test_pieces_cover_the_vocabulary_within_their_memory(tokens, vocab, dim):
     piece, splits = products.vocabulary_pieces(tokens, vocab, dim)
-    assert piece % 256 == 0 and piece > 0 and 1 <= splits <= (32 if tokens <= 128 else 16)
+    assert piece % 256 == 0 and piece > 0 and 1 <= splits <= 32
     # One tile's width is the least.
     assert 2 * tokens * (piece - 256) <= products._PIECE_BYTES
     assert piece - 256 < vocab or piece == 256
 
 
 def test_last_end_is_a_list_schedules():
-    assert products._last_end(((1, 5.0),)) == 5.0
-    assert products._last_end(((products._SLOTS, 5.0),)) == 5.0
-    assert products._last_end(((products._SLOTS + 1, 5.0),)) == 10.0
+    assert products._last_end(((1, 5.0),), 512) == 5.0
+    assert products._last_end(((512, 5.0),), 512) == 5.0
+    assert products._last_end(((513, 5.0),), 512) == 10.0
     # 3 slots' worth of long ones, the short ones in the others.
-    assert products._last_end(((3, 8.0), (2 * (products._SLOTS - 3), 4.0))) == 8.0
+    assert products._last_end(((3, 8.0), (2 * (256 - 3), 4.0)), 256) == 8.0
 
 
 def test_workspace_arrays_lie_apart_and_aligned():
