@@ -943,8 +943,8 @@ typedef struct {
 
 /* losses[n], and lse[n] for the backward call: log2 of sum_v exp(l[n][v]).  total: the
  * losses' sum, or with mean != 0 that over the number of tokens that count (one at
- * least); NULL: not written.  parts: working array of part_floats >= 4 * tokens *
- * ceil(vocab / 128), twice that for up to 32 tokens, 8-byte aligned.  index (1 + 2 *
+ * least); NULL: not written.  parts: working array of part_floats >= 8 * tokens *
+ * ceil(vocab / 256), of up to 32 tokens ceil(vocab / 128), 8-byte aligned.  index (1 + 2 *
  * tokens values) and gathered (tokens * dim values, 16-byte aligned): working arrays for
  * multiplying the tokens that count alone; NULL index: all are multiplied. */
 int32_t lct_cross_entropy_forward(const lct_cross_entropy *c, int32_t *index, int64_t index_size,

@@ -38,6 +38,13 @@ constexpr float kCapped = 1e18f;
 constexpr int kLogitRows = 192;
 template <bool kHalf>
 using LogitProduct = Product<kHalf, Lie::kRows, Lie::kRows, kLogitRows, 128, 2, 2, 64, 2>;
+// Deep products: us of a call with this | the tile above, of 8192 tokens 50176 x 768 612 | 582,
+// x 1024 758 | 748, x 1536 1066 | 1104, x 2048 1377 | 1439, 32000 x 4096 1703 | 1809; of 2048
+// tokens 50176 x 1536 306 | 298, 32000 x 4096 449 | 491; of 512 128 | 172; of 256 110 | 108, and 131072
+// x 2048 151 | 176.  One workgroup per compute unit, whose end no other's products hide.
+constexpr int32_t kDeep = 2048;
+template <bool kHalf>
+using DeepProduct = Product<kHalf, Lie::kRows, Lie::kRows, 256, 256, 4, 2, 64, 2>;
 // A few tokens, the vocabulary's rows streamed four steps ahead.  us of a call with this | the
 // wide tile: 50304 x 768, 1 token 26.2 | 26.3, 16 25.0 | 26.7, 32 24.9 | 27.2; 32000 x 4096, 1
 // token 64.8 | 80.3, 32 65.8 | 80.5.  The latter is 4.1 TB/s; of the former 14.6 us are the
@@ -271,7 +278,7 @@ __device__ __forceinline__ bool far_of(const P &p, const Cap &cap) {
 // ms, 1220 to 1070; 8192 x 50304 x 768, capped: 640 to 730 us, 990 to 870 (12 steps a tile;
 // matrix instructions busy 0.52 of the time, at 1.84 GHz: the power limit's).
 template <class P, bool kCap, bool kBias>
-__global__ __launch_bounds__(P::kThreads, 2) void logits_kernel(lct_cross_entropy c, Counted t,
+__global__ __launch_bounds__(P::kThreads, P::kThreads == 256 ? 2 : 1) void logits_kernel(lct_cross_entropy c, Counted t,
                                                                 int32_t vocab_tiles,
                                                                 int32_t token_tiles,
                                                                 Part *__restrict__ parts) {
@@ -882,6 +889,11 @@ void prepare(const lct_cross_entropy &c, const Counted &t, void *gathered,
     if (!here) gather_kernel<<<chunk_grid_of(c), 256, 0, stream>>>(c, t, gathered);
 }
 
+template <class T>
+struct Type {
+    using type = T;
+};
+
 template <class Launch>
 void by_form(const lct_cross_entropy &c, Launch launch) {
     const auto with = [&](auto half) {
@@ -908,10 +920,11 @@ extern "C" int32_t lct_cross_entropy_forward(const lct_cross_entropy *c, int32_t
                                              float *total, int32_t mean, hipStream_t stream) {
     if (const int32_t bad = check(c)) return bad;
     if (parts == nullptr || lse == nullptr || losses == nullptr) return LCT_E_NULL;
-    const bool few = c->tokens <= kFewTokens;
-    const int32_t vocab_tiles = tiles_of(c->vocab, few ? 128 : kLogitRows);
-    const int32_t token_tiles = tiles_of(c->tokens, few ? kFewTokens : 128);
-    const int32_t entries = (few ? 4 : 2) * vocab_tiles;
+    // (Up to 128 tokens would leave half of a deep tile without any.)
+    const bool few = c->tokens <= kFewTokens, deep = c->dim >= kDeep && c->tokens > 128;
+    const int32_t vocab_tiles = tiles_of(c->vocab, few ? 128 : deep ? 256 : kLogitRows);
+    const int32_t token_tiles = tiles_of(c->tokens, few ? kFewTokens : deep ? 256 : 128);
+    const int32_t entries = (few || deep ? 4 : 2) * vocab_tiles;
     if (part_floats < int64_t{2} * entries * c->tokens || !aligned(parts, 8)) return LCT_E_SIZE;
     Counted t{};
     if (index != nullptr) {
@@ -929,12 +942,14 @@ extern "C" int32_t lct_cross_entropy_forward(const lct_cross_entropy *c, int32_t
     auto *of = reinterpret_cast<Part *>(parts);
     by_form(*c, [&](auto half, auto cap, auto bias) {
         constexpr bool kHalf = decltype(half)::value;
-        if (few)
-            logits_kernel<FewProduct<kHalf>, decltype(cap)::value, decltype(bias)::value>
-                <<<grid, 256, 0, stream>>>(*c, t, vocab_tiles, token_tiles, of);
-        else
-            logits_kernel<LogitProduct<kHalf>, decltype(cap)::value, decltype(bias)::value>
-                <<<grid, 256, 0, stream>>>(*c, t, vocab_tiles, token_tiles, of);
+        const auto with = [&](auto product) {
+            using P = typename decltype(product)::type;
+            logits_kernel<P, decltype(cap)::value, decltype(bias)::value>
+                <<<grid, P::kThreads, 0, stream>>>(*c, t, vocab_tiles, token_tiles, of);
+        };
+        if (few) with(Type<FewProduct<kHalf>>{});
+        else if (deep) with(Type<DeepProduct<kHalf>>{});
+        else with(Type<LogitProduct<kHalf>>{});
     });
     const bool wide = c->tokens <= kWideJoin;
     const uint32_t joins = static_cast<uint32_t>(wide ? c->tokens : (c->tokens + 3) / 4);

@@ -92,7 +92,7 @@ def cross_entropy_forward(x: Tensor, weight: Tensor, bias, targets: Tensor, soft
     x, weight = _whole_rows(x), _whole_rows(weight)
     tokens, dim = x.shape
     device = x.device
-    floats = (8 if tokens <= _FEW_TOKENS else 4) * tokens * -(-weight.shape[0] // 128)
+    floats = 8 * tokens * -(-weight.shape[0] // (128 if tokens <= _FEW_TOKENS else 256))
     ints = 1 + 2 * tokens if tokens > _GATHER_TOKENS else 0
     halves = tokens * dim if ints else 0
     at = _places(4 * floats, 4 * ints, 2 * halves, 0 if keep else 8 * tokens)

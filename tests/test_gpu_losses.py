@@ -69,6 +69,16 @@ def test_sizes(tokens, vocab, dim, dtype, softcap):
     _check(x, weight, targets, bias if softcap else None, softcap=softcap)
 
 
+# From 2048 channels and 129 tokens on, the logits' tiles are 256 x 256.
+@pytest.mark.parametrize("softcap", [None, 15.0])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("tokens,vocab,dim", [(128, 300, 2048), (129, 255, 2048), (257, 513, 2056),
+                                              (300, 1100, 4096)])
+def test_deep_products(tokens, vocab, dim, dtype, softcap):
+    x, weight, targets, bias = _inputs(tokens, vocab, dim, dtype, bias=FP32)
+    _check(x, weight, targets, bias if softcap else None, softcap=softcap)
+
+
 @pytest.mark.parametrize("dim", [1, 2, 7, 13, 33, 70, 129])
 def test_odd_channels(dim):
     x, weight, targets, bias = _inputs(21, 67, dim, BF16, bias=FP32)
