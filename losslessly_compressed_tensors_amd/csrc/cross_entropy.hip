@@ -274,9 +274,9 @@ __device__ __forceinline__ bool far_of(const P &p, const Cap &cap) {
 // each): a token's maximum and sum need one exchange between two lanes.
 //
 // Bound by the matrix instructions: 2 * tokens * vocab * dim operations, and the exponentials
-// behind them.  14746 x 100352 x 2048: 5.19 ms, 1170 TFLOP/s; 4095 x 32000 x 4096: 0.88 to 1.0
-// ms, 1220 to 1070; 8192 x 50304 x 768, capped: 640 to 730 us, 990 to 870 (12 steps a tile;
-// matrix instructions busy 0.52 of the time, at 1.84 GHz: the power limit's).
+// behind them.  14746 x 100352 x 2048: 5.02 ms, 1210 TFLOP/s (at 1.3 GHz: the power limit's);
+// 4095 x 32000 x 4096: 0.83 to 0.93 ms, 1290 to 1150; 8192 x 50304 x 768, capped: 624 to 730 us,
+// 1010 to 870 (12 steps a tile; matrix instructions busy 0.54 of the time, at 1.81 GHz).
 template <class P, bool kCap, bool kBias>
 __global__ __launch_bounds__(P::kThreads, P::kThreads == 256 ? 2 : 1) void logits_kernel(lct_cross_entropy c, Counted t,
                                                                 int32_t vocab_tiles,
@@ -757,8 +757,9 @@ __device__ __forceinline__ void weight_gradient(const lct_cross_entropy &c, cons
 
 // Both, one launch: neither has as many tiles as fill the compute units evenly.
 //
-// Bound by the matrix instructions: a quarter of 8192 x 50304 x 768 337 to 350 us, 940 to 905
-// TFLOP/s (busy 0.52, at 1.85 GHz); a thirteenth of 14746 x 100352 x 2048 835 us, 1120.
+// Bound by the matrix instructions: a quarter of 8192 x 50304 x 768 314 us, 1010 TFLOP/s (96
+// tiles 400 steps deep and 150 of 256 fill the compute units to three quarters); a thirteenth of
+// 14746 x 100352 x 2048 794 us, 1180.
 template <bool kHalf, bool kExact>
 __global__ __launch_bounds__(kExact ? 256 : 512, kExact ? 2 : 1) void products_kernel(
     lct_cross_entropy c, Counted t, PieceProducts q, uint32_t weight_grid) {
