@@ -415,22 +415,39 @@ def test_several_pieces_and_many_token_tiles(dtype, monkeypatch):
         _check(x, weight, targets, bias, softcap=30.0)
 
 
-def test_offsets_past_32_bits():
-    """A vocabulary's matrix and a piece of more than 2^32 bytes."""
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_several_pieces_of_few_tokens(dtype, monkeypatch):
+    from losslessly_compressed_tensors_amd.kernels import products
+    x, weight, targets, bias = _inputs(101, 2000, 96, dtype, bias=FP32, ignored=0.1)
+    for piece, splits in ((256, 1), (512, 3), (768, 32), (2048, 7)):
+        monkeypatch.setattr(products, "vocabulary_pieces", lambda *a: (piece, splits))
+        _check(x, weight, targets, bias, softcap=30.0)
+
+
+@pytest.mark.parametrize("tokens", [1, 100, 200])
+def test_many_parts(tokens):
+    x, weight, targets, bias = _inputs(tokens, 17000, 64, BF16, bias=FP32)
+    _check(x, weight, targets, bias, reduction="sum")
+
+
+# Up to 128 tokens, and more: other tiles of all products.
+@pytest.mark.parametrize("tokens", [40, 150])
+def test_offsets_past_32_bits(tokens):
+    """A vocabulary's matrix, and its gradient, of more than 2^32 bytes."""
     dim, vocab = 4096, (1 << 19) + 321
     weight = torch.zeros(vocab, dim, dtype=BF16, device="cuda")
-    x = torch.zeros(40, dim, dtype=BF16, device="cuda")
+    x = torch.zeros(tokens, dim, dtype=BF16, device="cuda")
     x[:, 0] = 1.0
     weight[:, 0] = torch.linspace(-4, 4, vocab, device="cuda").to(BF16)
-    targets = torch.arange(vocab - 40, vocab, device="cuda")
+    targets = torch.arange(vocab - tokens, vocab, device="cuda")
     leaves = [x.requires_grad_(), weight.requires_grad_()]
     out = linear_cross_entropy(*leaves, targets, reduction="sum")
     grads = torch.autograd.grad(out, leaves)
     z = weight.detach()[:, 0].double()
     lse = torch.logsumexp(z, 0)
-    exact = 40 * lse - z[targets].sum()
+    exact = tokens * lse - z[targets].sum()
     assert abs(float(out) - float(exact)) < 1e-4 * float(exact)
-    p = 40 * (z - lse).exp()
+    p = tokens * (z - lse).exp()
     p[targets] -= 1.0
     assert_within(grads[1][:, 0], p.cpu(), (2.0 ** -6 * p.abs() + 1e-12).cpu(), "grad_weight")
     assert not grads[1][:, 1:].any()
