@@ -29,6 +29,8 @@ _MODULES = (
     "components.layers",
     "components.attention",
     "components.dropout",
+    "components.losses",
+    "components.orthogonal",
     "components.sparse_utils",
 )
 

@@ -48,8 +48,8 @@ from losslessly_compressed_tensors_amd.components.attention import (
 from losslessly_compressed_tensors_amd.components.dropout import dropout_add
 from losslessly_compressed_tensors_amd.components.layers import (
     Embedding, FlashAttention, Linear, RMSLinear, RMSLinearCrossEntropy, RMSNormFunction,
-    Relu2Linear, WindowAttention, compress_weight, dense_weight, flush_saved, named_trainable_tensors, prefetch_saved,
-    prefetch_weights, queued_saved, rms_norm_qkv,
+    Relu2Linear, WindowAttention, compress_weight, dense_weight, flush_saved,
+    named_trainable_tensors, prefetch_saved, prefetch_weights, queued_saved, rms_norm_qkv,
 )
 from losslessly_compressed_tensors_amd.components.sparse_utils import SparseAdamW, SparseMuon
 from losslessly_compressed_tensors_amd.tensor_buffer import TensorBuffer, _free_regions_snapshot

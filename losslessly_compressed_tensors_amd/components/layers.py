@@ -34,7 +34,8 @@ from .ops import rms_norm, rms_norm_backward
 
 __all__ = [
     "dense_weight", "prefetch_weights", "RMSLinear", "rms_norm_qkv", "RMSNormFunction",
-    "RMSLinearCrossEntropy", "Relu2Linear", "FlashAttention", "WindowAttention", "compress_weight", "Linear", "Embedding",
+    "RMSLinearCrossEntropy", "Relu2Linear", "FlashAttention", "WindowAttention",
+    "compress_weight", "Linear", "Embedding",
     "named_trainable_tensors", "flush_saved", "queued_saved", "prefetch_saved",
     "batch_saved_compression",
 ]

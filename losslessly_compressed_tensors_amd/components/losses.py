@@ -112,7 +112,8 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, targets: Tensor, bias: Tenso
     "none" for each token's loss.  Differentiable in ``x``, ``weight`` and ``bias``.
 
     No logits are kept: forward needs 16 bytes per token and 128 of the vocabulary
-    (of up to 32 tokens: twice that), backward their gradient in 16 bits for up to 256 MiB of the vocabulary at a time.
+    (of up to 32 tokens: twice that), backward their gradient in 16 bits for as much of
+    the vocabulary at a time as 256 MiB hold, and parts of the gradient of ``x`` in FP32.
     Logits, softmax and sums are FP32; the logits' gradients are rounded to 16 bits for
     their products with ``weight`` and ``x`` (of up to 128 tokens, kept in two numbers)."""
     softcap, ignore_index = check_cross_entropy(x, weight, targets, bias, softcap, ignore_index,

@@ -40,8 +40,8 @@ template <bool kHalf>
 using LogitProduct = Product<kHalf, Lie::kRows, Lie::kRows, kLogitRows, 128, 2, 2, 64, 2>;
 // Deep products: us of a call with this | the tile above, of 8192 tokens 50176 x 768 612 | 582,
 // x 1024 758 | 748, x 1536 1066 | 1104, x 2048 1377 | 1439, 32000 x 4096 1703 | 1809; of 2048
-// tokens 50176 x 1536 306 | 298, 32000 x 4096 449 | 491; of 512 128 | 172; of 256 110 | 108, and 131072
-// x 2048 151 | 176.  One workgroup per compute unit, whose end no other's products hide.
+// tokens 50176 x 1536 306 | 298, 32000 x 4096 449 | 491; of 512 128 | 172; of 256 110 | 108, and
+// 131072 x 2048 151 | 176.  One workgroup per compute unit, whose end no other's products hide.
 constexpr int32_t kDeep = 2048;
 template <bool kHalf>
 using DeepProduct = Product<kHalf, Lie::kRows, Lie::kRows, 256, 256, 4, 2, 64, 2>;
@@ -278,10 +278,9 @@ __device__ __forceinline__ bool far_of(const P &p, const Cap &cap) {
 // 4095 x 32000 x 4096: 0.83 to 0.93 ms, 1290 to 1150; 8192 x 50304 x 768, capped: 624 to 730 us,
 // 1010 to 870 (12 steps a tile; matrix instructions busy 0.54 of the time, at 1.81 GHz).
 template <class P, bool kCap, bool kBias>
-__global__ __launch_bounds__(P::kThreads, P::kThreads == 256 ? 2 : 1) void logits_kernel(lct_cross_entropy c, Counted t,
-                                                                int32_t vocab_tiles,
-                                                                int32_t token_tiles,
-                                                                Part *__restrict__ parts) {
+__global__ __launch_bounds__(P::kThreads, P::kThreads == 256 ? 2 : 1) void logits_kernel(
+    lct_cross_entropy c, Counted t, int32_t vocab_tiles, int32_t token_tiles,
+    Part *__restrict__ parts) {
     LCT_PRODUCT_STAGES(P);
     const int32_t count = t.count == nullptr ? c.tokens : *t.count;
     const int64_t item = xcd_item(int64_t{vocab_tiles} * token_tiles, blockIdx.x);

@@ -772,7 +772,8 @@ int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
 // | 1807 | 1779 | 1814; of 4096 x 4096 (528, 1024): 2380 | 1780 | 1698 | 1680; of 4096 x
 // 11008: | 3347 | 3217 | 3112.
 template <int kSize>
-using Symmetric = Product<true, Lie::kRows, Lie::kRows, kSize, kSize, 2, 2, 64, kSize == 64 ? 4 : 2>;
+using Symmetric =
+    Product<true, Lie::kRows, Lie::kRows, kSize, kSize, 2, 2, 64, kSize == 64 ? 4 : 2>;
 template <int kM, int kN, int kWavesN, int kStep, int kStages>
 using Update = Product<true, Lie::kColumns, Lie::kRows, kM, kN, 2, kWavesN, kStep, kStages>;
 constexpr int64_t kFewTiles = 160, kManyTiles = 800;   // of 128 x 128

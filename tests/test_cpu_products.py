@@ -241,6 +241,13 @@ def test_workspace_arrays_lie_apart_and_aligned():
     assert products._places(1, 0, 300, 256) == [0, 256, 256, 768, 1024]
 
 
+def test_the_packages_paths_are_the_modules():
+    import LCT.components.losses
+    import LCT.components.orthogonal
+    assert LCT.components.losses.linear_cross_entropy is linear_cross_entropy
+    assert LCT.components.orthogonal.orthogonalize is orthogonalize
+
+
 def test_muon_takes_the_option():
     p = torch.nn.Parameter(torch.zeros(4, 4))
     assert SparseMuon([p], compressed=False).fused is False
