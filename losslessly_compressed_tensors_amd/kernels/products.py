@@ -46,7 +46,14 @@ def _whole_rows(t: Tensor) -> Tensor:
     an address that the kernels read; zeros where it has to be widened."""
     rows, cols = t.shape
     if cols % 8:
-        out = t.new_zeros(rows, -(-cols // 8) * 8)
+        # Zeros in the last columns alone, where writing the others twice costs more than one
+        # more call: us of a call, either | all zeros first: 7 tokens against 53276 x 911 62 |
+        # 89, 2 against 37334 x 2250 with gradients 469 | 516, 37 against 307 x 71 202 | 194.
+        if rows * cols < 1 << 20:
+            out = t.new_zeros(rows, _up8(cols))
+        else:
+            out = t.new_empty(rows, _up8(cols))
+            out[:, cols:] = 0
         out[:, :cols] = t
         return out
     stride = t.stride(0) if rows > 1 else cols

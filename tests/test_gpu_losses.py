@@ -85,6 +85,12 @@ def test_odd_channels(dim):
     _check(x, weight, targets, bias, reduction="sum")
 
 
+def test_odd_channels_of_many_words():
+    # (Matrices of a million values are widened another way.)
+    x, weight, targets, bias = _inputs(130, 8200, 129, BF16, bias=FP32)
+    _check(x, weight, targets, bias)
+
+
 @pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
 @pytest.mark.parametrize("ignored", [0.0, 0.4, 1.0])
 @pytest.mark.parametrize("dtype", [BF16, FP16])
