@@ -911,9 +911,11 @@ extern "C" int32_t lct_orthogonalize(const lct_orthogonal *o, void *workspace,
     start_kernel<<<static_cast<uint32_t>(count * tiles), 256, 0, stream>>>(
         *o, parts, norms, it.rows, it.cols, it.x, it.x_rest);
     const int inner = o->out_stride[2] == 1 ? 2 : 1;
-    const int64_t length = inner == 2 ? o->cols : o->rows;
-    const bool whole = o->out_stride[inner] == 1 && length % 8 == 0
-                       && o->out_stride[3 - inner] % 8 == 0 && o->out_stride[0] % 8 == 0
+    const int64_t length = inner == 2 ? o->cols : o->rows, line = o->out_stride[3 - inner];
+    // (A tile's lines are addressed by 32-bit byte offsets: finish_kernel has no such limit.)
+    const bool whole = o->out_stride[inner] == 1 && length % 8 == 0 && line % 8 == 0
+                       && line >= length && line <= LCT_MAX_ORTHOGONAL_DIM
+                       && o->out_stride[0] % 8 == 0
                        && reinterpret_cast<uintptr_t>(o->out) % 16 == 0;
     // Two steps at once have 3 products with X, of rows^2 cols each, in place of 6 and 5 in
     // place of 2 of rows^3, the symmetric ones by half.  us of 12 or 5 steps one | two at a time:

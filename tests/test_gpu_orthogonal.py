@@ -7,6 +7,7 @@ import torch
 
 from gpu_util import require_gpu
 from losslessly_compressed_tensors_amd.components.orthogonal import orthogonalize
+from losslessly_compressed_tensors_amd.kernels import hip
 from product_oracle import polar, polar_floor, polar_off
 
 pytestmark = pytest.mark.gpu
@@ -216,3 +217,26 @@ def test_refusals():
         torch.jit.trace(lambda a: orthogonalize(a), g)
     # A result has no gradient, whoever asks.
     assert not orthogonalize(g.requires_grad_()).requires_grad
+
+
+# Lines of the result whose stride the tiles' stores take, or more than they take, past 32 bits
+# of bytes within a tile, or backwards: with rows or columns adjacent.
+@pytest.mark.parametrize("line", [272, 1 << 16, (1 << 16) + 8, 1 << 26, -272, -(1 << 26)])
+@pytest.mark.parametrize("tall", [False, True])
+def test_results_of_any_strides(tall, line):
+    rows, cols, steps = 136, 264, 3
+    g = _matrix((rows, cols)).to(BF16).cuda()
+    expected = orthogonalize(g, steps)
+    lines, length = (cols, rows) if tall else (rows, cols)
+    out = torch.full((lines, abs(line)), 7.0, dtype=BF16, device="cuda")
+    first = out.data_ptr() + (2 * (lines - 1) * -line if line < 0 else 0)
+    strides = (1, line) if tall else (line, 1)
+    workspace = torch.empty(1 << 23, dtype=torch.uint8, device="cuda")
+    record = hip.ORTHOGONAL.pack(g.data_ptr(), first, rows * cols, cols, 1, 0, *strides, 1, rows,
+                                 cols, steps, hip.BF16, 1.0, 1e-7)
+    hip.call("lct_orthogonalize", record, workspace.data_ptr(), workspace.numel(),
+             torch.cuda.current_stream().cuda_stream)
+    got = out[:, :length].flip(0) if line < 0 else out[:, :length]
+    assert torch.equal(got.mT if tall else got, expected)
+    for i in range(lines):
+        assert not (out[i, length:] != 7).any()
