@@ -13,10 +13,10 @@ import math
 
 import torch
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
 from ..kernels import products as kernels
 from .attention import _check_like, _check_memory, _check_tensor, _recorded, _whole
+from .autograd import first_order
 
 __all__ = ["linear_cross_entropy"]
 
@@ -37,24 +37,15 @@ class _LinearCrossEntropy(torch.autograd.Function):
         return out.clone() if reduction == "none" else out
 
     @staticmethod
+    @first_order
     def backward(ctx, grad):
-        # With a graph of the backward pass asked for, a second one is an error.
-        if torch.is_grad_enabled():
-            return _backward_once(ctx, grad)
-        return _backward(ctx, grad)
-
-
-def _backward(ctx, grad):
-    x, weight, bias, targets, stats = ctx.saved_tensors
-    grad_x, grad_weight, grad_bias = kernels.cross_entropy_backward(
-        grad.contiguous(), x, weight, None if bias is None else bias.float(), targets, stats,
-        *ctx.how, ctx.needs_input_grad[:3])
-    if grad_bias is not None:
-        grad_bias = grad_bias.to(bias.dtype)
-    return grad_x, grad_weight, grad_bias, None, None, None, None
-
-
-_backward_once = once_differentiable(_backward)
+        x, weight, bias, targets, stats = ctx.saved_tensors
+        grad_x, grad_weight, grad_bias = kernels.cross_entropy_backward(
+            grad.contiguous(), x, weight, None if bias is None else bias.float(), targets, stats,
+            *ctx.how, ctx.needs_input_grad[:3])
+        if grad_bias is not None:
+            grad_bias = grad_bias.to(bias.dtype)
+        return grad_x, grad_weight, grad_bias, None, None, None, None
 
 
 def check_cross_entropy(x, weight, targets, bias, softcap, ignore_index, reduction) -> tuple:

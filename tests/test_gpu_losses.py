@@ -457,3 +457,19 @@ def test_offsets_past_32_bits(tokens):
     p[targets] -= 1.0
     assert_within(grads[1][:, 0], p.cpu(), (2.0 ** -6 * p.abs() + 1e-12).cpu(), "grad_weight")
     assert not grads[1][:, 1:].any()
+
+
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_gradients_of_a_loss_are_no_constants(reduction):
+    """The incoming gradient is one here, which needs no gradient: a penalty on the loss's
+    gradient is refused, not left out."""
+    x, weight, targets, bias = _inputs(30, 60, 32, BF16, bias=FP32)
+    for at in range(3):
+        leaves = [t.cuda().requires_grad_(i == at) for i, t in enumerate((x, weight, bias))]
+        loss = linear_cross_entropy(leaves[0], leaves[1], targets.cuda(), leaves[2],
+                                    reduction=reduction)
+        plain, = torch.autograd.grad(loss.sum(), leaves[at], retain_graph=True)
+        grad, = torch.autograd.grad(loss.sum(), leaves[at], create_graph=True)
+        assert torch.equal(grad, plain)
+        with pytest.raises(RuntimeError, match="differentiated once only"):
+            (loss.sum() + grad.float().square().sum()).backward()
