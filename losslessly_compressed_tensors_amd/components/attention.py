@@ -28,6 +28,7 @@ from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from ..kernels import attention as kernels
+from .autograd import first_order
 
 __all__ = ["Rotary", "rotary_frequencies", "rotary_magnitude", "trainer_frequencies",
            "apply_rotary", "rotary_append", "window_attention", "decode_attention", "KVCache"]
@@ -335,19 +336,11 @@ class _WindowAttention(torch.autograd.Function):
         return out
 
     @staticmethod
+    @first_order
     def backward(ctx, grad):
-        if torch.is_grad_enabled():
-            return _attention_backward_once(ctx, grad)
-        return _attention_backward(ctx, grad)
-
-
-def _attention_backward(ctx, grad):
-    q, k, v, out, lse, lengths = ctx.saved_tensors
-    return (*kernels.attention_backward(grad, q, k, v, out, lse, *ctx.sight, lengths), None, None,
-            None, None)
-
-
-_attention_backward_once = once_differentiable(_attention_backward)
+        q, k, v, out, lse, lengths = ctx.saved_tensors
+        return (*kernels.attention_backward(grad, q, k, v, out, lse, *ctx.sight, lengths), None,
+                None, None, None)
 
 
 def check_attention(q, k, v, window, sinks, scale, lengths) -> tuple:

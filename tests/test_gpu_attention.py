@@ -546,3 +546,16 @@ def test_parts_of_one_kind_of_key_block(dim, splits, sink_splits, monkeypatch):
         assert bool(guarded.memory[floats:].isnan().all())
         # Every part's keys that exist are written: the last block's others are not.
         assert int(guarded.memory[:floats].isnan().sum()) <= floats // 2
+
+
+def test_gradients_of_a_sum_of_attention_are_no_constants():
+    """An incoming gradient of ones needs no gradient: a second derivative is refused, not left
+    out."""
+    for at in range(3):
+        leaves = [_values(1, 2, 9, 64).requires_grad_(i == at) for i in range(3)]
+        out = attention.window_attention(*leaves, window=4).float().sum()
+        plain, = torch.autograd.grad(out, leaves[at], retain_graph=True)
+        grad, = torch.autograd.grad(out, leaves[at], create_graph=True)
+        assert torch.equal(grad, plain)
+        with pytest.raises(RuntimeError, match="differentiated once only"):
+            (out + grad.float().square().sum()).backward()
