@@ -28,6 +28,7 @@ from ..kernels import fused
 from ..kernels import products
 from ..operations import compress, compress_batch, decompress
 from .attention import check_attention
+from .autograd import first_order
 from .dist_configs import act_dist, act_relu_dist, weight_dist
 from .losses import check_cross_entropy
 from .ops import rms_norm, rms_norm_backward
@@ -253,6 +254,7 @@ class RMSLinearCrossEntropy(torch.autograd.Function):
         return out.clone().view(targets.shape) if reduction == "none" else out
 
     @staticmethod
+    @first_order
     def backward(ctx, grad):
         norm_weight, rstd, weight, bias, targets, stats = ctx.saved_tensors
         x = ctx.saved.take()

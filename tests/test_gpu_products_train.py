@@ -220,3 +220,23 @@ def test_no_logits_are_kept():
     peak = torch.cuda.max_memory_allocated() - before
     # In 16 bits: 393 MiB.  Here: a piece of their gradient, parts, sums, both gradients.
     assert peak < 2 * tokens * vocab
+
+
+@pytest.mark.parametrize("reduction", ["sum", "none"])
+def test_heads_gradients_are_no_constants(reduction):
+    """A second derivative is refused: neither the loss's kernels nor the norm's saved values
+    have one."""
+    values = _head()
+    for at in range(4):
+        leaves = [t.detach().clone().requires_grad_(i == at) for i, t in enumerate(values[:4])]
+
+        def loss():
+            return layers.RMSLinearCrossEntropy.apply(*leaves, values[4], None, False, None, 1024,
+                                                      15.0, -100, reduction).sum()
+
+        plain, = torch.autograd.grad(loss(), leaves[at])
+        out = loss()
+        grad, = torch.autograd.grad(out, leaves[at], create_graph=True)
+        assert torch.equal(grad, plain)
+        with pytest.raises(RuntimeError, match="differentiated once only"):
+            grad.float().square().sum().backward()
