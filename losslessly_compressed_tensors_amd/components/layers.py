@@ -212,6 +212,7 @@ class RMSLinear(torch.autograd.Function):
         return output
 
     @staticmethod
+    @first_order
     def backward(ctx, grad):
         norm_weight, rstd, weight = ctx.saved_tensors
         x = ctx.saved.take()
@@ -294,6 +295,7 @@ class _RMSNormQKV(torch.autograd.Function):
         return outputs
 
     @staticmethod
+    @first_order
     def backward(ctx, grad_q, grad_k, grad_v):
         norm_weight, rstd, *weights = ctx.saved_tensors
         x = ctx.saved.take()
@@ -335,6 +337,7 @@ class RMSNormFunction(torch.autograd.Function):
         return output
 
     @staticmethod
+    @first_order
     def backward(ctx, grad):
         gains, rstd = ctx.saved_tensors
         x = ctx.saved.take()
@@ -367,6 +370,7 @@ class Relu2Linear(torch.autograd.Function):
         return output
 
     @staticmethod
+    @first_order
     def backward(ctx, grad):
         weight, = ctx.saved_tensors
         relu = ctx.saved.take()
@@ -424,6 +428,7 @@ class FlashAttention(torch.autograd.Function):
         return output
 
     @staticmethod
+    @first_order
     def backward(ctx, grad_output):
         q, k, v, out = ctx.state.unpack()
         batch, heads, length, head_dim = q.shape
@@ -462,6 +467,7 @@ class WindowAttention(torch.autograd.Function):
         return output
 
     @staticmethod
+    @first_order
     def backward(ctx, grad_output):
         q, k, v, out = ctx.state.unpack()
         batch, heads, length, head_dim = q.shape

@@ -14,6 +14,7 @@ import torch
 from torch import Tensor
 
 from ..kernels import fused
+from .autograd import first_order
 
 
 def _forward(x: Tensor, gain: Tensor | None) -> tuple[Tensor, Tensor]:
@@ -44,6 +45,7 @@ class _RMSNorm(torch.autograd.Function):
         return y, rstd
 
     @staticmethod
+    @first_order
     def backward(ctx, grad, grad_rstd):
         x, rstd, gain = ctx.saved_tensors
         return rms_norm_backward(grad, x, rstd, gain)
