@@ -980,8 +980,8 @@ int32_t lct_cross_entropy_backward(const lct_cross_entropy *c,
  * X) after `steps` of X <- 2 X + (-3/2 A + 1/2 A A) X, A = X X^T, from X = G / (|G|_F +
  * eps), for `count` matrices G of rows <= cols <= LCT_MAX_ORTHOGONAL_DIM (a tall one is
  * passed transposed).  input: type LCT_BF16, LCT_FP16 or LCT_FP32; strides in elements of
- * matrix, row and column, out's likewise.  X is the sum of two FP16 numbers, the products'
- * operands FP16 at powers of two, sums FP32, the norm FP64.  workspace (16-byte aligned):
+ * matrix, row and column, out's likewise.  X is held in two FP16 numbers (23 bits), the
+ * products' operands are FP16 at powers of two, sums FP32, the norm FP64.  workspace (16-byte aligned):
  * with both dimensions rounded up to 8, count * (8 LCT_ORTHOGONAL_NORM_PARTS + 6 rows cols
  * + 6 rows^2) bytes, and LCT_ORTHOGONAL_SPLIT_BYTES where there are
  * LCT_ORTHOGONAL_SPLIT_DEPTH columns; none, and NULL, for matrices within

@@ -3,7 +3,7 @@
 ``components/sparse_utils.py``'s ``zeropower_via_newtonschulz5`` (the reference's,
 ``LCT/components/sparse_utils.py:71-86``) iterates in BF16 on the library's products.
 :func:`orthogonalize` computes the same polynomial with the symmetric products by
-half and the iterate in 22 bits; ``SparseMuon(fused=True)`` steps with it.
+half and the iterate in 32 bits; ``SparseMuon(fused=True)`` steps with it.
 """
 from __future__ import annotations
 
@@ -28,12 +28,16 @@ def orthogonalize(G: Tensor, steps: int = 5, *, scale: float = 1.0) -> Tensor:
     strides; BF16, contiguous, in ``G``'s orientation.
 
     Each matrix is divided by its Frobenius norm plus 1e-7, then ``steps`` times ``X <- 2 X
-    + (-1.5 A + 0.5 A A) X`` with ``A = X X^T`` (of a tall one: transposed).  X is kept in
-    22 bits between steps, and the products' operands are FP16 at fixed powers of two:
-    results are within 1.5e-3 of the exact iteration's norm, the rounding to BF16 (1.7e-3)
-    aside, for matrices of a norm of 1e-11 or more.  A call's results are the same in every
-    run; in another batch, or at another place of it, a matrix's may differ in roundings.
-    Not differentiable."""
+    + (-1.5 A + 0.5 A A) X`` with ``A = X X^T`` (of a tall one: transposed).  X is held in 32
+    bits (two FP16 numbers), the products' operands are FP16 at fixed powers of two, their
+    sums FP32.  Results, their rounding to BF16 (1.7e-3) aside, are off by up to 7e-4
+    sqrt(steps) of the exact iteration's norm (2e-4 sqrt(steps) of matrices of a hundred rows
+    or more), whatever the norm of ``G``.  In directions in which ``G`` has next to nothing,
+    FP32's roundings double with each step, as they do in any FP32 iteration: a matrix of
+    rank 1 ends another 2^(steps - 22) of the norm off, 1e-3 after 12 steps but 1e-2 after
+    16, so that steps past about 14 are for matrices of full rank.  A call's results are the
+    same in every run; in another batch, or at another place of it, a matrix's may differ in
+    roundings.  Not differentiable."""
     if not isinstance(G, Tensor) or G.ndim < 2:
         raise TypeError("G must be a torch.Tensor of at least two dimensions")
     _check_tensor(G, "G", G.ndim, tuple(kernels.TYPES))

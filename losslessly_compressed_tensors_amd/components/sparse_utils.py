@@ -28,7 +28,7 @@ How this build runs them on one MI355X:
   GPT-2-small step's 72 block matrices form two groups (48 of 768x768, 24 of
   768x3072), so 12 iterations take 72 GEMM launches instead of 2592.  With
   ``fused=True`` the iteration is ``components/orthogonal.py``'s kernels, whose
-  iterate is kept in 22 bits.
+  iterate is held in 32 bits.
 * **Multi-tensor AdamW.**  Parameters with the same dtype and step count are
   updated together with ``torch._foreach_*`` operations.
 * **No host synchronisation.**  Scalars that the fused kernels read live on

@@ -8,14 +8,17 @@
 // Three products a step, each a launch over all matrices: A and P are symmetric, so
 // tiles above the diagonal are not computed but written from below it.
 //
-// X is kept in 22 bits, as the sum of two FP16 numbers; the products take the first of
-// them, and A and P in FP16, all at fixed powers of two.  Small singular directions only
+// X is held in 32 bits, as the sum of two FP16 numbers, the second at 2^11 times the first's
+// power of two: 23 bits, rounded 1.5 times as far off as FP32 (root mean square), and what is
+// below FP16's range in the first number is in the second's.  The products take the first
+// of them, and A and P in FP16, all at fixed powers of two.  Small singular directions only
 // double in the early steps.  What rounds X itself adds noise in all directions, and the
 // steps that follow double that too: with X in 16 bits, 12 steps of a matrix whose
 // singular values fall off as 1/i end 0.1 (BF16) or 0.01 (FP16) of the norm away.  P X is
 // small in the small directions on either side, so that rounding P's and X's operands
-// there is harmless: 4e-4.  No value exceeds 1 by more than roundings, so FP16's range
-// suffices and its three more bits are free.
+// there is harmless: 4e-4.  Near the end, where P is -1, each step leaves what its operands'
+// rounding took from X: 2e-4 sqrt(steps) of the norm after many.  No value exceeds 1 by more
+// than roundings, so FP16's range suffices and its three more bits are free.
 #include <algorithm>
 
 #include "product_core.h"
@@ -26,6 +29,8 @@ namespace {
 constexpr float kA = 2.0f, kB = -1.5f, kC = 0.5f;
 // The operands' powers of two: X within 1 + 2^-8 (2^10 of 65504), A likewise, |P| <= 1.2.
 constexpr float kHoldX = 1024.0f, kHoldA = 4096.0f;
+// X's second number, over the first's: at most half a step of that, 2^-12 of 2^10.
+constexpr float kHoldRest = 2048.0f;
 
 using Half = Element<true>;
 
@@ -155,9 +160,14 @@ __global__ __launch_bounds__(256) void norm_kernel(lct_orthogonal o, int32_t par
     if (threadIdx.x == 0) out[blockIdx.x] = sums[0] + sums[1] + sums[2] + sums[3];
 }
 
-// Two adjacent values as FP16, and what that leaves.
+// X's second number of two adjacent values, whose first ones are `pair`.
 __device__ __forceinline__ uint32_t rest(float x, float y, uint32_t pair) {
-    return Half::round_pair(x - Half::low(pair), y - Half::high(pair));
+    return Half::round_pair((x - Half::low(pair)) * kHoldRest, (y - Half::high(pair)) * kHoldRest);
+}
+
+// 2^10 X of both numbers.
+__device__ __forceinline__ float both(float first, float second) {
+    return __builtin_fmaf(1.0f / kHoldRest, second, first);
 }
 
 // X from G, in rows of whole 16-byte pieces; zeros in what both dimensions are widened by.
@@ -224,8 +234,8 @@ __global__ __launch_bounds__(256) void finish_kernel(lct_orthogonal o, int32_t r
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
             const uint32_t pair =
-                Element<false>::round_pair((Half::low(p[n]) + Half::low(q[n])) * factor,
-                                           (Half::high(p[n]) + Half::high(q[n])) * factor);
+                Element<false>::round_pair(both(Half::low(p[n]), Half::low(q[n])) * factor,
+                                           both(Half::high(p[n]), Half::high(q[n])) * factor);
             tile[i][j + 2 * n] = static_cast<uint16_t>(pair);
             tile[i][j + 2 * n + 1] = static_cast<uint16_t>(pair >> 16);
         }
@@ -322,7 +332,7 @@ __global__ __launch_bounds__(kWaves *kWave) void small_kernel(lct_orthogonal o) 
         kRowBlocks * kRowBlocks < kWaves ? 1 : kRowBlocks * kRowBlocks / kWaves;
     constexpr int kPitch = kCols + kSmallPad, kSquarePitch = kRows + kSmallPad;
     static_assert(kTiles <= kRowBlocks && kSquares <= kRowBlocks);
-    // At the start, what X's rounding leaves lies where A and P will.
+    // At the start, X's second number lies where A and P will.
     constexpr int kSquareValues = kRows * kSquarePitch;
     constexpr int kRest = kRows * kPitch > 2 * kSquareValues ? kRows * kPitch : 2 * kSquareValues;
     __shared__ __attribute__((aligned(16))) uint16_t operand[kRows * kPitch];
@@ -409,8 +419,9 @@ __global__ __launch_bounds__(kWaves *kWave) void small_kernel(lct_orthogonal o) 
             const u32x2 q = *reinterpret_cast<const u32x2 *>(squares + at + 8 * g);
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                x[t][4 * g + 2 * r] = (Half::low(p[r]) + Half::low(q[r])) * (1.0f / kHoldX);
-                x[t][4 * g + 2 * r + 1] = (Half::high(p[r]) + Half::high(q[r])) * (1.0f / kHoldX);
+                x[t][4 * g + 2 * r] = both(Half::low(p[r]), Half::low(q[r])) * (1.0f / kHoldX);
+                x[t][4 * g + 2 * r + 1] =
+                    both(Half::high(p[r]), Half::high(q[r])) * (1.0f / kHoldX);
             }
         }
     }
@@ -729,11 +740,12 @@ __global__ __launch_bounds__(P::kThreads, P::kThreads == 256 ? 2 : 1) void updat
                         p.sum[m][n][r + 1] = __builtin_fmaf(1.0f / kHoldA, p.sum[m][n][r + 1],
                                                             share * Half::high(old));
                     });
+    const float share_rest = share * (1.0f / kHoldRest);
     load_columns<P>(x_rest + at, cols, rows - row, cols - column, mine,
                     [&](int m, int n, int r, uint32_t old) __attribute__((always_inline)) {
-                        p.sum[m][n][r] = __builtin_fmaf(share, Half::low(old), p.sum[m][n][r]);
+                        p.sum[m][n][r] = __builtin_fmaf(share_rest, Half::low(old), p.sum[m][n][r]);
                         p.sum[m][n][r + 1] =
-                            __builtin_fmaf(share, Half::high(old), p.sum[m][n][r + 1]);
+                            __builtin_fmaf(share_rest, Half::high(old), p.sum[m][n][r + 1]);
                     });
     if constexpr (kLast) {
         const float factor = o.scale * (1.0f / kHoldX);
@@ -889,7 +901,7 @@ extern "C" int32_t lct_orthogonalize(const lct_orthogonal *o, void *workspace,
     if (count * tiles >= LCT_MAX_ORTHOGONAL_TILES) return LCT_E_SIZE;
     const int32_t parts =
         static_cast<int32_t>(std::min<int64_t>(LCT_ORTHOGONAL_NORM_PARTS, (tiles + 3) / 4));
-    // Norms, X as it is and to be, what X's rounding leaves, and three square matrices.
+    // Norms, X's first number as it is and to be, its second, and three square matrices.
     const int64_t norm_bytes = count * LCT_ORTHOGONAL_NORM_PARTS * 8;
     // (Parts of up to kSlots tiles.)
     const int64_t part_bytes = cols >= kSplitDepth ? LCT_ORTHOGONAL_SPLIT_BYTES : 0;

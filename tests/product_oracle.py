@@ -134,3 +134,20 @@ def polar_floor(steps, values) -> float:
     FP16's smallest: X times 2^10 is held to half of their spacing, 2^-25, and a step at most
     doubles what the steps before have left: 2^-35 (1 + 2 + .. + 2^steps) a value."""
     return values ** 0.5 * 2.0 ** (steps + 1 - 35)
+
+
+def polar_rest_floor(steps, values) -> float:
+    """:func:`polar_floor` with what the second number of X holds: that is 2^11 larger than the
+    first, so half of the spacing of its smallest is 2^-46 of X."""
+    return polar_floor(steps, values) * 2.0 ** -11
+
+
+def polar_off_in_empty_directions(steps, rows) -> float:
+    """What a matrix of rank 1 may be off beside :func:`polar_off`, relative to the norm: in
+    directions that it does not have, what a step rounds is doubled by each step after it.
+
+    A step's sums of `rows` products (FP32, 16 at a time) are off by 2^-23 of what they have
+    come to, half of 1.2 |X| on average, each time; adding 2 X and X's two numbers round by
+    2^-24 and 2^-23 of 2 |X| and |X|: ((rows / 16 + 1) 0.6 + 2) 2^-23 of |X| = 1 at most.
+    Steps are independent: sqrt(4^steps + 4^(steps - 1) + ..) = 1.16 2^steps of that."""
+    return 1.16 * 2.0 ** steps * ((rows / 16 + 1) * 0.6 + 2) * 2.0 ** -23

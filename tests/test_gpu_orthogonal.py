@@ -8,7 +8,9 @@ import torch
 from gpu_util import require_gpu
 from losslessly_compressed_tensors_amd.components.orthogonal import orthogonalize
 from losslessly_compressed_tensors_amd.kernels import hip
-from product_oracle import polar, polar_floor, polar_off
+from product_oracle import (
+    polar, polar_floor, polar_off, polar_off_in_empty_directions, polar_rest_floor,
+)
 
 pytestmark = pytest.mark.gpu
 BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
@@ -240,3 +242,33 @@ def test_results_of_any_strides(tall, line):
     assert torch.equal(got.mT if tall else got, expected)
     for i in range(lines):
         assert not (out[i, length:] != 7).any()
+
+
+@pytest.mark.parametrize("size", [1e-11, 1e-13, 1e-14, 1e-16])
+@pytest.mark.parametrize("rows,cols", [(72, 136), (300, 300), (264, 1000), (2048, 2048)])
+def test_norms_far_below_eps(rows, cols, size):
+    """X is then small as a whole, and held to its own precision all the same."""
+    g = _matrix((rows, cols))
+    g *= size / g.norm()
+    out = orthogonalize(g.cuda(), 5)
+    exact = polar(g, 5)
+    off = (out.cpu().double() - exact).norm()
+    assert off <= polar_off(5) * exact.norm() + polar_rest_floor(5, rows * cols)
+
+
+@pytest.mark.parametrize("shape", [(96, 160), (300, 140), (256, 256), (768, 768)])
+@pytest.mark.parametrize("steps", [14, 16, 18])
+def test_directions_that_a_matrix_does_not_have(steps, shape):
+    """FP32's roundings there double with every step."""
+    g = _matrix(shape, "rank 1")
+    exact = polar(g, steps)
+    off = float((orthogonalize(g.cuda(), steps).cpu().double() - exact).norm() / exact.norm())
+    assert off <= polar_off(steps) + polar_off_in_empty_directions(steps, min(shape))
+
+
+@pytest.mark.parametrize("shape", [(96, 160), (160, 96), (300, 300)])
+@pytest.mark.parametrize("steps", [30, 101, 300])
+def test_many_steps(steps, shape):
+    g = _matrix(shape)
+    _assert_polar(orthogonalize(g.cuda(), steps), g, steps)
+    assert polar_off(300) < 0.03      # (a bound that says something)
