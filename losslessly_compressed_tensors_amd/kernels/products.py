@@ -162,9 +162,15 @@ def _parts(tokens: int, piece: int, vocab: int, dims: int) -> int:
     return best[1]
 
 
+def _dz_values(tokens: int) -> int:
+    """Values of the logits' gradients per word: whole 16-byte pieces, twice where what
+    rounding them leaves is kept."""
+    return _up8(tokens) * (2 if tokens <= _EXACT_TOKENS else 1)
+
+
 def vocabulary_pieces(tokens: int, vocab: int, dim: int) -> tuple:
     """The size of a piece and the parts of its sum for the gradient of x."""
-    pieces = -(-2 * vocab * tokens // _PIECE_BYTES)
+    pieces = -(-vocab * _dz_values(tokens) * 2 // _PIECE_BYTES)
     piece = -(-vocab // (256 * pieces)) * 256
     # (By whole tiles: choosing takes milliseconds.)
     return piece, _parts(-(-tokens // 128) * 128, piece, vocab, -(-dim // 256))
@@ -188,7 +194,7 @@ def cross_entropy_backward(grad: Tensor, x: Tensor, weight: Tensor, bias, target
     ints, floats, halves = 1 + 2 * tokens, 1 + 3 * tokens, tokens * width
     dz_size = 0
     if need_x or need_weight:
-        dz_size = min(piece, vocab) * _up8(tokens) * (2 if tokens <= _EXACT_TOKENS else 1)
+        dz_size = min(piece, vocab) * _dz_values(tokens)
     hidden_floats = splits * tokens * width if need_x else 0
     bias_floats = 2 * -(-tokens // 128) * vocab if need_bias else 0
     *places, size = _places(4 * ints, 4 * floats, 2 * halves, 2 * dz_size, 4 * hidden_floats,

@@ -252,3 +252,13 @@ def test_muon_takes_the_option():
     p = torch.nn.Parameter(torch.zeros(4, 4))
     assert SparseMuon([p], compressed=False).fused is False
     assert SparseMuon([p], compressed=False, fused=True).fused is True
+
+
+@pytest.mark.parametrize("tokens", [1, 8, 37, 128, 129, 4096])
+@pytest.mark.parametrize("vocab", [50304, (1 << 20) + 7, 1 << 24])
+def test_both_numbers_of_a_piece_are_within_its_memory(tokens, vocab):
+    """Of up to 128 tokens the logits' gradients are held in two numbers, each token's in whole
+    pieces of eight."""
+    piece, _ = products.vocabulary_pieces(tokens, vocab, 64)
+    numbers = 2 if tokens <= 128 else 1
+    assert 2 * numbers * -(-tokens // 8) * 8 * (piece - 256) <= 256 << 20
