@@ -932,6 +932,7 @@ int32_t lct_dropout(const void *x, const void *residual, void *out, int64_t n, i
 #define LCT_MAX_CROSS_ENTROPY_LOGITS ((int64_t)1 << 37)    /* tokens * vocab */
 #define LCT_MAX_CROSS_ENTROPY_SPLITS 32
 #define LCT_CROSS_ENTROPY_EXACT_TOKENS 128
+#define LCT_CROSS_ENTROPY_BIAS_TOKENS 192
 typedef struct {
     const void *x, *weight;
     const float *bias;
@@ -959,8 +960,8 @@ int32_t lct_cross_entropy_forward(const lct_cross_entropy *c, int32_t *index, in
  * Working arrays: index (1 + 2 * tokens), values (1 + 3 * tokens), gathered (tokens * dim
  * 16-bit values), dz (min(piece, vocab) * (tokens rounded up to 8) 16-bit values,
  * twice that for up to LCT_CROSS_ENTROPY_EXACT_TOKENS), hidden_parts (splits * tokens *
- * dim), bias_parts (2 * ceil(tokens / 128) * vocab); those of 16 bits and hidden_parts
- * 16-byte aligned. */
+ * dim), bias_parts (2 * ceil(tokens / LCT_CROSS_ENTROPY_BIAS_TOKENS) * vocab); those of 16
+ * bits and hidden_parts 16-byte aligned. */
 typedef struct {
     const float *grad, *lse, *losses;
     void *grad_x, *grad_weight;

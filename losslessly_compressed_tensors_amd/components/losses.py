@@ -104,7 +104,11 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, targets: Tensor, bias: Tenso
 
     No logits are kept: forward needs 16 bytes per token and 128 of the vocabulary
     (of up to 32 tokens: twice that), backward their gradient in 16 bits for as much of
-    the vocabulary at a time as 256 MiB hold, and parts of the gradient of ``x`` in FP32.
+    the vocabulary at a time as 256 MiB hold (256 words at least), 1 to 32 parts of the
+    gradient of ``x`` in FP32 (the more, the fewer tokens), and of ``bias``'s gradient 8 bytes
+    per 192 tokens and word.  Both directions also take a copy of ``x`` (forward of more than
+    256 tokens), whether all tokens count or not, and with channels that are no multiple of 8
+    widened copies of ``x``, ``weight`` and their gradients.
     Logits, softmax and sums are FP32; the logits' gradients are rounded to 16 bits for
     their products with ``weight`` and ``x`` (of up to 128 tokens, kept in two numbers)."""
     softcap, ignore_index = check_cross_entropy(x, weight, targets, bias, softcap, ignore_index,

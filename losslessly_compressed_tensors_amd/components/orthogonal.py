@@ -37,7 +37,10 @@ def orthogonalize(G: Tensor, steps: int = 5, *, scale: float = 1.0) -> Tensor:
     rank 1 ends another 2^(steps - 22) of the norm off, 1e-3 after 12 steps but 1e-2 after
     16, so that steps past about 14 are for matrices of full rank.  A call's results are the
     same in every run; in another batch, or at another place of it, a matrix's may differ in
-    roundings.  Not differentiable."""
+    roundings.  Not differentiable.
+
+    Matrices past 128 x 256 need 6 bytes per value and per value of ``X X^T`` and 8 KiB each
+    (with 2048 columns 32 MiB more) while the call runs."""
     if not isinstance(G, Tensor) or G.ndim < 2:
         raise TypeError("G must be a torch.Tensor of at least two dimensions")
     _check_tensor(G, "G", G.ndim, tuple(kernels.TYPES))

@@ -35,7 +35,7 @@ constexpr float kCapped = 1e18f;
 // leave the larger tile.  us of a step of 8192 x 50304 x 768 | 1013 x 50257 x 1024 | 16384 x
 // 100352 x 2048 with these: 2760 | 409 | 21608; logits by 256 x 128, three steps of 32: 2937 |
 // 439 | 23543; by 128 x 128, two of 64: 3065 | 439 | 22403.
-constexpr int kLogitRows = 192;
+constexpr int kLogitRows = LCT_CROSS_ENTROPY_BIAS_TOKENS;
 template <bool kHalf>
 using LogitProduct = Product<kHalf, Lie::kRows, Lie::kRows, kLogitRows, 128, 2, 2, 64, 2>;
 // Deep products: us of a call with this | the tile above, of 8192 tokens 50176 x 768 612 | 582,
@@ -987,7 +987,7 @@ extern "C" int32_t lct_cross_entropy_backward(const lct_cross_entropy *c,
         || (products && d->dz_size < std::min(d->piece, c->vocab) * pitch * (exact ? 2 : 1))
         || (d->grad_x != nullptr && d->hidden_floats < d->splits * tokens * c->dim)
         || (d->grad_bias != nullptr
-            && d->bias_floats < int64_t{2} * tiles_of(tokens, 128) * c->vocab))
+            && d->bias_floats < int64_t{2} * token_tiles * c->vocab))
         return LCT_E_SIZE;
     if (!aligned(d->gathered, 16) || !aligned(d->dz, 16) || !aligned(d->hidden_parts, 16)
         || !aligned(d->grad_x, 16) || !aligned(d->grad_weight, 16))

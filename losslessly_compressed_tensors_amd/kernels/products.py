@@ -25,6 +25,7 @@ MAX_LOGITS = 1 << 37    # LCT_MAX_CROSS_ENTROPY_LOGITS
 
 _CUS = 256
 _EXACT_TOKENS = 128     # LCT_CROSS_ENTROPY_EXACT_TOKENS
+_BIAS_TOKENS = 192      # LCT_CROSS_ENTROPY_BIAS_TOKENS
 _PIECE_BYTES = 256 << 20
 # Parts of the sum for the gradient of x, of which vocabulary_pieces chooses; 32
 # (LCT_MAX_CROSS_ENTROPY_SPLITS) at most.  us of a step with 1 | 2 | 4 | 8 | 16 | 32 parts,
@@ -196,7 +197,7 @@ def cross_entropy_backward(grad: Tensor, x: Tensor, weight: Tensor, bias, target
     if need_x or need_weight:
         dz_size = min(piece, vocab) * _dz_values(tokens)
     hidden_floats = splits * tokens * width if need_x else 0
-    bias_floats = 2 * -(-tokens // 128) * vocab if need_bias else 0
+    bias_floats = 2 * -(-tokens // _BIAS_TOKENS) * vocab if need_bias else 0
     *places, size = _places(4 * ints, 4 * floats, 2 * halves, 2 * dz_size, 4 * hidden_floats,
                             4 * bias_floats)
     memory = torch.empty(size, dtype=torch.uint8, device=x.device)

@@ -262,3 +262,13 @@ def test_both_numbers_of_a_piece_are_within_its_memory(tokens, vocab):
     piece, _ = products.vocabulary_pieces(tokens, vocab, 64)
     numbers = 2 if tokens <= 128 else 1
     assert 2 * numbers * -(-tokens // 8) * 8 * (piece - 256) <= 256 << 20
+
+
+def test_the_biases_parts_are_a_tile_of_tokens_each(lib):
+    """Two of 192 tokens and a word: no fewer, and no more are asked for."""
+    record = _cross_entropy(tokens=1000, bias=1 << 20)
+    for floats, hidden, code in ((2 * 6 * 5 - 1, 1 << 40, E_SIZE), (2 * 6 * 5, 1 << 40, E_ARG)):
+        # (An odd address, which is looked at behind the sizes.)
+        gradients = _gradients(grad_bias=1 << 20, columns=1 << 20, bias_floats=floats,
+                               hidden_floats=hidden, dz=(1 << 20) + 8)
+        assert lib.lct_cross_entropy_backward(record, gradients, None) == code

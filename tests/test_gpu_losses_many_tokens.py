@@ -102,3 +102,30 @@ def test_a_trainers_size(ignored):
     assert_within(out, exact.total.cpu(), exact.total_off.cpu(), "total")
     for name, got in zip(("grad_x", "grad_weight", "grad_bias"), grads):
         assert_within(got, getattr(exact, name).cpu(), getattr(exact, name + "_off").cpu(), name)
+
+
+def _backward_peak(tokens, vocab, dim):
+    x = torch.randn(tokens, dim, device="cuda").to(BF16).requires_grad_()
+    weight = torch.randn(vocab, dim, device="cuda").to(BF16).requires_grad_()
+    bias = torch.zeros(vocab, device="cuda", requires_grad=True)
+    loss = linear_cross_entropy(x, weight, torch.zeros(tokens, dtype=torch.int64, device="cuda"),
+                                bias, reduction="sum")
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    grads = torch.autograd.grad(loss, (x, weight, bias))
+    return (torch.cuda.max_memory_allocated() - before
+            - sum(g.numel() * g.element_size() for g in grads))
+
+
+@pytest.mark.parametrize("tokens,vocab,dim", [(1, (1 << 22) + 5, 8), (128, (1 << 21) + 5, 8),
+                                              (24000, 30000, 16), (4096, 50304, 256)])
+def test_memory_as_stated(tokens, vocab, dim):
+    piece, splits = products.vocabulary_pieces(tokens, vocab, dim)
+    stated = (2 * tokens * dim                          # the counted tokens' x
+              + (256 << 20) + 512 * (tokens + 7)        # the logits' gradients: a tile more
+              + 4 * splits * tokens * dim               # parts of grad_x
+              + 8 * -(-tokens // 192) * vocab           # of the bias's gradient
+              + 20 * tokens + 8)                        # lists
+    assert splits <= 32
+    assert _backward_peak(tokens, vocab, dim) <= stated + (1 << 20)     # (alignment)
