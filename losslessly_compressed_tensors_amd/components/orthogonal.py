@@ -45,8 +45,8 @@ def orthogonalize(G: Tensor, steps: int = 5, *, scale: float = 1.0) -> Tensor:
         raise TypeError("G must be a torch.Tensor of at least two dimensions")
     _check_tensor(G, "G", G.ndim, tuple(kernels.TYPES))
     steps = _whole(steps, "steps", 0, 1000)
-    if not math.isfinite(scale):
-        raise ValueError("scale must be finite")
+    if not abs(scale) <= torch.finfo(torch.float32).max:
+        raise ValueError("scale must be finite, in FP32")
     rows, cols = G.shape[-2:]
     if max(rows, cols) > kernels.MAX_MATRIX_DIM:
         raise ValueError(f"at most {kernels.MAX_MATRIX_DIM} rows and columns")

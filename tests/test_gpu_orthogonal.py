@@ -272,3 +272,12 @@ def test_many_steps(steps, shape):
     g = _matrix(shape)
     _assert_polar(orthogonalize(g.cuda(), steps), g, steps)
     assert polar_off(300) < 0.03      # (a bound that says something)
+
+
+def test_scales_that_fp32_does_not_hold_are_refused():
+    g = torch.randn(4, 6, device="cuda")
+    for scale in (1e39, -1e300, float("inf")):
+        with pytest.raises(ValueError, match="scale"):
+            orthogonalize(g, 5, scale=scale)
+    largest = torch.finfo(FP32).max
+    assert not orthogonalize(g, 5, scale=largest).isnan().any()
