@@ -248,18 +248,22 @@ class RMSLinearCrossEntropy(torch.autograd.Function):
             None if bias is None else bias.float().contiguous(), flat, softcap, ignore_index,
             reduction, True)
         del normalized
-        ctx.saved = _SavedActivation(x, compressed and x.numel() >= min_elements,
-                                     distribution or act_dist, buffer)
-        ctx.save_for_backward(norm_weight, rstd, weight, bias, flat, stats)
+        # (An input that is kept as it is: autograd notices a change of it.)
+        packed = compressed and x.numel() >= min_elements
+        ctx.saved = _SavedActivation(x, True, distribution or act_dist, buffer) if packed else None
+        ctx.save_for_backward(None if packed else x, norm_weight, rstd, weight, bias, flat, stats)
         ctx.how = softcap, ignore_index, reduction
         return out.clone().view(targets.shape) if reduction == "none" else out
 
     @staticmethod
     @first_order
     def backward(ctx, grad):
-        norm_weight, rstd, weight, bias, targets, stats = ctx.saved_tensors
-        x = ctx.saved.take()
-        ctx.saved = None
+        x, norm_weight, rstd, weight, bias, targets, stats = ctx.saved_tensors
+        if x is None:
+            if ctx.saved is None:
+                raise RuntimeError("the compressed input was freed by an earlier backward pass")
+            x = ctx.saved.take()
+            ctx.saved = None
         need = ctx.needs_input_grad
         normalized, _ = _norm(x, norm_weight)
         grad_normalized, grad_weight, grad_bias = products.cross_entropy_backward(

@@ -240,3 +240,28 @@ def test_heads_gradients_are_no_constants(reduction):
         assert torch.equal(grad, plain)
         with pytest.raises(RuntimeError, match="differentiated once only"):
             grad.float().square().sum().backward()
+
+
+def test_changed_inputs_of_the_head_are_noticed():
+    x, weight, gain, bias, targets = _head()
+    leaf, hidden = gain.requires_grad_(), x.clone()
+    out = layers.RMSLinearCrossEntropy.apply(hidden, weight, leaf, bias, targets)
+    hidden.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.backward()
+
+
+def test_a_second_backward_pass_of_the_head():
+    """An input that is not compressed is still there; a compressed one was freed."""
+    for compressed in (False, True):
+        x, weight, gain, bias, targets = _head()
+        leaves = [t.requires_grad_() for t in (x, weight, gain, bias)]
+        buffer = TensorBuffer(8 * 2 ** 20, device=x.device) if compressed else None
+        out = layers.RMSLinearCrossEntropy.apply(*leaves, targets, buffer, compressed,
+                                                 layers.act_dist, 1024)
+        first = torch.autograd.grad(out, leaves, retain_graph=True)
+        if compressed:
+            with pytest.raises(RuntimeError, match="freed by an earlier backward pass"):
+                out.backward()
+        else:
+            assert all(map(torch.equal, first, torch.autograd.grad(out, leaves)))
