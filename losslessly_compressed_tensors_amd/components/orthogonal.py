@@ -20,6 +20,21 @@ __all__ = ["orthogonalize"]
 _EPS = 1e-7
 
 
+def check_orthogonalize(G, steps, count: int | None = None) -> int:
+    """``steps`` of checked arguments; ``count``: of matrices like ``G``'s, if not its own."""
+    if not isinstance(G, Tensor) or G.ndim < 2:
+        raise TypeError("G must be a torch.Tensor of at least two dimensions")
+    _check_tensor(G, "G", G.ndim, tuple(kernels.TYPES))
+    steps = _whole(steps, "steps", 0, 1000)
+    rows, cols = G.shape[-2:]
+    if max(rows, cols) > kernels.MAX_MATRIX_DIM:
+        raise ValueError(f"at most {kernels.MAX_MATRIX_DIM} rows and columns")
+    count = math.prod(G.shape[:-2]) if count is None else count
+    if kernels.orthogonal_tiles(count, rows, cols) >= kernels.MAX_TILES:
+        raise ValueError(f"too many matrices: {count} of {rows} x {cols}")
+    return steps
+
+
 @torch.compiler.disable
 @torch.no_grad()
 def orthogonalize(G: Tensor, steps: int = 5, *, scale: float = 1.0) -> Tensor:
@@ -41,19 +56,10 @@ def orthogonalize(G: Tensor, steps: int = 5, *, scale: float = 1.0) -> Tensor:
 
     Matrices past 128 x 256 need 6 bytes per value and per value of ``X X^T`` and 8 KiB each
     (with 2048 columns 32 MiB more) while the call runs."""
-    if not isinstance(G, Tensor) or G.ndim < 2:
-        raise TypeError("G must be a torch.Tensor of at least two dimensions")
-    _check_tensor(G, "G", G.ndim, tuple(kernels.TYPES))
-    steps = _whole(steps, "steps", 0, 1000)
+    steps = check_orthogonalize(G, steps)
     if not abs(scale) <= torch.finfo(torch.float32).max:
         raise ValueError("scale must be finite, in FP32")
-    rows, cols = G.shape[-2:]
-    if max(rows, cols) > kernels.MAX_MATRIX_DIM:
-        raise ValueError(f"at most {kernels.MAX_MATRIX_DIM} rows and columns")
-    count = math.prod(G.shape[:-2])
-    if kernels.orthogonal_tiles(count, rows, cols) >= kernels.MAX_TILES:
-        raise ValueError(f"too many matrices: {count} of {rows} x {cols}")
     if G.numel() == 0:
         return torch.empty(G.shape, dtype=torch.bfloat16, device=G.device)
-    out = kernels.orthogonalize(G.reshape(-1, rows, cols), steps, float(scale), _EPS)
+    out = kernels.orthogonalize(G.reshape(-1, *G.shape[-2:]), steps, float(scale), _EPS)
     return out.view(G.shape)

@@ -42,6 +42,7 @@ the dense update rounds after each operation.
 from __future__ import annotations
 
 import math
+from collections import Counter
 from typing import Iterable
 
 import torch
@@ -52,7 +53,7 @@ from ..codec.decode import decode_batch
 from ..operations import a_compA_add_B
 from ..tensor_buffer import TensorBuffer
 from .dist_configs import momentum_dist, momentum_first_dist
-from .orthogonal import orthogonalize
+from .orthogonal import check_orthogonalize, orthogonalize
 
 # Newton-Schulz polynomial p(s) = a s + b s^3 + c s^5 on the singular values:
 # p(1) = 1 and p'(1) = 0, so unit singular values attract quadratically.
@@ -263,6 +264,12 @@ class SparseMuon:
         groups: dict[tuple, list[tuple[int, Tensor, bool]]] = {}
         active = [(index, param.grad) for index, param in enumerate(self.params)
                   if param.grad is not None]
+        if self.fused:
+            # A refused step leaves gradients and momenta as they were.
+            shapes = Counter(grad.shape for _, grad in active)
+            for _, grad in active:
+                check_orthogonalize(grad, self.ns_iters,
+                                    shapes[grad.shape] * math.prod(grad.shape[:-2]))
         # Momenta are checked out 16 at a time: one decode launch for the 16
         # (each is a few codec blocks, so its own decode would be bound by one
         # block's latency), and at most 16 dense momenta at once.

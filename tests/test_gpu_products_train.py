@@ -265,3 +265,33 @@ def test_a_second_backward_pass_of_the_head():
                 out.backward()
         else:
             assert all(map(torch.equal, first, torch.autograd.grad(out, leaves)))
+
+
+@pytest.mark.parametrize("compressed", [False, True])
+def test_a_refused_step_of_muon_changes_nothing(compressed):
+    shapes = [(256, 128), ((1 << 16) + 1, 2)]
+    g = torch.Generator().manual_seed(0)
+    params = [torch.nn.Parameter(torch.randn(*s, generator=g).to(BF16).cuda()) for s in shapes]
+    buffer = TensorBuffer(16 * 2 ** 20, device="cuda") if compressed else None
+    muon = SparseMuon(params, compressed=compressed, buffer=buffer, fused=True)
+    params[0].grad = torch.randn(*shapes[0], generator=g).to(BF16).cuda()
+    muon.step()
+    for p in params:
+        p.grad = torch.randn(p.shape, generator=g).to(BF16).cuda()
+
+    def held():
+        momenta = [m.decompress() if isinstance(m, LCTTensor) else m
+                   for m in muon.momentums if m is not None]
+        return [t.detach().clone() for t in (*params, *(p.grad for p in params), *momenta)]
+
+    before = held()
+    with pytest.raises(ValueError, match="at most 65536 rows"):
+        muon.step()
+    assert len(before) == len(held()) and all(map(torch.equal, before, held()))
+    muon.ns_iters = 1001
+    params[1].grad = None
+    with pytest.raises(ValueError, match="steps"):
+        muon.step()
+    muon.ns_iters = 5
+    muon.step()
+    assert not torch.equal(before[0], params[0])
