@@ -230,7 +230,8 @@ class RMSLinearCrossEntropy(torch.autograd.Function):
     """:class:`RMSLinear` and the cross entropy of its output, whose logits are never kept
     (``components/losses.py``'s ``linear_cross_entropy``; the reference's head keeps those
     of a chunk of tokens, ``examples/nanogpt/train_gpt_lct.py:88-140``); saves the norm
-    input.  Returns the FP32 sum, mean or per-token losses."""
+    input.  Returns the FP32 sum, mean or per-token losses.  What tokens whose target is
+    ``ignore_index`` hold reaches nothing, the norm's gradients included."""
 
     @staticmethod
     def forward(ctx, x, weight, norm_weight, bias, targets, buffer=None, compressed=False,
@@ -241,7 +242,7 @@ class RMSLinearCrossEntropy(torch.autograd.Function):
                                                     reduction)
         if targets.numel() == 0:
             raise ValueError("the head needs a token")
-        normalized, rstd = _norm(x, norm_weight)
+        normalized, _ = _norm(x, norm_weight)
         flat = targets.reshape(-1).contiguous()
         out, stats = products.cross_entropy_forward(
             normalized.reshape(-1, x.shape[-1]), W,
@@ -251,21 +252,25 @@ class RMSLinearCrossEntropy(torch.autograd.Function):
         # (An input that is kept as it is: autograd notices a change of it.)
         packed = compressed and x.numel() >= min_elements
         ctx.saved = _SavedActivation(x, True, distribution or act_dist, buffer) if packed else None
-        ctx.save_for_backward(None if packed else x, norm_weight, rstd, weight, bias, flat, stats)
+        ctx.save_for_backward(None if packed else x, norm_weight, weight, bias, flat, stats)
         ctx.how = softcap, ignore_index, reduction
         return out.clone().view(targets.shape) if reduction == "none" else out
 
     @staticmethod
     @first_order
     def backward(ctx, grad):
-        x, norm_weight, rstd, weight, bias, targets, stats = ctx.saved_tensors
-        if x is None:
+        x, norm_weight, weight, bias, targets, stats = ctx.saved_tensors
+        packed = x is None
+        if packed:
             if ctx.saved is None:
                 raise RuntimeError("the compressed input was freed by an earlier backward pass")
             x = ctx.saved.take()
             ctx.saved = None
+        # Ignored tokens' gradients of zero would meet what they hold.
+        ignored = (targets == ctx.how[1]).view(*x.shape[:-1], 1)
+        x = x.masked_fill_(ignored, 0) if packed else x.masked_fill(ignored, 0)
         need = ctx.needs_input_grad
-        normalized, _ = _norm(x, norm_weight)
+        normalized, rstd = _norm(x, norm_weight)
         grad_normalized, grad_weight, grad_bias = products.cross_entropy_backward(
             grad.contiguous(), normalized.reshape(-1, x.shape[-1]), dense_weight(weight),
             None if bias is None else bias.float().contiguous(), targets, stats, *ctx.how,

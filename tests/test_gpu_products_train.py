@@ -295,3 +295,22 @@ def test_a_refused_step_of_muon_changes_nothing(compressed):
     muon.ns_iters = 5
     muon.step()
     assert not torch.equal(before[0], params[0])
+
+
+@pytest.mark.parametrize("compressed", [False, True])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -3e38])
+def test_what_ignored_tokens_hold_reaches_nothing_of_the_head(value, compressed):
+    results = []
+    for dirty in (False, True):
+        x, weight, gain, bias, targets = _head()
+        if dirty:
+            x[targets == -100] = value
+        held = x.clone()
+        leaves = [t.requires_grad_() for t in (x, weight, gain, bias)]
+        buffer = TensorBuffer(8 * 2 ** 20, device=x.device) if compressed else None
+        out = layers.RMSLinearCrossEntropy.apply(*leaves, targets, buffer, compressed,
+                                                 layers.act_dist, 1024, 15.0)
+        results.append([out.detach(), *torch.autograd.grad(out, leaves)])
+        assert torch.equal(x.detach().view(torch.int16), held.view(torch.int16))
+    assert (targets == -100).any() and not results[1][1][targets == -100].any()
+    assert all(map(torch.equal, *results))
