@@ -7,9 +7,11 @@
 //     loss = log(sum_v exp(l_v)) - l_t = log(1 + sum_{v != t} exp(l_v - l_t)),
 //     dz_v = g (exp(l_v) / sum - [v = t]) (1 + (z / s)^2)^(-3/2),
 //     dx = dz W,  dW = dz^T x,  dbias = the columns' sums of dz.
-// dz is rounded to 16 bits for its products, as far off as their results' own rounding.  Of
-// up to 128 tokens, whose products wait for memory in any case, what the rounding leaves
-// is multiplied too: there a few large values carry the results.
+// dz is rounded to 16 bits for its products, as far off as their results' own rounding: the
+// gradients end up to 1.25 times as far from those in 64 bits as ones rounded once.  Multiplying
+// what the rounding leaves too would double both products (1.26 of 2.6 ms of 8192 x 50304 x 768).
+// Of up to 128 tokens, whose products wait for memory in any case, that is done: there a few
+// large values carry the results.
 // The second form of the loss keeps its precision where the target is likely:
 // the target is left out of the sums, and its own gradient is exp(-loss) - 1.
 //
@@ -42,6 +44,8 @@ using LogitProduct = Product<kHalf, Lie::kRows, Lie::kRows, kLogitRows, 128, 2, 
 // x 1024 758 | 748, x 1536 1066 | 1104, x 2048 1377 | 1439, 32000 x 4096 1703 | 1809; of 2048
 // tokens 50176 x 1536 306 | 298, 32000 x 4096 449 | 491; of 512 128 | 172; of 256 110 | 108, and
 // 131072 x 2048 151 | 176.  One workgroup per compute unit, whose end no other's products hide.
+// The rule goes by channels alone, of more than 128 tokens: 1536 channels lose 3 % of 8192 tokens
+// by it and gain 3 % of 2048, and 4096 channels lose 2 % of 256.
 constexpr int32_t kDeep = 2048;
 template <bool kHalf>
 using DeepProduct = Product<kHalf, Lie::kRows, Lie::kRows, 256, 256, 4, 2, 64, 2>;
@@ -274,9 +278,10 @@ __device__ __forceinline__ bool far_of(const P &p, const Cap &cap) {
 // each): a token's maximum and sum need one exchange between two lanes.
 //
 // Bound by the matrix instructions: 2 * tokens * vocab * dim operations, and the exponentials
-// behind them.  14746 x 100352 x 2048: 5.02 ms, 1210 TFLOP/s (at 1.3 GHz: the power limit's);
-// 4095 x 32000 x 4096: 0.83 to 0.93 ms, 1290 to 1150; 8192 x 50304 x 768, capped: 624 to 730 us,
-// 1010 to 870 (12 steps a tile; matrix instructions busy 0.54 of the time, at 1.81 GHz).
+// behind them.  14746 x 100352 x 2048: 5.0 to 5.2 ms, 1210 to 1170 TFLOP/s (matrix instructions
+// busy 0.66 of the time, at the power limit's 1.74 GHz); 4095 x 32000 x 4096: 0.83 to 0.97 ms, 1290
+// to 1100 (0.69, 1.6 GHz); 8192 x 50304 x 768, capped: 623 to 730 us, 1010 to 870 (12 steps a tile;
+// 0.54, 1.78 GHz).
 template <class P, bool kCap, bool kBias>
 __global__ __launch_bounds__(P::kThreads, P::kThreads == 256 ? 2 : 1) void logits_kernel(
     lct_cross_entropy c, Counted t, int32_t vocab_tiles, int32_t token_tiles,
@@ -512,9 +517,9 @@ __global__ __launch_bounds__(kPrepareThreads) void total_kernel(lct_cross_entrop
 // that follow read, and its sums over these tokens.
 //
 // As the logits' kernel, and 2 bytes written a logit: a quarter of 8192 x 50304 x 768, capped,
-// 199 to 220 us, 800 to 710 TFLOP/s (matrix instructions busy 0.38 of the time, at 1.98 GHz; the
+// 194 to 220 us, 820 to 720 TFLOP/s (matrix instructions busy 0.39 of the time, at 2.0 GHz; the
 // epilogue's exponential, root and stores take as long as the 12 steps); a thirteenth of 14746
-// x 100352 x 2048 466 us, 1000.  The parts a workgroup works in, of both on a compute unit,
+// x 100352 x 2048 462 to 475 us, 1010 to 980.  The parts a workgroup works in, of both on a compute unit,
 // overlap: starting half of them late, or stores past the caches, changed nothing.
 template <class P, bool kHalf, bool kCap, bool kBias>
 __global__ __launch_bounds__(P::kThreads, 2) void gradient_kernel(
@@ -756,9 +761,10 @@ __device__ __forceinline__ void weight_gradient(const lct_cross_entropy &c, cons
 
 // Both, one launch: neither has as many tiles as fill the compute units evenly.
 //
-// Bound by the matrix instructions: a quarter of 8192 x 50304 x 768 314 us, 1010 TFLOP/s (96
-// tiles 400 steps deep and 150 of 256 fill the compute units to three quarters); a thirteenth of
-// 14746 x 100352 x 2048 794 us, 1180.
+// Bound by the matrix instructions: a quarter of 8192 x 50304 x 768 314 to 322 us, 1010 to 980
+// TFLOP/s (96 tiles 400 steps deep and 150 of 256 fill the compute units to three quarters: busy
+// 0.66 of the time, matrix instructions 0.50, at 1.93 GHz); a thirteenth of 14746 x 100352 x 2048
+// 794 to 820 us, 1180 to 1140 (0.86, 0.63, 1.77 GHz).
 template <bool kHalf, bool kExact>
 __global__ __launch_bounds__(kExact ? 256 : 512, kExact ? 2 : 1) void products_kernel(
     lct_cross_entropy c, Counted t, PieceProducts q, uint32_t weight_grid) {

@@ -528,7 +528,7 @@ __global__ __launch_bounds__(kWaves *kWave) void small_kernel(lct_orthogonal o) 
 
 // The smallest that holds the matrices.  Bound by the steps' order: three products, each with
 // its barriers and its reads of LDS, of one compute unit.  Up to 256 of them run at once: 8 of
-// 96 x 160, 5 steps, 30.3 us (of which 12 without a step), where the launches for larger
+// 96 x 160, 5 steps, 30.6 us (of which 12 without a step), where the launches for larger
 // matrices took 68; one of 64 x 64, 12 steps: 25 us.
 void small(const lct_orthogonal &o, hipStream_t stream) {
     const uint32_t count = static_cast<uint32_t>(o.count);
@@ -706,8 +706,8 @@ __global__ __launch_bounds__(P::kThreads, 1) void symmetric_join_kernel(Symmetri
 // rows are whole 16-byte pieces.
 //
 // Bound by the products and by X's way in and out (4 bytes a value each way, through LDS), which
-// a tile's waves do one after the other: 48 x 768 x 768 82.5 us, 530 TFLOP/s; 4096 x 4096 by
-// 11008 395 us, 935; 16 x 1024 x 4096 221 us, 620.
+// a tile's waves do one after the other: 48 x 768 x 768 82 to 84 us, 530 TFLOP/s; 4096 x 4096 by
+// 11008 395 to 411 us, 935 to 900; 16 x 1024 x 4096 219 us, 620.
 template <class P, bool kLast>
 __global__ __launch_bounds__(P::kThreads, P::kThreads == 256 ? 2 : 1) void update_kernel(
     const uint16_t *poly, const uint16_t *x, int32_t count, int32_t rows, int32_t cols,
@@ -932,7 +932,7 @@ extern "C" int32_t lct_orthogonalize(const lct_orthogonal *o, void *workspace,
     // Two steps at once have 3 products with X, of rows^2 cols each, in place of 6 and 5 in
     // place of 2 of rows^3, the symmetric ones by half.  us of 12 or 5 steps one | two at a time:
     // 48 x 768 x 768 1765 | 1858; 16 x 4096 x 1024 1907 | 1409; 4096 x 11008 3955 | 3217; of few
-    // tiles, which cost their launches, 768 x 768 138 | 138, 8 x 96 x 160 76 | 81.
+    // tiles, which cost their launches, 768 x 768 138 | 138.
     const bool pairs = 2 * cols >= 3 * rows && it.all_tiles() >= kFewTiles;
     for (int32_t s = 0; s < o->steps;) {
         uint16_t *const m = it.square[0], *const p = it.square[1], *const r = it.square[2];

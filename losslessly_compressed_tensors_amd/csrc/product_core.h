@@ -18,7 +18,7 @@ namespace lct {
 
 enum class Lie { kRows, kColumns };
 
-// One operand's tile of kTile rows by 32 of k: how it comes to LDS and how an
+// One operand's tile of kTile rows by kStep of k: how it comes to LDS and how an
 // instruction's 32 rows by 16 of k are read from there.
 //
 // LDS returns 256 bytes a clock: the chunks of 16 bytes that 16 rows are read at (by
@@ -59,7 +59,7 @@ struct Operand {
         }
     }
 
-    // k .. k + 31 of `depth`; zeros past it and past the last row.
+    // k .. k + kStep - 1 of `depth`; zeros past it and past the last row.
     __device__ __forceinline__ void issue(int32_t k, int32_t depth, uint16_t *tile) const {
         const int32_t left = depth - k;
         const int32_t lines = kLie == Lie::kRows ? valid : min(left, kStep);

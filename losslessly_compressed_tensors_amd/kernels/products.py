@@ -141,7 +141,8 @@ def _last_end(lengths, slots: int) -> float:
 @lru_cache(maxsize=4096)
 def _parts(tokens: int, piece: int, vocab: int, dims: int) -> int:
     """Into how many parts the sum for the gradient of x is divided: those with which a
-    piece's products end first, counted in their steps of 32."""
+    piece's products end first, counted in their steps of 32 (as if the weight's gradient
+    were needed too)."""
     # The kernel for up to _EXACT_TOKENS takes tiles of 128, two at once per compute unit,
     # and multiplies twice; that for more takes tiles of 256, one at once.
     tile, at_once, twice = (128, 2, 2) if tokens <= _EXACT_TOKENS else (256, 1, 1)
