@@ -917,7 +917,8 @@ int32_t lct_dropout(const void *x, const void *residual, void *out, int64_t n, i
 
 /* ---- softmax cross entropy of a projection onto a vocabulary, in pieces of the
  * vocabulary (examples/nanogpt/train_gpt_lct.py:88-140, which keeps the logits of a
- * chunk of tokens): z = x W^T + bias, l = z / sqrt(1 + (z / softcap)^2) (softcap 0: z),
+ * chunk of tokens): z = x W^T + bias, l = z / sqrt(1 + (z / softcap)^2) (softcap 0: z; else
+ * between 1e-19 and 1e19),
  * losses[n] = log(sum_v exp(l[n][v])) - l[n][targets[n]].
  *
  * x [tokens, dim] and weight [vocab, dim]: BF16, or FP16 where fp16 != 0, rows by

@@ -869,7 +869,7 @@ int32_t check(const lct_cross_entropy *c) {
         || c->weight_stride > LCT_MAX_CROSS_ENTROPY_DIM || !aligned(c->x, 16)
         || !aligned(c->weight, 16) || !aligned(c->bias, 4)
         || !aligned(c->targets, c->targets_64 ? 8 : 4) || !(c->softcap >= 0.0f)
-        || !(c->softcap < 1e19f))
+        || !(c->softcap < 1e19f) || (c->softcap > 0.0f && c->softcap < 1e-19f))
         return LCT_E_ARG;
     return 0;
 }

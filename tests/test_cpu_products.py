@@ -272,3 +272,12 @@ def test_the_biases_parts_are_a_tile_of_tokens_each(lib):
         gradients = _gradients(grad_bias=1 << 20, columns=1 << 20, bias_floats=floats,
                                hidden_floats=hidden, dz=(1 << 20) + 8)
         assert lib.lct_cross_entropy_backward(record, gradients, None) == code
+
+
+@pytest.mark.parametrize("softcap", [1e-45, 1e-39, 9e-20])
+def test_caps_whose_inverse_may_not_fit_are_refused(lib, softcap):
+    """1 / softcap of a subnormal number is infinite, and 0 / softcap then no number."""
+    record, at = _cross_entropy(softcap=softcap), 1 << 20
+    assert lib.lct_cross_entropy_forward(record, None, 0, None, 0, at, 1 << 40, at, at, None, 0,
+                                         None) == E_ARG
+    assert lib.lct_cross_entropy_backward(record, _gradients(), None) == E_ARG
